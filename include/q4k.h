@@ -237,6 +237,133 @@ int q4k_rms_norm(void* stream, const void* x, const float* w, void* y, uint32_t 
 int q4k_rms_norm_gather(void* stream, const void* x, const float* w, void* out, uint32_t k, const uint32_t* counts, const uint32_t* samples,
                         uint32_t nqueries, float eps, uint32_t dtype, uint32_t* rows_out);
 
+/* ---- Rotary positions and head norms --------------------------------------
+ * Between the QKV projection and attention: the reference's
+ * attention_prepare (attention.metal:15, init_rope native_ops.metal:115),
+ * here for any head size, two pair layouts, a rotated part of the head, and
+ * frequencies scaled for long contexts.  `device` is the GPU of the pointers
+ * and of `stream`; the caller's current device is left as it was. */
+#define Q4K_ROPE_HALF 0u        /* pair i: elements i and i + rot_dim / 2 */
+#define Q4K_ROPE_INTERLEAVED 1u /* pair i: elements 2i and 2i + 1 */
+
+#define Q4K_ROPE_SCALING_NONE 0u   /* f_i = base^(-2i / rot_dim) */
+#define Q4K_ROPE_SCALING_LINEAR 1u /* f_i / factor: positions interpolated */
+#define Q4K_ROPE_SCALING_NTK 2u    /* base * factor^(rot_dim / (rot_dim - 2)) */
+#define Q4K_ROPE_SCALING_YARN 3u   /* f_i / factor below beta_slow turns in the original context, f_i above beta_fast, a ramp between */
+
+#define Q4K_MAX_HEAD_DIM 1024u
+
+/* The rot_dim / 2 angles per position, in radians, of a rotation, in 64 bits
+ * (host memory), and the factor of the rotated values that goes with them
+ * (*scale: 0.1 ln(factor) + 1 for YARN with factor > 1, else 1; may be NULL).  original_context,
+ * beta_slow and beta_fast are read for YARN only (0 < beta_slow < beta_fast;
+ * 1 and 32 in the published method). */
+int q4k_rope_frequencies(uint32_t rot_dim, double base, uint32_t scaling, double factor, uint32_t original_context, double beta_slow,
+                         double beta_fast, double* inv_freq, float* scale);
+
+/* Heads of a packed batch: row r, head j, element d is at
+ * r * row_stride + j * head_stride + d (strides in elements).  `out` is `in`
+ * with the same strides, or none of its elements is one of `in`'s; the
+ * outputs of a call must not overlap each other. */
+typedef struct q4k_heads {
+  const void* in;
+  void* out;
+  const float* weight; /* norm weights [head_dim] (q4k_qk_norm_rope) */
+  int64_t in_row_stride, in_head_stride, out_row_stride, out_head_stride;
+  uint32_t heads;
+} q4k_heads;
+
+typedef struct q4k_rotation {
+  const double* inv_freq;   /* device, rot_dim / 2 */
+  const int32_t* positions; /* device, one per row; any value, read when the call runs */
+  uint32_t rot_dim;         /* even, <= head_dim; elements behind it are not rotated */
+  uint32_t layout;
+  float scale; /* of the rotated part */
+} q4k_rotation;
+
+/* Rotates the pairs of every head by position * inv_freq: with c, n = scale *
+ * (cos, sin), (a, b) becomes (a c - b n, b c + a n).  Angles are formed in 64
+ * bits, the rest in fp32 with one rounding to the dtype.  rows may be 0. */
+int q4k_rope(void* stream, int device, const q4k_heads* x, const q4k_rotation* rotation, uint32_t rows, uint32_t head_dim, uint32_t dtype);
+
+/* RMS norm of every query and key head (x * weight / sqrt(sum(x^2) / head_dim
+ * + eps)), then the rotation, in one launch and one rounding.  Typically q and
+ * k are parts of the QKV projection's output, in place or not.  rot_dim 0
+ * norms only. */
+int q4k_qk_norm_rope(void* stream, int device, const q4k_heads* q, const q4k_heads* k, const q4k_rotation* rotation, uint32_t rows,
+                     uint32_t head_dim, float eps, uint32_t dtype);
+
+/* ---- Low-rank adapters beside a projection ---------------------------------
+ * No counterpart in the reference.  Up to `slots` adapters of one projection
+ * [n, k], stacked: a [slots, rank, k] and b [slots, n, rank], fp16, device.
+ * Sequence q of a packed batch takes adapter ids[q]; an id outside
+ * [0, slots) means none.  ids, ranks and scales are read when the call runs, so
+ * a captured call follows them from replay to replay. */
+#define Q4K_LORA_MAX_RANK 512u
+typedef struct q4k_adapters {
+  const void* a;
+  const void* b;
+  const int32_t* ids;    /* device, one per sequence */
+  const int32_t* ranks;  /* device, [slots]: ranks in use, clamped to [0, rank]; NULL: all `rank` */
+  const float* scales;   /* device, [slots]; NULL: 1 */
+  uint32_t slots, rank;
+} q4k_adapters;
+
+/* y[m, n] = aux + scale * (x[m, k] A^T) B^T, row by row with the adapter of the
+ * row's sequence (aux NULL: 0; aux may be y, which then keeps its bits in rows
+ * without an adapter).  query_counts as for q4k_linear (NULL: one sequence);
+ * k a multiple of 256, n of 16.  x, a and b are used as they are (x A^T sums
+ * in fp32; fp32 x is not rounded), (x A^T) stays fp32, y is rounded once.
+ * Elements of a and b past an adapter's rank are not used.  The sums of K-slices
+ * live in the device's workspace. */
+int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m, uint32_t k, uint32_t n,
+             const uint32_t* query_counts, uint32_t nqueries, uint32_t dtype);
+
+/* q4k_linear with adapters: y = post(x W^T + scale (x A^T) B^T, aux).  The
+ * adapters' part is written first (post 0 and 1: into y with aux added, rounded to the
+ * dtype; post 2: into a workspace buffer of m * n) and the projection adds to it. */
+int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
+                    const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);
+
+/* ---- Logits -----------------------------------------------------------------
+ * No counterpart in the reference (its sample_logits, native_ops.metal:122,
+ * takes them as they are).  Every pointer is a device pointer, read when the
+ * call runs; a group whose pointers are NULL is left out. */
+typedef struct q4k_logits_params {
+  /* The rows' texts, in the request token buffer of q4k_embedding_batch:
+   * token_slots rows of `capacity` tokens.  Row r's text is the first
+   * lengths[r] tokens of slot slots[r] (NULL: slot r); those before prompts[r]
+   * (NULL: 0) were given, the others generated.  A slot outside the buffer has
+   * no text, a length is clamped to the capacity, tokens outside the vocabulary
+   * do not count. */
+  const int32_t* tokens;
+  const int32_t* slots;
+  const int32_t* lengths;
+  const int32_t* prompts;
+  const float* repetition; /* [rows]: tokens of the text, l > 0 ? l / p : l * p */
+  const float* frequency;  /* [rows]: minus f * (generated occurrences) */
+  const float* presence;   /* [rows]: minus p for a generated token */
+  /* Row r's biases: entries bias_offsets[r] .. bias_offsets[r + 1] - 1 of
+   * bias_tokens / bias_values (bias_count entries); the last entry of a token
+   * counts. */
+  const int32_t* bias_offsets; /* [rows + 1] */
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  /* mask_count bit masks of mask_stride words (>= vocab / 32, rounded up): bit
+   * v % 32 of word v / 32 allows token v.  Row r takes mask mask_rows[r] (NULL:
+   * r; outside [0, mask_count): none). */
+  const uint32_t* mask;
+  const int32_t* mask_rows;
+  uint32_t token_slots, capacity, bias_count, mask_count, mask_stride;
+} q4k_logits_params;
+
+/* out[r] = logits[r] with repetition, then frequency and presence, then the
+ * bias, then -inf where the mask forbids (whatever was there, NaN too).  fp32
+ * arithmetic, one rounding to the dtype.  Row strides in elements; out is logits
+ * with the same stride, or does not overlap it.  rows may be 0. */
+int q4k_process_logits(void* stream, int device, const void* logits, void* out, uint32_t rows, uint32_t vocab, int64_t logits_stride,
+                       int64_t out_stride, const q4k_logits_params* params, uint32_t dtype);
+
 /* ---- GGUF reader ---------------------------------------------------------
  * Replaces the reference's ggml gguf_init_from_buffer over the mapped model
  * file (model/qwen35/forward.cpp:12-23, loadWeights).  The file is mapped
@@ -290,7 +417,7 @@ int q4k_workspace_allocations(uint64_t* count);
 #define Q4K_KERNEL_GEMV 1u       /* MFMA GEMV, phases 0/2 and small prefill */
 #define Q4K_KERNEL_GEMV_GATED 2u /* fused gate/up GEMV, phase 3 */
 #define Q4K_KERNEL_GEMM 3u       /* LDS-tiled MFMA GEMM, phase 1 */
-#define Q4K_KERNEL_AUX 4u        /* token embedding, RMS norm, rms_norm_gather */
+#define Q4K_KERNEL_AUX 4u        /* token embedding, RMS norm, rms_norm_gather, rotary positions, adapters, logits */
 
 /* Event timing of every kernel launch (no counterpart in the reference, whose
  * method is paired A/B timing, agents/KERNELS.md:13-21).  While enabled, each

@@ -74,6 +74,14 @@ def _load():
         "q4k_embedding_batch": (c_int, [p, p, p, u32, pu32, pu32, pu32, u32, p, u32, pu32]),
         "q4k_rms_norm": (c_int, [p, p, p, p, u32, u32, ctypes.c_float, u32]),
         "q4k_rms_norm_gather": (c_int, [p, p, p, p, u32, pu32, pu32, u32, ctypes.c_float, u32, pu32]),
+        # Structures and count tables of these arrive packed (bytes).
+        "q4k_rope_frequencies": (c_int, [u32, ctypes.c_double, u32, ctypes.c_double, u32, ctypes.c_double, ctypes.c_double,
+                                         ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_float)]),
+        "q4k_rope": (c_int, [p, c_int, p, p, u32, u32, u32]),
+        "q4k_qk_norm_rope": (c_int, [p, c_int, p, p, p, u32, u32, ctypes.c_float, u32]),
+        "q4k_lora": (c_int, [p, c_int, p, p, p, p, u32, u32, u32, p, u32, u32]),
+        "q4k_linear_lora": (c_int, [p, p, p, p, p, p, u32, p, u32, u32, u32]),
+        "q4k_process_logits": (c_int, [p, c_int, p, p, u32, u32, ctypes.c_int64, ctypes.c_int64, p, u32]),
         "q4k_profile_enable": (c_int, [c_int]),
         "q4k_profile_query": (c_int, [u32, pu32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),
                                       ctypes.POINTER(ctypes.c_double)]),

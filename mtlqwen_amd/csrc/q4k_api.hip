@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -83,6 +84,8 @@ struct Workspace {
   size_t pack_bytes = 0;
   uint8_t* normed = nullptr;  // q4k_mlp's RMS-normalised x when the norm is not fused
   size_t normed_bytes = 0;
+  uint8_t* adapted = nullptr;  // q4k_linear_lora: the gated projection before its gate
+  size_t adapted_bytes = 0;
   std::vector<void*> retired;
   // Fixed-size buffers in the no-allocation scratch: never grown; a call
   // that needs more fails (ensure_buffer).
@@ -1708,6 +1711,413 @@ int q4k_rms_norm_gather(void* stream, const void* x, const float* w, void* out, 
     return fail(Q4K_EALIAS, "out must not overlap x");
   LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_rms_norm(static_cast<hipStream_t>(stream), x, w, out, (int)idx.rows, (int)k, eps, (int)dtype, &idx), "rms_norm_gather launch");
+  return Q4K_OK;
+}
+
+}  // extern "C"
+
+// ---- rotary positions, head norms, adapters, logits -----------------------
+
+namespace {
+
+// Makes `device` current and restores the caller's device on leaving.
+struct DeviceScope {
+  int before = -1, rc = Q4K_OK;
+  explicit DeviceScope(int device) {
+    hipError_t e = hipGetDevice(&before);
+    if (e == hipSuccess && before != device) {
+      e = hipSetDevice(device);
+      if (e != hipSuccess)
+        before = -1;
+    } else {
+      before = -1;
+    }
+    if (e != hipSuccess)
+      rc = hip_fail(e, "hipSetDevice");
+  }
+  ~DeviceScope() {
+    if (before >= 0)
+      (void)hipSetDevice(before);
+  }
+};
+
+// The elements of a set of heads as two nested runs: `inner` contiguous values
+// from the base on, repeated `count` times every `step` values (the outer of
+// rows and heads).  False if two of its elements share a place, or a stride is
+// negative.
+struct HeadSpan {
+  uintptr_t base = 0;
+  uint64_t inner = 0, step = 0, count = 0;  // bytes, bytes, repetitions
+  uint64_t extent() const { return count ? (count - 1) * step + inner : 0; }
+};
+
+bool head_span(const void* p, int64_t row_stride, int64_t head_stride, uint32_t rows, uint32_t heads, uint32_t dim, size_t es, HeadSpan* span) {
+  uint64_t s[2] = {(uint64_t)row_stride, (uint64_t)head_stride}, c[2] = {rows, heads};
+  if (c[0] <= 1)
+    s[0] = 0;
+  if (c[1] <= 1)
+    s[1] = 0;
+  const int outer = c[1] <= 1 || (c[0] > 1 && s[0] >= s[1]) ? 0 : 1, in = 1 - outer;
+  const bool apart = (c[in] <= 1 || s[in] >= dim) && (c[outer] <= 1 || s[outer] >= (c[in] - 1) * s[in] + dim);
+  span->base = (uintptr_t)p;
+  span->inner = ((c[in] - 1) * s[in] + dim) * es;
+  span->step = s[outer] * es;
+  span->count = c[outer];
+  return apart;
+}
+
+// Whether two sets may share an element: their runs are taken as solid, and
+// sets of one step (columns of one matrix) are compared within the step.
+bool spans_meet(const HeadSpan& a, const HeadSpan& b) {
+  if (!overlaps(reinterpret_cast<const void*>(a.base), a.extent(), reinterpret_cast<const void*>(b.base), b.extent()))
+    return false;
+  const uint64_t step = a.count > 1 ? a.step : b.step;
+  if (step == 0 || (a.count > 1 && b.count > 1 && a.step != b.step) || a.inner > step || b.inner > step)
+    return true;
+  const uint64_t d = b.base >= a.base ? (b.base - a.base) % step : (step - (a.base - b.base) % step) % step;
+  return d < a.inner || d + b.inner > step;
+}
+
+int check_heads(const char* what, const q4k_heads* h, uint32_t rows, uint32_t dim, size_t es, HeadSpan* in, HeadSpan* out) {
+  if (h->heads == 0 || h->heads > 65535)
+    return fail(Q4K_ESHAPE, "%s: heads must be 1..65535 (got %u)", what, h->heads);
+  constexpr int64_t kMaxStride = 1ll << 40;
+  const int64_t strides[4] = {h->in_row_stride, h->in_head_stride, h->out_row_stride, h->out_head_stride};
+  for (int64_t s : strides)
+    if (s < 0 || s > kMaxStride)
+      return fail(Q4K_ESHAPE, "%s: strides must be 0..2^40 elements (got %lld)", what, (long long)s);
+  if (rows == 0)
+    return Q4K_OK;
+  if (!h->in || !h->out)
+    return fail(Q4K_EINVAL, "%s: in and out must be non-NULL", what);
+  (void)head_span(h->in, h->in_row_stride, h->in_head_stride, rows, h->heads, dim, es, in);
+  if (!head_span(h->out, h->out_row_stride, h->out_head_stride, rows, h->heads, dim, es, out))
+    return fail(Q4K_ESHAPE, "%s: elements of the output share a place (row stride %lld, head stride %lld, %u heads of %u)", what,
+                (long long)h->out_row_stride, (long long)h->out_head_stride, h->heads, dim);
+  const bool same = h->in == h->out && (rows <= 1 || h->in_row_stride == h->out_row_stride) &&
+                    (h->heads <= 1 || h->in_head_stride == h->out_head_stride);
+  if (!same && spans_meet(*in, *out))
+    return fail(Q4K_EALIAS, "%s: out must be in with the same strides, or not overlap it", what);
+  return Q4K_OK;
+}
+
+bool span_meets(const HeadSpan& s, const void* p, size_t bytes) {
+  return p && bytes && overlaps(reinterpret_cast<const void*>(s.base), s.extent(), p, bytes);
+}
+
+int run_heads(void* stream, int device, const q4k_heads* sets, int nsets, const q4k_rotation* rot, uint32_t rows, uint32_t dim, bool norm, float eps,
+              uint32_t dtype) {
+  if (dtype > Q4K_DTYPE_F16)
+    return fail(Q4K_EINVAL, "bad dtype %u", dtype);
+  if (dim == 0 || dim > kMaxHeadDim)
+    return fail(Q4K_ESHAPE, "head_dim must be 1..%u (got %u)", kMaxHeadDim, dim);
+  if (rows > 0x7fffffffu)
+    return fail(Q4K_ESHAPE, "at most 2^31 - 1 rows (got %u)", rows);
+  if (rot->rot_dim % 2 != 0 || rot->rot_dim > dim || (rot->rot_dim == 0 && !norm))
+    return fail(Q4K_ESHAPE, "rot_dim must be even and 2..head_dim (got %u of %u)", rot->rot_dim, dim);
+  if (rot->layout > Q4K_ROPE_INTERLEAVED)
+    return fail(Q4K_EINVAL, "bad rotary layout %u", rot->layout);
+  if (norm && !(eps >= 0.0f))
+    return fail(Q4K_EINVAL, "eps must be a non-negative number");
+  if (rot->rot_dim && rows && (!rot->inv_freq || !rot->positions))
+    return fail(Q4K_EINVAL, "inv_freq and positions must be non-NULL");
+  static const char* const names[2][2] = {{"x", ""}, {"q", "k"}};
+  const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2;
+  HeadSpan in[2], out[2];
+  for (int i = 0; i < nsets; ++i) {
+    if (norm && rows && !sets[i].weight)
+      return fail(Q4K_EINVAL, "%s: weight must be non-NULL", names[1][i]);
+    int rc = check_heads(names[nsets - 1][i], &sets[i], rows, dim, es, &in[i], &out[i]);
+    if (rc)
+      return rc;
+  }
+  if (rows == 0)
+    return Q4K_OK;
+  if (nsets == 2 && (spans_meet(out[0], out[1]) || spans_meet(out[0], in[1]) || spans_meet(in[0], out[1])))
+    return fail(Q4K_EALIAS, "the outputs of q and k must not overlap each other or the other's input");
+  for (int i = 0; i < nsets; ++i) {
+    bool meets = span_meets(out[i], rot->positions, rot->rot_dim ? (size_t)rows * 4 : 0) || span_meets(out[i], rot->inv_freq, (size_t)rot->rot_dim * 4);
+    for (int j = 0; j < nsets && norm; ++j)
+      meets = meets || span_meets(out[i], sets[j].weight, (size_t)dim * 4);
+    if (meets)
+      return fail(Q4K_EALIAS, "an output must not overlap the positions, frequencies or norm weights");
+  }
+  HeadsArgs a;
+  for (int i = 0; i < nsets; ++i) {
+    a.in[i] = sets[i].in;
+    a.out[i] = sets[i].out;
+    a.w[i] = sets[i].weight;
+    a.heads[i] = sets[i].heads;
+    a.row_in[i] = sets[i].in_row_stride;
+    a.head_in[i] = sets[i].in_head_stride;
+    a.row_out[i] = sets[i].out_row_stride;
+    a.head_out[i] = sets[i].out_head_stride;
+  }
+  a.inv_freq = rot->inv_freq;
+  a.positions = rot->positions;
+  a.rows = rows;
+  a.dim = (int)dim;
+  a.rot = (int)rot->rot_dim;
+  a.scale = rot->scale;
+  a.eps = eps;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_heads(static_cast<hipStream_t>(stream), a, norm, rot->layout == Q4K_ROPE_INTERLEAVED, (int)dtype, device_cus(device)),
+              "head rotation launch");
+  return Q4K_OK;
+}
+
+// Argument checks of the adapters beside a projection of k inputs and n outputs.
+int check_lora(const q4k_adapters* ad, const void* x, const void* y, const void* aux, uint32_t m, uint32_t k, uint32_t n,
+               const uint32_t* counts, uint32_t nq, uint32_t dtype) {
+  if (!ad)
+    return fail(Q4K_EINVAL, "adapters is NULL");
+  if (dtype > Q4K_DTYPE_F16)
+    return fail(Q4K_EINVAL, "bad dtype %u", dtype);
+  if (k == 0 || k % 256 != 0 || k > (1u << 24) || n == 0 || n % 16 != 0 || n > (1u << 24))
+    return fail(Q4K_ESHAPE, "k must be a positive multiple of 256 and n of 16, both up to 2^24 (got k=%u, n=%u)", k, n);
+  if (m == 0 || m > (1u << 24))
+    return fail(Q4K_ESHAPE, "m must be 1..2^24 (got %u)", m);
+  if (ad->rank == 0 || ad->rank > Q4K_LORA_MAX_RANK)
+    return fail(Q4K_ESHAPE, "the adapters' rank must be 1..%u (got %u)", Q4K_LORA_MAX_RANK, ad->rank);
+  if (ad->slots == 0 || ad->slots > 65536)
+    return fail(Q4K_ESHAPE, "slots must be 1..65536 (got %u)", ad->slots);
+  if (!ad->a || !ad->b || !ad->ids || !x || !y)
+    return fail(Q4K_EINVAL, "a, b, ids, x and y must be non-NULL");
+  int rc = check_counts(counts, nq, m);
+  if (rc)
+    return rc;
+  const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2, yb = (size_t)m * n * es;
+  const uint32_t sequences = counts ? nq : 1;
+  if (overlaps(x, (size_t)m * k * es, y, yb))
+    return fail(Q4K_EALIAS, "x must not overlap y");
+  if (aux && aux != y && overlaps(aux, yb, y, yb))
+    return fail(Q4K_EALIAS, "aux must be y itself or disjoint from it");
+  if (overlaps(ad->a, (size_t)ad->slots * ad->rank * k * 2, y, yb) || overlaps(ad->b, (size_t)ad->slots * ad->rank * n * 2, y, yb) ||
+      overlaps(ad->ids, (size_t)sequences * 4, y, yb) || (ad->ranks && overlaps(ad->ranks, (size_t)ad->slots * 4, y, yb)) ||
+      (ad->scales && overlaps(ad->scales, (size_t)ad->slots * 4, y, yb)))
+    return fail(Q4K_EALIAS, "y must not overlap the adapters");
+  return Q4K_OK;
+}
+
+// The adapters' part of a projection, with the device's workspace lock held.
+int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_adapters* ad, const void* x, void* y, const void* aux, uint32_t m,
+                    uint32_t k, uint32_t n, const uint32_t* counts, uint32_t nq, uint32_t dtype) {
+  LoraArgs a;
+  a.x = x;
+  a.y = y;
+  a.aux = aux;
+  a.a = static_cast<const _Float16*>(ad->a);
+  a.b = static_cast<const _Float16*>(ad->b);
+  a.ids = ad->ids;
+  a.ranks = ad->ranks;
+  a.scales = ad->scales;
+  a.m = (int)m;
+  a.k = (int)k;
+  a.n = (int)n;
+  a.r = (int)ad->rank;
+  a.rpad = (a.r + 15) / 16 * 16;
+  a.slots = (int)ad->slots;
+  a.nq = counts ? (int)nq : 1;
+  uint32_t start = 0;
+  for (int q = 0; q < a.nq; ++q) {
+    a.start[q] = (int)start;
+    a.count[q] = counts ? (int)counts[q] : (int)m;
+    start += (uint32_t)a.count[q];
+  }
+  a.slices = lora_slices(a, device_cus(device));
+  int rc = ensure_buffer(stream, ws, device, ws.part, ws.part_elems, (size_t)a.slices * a.m * a.rpad, "split-K workspace");
+  if (rc)
+    return rc;
+  a.part = ws.part;
+  {
+    LaunchTimer timer(stream, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_lora_shrink(stream, a, (int)dtype), "adapter shrink launch");
+  }
+  LaunchTimer timer(stream, Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_lora_expand(stream, a, (int)dtype), "adapter expand launch");
+  return Q4K_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int q4k_rope_frequencies(uint32_t rot_dim, double base, uint32_t scaling, double factor, uint32_t original_context, double beta_slow,
+                         double beta_fast, double* inv_freq, float* scale) {
+  if (!inv_freq)
+    return fail(Q4K_EINVAL, "inv_freq is NULL");
+  if (rot_dim == 0 || rot_dim % 2 != 0 || rot_dim > Q4K_MAX_HEAD_DIM)
+    return fail(Q4K_ESHAPE, "rot_dim must be even and 2..%u (got %u)", Q4K_MAX_HEAD_DIM, rot_dim);
+  if (scaling > Q4K_ROPE_SCALING_YARN)
+    return fail(Q4K_EINVAL, "bad rotary scaling %u", scaling);
+  if (!(base > 0.0) || !std::isfinite(base))
+    return fail(Q4K_EINVAL, "base must be a positive number");
+  if (scaling != Q4K_ROPE_SCALING_NONE && (!(factor > 0.0) || !std::isfinite(factor)))
+    return fail(Q4K_EINVAL, "factor must be a positive number");
+  if (scaling == Q4K_ROPE_SCALING_NTK && rot_dim == 2)
+    return fail(Q4K_ESHAPE, "NTK scaling needs a rot_dim of at least 4");
+  if (scaling == Q4K_ROPE_SCALING_YARN && (original_context == 0 || !(beta_slow > 0.0) || !(beta_fast > beta_slow) || !std::isfinite(beta_fast)))
+    return fail(Q4K_EINVAL, "YARN scaling needs an original context and 0 < beta_slow < beta_fast");
+  const double b = scaling == Q4K_ROPE_SCALING_NTK ? base * std::pow(factor, (double)rot_dim / (rot_dim - 2.0)) : base;
+  for (uint32_t i = 0; i < rot_dim / 2; ++i) {
+    double f = std::pow(b, -2.0 * i / rot_dim);
+    if (scaling == Q4K_ROPE_SCALING_LINEAR)
+      f /= factor;
+    if (scaling == Q4K_ROPE_SCALING_YARN) {
+      const double turns = original_context * f / 6.283185307179586477;
+      const double ramp = (turns - beta_slow) / (beta_fast - beta_slow), kept = ramp < 0.0 ? 0.0 : ramp > 1.0 ? 1.0 : ramp;
+      f = (1.0 - kept) * f / factor + kept * f;
+    }
+    inv_freq[i] = f;
+  }
+  if (scale)
+    *scale = scaling == Q4K_ROPE_SCALING_YARN && factor > 1.0 ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+  return Q4K_OK;
+}
+
+int q4k_rope(void* stream, int device, const q4k_heads* x, const q4k_rotation* rotation, uint32_t rows, uint32_t head_dim, uint32_t dtype) {
+  if (!x || !rotation)
+    return fail(Q4K_EINVAL, "null argument");
+  return run_heads(stream, device, x, 1, rotation, rows, head_dim, false, 0.0f, dtype);
+}
+
+int q4k_qk_norm_rope(void* stream, int device, const q4k_heads* q, const q4k_heads* k, const q4k_rotation* rotation, uint32_t rows,
+                     uint32_t head_dim, float eps, uint32_t dtype) {
+  if (!q || !k || !rotation)
+    return fail(Q4K_EINVAL, "null argument");
+  const q4k_heads sets[2] = {*q, *k};
+  return run_heads(stream, device, sets, 2, rotation, rows, head_dim, true, eps, dtype);
+}
+
+int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m, uint32_t k, uint32_t n,
+             const uint32_t* query_counts, uint32_t nqueries, uint32_t dtype) {
+  int rc = check_lora(adapters, x, y, aux, m, k, n, query_counts, nqueries, dtype);
+  if (rc)
+    return rc;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Workspace& ws = workspace(device);
+  std::lock_guard<std::mutex> lock(ws.mu);
+  reserve_workspace(s, ws, device);
+  return run_lora_locked(s, ws, device, adapters, x, y, aux, m, k, n, query_counts, nqueries, dtype);
+}
+
+int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
+                    const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype) {
+  uint32_t phase = 0;
+  int rc = check_linear(w, x, y, aux, m, query_counts, nqueries, post, dtype, &phase);
+  if (!rc)
+    rc = check_lora(adapters, x, y, post == Q4K_POST_STORE ? nullptr : aux, m, w->k, w->n, query_counts, nqueries, dtype);
+  if (rc)
+    return rc;
+  DeviceScope scope(w->device);
+  if (scope.rc)
+    return scope.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Workspace& ws = workspace(w->device);
+  std::lock_guard<std::mutex> lock(ws.mu);
+  reserve_workspace(s, ws, w->device);
+  // What the projection adds to: y itself, or for the gated epilogue (whose
+  // gate multiplies projection and adapters alike) a buffer of its own.
+  void* sum = y;
+  if (post == Q4K_POST_GATE) {
+    const size_t bytes = (size_t)m * w->n * (dtype == Q4K_DTYPE_F32 ? 4 : 2);
+    rc = ensure_buffer(s, ws, w->device, ws.adapted, ws.adapted_bytes, bytes, "adapted-projection buffer");
+    if (rc)
+      return rc;
+    sum = ws.adapted;
+  }
+  rc = run_lora_locked(s, ws, w->device, adapters, x, sum, post == Q4K_POST_ADD ? aux : nullptr, m, w->k, w->n, query_counts, nqueries, dtype);
+  if (rc)
+    return rc;
+  rc = run_linear_locked(s, ws, w, nullptr, x, sum, sum, m, Q4K_POST_ADD, dtype, phase, true);
+  if (rc || post != Q4K_POST_GATE)
+    return rc;
+  LaunchTimer timer(s, Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_gate(s, sum, aux, y, (size_t)m * w->n, (int)dtype), "gate launch");
+  return Q4K_OK;
+}
+
+int q4k_process_logits(void* stream, int device, const void* logits, void* out, uint32_t rows, uint32_t vocab, int64_t logits_stride,
+                       int64_t out_stride, const q4k_logits_params* p, uint32_t dtype) {
+  if (!p)
+    return fail(Q4K_EINVAL, "params is NULL");
+  if (dtype > Q4K_DTYPE_F16)
+    return fail(Q4K_EINVAL, "bad dtype %u", dtype);
+  if (vocab == 0 || vocab > (1u << 30))
+    return fail(Q4K_ESHAPE, "vocab must be 1..2^30 (got %u)", vocab);
+  if (rows > 65535)
+    return fail(Q4K_ESHAPE, "at most 65535 rows (got %u)", rows);
+  constexpr int64_t kMaxStride = 1ll << 40;
+  if (logits_stride < 0 || logits_stride > kMaxStride || out_stride < 0 || out_stride > kMaxStride || (rows > 1 && out_stride < (int64_t)vocab))
+    return fail(Q4K_ESHAPE, "row strides must be 0..2^40, the output's at least vocab (got %lld, %lld)", (long long)logits_stride,
+                (long long)out_stride);
+  if (p->tokens ? !p->lengths : p->slots || p->lengths || p->prompts || p->repetition || p->frequency || p->presence)
+    return fail(Q4K_EINVAL, "tokens and lengths go together; slots, prompts and penalties need them");
+  if (p->tokens && (p->capacity > (1u << 30) || (!p->slots && p->token_slots < rows)))
+    return fail(Q4K_ESHAPE, "capacity must be up to 2^30, and without slots every row needs a text (%u rows, %u texts)", rows, p->token_slots);
+  if ((p->bias_offsets != nullptr) != (p->bias_tokens != nullptr) || (p->bias_offsets != nullptr) != (p->bias_values != nullptr))
+    return fail(Q4K_EINVAL, "bias_offsets, bias_tokens and bias_values go together");
+  if (p->bias_count > (1u << 30))
+    return fail(Q4K_ESHAPE, "at most 2^30 biases (got %u)", p->bias_count);
+  if (p->mask ? p->mask_stride < (vocab + 31) / 32 : p->mask_rows != nullptr)
+    return fail(p->mask ? Q4K_ESHAPE : Q4K_EINVAL, "mask_rows needs a mask, and a mask of %u tokens %u words a row (got %u)", vocab, (vocab + 31) / 32,
+                p->mask_stride);
+  if (p->mask && !p->mask_rows && p->mask_count < rows)
+    return fail(Q4K_ESHAPE, "without mask_rows every row needs a mask (%u rows, %u masks)", rows, p->mask_count);
+  if (rows == 0)
+    return Q4K_OK;
+  if (!logits || !out)
+    return fail(Q4K_EINVAL, "logits and out must be non-NULL");
+  const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2;
+  const size_t ib = ((size_t)(rows - 1) * logits_stride + vocab) * es, ob = ((size_t)(rows - 1) * out_stride + vocab) * es;
+  if (!(logits == out && (rows == 1 || logits_stride == out_stride)) && overlaps(logits, ib, out, ob))
+    return fail(Q4K_EALIAS, "out must be logits with the same stride, or not overlap it");
+  const struct {
+    const void* p;
+    size_t bytes;
+  } read[] = {{p->tokens, (size_t)p->token_slots * p->capacity * 4}, {p->slots, (size_t)rows * 4}, {p->lengths, (size_t)rows * 4},
+              {p->prompts, (size_t)rows * 4}, {p->repetition, (size_t)rows * 4}, {p->frequency, (size_t)rows * 4},
+              {p->presence, (size_t)rows * 4}, {p->bias_offsets, (size_t)rows * 4 + 4}, {p->bias_tokens, (size_t)p->bias_count * 4},
+              {p->bias_values, (size_t)p->bias_count * 4}, {p->mask, (size_t)p->mask_count * p->mask_stride * 4},
+              {p->mask_rows, (size_t)rows * 4}};
+  for (const auto& r : read)
+    if (r.p && r.bytes && overlaps(r.p, r.bytes, out, ob))
+      return fail(Q4K_EALIAS, "out must not overlap the parameters");
+  LogitsArgs a;
+  a.in = logits;
+  a.out = out;
+  a.in_stride = logits_stride;
+  a.out_stride = out_stride;
+  a.tokens = p->tokens;
+  a.slots = p->slots;
+  a.lengths = p->lengths;
+  a.prompts = p->prompts;
+  a.repetition = p->repetition;
+  a.frequency = p->frequency;
+  a.presence = p->presence;
+  a.bias_offsets = p->bias_offsets;
+  a.bias_tokens = p->bias_tokens;
+  a.bias_values = p->bias_values;
+  a.mask = p->mask;
+  a.mask_rows = p->mask_rows;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.nslots = p->token_slots;
+  a.capacity = p->capacity;
+  a.nbias = p->bias_count;
+  a.nmasks = p->mask_count;
+  a.mask_stride = p->mask_stride;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_logits(static_cast<hipStream_t>(stream), a, (int)dtype, device_cus(device)), "logits launch");
   return Q4K_OK;
 }
 

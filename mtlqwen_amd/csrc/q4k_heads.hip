@@ -1,0 +1,252 @@
+// Rotary positions of attention heads, alone or after the RMS norm of each
+// query and key head: heads_kernel.
+//
+// Both read and write every value once, so they are bound by memory; what
+// decides is that a row's angles are made once for many heads.
+#include "q4k_device.h"
+
+namespace q4k {
+namespace {
+
+// ----------------------------------------------------------------------------
+// One head of `dim` values x, position p, h = rot / 2, pair i < h turned by
+// p f_i (f = inv_freq): with c = scale cos(p f_i) and n = scale sin(p f_i),
+//   half layout (INTER = 0):   y[i] = x[i] c - x[i + h] n, y[i + h] = x[i + h] c + x[i] n
+//   interleaved (INTER = 1):   the same of x[2i] and x[2i + 1]
+// and y[d] = x[d] for d >= rot.  NORM: x is x * w / sqrt(sum(x^2) / dim + eps)
+// first, in fp32, without a rounding in between.
+//
+// A lane holds two vectors of V values (a "slot"): of the rotated part the two
+// that turn into each other, behind it two neighbours; glog = log2 of the lanes
+// of a head, so that a wave reduces the sums of squares of its heads without
+// LDS.  A lane keeps its head (and the norm weights of its slot) and walks over
+// U rows, whose values are all asked for before the first is used.  P slots per
+// lane cover heads that 64 lanes of one slot do not.
+//
+// The workgroup's angles are made once, in LDS: rows x h of them for hb heads.
+// Angles are 64-bit products of the position and the frequency in turns, whose
+// fraction is rounded to 32 bits: at position 2^20 a product in 32 bits would
+// be off by 0.06 rad, at any position below 2^31 this one is by 5e-7.
+// ----------------------------------------------------------------------------
+template <typename T, int V>
+struct VecOf {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+template <typename T>
+struct VecOf<T, 1> {
+  typedef T type;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  if constexpr (V == 1) {
+    v[0] = (float)p[0];
+  } else {
+    const typename VecOf<T, V>::type a = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      v[i] = (float)a[i];
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  if constexpr (V == 1) {
+    p[0] = (T)v[0];
+  } else {
+    typename VecOf<T, V>::type a;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      a[i] = (T)v[i];
+    *reinterpret_cast<typename VecOf<T, V>::type*>(p) = a;
+  }
+}
+
+template <typename T, int V, int P, int U, bool NORM, bool INTER>
+__global__ __launch_bounds__(256) void heads_kernel(HeadsArgs a) {
+  extern __shared__ float cs[];  // [rows of the workgroup][2][h]: cosines, sines
+  const int tid = threadIdx.x, lane = tid & ((1 << a.glog) - 1), slot = tid >> a.glog;
+  const int hb = 1 << a.hblog, rb = 256 >> (a.glog + a.hblog);
+  const uint32_t head = blockIdx.y * (uint32_t)hb + (uint32_t)(slot & (hb - 1));
+  const uint32_t row0 = blockIdx.x * (uint32_t)(rb * U) + (uint32_t)(slot >> a.hblog);
+  const int h = a.rot >> 1, nslots = a.nslots, rslots = INTER ? 0 : h / V;
+  const bool key = head >= a.heads[0], live_head = head < a.heads[0] + a.heads[1];
+  const uint32_t hi = key ? head - a.heads[0] : head;
+  const T* in = static_cast<const T*>(key ? a.in[1] : a.in[0]) + (int64_t)hi * (key ? a.head_in[1] : a.head_in[0]);
+  T* out = static_cast<T*>(key ? a.out[1] : a.out[0]) + (int64_t)hi * (key ? a.head_out[1] : a.head_out[0]);
+  const int64_t row_in = key ? a.row_in[1] : a.row_in[0], row_out = key ? a.row_out[1] : a.row_out[0];
+
+  int o1[P], o2[P];
+  bool on1[P], on2[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int j = lane + (p << a.glog);
+    o1[p] = INTER ? 2 * V * j : j < rslots ? V * j : a.rot + 2 * V * (j - rslots);
+    o2[p] = !INTER && j < rslots ? o1[p] + h : o1[p] + V;
+    on1[p] = live_head && j < nslots && o1[p] < a.dim;
+    on2[p] = on1[p] && o2[p] < a.dim;
+  }
+
+  float v1[U][P][V], v2[U][P][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + (uint32_t)(u * rb);
+    const T* x = in + (int64_t)row * row_in;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        v1[u][p][i] = v2[u][p][i] = 0.0f;
+      if (row < a.rows && on1[p])
+        load_vec<T, V>(x + o1[p], v1[u][p]);
+      if (row < a.rows && on2[p])
+        load_vec<T, V>(x + o2[p], v2[u][p]);
+    }
+  }
+  float w1[NORM ? P : 1][V], w2[NORM ? P : 1][V];
+  if constexpr (NORM) {
+    const float* w = key ? a.w[1] : a.w[0];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (on1[p])
+        load_vec<float, V>(w + o1[p], w1[p]);
+      if (on2[p])
+        load_vec<float, V>(w + o2[p], w2[p]);
+    }
+  }
+
+  // The angles of the workgroup's rows.
+  for (int i = tid; i < rb * U * h; i += 256) {
+    const int r = i / h, f = i - r * h;
+    const uint32_t row = blockIdx.x * (uint32_t)(rb * U) + (uint32_t)r;
+    if (row < a.rows) {
+      const double turns = (double)a.positions[row] * (a.inv_freq[f] * 0.15915494309189533577);
+      float s, c;
+      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+      cs[(2 * r) * h + f] = a.scale * c;
+      cs[(2 * r + 1) * h + f] = a.scale * s;
+    }
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + (uint32_t)(u * rb);
+    if constexpr (NORM) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          ss = fmaf(v1[u][p][i], v1[u][p][i], fmaf(v2[u][p][i], v2[u][p][i], ss));
+      for (int off = (1 << a.glog) >> 1; off > 0; off >>= 1)
+        ss += __shfl_xor(ss, off);
+      const float r = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          v1[u][p][i] = on1[p] ? v1[u][p][i] * r * w1[p][i] : 0.0f;
+          v2[u][p][i] = on2[p] ? v2[u][p][i] * r * w2[p][i] : 0.0f;
+        }
+    }
+    if (row >= a.rows)
+      continue;
+    const float* ct = cs + 2 * ((slot >> a.hblog) + u * rb) * h;
+    const float* st = ct + h;
+    T* y = out + (int64_t)row * row_out;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (on1[p] && o1[p] < a.rot) {
+        if constexpr (!INTER || V == 1) {
+          const int f = INTER ? o1[p] >> 1 : o1[p];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float c = ct[f + i], n = st[f + i], x1 = v1[u][p][i], x2 = v2[u][p][i];
+            v1[u][p][i] = x1 * c - x2 * n;
+            v2[u][p][i] = x2 * c + x1 * n;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            const float c = ct[(o1[p] + i) >> 1], n = st[(o1[p] + i) >> 1], x1 = v1[u][p][i], x2 = v1[u][p][i + 1];
+            v1[u][p][i] = x1 * c - x2 * n;
+            v1[u][p][i + 1] = x2 * c + x1 * n;
+          }
+          if (o2[p] < a.rot) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+              const float c = ct[(o2[p] + i) >> 1], n = st[(o2[p] + i) >> 1], x1 = v2[u][p][i], x2 = v2[u][p][i + 1];
+              v2[u][p][i] = x1 * c - x2 * n;
+              v2[u][p][i + 1] = x2 * c + x1 * n;
+            }
+          }
+        }
+      }
+      if (on1[p])
+        store_vec<T, V>(y + o1[p], v1[u][p]);
+      if (on2[p])
+        store_vec<T, V>(y + o2[p], v2[u][p]);
+    }
+  }
+}
+
+// The widest vector that a head's layout allows: chunks of V values must not
+// straddle the halves (or the end) of the rotated part, nor the head's end.
+int heads_vec(int dim, int rot, bool inter, int widest) {
+  for (int v = widest; v > 1; v >>= 1)
+    if (dim % v == 0 && (inter ? rot : rot / 2) % v == 0)
+      return v;
+  return 1;
+}
+
+template <typename T, bool NORM, bool INTER>
+hipError_t heads_launch(hipStream_t s, HeadsArgs a, int cus) {
+  constexpr int kWide = 16 / (int)sizeof(T);
+  int v = heads_vec(a.dim, a.rot, INTER, kWide);
+  auto slots_of = [&](int vec) {
+    const int turned = INTER ? 0 : a.rot / (2 * vec), rest = INTER ? a.dim : a.dim - a.rot;
+    return turned + (rest + 2 * vec - 1) / (2 * vec);
+  };
+  if (v != kWide || slots_of(v) > 64)
+    v = v >= 2 ? 2 : 1;
+  a.nslots = slots_of(v);
+  const uint32_t heads = a.heads[0] + a.heads[1];
+  a.glog = 0;
+  while ((1 << a.glog) < a.nslots && a.glog < 6)
+    ++a.glog;
+  // Heads side by side: as many as a workgroup holds and the heads fill to an
+  // eighth, so that few lanes idle.
+  a.hblog = 8 - a.glog;
+  while (a.hblog > 0 && ((heads + (1u << a.hblog) - 1) >> a.hblog << a.hblog) - heads > heads / 8)
+    --a.hblog;
+  const uint32_t rb = 256u >> (a.glog + a.hblog), groups = (heads + (1u << a.hblog) - 1) >> a.hblog;
+  // Four rows per lane once that still leaves every CU four workgroups.
+  const bool deep = v == kWide && (uint64_t)((a.rows + 4 * rb - 1) / (4 * rb)) * groups >= 4ull * (uint32_t)cus &&
+                    (size_t)rb * 4 * a.rot * sizeof(float) <= 32768;
+  const uint32_t rows = rb * (deep ? 4u : 1u);
+  const dim3 grid((a.rows + rows - 1) / rows, groups), block(256);
+  const size_t lds = (size_t)rows * a.rot * sizeof(float);
+  if (v == kWide && deep)
+    return dispatch_lds(heads_kernel<T, kWide, 1, 4, NORM, INTER>, grid, block, lds, s, a);
+  if (v == kWide)
+    return dispatch_lds(heads_kernel<T, kWide, 1, 1, NORM, INTER>, grid, block, lds, s, a);
+  if (v == 2)
+    return dispatch_lds(heads_kernel<T, 2, 4, 1, NORM, INTER>, grid, block, lds, s, a);
+  return dispatch_lds(heads_kernel<T, 1, 8, 1, NORM, INTER>, grid, block, lds, s, a);
+}
+
+template <typename T>
+hipError_t heads_launch_t(hipStream_t s, const HeadsArgs& a, bool norm, bool inter, int cus) {
+  if (norm)
+    return inter ? heads_launch<T, true, true>(s, a, cus) : heads_launch<T, true, false>(s, a, cus);
+  return inter ? heads_launch<T, false, true>(s, a, cus) : heads_launch<T, false, false>(s, a, cus);
+}
+
+}  // namespace
+
+hipError_t launch_heads(hipStream_t s, const HeadsArgs& a, bool norm, bool inter, int dtype, int cus) {
+  return dtype == kF32 ? heads_launch_t<float>(s, a, norm, inter, cus) : heads_launch_t<_Float16>(s, a, norm, inter, cus);
+}
+
+}  // namespace q4k

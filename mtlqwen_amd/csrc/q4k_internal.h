@@ -512,6 +512,68 @@ hipError_t launch_embedding_batch(hipStream_t s, const uint8_t* w, const int32_t
 // otherwise x row idx->src[r]).
 hipError_t launch_rms_norm(hipStream_t s, const void* x, const float* w, void* y, int rows, int k, float eps, int dtype, const GatherIndex* idx);
 
+// Rotary positions of one (heads[1] = 0) or two sets of heads (queries and
+// keys), after an RMS norm of each head where `norm` (q4k_heads.hip).  Strides
+// count elements; in and out are the same storage or do not overlap.
+struct HeadsArgs {
+  const void* in[2] = {nullptr, nullptr};
+  void* out[2] = {nullptr, nullptr};
+  const float* w[2] = {nullptr, nullptr};  // norm weights [dim]
+  int64_t row_in[2] = {0, 0}, head_in[2] = {0, 0}, row_out[2] = {0, 0}, head_out[2] = {0, 0};
+  const double* inv_freq = nullptr;  // rot / 2 angles per position, in radians
+  const int32_t* positions = nullptr;
+  uint32_t heads[2] = {0, 0}, rows = 0;
+  int dim = 0, rot = 0;
+  float scale = 1.0f, eps = 0.0f;
+  int nslots = 0, glog = 0, hblog = 0;  // set by the launch
+};
+constexpr uint32_t kMaxHeadDim = 1024;
+hipError_t launch_heads(hipStream_t s, const HeadsArgs& a, bool norm, bool inter, int dtype, int cus);
+
+// Low-rank adapters of a packed batch (q4k_lora.hip): u = x A^T into the
+// slices of `part`, then y = aux + s u B^T.
+constexpr uint32_t kLoraMaxRank = 512;
+struct LoraArgs {
+  const void* x = nullptr;
+  const void* aux = nullptr;  // nullptr: zero; may be y
+  void* y = nullptr;
+  const _Float16* a = nullptr;  // [slots, r, k]
+  const _Float16* b = nullptr;  // [slots, n, r]
+  const int32_t* ids = nullptr;    // [nq]: the adapter of each sequence, others than 0 .. slots - 1: none
+  const int32_t* ranks = nullptr;  // [slots] or nullptr: r
+  const float* scales = nullptr;   // [slots] or nullptr: 1
+  float* part = nullptr;           // [slices, m, rpad]
+  int m = 0, k = 0, n = 0, r = 0, rpad = 0, slots = 0, nq = 0, slices = 1;
+  int start[8] = {}, count[8] = {};  // rows of the sequences
+};
+int lora_slices(const LoraArgs& a, int cus);
+hipError_t launch_lora_shrink(hipStream_t s, const LoraArgs& a, int dtype);
+hipError_t launch_lora_expand(hipStream_t s, const LoraArgs& a, int dtype);
+// y = silu(aux) * t over `elems` (a multiple of 16) values; y may be aux.
+hipError_t launch_gate(hipStream_t s, const void* t, const void* aux, void* y, size_t elems, int dtype);
+
+// Penalties, biases and masks on rows of logits (q4k_logits.hip).  Strides
+// count elements; out is in with the same stride or does not overlap it.
+struct LogitsArgs {
+  const void* in = nullptr;
+  void* out = nullptr;
+  int64_t in_stride = 0, out_stride = 0;
+  const int32_t* tokens = nullptr;  // [nslots, capacity] or nullptr: no text
+  const int32_t* slots = nullptr;   // [rows] or nullptr: row r reads slot r
+  const int32_t* lengths = nullptr;
+  const int32_t* prompts = nullptr;  // [rows] or nullptr: 0
+  const float* repetition = nullptr;
+  const float* frequency = nullptr;
+  const float* presence = nullptr;
+  const int32_t* bias_offsets = nullptr;  // [rows + 1] or nullptr: no biases
+  const int32_t* bias_tokens = nullptr;
+  const float* bias_values = nullptr;
+  const uint32_t* mask = nullptr;  // [nmasks, mask_stride] words or nullptr
+  const int32_t* mask_rows = nullptr;  // [rows] or nullptr: row r takes mask r
+  uint32_t rows = 0, vocab = 0, nslots = 0, capacity = 0, nbias = 0, nmasks = 0, mask_stride = 0;
+};
+hipError_t launch_logits(hipStream_t s, const LogitsArgs& a, int dtype, int cus);
+
 // Device-side GGUF -> tiled re-layout (src and dst are device buffers).
 hipError_t launch_relayout(hipStream_t s, const uint8_t* src, uint8_t* dst, uint32_t n, uint32_t k);
 
@@ -550,6 +612,14 @@ template <typename... P, typename... A>
 hipError_t dispatch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t s, A... args) {
   const DispatchEvents& e = dispatch_events();
   hipExtLaunchKernelGGL(kernel, grid, block, 0, s, e.start, e.stop, 0, static_cast<P>(args)...);
+  return hipGetLastError();
+}
+
+// The same with `lds` bytes of dynamic LDS.
+template <typename... P, typename... A>
+hipError_t dispatch_lds(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, A... args) {
+  const DispatchEvents& e = dispatch_events();
+  hipExtLaunchKernelGGL(kernel, grid, block, lds, s, e.start, e.stop, 0, static_cast<P>(args)...);
   return hipGetLastError();
 }
 
