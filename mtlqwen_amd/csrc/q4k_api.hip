@@ -2049,8 +2049,8 @@ int q4k_process_logits(void* stream, int device, const void* logits, void* out, 
     return fail(Q4K_EINVAL, "params is NULL");
   if (dtype > Q4K_DTYPE_F16)
     return fail(Q4K_EINVAL, "bad dtype %u", dtype);
-  if (vocab == 0 || vocab > (1u << 30))
-    return fail(Q4K_ESHAPE, "vocab must be 1..2^30 (got %u)", vocab);
+  if (vocab == 0 || vocab > (1u << 24))
+    return fail(Q4K_ESHAPE, "vocab must be 1..2^24 (got %u)", vocab);
   if (rows > 65535)
     return fail(Q4K_ESHAPE, "at most 65535 rows (got %u)", rows);
   constexpr int64_t kMaxStride = 1ll << 40;

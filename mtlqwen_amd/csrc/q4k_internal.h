@@ -571,8 +571,10 @@ struct LogitsArgs {
   const uint32_t* mask = nullptr;  // [nmasks, mask_stride] words or nullptr
   const int32_t* mask_rows = nullptr;  // [rows] or nullptr: row r takes mask r
   uint32_t rows = 0, vocab = 0, nslots = 0, capacity = 0, nbias = 0, nmasks = 0, mask_stride = 0;
+  uint32_t stagger = 1;
+  uint32_t count_bits = 0;  // set by the launch: the bits that hold a count of up to `capacity`
 };
-hipError_t launch_logits(hipStream_t s, const LogitsArgs& a, int dtype, int cus);
+hipError_t launch_logits(hipStream_t s, LogitsArgs a, int dtype, int cus);
 
 // Device-side GGUF -> tiled re-layout (src and dst are device buffers).
 hipError_t launch_relayout(hipStream_t s, const uint8_t* src, uint8_t* dst, uint32_t n, uint32_t k);

@@ -178,7 +178,7 @@ def logits(q4k, p, i=X, o=Y, rows=4, vocab=1000, si=1000, so=1000, dtype=0):
     (None, {}, EINVAL),
     (params(), {"dtype": 2}, EINVAL),
     (params(), {"vocab": 0}, ESHAPE),
-    (params(), {"vocab": (1 << 30) + 1}, ESHAPE),
+    (params(), {"vocab": (1 << 24) + 1}, ESHAPE),
     (params(), {"rows": 65536}, ESHAPE),
     (params(), {"so": 999}, ESHAPE),
     (params(), {"si": -1}, ESHAPE),
