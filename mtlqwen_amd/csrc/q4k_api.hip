@@ -1927,7 +1927,7 @@ int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_ada
     a.count[q] = counts ? (int)counts[q] : (int)m;
     start += (uint32_t)a.count[q];
   }
-  a.slices = lora_slices(a, device_cus(device));
+  lora_plan(a, device_cus(device));
   int rc = ensure_buffer(stream, ws, device, ws.part, ws.part_elems, (size_t)a.slices * a.m * a.rpad, "split-K workspace");
   if (rc)
     return rc;
@@ -1936,8 +1936,13 @@ int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_ada
     LaunchTimer timer(stream, Q4K_KERNEL_AUX);
     Q4K_TRY_HIP(launch_lora_shrink(stream, a, (int)dtype), "adapter shrink launch");
   }
+  if (a.tall && a.slices > 1) {
+    LaunchTimer timer(stream, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_lora_reduce(stream, a), "adapter reduce launch");
+    a.slices = 1;
+  }
   LaunchTimer timer(stream, Q4K_KERNEL_AUX);
-  Q4K_TRY_HIP(launch_lora_expand(stream, a, (int)dtype), "adapter expand launch");
+  Q4K_TRY_HIP(launch_lora_expand(stream, a, (int)dtype, device_cus(device)), "adapter expand launch");
   return Q4K_OK;
 }
 

@@ -1,29 +1,35 @@
 // Low-rank adapters of a packed batch, one per sequence, beside a projection:
-// lora_shrink_kernel (u = x A^T), lora_expand_kernel (y = aux + s u B^T) and
-// gate_kernel (the gated epilogue of a projection with adapters).
+// u = x A^T (lora_shrink_kernel; lora_shrink_tall_kernel and lora_reduce_kernel)
+// and y = aux + s u B^T (lora_expand_kernel), and gate_kernel, the gated epilogue of a
+// projection with adapters.
 #include "q4k_device.h"
 
 namespace q4k {
 namespace {
 
-// A block of up to 16 rows that lie in one sequence: its first row, its rows,
-// and the sequence's adapter (-1: none) with its rank.
+constexpr int kLoraMaxSlices = 8, kLoraTallSlices = 16;
+
+// Up to 16 RT rows that lie in one sequence: the first row, the rows, and the
+// sequence's adapter (-1: none) with its rank.
 struct LoraBlock {
   int row, rows, adapter, rank;
 };
 
 __device__ __forceinline__ LoraBlock lora_block(const LoraArgs& a, int tile, int tile_rows) {
-  int q = 0, t = tile;
-  while (q + 1 < a.nq) {
-    const int tiles = (a.count[q] + tile_rows - 1) / tile_rows;
-    if (t < tiles)
-      break;
-    t -= tiles;
-    ++q;
-  }
+  // a.tile[q] = tiles before sequence q; constant indices, so that the tables
+  // are read in one go.
+  int q = 0, row = a.start[0], rows = a.count[0], first = 0;
+#pragma unroll
+  for (int i = 1; i < 8; ++i)
+    if (i < a.nq && tile >= a.tile[i]) {
+      q = i;
+      row = a.start[i];
+      rows = a.count[i];
+      first = a.tile[i];
+    }
   LoraBlock b;
-  b.row = a.start[q] + t * tile_rows;
-  b.rows = min(a.count[q] - t * tile_rows, tile_rows);
+  b.row = row + (tile - first) * tile_rows;
+  b.rows = min(rows - (tile - first) * tile_rows, tile_rows);
   b.adapter = a.ids[q];
   if (b.adapter < 0 || b.adapter >= a.slots)
     b.adapter = -1;
@@ -33,168 +39,569 @@ __device__ __forceinline__ LoraBlock lora_block(const LoraArgs& a, int tile, int
   return b;
 }
 
+// Power of two that brings a largest magnitude m to [2^14, 2^15), and its
+// inverse: values scaled by it split into two fp16 parts, hi = fp16(v) and lo =
+// fp16(v - hi), that keep 22 of v's bits down to 2^-17 of the largest, and every
+// bit above 2^-25 of 1 below that.  (m below 2^-112, infinities and NaN: the
+// nearest such power.)
+__device__ __forceinline__ float split_scale(float m, float* inverse) {
+  const int e = min(max((int)(__builtin_bit_cast(uint32_t, m) >> 23), 15), 254);
+  *inverse = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+  return __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
+}
+
+// The parts of 8 scaled values.  The low part of an infinity is finite (its
+// difference is no number), so that the infinity stays one.
+__device__ __forceinline__ void split8(const float* v, float scale, h8_t* hi, h8_t* lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float s = v[e] * scale;
+    (*hi)[e] = (_Float16)s;
+    (*lo)[e] = (_Float16)__builtin_amdgcn_fmed3f(s - (float)(*hi)[e], -64.0f, 64.0f);
+  }
+}
+
+// The 16 bytes of lane 4 (lane % 16) + lane / 16: loads give each four lanes 64
+// contiguous bytes of one row (16 cache lines an instruction), the matrix
+// instructions want lane % 16 to be the row (loaded so, every lane of a
+// quarter wave is in a line of its own, 64 an instruction, and a CU takes in 13
+// bytes a cycle: 3.9 us for 128 KB).
+__device__ __forceinline__ u4_t to_rows(u4_t v, int from) {
+  u4_t o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    o[e] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)v[e]);
+  return o;
+}
+
+typedef uint32_t u4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
 // ----------------------------------------------------------------------------
-// u[row][j] = sum over k of x[row][k] A[j][k], in K-slices: one workgroup per
-// 16 rows, slice and 16 * NT ranks; its eight waves share the slice's blocks of
-// 256 k, 32 k each, and add their sums in LDS.  fp16 x: v_mfma_f32_16x16x32_f16,
-// whose products are exact.  fp32 x: v_mfma_f32_16x16x4_f32 on A converted to
-// fp32, so that x keeps its 24 bits and its range.
+// One wave's share of u[row][j] = sum over k of x[row][k] A[j][k]: 16 RT rows, 16
+// NT ranks, `steps` times 32 k, from the addresses x[r] and w on (row or rank lane / 4 of
+// their tile, k 8 (lane % 4)), the loads of SEG steps on their way together.
+// v_mfma_f32_16x16x32_f16, whose products are exact; fp32 x as two fp16 parts
+// (split_scale), which costs two of these instructions where eight fp32 ones of
+// twice the time each would be needed.  The scale of a row follows the largest
+// value so far; the sums follow it where it changes.
+// acc[r][t][c]: row 16 r + 4 (lane / 16) + c, rank 16 t + lane % 16.
 // ----------------------------------------------------------------------------
-template <typename T, int NT>
-__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a) {
-  __shared__ float red[8][NT * 256];
-  const LoraBlock b = lora_block(a, blockIdx.x, 16);
+template <typename T, int RT, int NT, int SEG>
+__device__ __forceinline__ void lora_sum(const T* const* x, const _Float16* w, int steps, int k, int live, int lane, f4_t (*acc)[NT]) {
+  constexpr int kX = (int)sizeof(T) / 2;  // 16-byte loads of 8 values
+  const int g = lane >> 4, from = 4 * (4 * (lane & 15) + g);
+  float scale[RT], inverse[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    scale[r] = split_scale(0.0f, &inverse[r]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      acc[r][t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (int s0 = 0; s0 < steps; s0 += SEG) {
+    u4_t wv[SEG][NT], xv[SEG][RT][kX];
+#pragma unroll
+    for (int s = 0; s < SEG; ++s)
+      if (s0 + s < steps)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int h = 0; h < kX; ++h)
+            xv[s][r][h] = *reinterpret_cast<const u4_any_t*>(x[r] + 32 * (s0 + s) + 4 * h);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int s = 0; s < SEG; ++s)
+        wv[s][t] = u4_t{0u, 0u, 0u, 0u};
+      if (16 * t + (lane >> 2) < live)
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+          if (s0 + s < steps)
+            wv[s][t] = *reinterpret_cast<const u4_any_t*>(w + (size_t)(16 * t) * k + 32 * (s0 + s));
+    }
+    if constexpr (kX == 2) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float m = 0.0f;
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+          if (s0 + s < steps)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              m = fmaxf(m, fabsf(__builtin_bit_cast(float, (uint32_t)xv[s][r][e >> 2][e & 3])));
+        m = fmaxf(m, __shfl_xor(m, 1));
+        m = fmaxf(m, __shfl_xor(m, 2));
+        // Lanes 4 i .. 4 i + 3 hold row i: its scale stays with them.
+        float undo;
+        const float now = split_scale(m, &undo);
+        if (__any(now < scale[r])) {
+          const float ratio = now < scale[r] ? now * inverse[r] : 1.0f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float q = __shfl(ratio, 4 * (4 * g + c));
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[r][t][c] *= q;
+          }
+          if (now < scale[r]) {
+            scale[r] = now;
+            inverse[r] = undo;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < SEG; ++s)
+      if (s0 + s < steps) {
+        h8_t a[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          a[t] = __builtin_bit_cast(h8_t, to_rows(wv[s][t], from));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if constexpr (kX == 1) {
+            const h8_t v = __builtin_bit_cast(h8_t, to_rows(xv[s][r][0], from));
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, a[t], acc[r][t], 0, 0, 0);
+          } else {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              v[e] = __builtin_bit_cast(float, (uint32_t)xv[s][r][e >> 2][e & 3]);
+            h8_t hi, lo;
+            split8(v, scale[r], &hi, &lo);
+            hi = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, hi), from));
+            lo = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, lo), from));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, a[t], acc[r][t], 0, 0, 0);
+              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, a[t], acc[r][t], 0, 0, 0);
+            }
+          }
+        }
+      }
+  }
+  if constexpr (kX == 2)
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float undo = __shfl(inverse[r], 4 * (4 * g + c));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          acc[r][t][c] *= undo;
+      }
+}
+
+// The waves' sums of one row and rank, added in pairs.
+template <int WAVES>
+__device__ __forceinline__ float sum_waves(const float* p, int stride) {
+  float v[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+    v[w] = p[w * stride];
+#pragma unroll
+  for (int n = WAVES / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int w = 0; w < n; ++w)
+      v[w] += v[w + n];
+  return v[0];
+}
+
+// K in slices: one workgroup per 16 RT rows, slice and 16 NT ranks; its WAVES
+// waves take a part of the slice each and add their sums in LDS.
+template <typename T, int RT, int NT, int WAVES, int SEG>
+__global__ __launch_bounds__(64 * WAVES, 4) void lora_shrink_kernel(LoraArgs a) {
+  constexpr int kSums = RT * NT * 256;
+  __shared__ float red[WAVES * kSums];
+  const LoraBlock b = lora_block(a, blockIdx.x, 16 * RT);
   const int j0 = (int)blockIdx.z * 16 * NT;
   if (b.adapter < 0 || j0 >= b.rank)
     return;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, i = lane & 15, g = lane >> 4;
-  const int nb = a.k >> 8, b0 = (int)((int64_t)nb * blockIdx.y / a.slices), b1 = (int)((int64_t)nb * (blockIdx.y + 1) / a.slices);
-  const T* x = static_cast<const T*>(a.x) + (size_t)(b.row + min(i, b.rows - 1)) * a.k + 32 * wave + 8 * g;
-  const _Float16* w = a.a + ((size_t)b.adapter * a.r + j0) * a.k + 32 * wave + 8 * g;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
+  // Units of 32 k per wave.
+  const int units = a.k / (32 * WAVES), u0 = (int)((int64_t)units * blockIdx.y / a.slices), u1 = (int)((int64_t)units * (blockIdx.y + 1) / a.slices);
+  const int k0 = 32 * (WAVES * u0 + wave * (u1 - u0)) + 8 * (lane & 3);
+  f4_t acc[RT][NT];
+  const T* x[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+    x[r] = static_cast<const T*>(a.x) + (size_t)(b.row + min(16 * r + (lane >> 2), b.rows - 1)) * a.k + k0;
+  lora_sum<T, RT, NT, SEG>(x, a.a + ((size_t)b.adapter * a.r + j0 + (lane >> 2)) * a.k + k0, u1 - u0, a.k, b.rank - j0, lane, acc);
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        red[wave * kSums + (16 * r + 4 * g + c) * (16 * NT) + 16 * t + i] = acc[r][t][c];
+  __syncthreads();
+  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row) * a.rpad + j0;
+  for (int o = tid; o < kSums; o += 64 * WAVES) {
+    const int row = o / (16 * NT), j = o % (16 * NT);
+    if (row < b.rows && j0 + j < b.rank)
+      part[(size_t)row * a.rpad + j] = sum_waves<WAVES>(red + o, kSums);
+  }
+}
+
+// The same for many rows: one workgroup of four waves per 64 rows, slice and 16 NT
+// ranks.  A wave reads, splits and multiplies its own 16 rows, 64 k at a time;
+// A's 64 k are shared through LDS, so that they cross from the L2 once per 64
+// rows.  The next 64 k are read while these are multiplied.
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void lora_shrink_tall_kernel(LoraArgs a) {
+  constexpr int kPad = 72, kParts = sizeof(T) == 4 ? 2 : 1, kA = NT * 16 / 32;
+  __shared__ _Float16 as[2][NT * 16 * kPad], xs[4][kParts][16 * kPad];
+  const LoraBlock b = lora_block(a, blockIdx.x, 64);
+  const int j0 = (int)blockIdx.z * 16 * NT;
+  if (b.adapter < 0 || j0 >= b.rank)
+    return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
+  const int chunks = a.k >> 6, c0 = (int)((int64_t)chunks * blockIdx.y / a.slices), c1 = (int)((int64_t)chunks * (blockIdx.y + 1) / a.slices);
+  // Register q of lane group g holds row 4 g + q of the wave: the rows whose sums
+  // acc[.][q] of the same lanes will be.
+  const T* x[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    x[q] = static_cast<const T*>(a.x) + (size_t)(b.row + min(16 * wave + 4 * g + q, b.rows - 1)) * a.k + 4 * i;
+  // Lane's share of A: rank tid / 8 (+ 32 h), 8 k from 8 (tid % 8) on.
+  const _Float16* w = a.a + ((size_t)b.adapter * a.r + j0) * a.k + 8 * (tid & 7);
+  typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  t4 xv[4];
+  u4_t wv[kA < 1 ? 1 : kA];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      xv[q] = *reinterpret_cast<const t4*>(x[q] + 64 * c);
+#pragma unroll
+    for (int h = 0; h < (kA < 1 ? 1 : kA); ++h) {
+      const int j = (tid >> 3) + 32 * h;
+      wv[h] = u4_t{0u, 0u, 0u, 0u};
+      if (j < 16 * NT && j0 + j < b.rank)
+        wv[h] = *reinterpret_cast<const u4_any_t*>(w + (size_t)j * a.k + 64 * c);
+    }
+  };
   f4_t acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     acc[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb = b0; kb < b1; ++kb) {
-    h8_t wv[NT];
+  float scale[4], inverse[4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      wv[t] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
-      if (j0 + 16 * t + i < b.rank)
-        wv[t] = *reinterpret_cast<const h8_any_t*>(w + (size_t)(16 * t + i) * a.k + kb * 256);
+  for (int q = 0; q < 4; ++q)
+    scale[q] = split_scale(0.0f, &inverse[q]);
+  load(c0);
+  for (int c = c0; c < c1; ++c) {
+    _Float16* at = as[c & 1];
+#pragma unroll
+    for (int h = 0; h < (kA < 1 ? 1 : kA); ++h) {
+      const int j = (tid >> 3) + 32 * h;
+      if (j < 16 * NT)
+        *reinterpret_cast<u4_t*>(at + j * kPad + 8 * (tid & 7)) = wv[h];
     }
-    if constexpr (sizeof(T) == 2) {
-      const h8_t xv = *reinterpret_cast<const h8_any_t*>(x + kb * 256);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      _Float16* to = &xs[wave][0][(4 * g + q) * kPad + 4 * i];
+      if constexpr (kParts == 1) {
+        *reinterpret_cast<h4_t*>(to) = __builtin_bit_cast(h4_t, xv[q]);
+      } else {
+        float m = fmaxf(fmaxf(fabsf(xv[q][0]), fabsf(xv[q][1])), fmaxf(fabsf(xv[q][2]), fabsf(xv[q][3])));
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1)
+          m = fmaxf(m, __shfl_xor(m, off));
+        float undo;
+        const float now = split_scale(m, &undo);
+        if (now < scale[q]) {
+          const float ratio = now * inverse[q];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            acc[t][q] *= ratio;
+          scale[q] = now;
+          inverse[q] = undo;
+        }
+        h4_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = xv[q][e] * scale[q];
+          hi[e] = (_Float16)v;
+          lo[e] = (_Float16)__builtin_amdgcn_fmed3f(v - (float)hi[e], -64.0f, 64.0f);
+        }
+        *reinterpret_cast<h4_t*>(to) = hi;
+        *reinterpret_cast<h4_t*>(to + 16 * kPad) = lo;
+      }
+    }
+    if (c + 1 < c1)
+      load(c + 1);
+    // One barrier: A's other buffer is not written before every wave has left
+    // the previous round's reads of it; a wave's rows are its own.
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      h8_t av[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv, wv[t], acc[t], 0, 0, 0);
-    } else {
-      float xv[8];
-      load8(x + kb * 256, xv);
+        av[t] = *reinterpret_cast<const h8_t*>(at + (16 * t + i) * kPad + 32 * s + 8 * g);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int part = 0; part < kParts; ++part) {
+        const h8_t v = *reinterpret_cast<const h8_t*>(&xs[wave][part][i * kPad + 32 * s + 8 * g]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[e], (float)wv[t][e], acc[t], 0, 0, 0);
+        for (int t = 0; t < NT; ++t)
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, av[t], acc[t], 0, 0, 0);
+      }
     }
   }
+  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row + 16 * wave) * a.rpad + j0;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      red[wave][(4 * g + c) * (16 * NT) + 16 * t + i] = acc[t][c];
-  __syncthreads();
-  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row) * a.rpad + j0;
-  for (int o = tid; o < 256 * NT; o += 512) {
-    const int row = o / (16 * NT), j = o % (16 * NT);
-    if (row < b.rows && j0 + j < b.rank) {
-      float p[8];
+      if (16 * wave + 4 * g + c < b.rows && j0 + 16 * t + i < b.rank)
+        part[(size_t)(4 * g + c) * a.rpad + 16 * t + i] = kParts == 2 ? acc[t][c] * inverse[c] : acc[t][c];
+}
+
+// The slices' sums, low slices first, into the first slice: four values per thread.
+__global__ __launch_bounds__(256) void lora_reduce_kernel(LoraArgs a) {
+  const size_t quads = (size_t)a.m * a.rpad / 4, q = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= quads)
+    return;
+  f4_t* p = reinterpret_cast<f4_t*>(a.part) + q;
+  f4_t v[kLoraTallSlices];
 #pragma unroll
-      for (int wv = 0; wv < 8; ++wv)
-        p[wv] = red[wv][o];
-      part[(size_t)row * a.rpad + j] = sum8_pairs(p);
-    }
-  }
+  for (int s = 0; s < kLoraTallSlices; ++s)
+    v[s] = s < a.slices ? p[s * quads] : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  f4_t sum = v[0];
+#pragma unroll
+  for (int s = 1; s < kLoraTallSlices; ++s)
+    sum += v[s];
+  *p = sum;
 }
 
 // ----------------------------------------------------------------------------
-// y[row][n] = aux[row][n] + sum over j of (s u[row][j]) B[n][j]: one workgroup
-// per 16 * RT rows of a sequence and 128 * CT columns.  The slices' sums are
-// added (low slices first) into LDS, scaled, as fp32; the products are
-// v_mfma_f32_16x16x4_f32 with B as the row operand, so that a lane ends up with
-// consecutive columns of one row: two tiles cover 32 columns, lane group g
-// holding 8g .. 8g + 7.  Rows without an adapter copy aux (or store zero).
+// y[row][n] = aux[row][n] + sum over j of (s u[row][j]) B[n][j] for up to 16 a.rt
+// rows and 64 columns a step: u (scaled by s) lies in LDS as two fp16 parts per
+// row (split_scale); v_mfma_f32_16x16x32_f16.  Tile p holds columns 4 i + p, so
+// that lane i of a lane group ends up with four consecutive columns of rows 4
+// (lane / 16) .. + 3, and 16 lanes read and write one contiguous piece of a row.
+// NC = 0: up to 16 ranks, both parts of u in one instruction (k groups 0, 1 the
+// high part, 2, 3 the low, B given twice); NC = 1, 2: up to 32 NC ranks; NC = 3:
+// any number, B read anew for each row tile.  A wave takes every WAVES-th step of
+// the workgroup's columns; the loads of its first B and aux are on their way
+// before u is there, those of the next aux before its products.
 // ----------------------------------------------------------------------------
-template <typename T, int RT, int CT>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
-  extern __shared__ float u[];  // [16 * RT][upad]
-  const LoraBlock b = lora_block(a, blockIdx.x, 16 * RT);
+struct LoraU {
+  _Float16* part[2];  // [16 rt][pad] each
+  float* undo;        // [16 rt]
+  int pad;
+};
+
+template <typename T, int NC, int WAVES>
+struct LoraColumns {
+  static constexpr int kChunks = NC == 0 ? 1 : NC == 3 ? 1 : NC, P = 4;
+  typedef T vec_t __attribute__((ext_vector_type(P), aligned(sizeof(T))));
+  const LoraArgs& a;
+  const LoraBlock& b;
+  const _Float16* w;
+  int i, g, end;
+  h8_t bv[P][kChunks];
+  vec_t x[4];
+
+  __device__ __forceinline__ LoraColumns(const LoraArgs& args, const LoraBlock& block, int lane, int last)
+      : a(args), b(block), w(args.b + (size_t)max(block.adapter, 0) * args.n * args.r), i(lane & 15), g(lane >> 4), end(last) {}
+
+  // Ranks j .. j + 7 of column n, zero behind the adapter's rank.
+  __device__ __forceinline__ h8_t ranks8(int n, int j) const {
+    h8_t v = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    if (j + 8 <= b.rank) {
+      if (n < a.n)
+        v = *reinterpret_cast<const h8_any_t*>(w + (size_t)n * a.r + j);
+      return v;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n < a.n && j + e < b.rank)
+        v[e] = w[(size_t)n * a.r + j + e];
+    return v;
+  }
+
+  __device__ __forceinline__ void load_b(int n0) {
+    if constexpr (NC != 3)
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          bv[p][c] = ranks8(n0 + P * i + p, NC == 0 ? 8 * (g & 1) : 32 * c + 8 * g);
+  }
+
+  __device__ __forceinline__ size_t at(int n0, int t, int c) const { return (size_t)(b.row + 16 * t + 4 * g + c) * a.n + n0 + P * i; }
+
+  __device__ __forceinline__ void load_aux(int n0, int t) {
+    if (a.aux && n0 + P * i < a.n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (16 * t + 4 * g + c < b.rows)
+          x[c] = __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(static_cast<const T*>(a.aux) + at(n0, t, c)));
+  }
+
+  __device__ __forceinline__ void first(int n0) {
+    if (n0 < end) {
+      load_b(n0);
+      load_aux(n0, 0);
+    }
+  }
+
+  // All columns of the wave, from n0 on.
+  __device__ __forceinline__ void run(int n0, const LoraU& u) {
+    const int tiles = (b.rows + 15) >> 4;
+    const _Float16* const frag = (NC == 0 && g >= 2 ? u.part[1] : u.part[0]) + i * u.pad + (NC == 0 ? 8 * (g & 1) : 8 * g);
+    const _Float16* const low = u.part[1] + i * u.pad + 8 * g;
+    while (n0 < end) {
+      for (int t = 0; t < tiles; ++t) {
+        const bool last = t + 1 == tiles;
+        const int next = n0 + 16 * P * WAVES;
+        f4_t acc[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          acc[p] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        float undo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (b.adapter >= 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            undo[c] = u.undo[16 * t + 4 * g + c];
+          const int ro = 16 * t * u.pad;
+          if constexpr (NC == 3) {
+            for (int j = 0; j < b.rank; j += 32) {
+              const h8_t hi = *reinterpret_cast<const h8_t*>(frag + ro + j), lo = *reinterpret_cast<const h8_t*>(low + ro + j);
+#pragma unroll
+              for (int p = 0; p < P; ++p) {
+                const h8_t v = ranks8(n0 + P * i + p, j + 8 * g);
+                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, v, acc[p], 0, 0, 0);
+                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, v, acc[p], 0, 0, 0);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              const h8_t hi = *reinterpret_cast<const h8_t*>(frag + ro + 32 * c);
+#pragma unroll
+              for (int p = 0; p < P; ++p)
+                acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, bv[p][c], acc[p], 0, 0, 0);
+              if constexpr (NC != 0) {
+                const h8_t lo = *reinterpret_cast<const h8_t*>(low + ro + 32 * c);
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                  acc[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, bv[p][c], acc[p], 0, 0, 0);
+              }
+            }
+          }
+        }
+        if (last && next < end)
+          load_b(next);
+        vec_t y[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            float o = a.aux ? (float)x[c][p] : 0.0f;
+            if (b.adapter >= 0)
+              o = fmaf(acc[p][c], undo[c], o);
+            y[c][p] = (T)o;
+          }
+        if (!last)
+          load_aux(n0, t + 1);
+        else if (next < end)
+          load_aux(next, 0);
+        if (n0 + P * i < a.n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (16 * t + 4 * g + c < b.rows)
+              __builtin_nontemporal_store(y[c], reinterpret_cast<vec_t*>(static_cast<T*>(a.y) + at(n0, t, c)));
+      }
+      n0 += 16 * P * WAVES;
+    }
+  }
+};
+
+// Rank columns of u's parts in LDS: a multiple of 32 (16 for NC = 0) and 8, so that
+// the rows of a tile start in different banks.
+__host__ __device__ inline int lora_upad(int r) {
+  return (r <= 16 ? 16 : (r + 31) / 32 * 32) + 8;
+}
+
+__host__ __device__ inline size_t lora_ubytes(int rows, int r) {
+  return (size_t)rows * (2 * lora_upad(r) * sizeof(_Float16) + sizeof(float));
+}
+
+// The second launch: one workgroup per 16 a.rt rows of a sequence and a.span
+// columns.  2^a.glog lanes take one row of u, four ranks each (Q times), add the slices'
+// sums, low slices first, and split them.
+template <typename T, int NC>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && NC == 2 ? 3 : 4) void lora_expand_kernel(LoraArgs a) {
+  extern __shared__ _Float16 lds[];
+  const LoraBlock b = lora_block(a, blockIdx.x, 16 * a.rt);
   if (b.adapter < 0 && a.aux == a.y)
     return;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, i = lane & 15, g = lane >> 4;
-  const int rtiles = (b.rank + 15) >> 4, upad = a.rpad + 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int start = (int)blockIdx.y * a.span, n0 = start + 64 * wave;
+  LoraU u;
+  u.pad = lora_upad(a.r);
+  u.part[0] = lds;
+  u.part[1] = lds + 16 * a.rt * u.pad;
+  u.undo = reinterpret_cast<float*>(lds + 32 * a.rt * u.pad);
+  LoraColumns<T, NC, 4> cols(a, b, lane, min(start + a.span, a.n));
+  cols.first(n0);
   if (b.adapter >= 0) {
+    constexpr int Q = NC == 3 ? 2 : 1;
     const float scale = a.scales ? a.scales[b.adapter] : 1.0f;
-    for (int o = tid; o < 16 * RT * rtiles * 16; o += 256) {
-      const int row = o / (rtiles * 16), j = o - row * (rtiles * 16);
-      float s = 0.0f;
-      if (row < b.rows && j < b.rank) {
-        const float* p = a.part + (size_t)(b.row + row) * a.rpad + j;
-        for (int sl = 0; sl < a.slices; ++sl)
-          s += p[(size_t)sl * a.m * a.rpad];
-        s *= scale;
+    const int q = tid & ((1 << a.glog) - 1), width = u.pad - 8;
+    for (int row = tid >> a.glog; row < ((b.rows + 15) & ~15); row += 256 >> a.glog) {
+      f4_t v[Q][kLoraMaxSlices];
+#pragma unroll
+      for (int h = 0; h < Q; ++h)
+#pragma unroll
+        for (int sl = 0; sl < kLoraMaxSlices; ++sl) {
+          const int j = 4 * (q + (h << a.glog));
+          v[h][sl] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+          if (row < b.rows && j < b.rank && sl < a.slices)
+            v[h][sl] = *reinterpret_cast<const f4_t*>(a.part + ((size_t)sl * a.m + b.row + row) * a.rpad + j);
+        }
+      float m = 0.0f;
+#pragma unroll
+      for (int h = 0; h < Q; ++h) {
+        const int j = 4 * (q + (h << a.glog));
+#pragma unroll
+        for (int sl = 1; sl < kLoraMaxSlices; ++sl)
+          v[h][0] += v[h][sl];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[h][0][e] = j + e < b.rank ? v[h][0][e] * scale : 0.0f;
+          m = fmaxf(m, fabsf(v[h][0][e]));
+        }
       }
-      u[row * upad + j] = s;
+      for (int off = (1 << a.glog) >> 1; off > 0; off >>= 1)
+        m = fmaxf(m, __shfl_xor(m, off));
+      float inverse;
+      const float up = split_scale(m, &inverse);
+#pragma unroll
+      for (int h = 0; h < Q; ++h) {
+        const int j = 4 * (q + (h << a.glog));
+        if (j < width) {
+          h4_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = v[h][0][e] * up;
+            hi[e] = (_Float16)x;
+            lo[e] = (_Float16)__builtin_amdgcn_fmed3f(x - (float)hi[e], -64.0f, 64.0f);
+          }
+          *reinterpret_cast<h4_t*>(u.part[0] + row * u.pad + j) = hi;
+          *reinterpret_cast<h4_t*>(u.part[1] + row * u.pad + j) = lo;
+        }
+      }
+      if (q == 0)
+        u.undo[row] = inverse;
     }
     __syncthreads();
   }
-  const _Float16* w = a.b + (size_t)max(b.adapter, 0) * a.n * a.r;
-  typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int n0 = ((int)blockIdx.y * CT + ct) * 128 + 32 * wave;
-    if (n0 >= a.n)
-      continue;
-    const int nl = n0 + 8 * g;  // the lane's 8 columns
-    f4_t acc[2][RT];
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-        acc[p][t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int jt = 0; jt < rtiles; ++jt) {
-      const int j = 16 * jt + 4 * g;
-      float bv[2][4];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int n = n0 + 8 * (i >> 2) + 4 * p + (i & 3);
-        const _Float16* src = w + (size_t)n * a.r + j;
-        if (n < a.n && j + 4 <= a.r) {
-          const h4_t v = *reinterpret_cast<const h4_any_t*>(src);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            bv[p][e] = j + e < b.rank ? (float)v[e] : 0.0f;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            bv[p][e] = n < a.n && j + e < b.rank ? (float)src[e] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const f4_t uv = *reinterpret_cast<const f4_t*>(&u[(16 * t + i) * upad + j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-            acc[p][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[p][e], uv[e], acc[p][t], 0, 0, 0);
-      }
-    }
-    if (nl >= a.n)
-      continue;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      if (16 * t + i >= b.rows)
-        continue;
-      const size_t at = (size_t)(b.row + 16 * t + i) * a.n + nl;
-      float o[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        o[c] = acc[c >> 2][t][c & 3];
-      if (a.aux) {
-        float x[8];
-        load8(static_cast<const T*>(a.aux) + at, x);
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          o[c] = b.adapter < 0 ? x[c] : x[c] + o[c];
-      }
-      t8 y;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        y[c] = (T)o[c];
-      *reinterpret_cast<t8*>(static_cast<T*>(a.y) + at) = y;
-    }
-  }
+  cols.run(n0, u);
 }
 
 // y = silu(aux) * t, 8 elements per thread.
@@ -220,40 +627,92 @@ int lora_tiles(const LoraArgs& a, int rows) {
   return t;
 }
 
-template <typename T>
-hipError_t lora_shrink(hipStream_t s, const LoraArgs& a) {
-  const int tiles = lora_tiles(a, 16), rt = (a.r + 15) / 16;
-  if (rt == 1)
-    return dispatch(lora_shrink_kernel<T, 1>, dim3(tiles, a.slices, 1), dim3(512), s, a);
-  if (rt == 2)
-    return dispatch(lora_shrink_kernel<T, 2>, dim3(tiles, a.slices, 1), dim3(512), s, a);
-  return dispatch(lora_shrink_kernel<T, 4>, dim3(tiles, a.slices, (rt + 3) / 4), dim3(512), s, a);
+// Fills a.tile for tiles of `rows` rows and returns their number.
+int lora_lay_tiles(LoraArgs& a, int rows) {
+  int t = 0;
+  for (int q = 0; q < a.nq; ++q) {
+    a.tile[q] = t;
+    t += (a.count[q] + rows - 1) / rows;
+  }
+  return t;
+}
+
+int lora_env(const char* n, int d) {
+  const char* v = getenv(n);
+  return v ? atoi(v) : d;
 }
 
 template <typename T>
-hipError_t lora_expand(hipStream_t s, const LoraArgs& a) {
-  const int upad = a.rpad + 4;
-  // Four row tiles share a load of B where the rows of a sequence fill them.
-  if (a.m >= 64 * a.nq && (size_t)64 * upad * sizeof(float) <= 65536)
-    return dispatch_lds(lora_expand_kernel<T, 4, 1>, dim3(lora_tiles(a, 64), (a.n + 127) / 128), dim3(256), 64 * upad * sizeof(float), s, a);
-  return dispatch_lds(lora_expand_kernel<T, 1, 2>, dim3(lora_tiles(a, 16), (a.n + 255) / 256), dim3(256), 16 * upad * sizeof(float), s, a);
+hipError_t lora_shrink(hipStream_t s, LoraArgs a) {
+  const int rt = (a.r + 15) / 16;
+  if (a.tall) {
+    const dim3 grid(lora_lay_tiles(a, 64), a.slices, (rt + 3) / 4), block(256);
+    hipError_t e = rt == 1   ? dispatch(lora_shrink_tall_kernel<T, 1>, grid, block, s, a)
+                   : rt == 2 ? dispatch(lora_shrink_tall_kernel<T, 2>, grid, block, s, a)
+                             : dispatch(lora_shrink_tall_kernel<T, 4>, grid, block, s, a);
+    return e;
+  }
+  const dim3 grid(lora_lay_tiles(a, 16), a.slices, (rt + 3) / 4), block(512);
+  if (rt == 1)
+    return dispatch(lora_shrink_kernel<T, 1, 1, 8, 4>, grid, block, s, a);
+  if (rt == 2)
+    return dispatch(lora_shrink_kernel<T, 1, 2, 8, 2>, grid, block, s, a);
+  return dispatch(lora_shrink_kernel<T, 1, 4, 8, 2>, grid, block, s, a);
+}
+
+template <typename T>
+hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
+  // Row tiles that share a load of B: as many as the sequences' mean fills, up to four.
+  static const int cap = lora_env("LR", 4);
+  a.rt = a.r > 256 ? 1 : a.m / (16 * a.nq);
+  a.rt = a.rt < 1 ? 1 : a.rt > cap ? cap : a.rt;
+  const int tiles = lora_lay_tiles(a, 16 * a.rt);
+  static const int per = lora_env("LX", 4);
+  // Columns of a workgroup: at least `per` workgroups per CU.
+  int steps = (int)(((int64_t)tiles * ((a.n + 255) / 256)) / ((int64_t)per * cus));
+  steps = steps < 1 ? 1 : steps > 16 ? 16 : steps;
+  a.span = 256 * steps;
+  // Lanes of a row of u: four ranks each, twice beyond 256 ranks.
+  const int quads = (lora_upad(a.r) - 8) / 4;
+  a.glog = 2;
+  while ((1 << a.glog) < quads && a.glog < 6)
+    ++a.glog;
+  const dim3 grid(tiles, (a.n + a.span - 1) / a.span), block(256);
+  const size_t lds = lora_ubytes(16 * a.rt, a.r);
+  if (a.r <= 16)
+    return dispatch_lds(lora_expand_kernel<T, 0>, grid, block, lds, s, a);
+  if (a.r <= 32)
+    return dispatch_lds(lora_expand_kernel<T, 1>, grid, block, lds, s, a);
+  if (a.r <= 64)
+    return dispatch_lds(lora_expand_kernel<T, 2>, grid, block, lds, s, a);
+  return dispatch_lds(lora_expand_kernel<T, 3>, grid, block, lds, s, a);
 }
 
 }  // namespace
 
-int lora_slices(const LoraArgs& a, int cus) {
-  // Two workgroups per CU, each at least one block of 256 k.
-  const int tiles = lora_tiles(a, 16), nb = a.k / 256;
-  const int want = (2 * cus + tiles - 1) / tiles;
-  return want < 1 ? 1 : want > nb ? nb : want > 16 ? 16 : want;
+void lora_plan(LoraArgs& a, int cus) {
+  static const int tall = lora_env("LT", 64), per = lora_env("LS", 2);
+  a.tall = a.m >= tall * a.nq;
+  const int groups = (a.r + 63) / 64, tiles = lora_tiles(a, a.tall ? 64 : 16) * groups, units = a.k / (a.tall ? 64 : 256);
+  // Workgroups for every CU, each with at least 256 k.
+  int want = ((a.tall ? per : 1) * cus + tiles - 1) / (tiles > 0 ? tiles : 1);
+  want = want > (a.tall ? kLoraTallSlices : kLoraMaxSlices) ? (a.tall ? kLoraTallSlices : kLoraMaxSlices) : want;
+  want = want > a.k / 256 ? a.k / 256 : want;
+  a.slices = want < 1 ? 1 : want;
+  (void)units;
 }
 
 hipError_t launch_lora_shrink(hipStream_t s, const LoraArgs& a, int dtype) {
   return dtype == kF32 ? lora_shrink<float>(s, a) : lora_shrink<_Float16>(s, a);
 }
 
-hipError_t launch_lora_expand(hipStream_t s, const LoraArgs& a, int dtype) {
-  return dtype == kF32 ? lora_expand<float>(s, a) : lora_expand<_Float16>(s, a);
+hipError_t launch_lora_reduce(hipStream_t s, const LoraArgs& a) {
+  const size_t quads = (size_t)a.m * a.rpad / 4;
+  return dispatch(lora_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), s, a);
+}
+
+hipError_t launch_lora_expand(hipStream_t s, const LoraArgs& a, int dtype, int cus) {
+  return dtype == kF32 ? lora_expand<float>(s, a, cus) : lora_expand<_Float16>(s, a, cus);
 }
 
 hipError_t launch_gate(hipStream_t s, const void* t, const void* aux, void* y, size_t elems, int dtype) {
