@@ -1928,6 +1928,11 @@ int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_ada
     start += (uint32_t)a.count[q];
   }
   lora_plan(a, device_cus(device));
+  if (a.one) {
+    LaunchTimer timer(stream, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_lora_token(stream, a, (int)dtype, device_cus(device)), "adapter launch");
+    return Q4K_OK;
+  }
   int rc = ensure_buffer(stream, ws, device, ws.part, ws.part_elems, (size_t)a.slices * a.m * a.rpad, "split-K workspace");
   if (rc)
     return rc;
@@ -1935,11 +1940,6 @@ int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_ada
   {
     LaunchTimer timer(stream, Q4K_KERNEL_AUX);
     Q4K_TRY_HIP(launch_lora_shrink(stream, a, (int)dtype), "adapter shrink launch");
-  }
-  if (a.tall && a.slices > 1) {
-    LaunchTimer timer(stream, Q4K_KERNEL_AUX);
-    Q4K_TRY_HIP(launch_lora_reduce(stream, a), "adapter reduce launch");
-    a.slices = 1;
   }
   LaunchTimer timer(stream, Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_lora_expand(stream, a, (int)dtype, device_cus(device)), "adapter expand launch");

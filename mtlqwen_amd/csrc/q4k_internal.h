@@ -545,16 +545,15 @@ struct LoraArgs {
   float* part = nullptr;           // [slices, m, rpad]
   int m = 0, k = 0, n = 0, r = 0, rpad = 0, slots = 0, nq = 0, slices = 1;
   int start[8] = {}, count[8] = {};  // rows of the sequences
-  bool tall = false;                 // many rows: the shrink shares A between 64 of them
+  bool one = false;                  // few rows and ranks: one launch
   // Set by the launches: row tiles before a sequence and in a workgroup, columns
   // per workgroup, log2 of the lanes of a row of u.
   int tile[8] = {}, rt = 1, span = 0, glog = 0;
 };
-// Sets tall and slices.
+// Sets one and slices.
 void lora_plan(LoraArgs& a, int cus);
+hipError_t launch_lora_token(hipStream_t s, const LoraArgs& a, int dtype, int cus);
 hipError_t launch_lora_shrink(hipStream_t s, const LoraArgs& a, int dtype);
-// Adds the slices into the first one.
-hipError_t launch_lora_reduce(hipStream_t s, const LoraArgs& a);
 hipError_t launch_lora_expand(hipStream_t s, const LoraArgs& a, int dtype, int cus);
 // y = silu(aux) * t over `elems` (a multiple of 16) values; y may be aux.
 hipError_t launch_gate(hipStream_t s, const void* t, const void* aux, void* y, size_t elems, int dtype);

@@ -1,13 +1,13 @@
 // Low-rank adapters of a packed batch, one per sequence, beside a projection:
-// u = x A^T (lora_shrink_kernel; lora_shrink_tall_kernel and lora_reduce_kernel)
-// and y = aux + s u B^T (lora_expand_kernel), and gate_kernel, the gated epilogue of a
-// projection with adapters.
+// u = x A^T (lora_shrink_kernel) and y = aux + s u B^T (lora_expand_kernel), both in
+// one launch for single rows and few ranks (lora_token_kernel), and gate_kernel, the
+// gated epilogue of a projection with adapters.
 #include "q4k_device.h"
 
 namespace q4k {
 namespace {
 
-constexpr int kLoraMaxSlices = 8, kLoraTallSlices = 16;
+constexpr int kLoraMaxSlices = 8;
 
 // Up to 16 RT rows that lie in one sequence: the first row, the rows, and the
 // sequence's adapter (-1: none) with its rank.
@@ -50,15 +50,30 @@ __device__ __forceinline__ float split_scale(float m, float* inverse) {
   return __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
 }
 
-// The parts of 8 scaled values.  The low part of an infinity is finite (its
+// The parts of N values scaled.  The low part of an infinity is finite (its
 // difference is no number), so that the infinity stays one.
-__device__ __forceinline__ void split8(const float* v, float scale, h8_t* hi, h8_t* lo) {
+template <int N, typename H>
+__device__ __forceinline__ void split(const float* v, float scale, H* hi, H* lo) {
+  typedef float f2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float s = v[e] * scale;
-    (*hi)[e] = (_Float16)s;
-    (*lo)[e] = (_Float16)__builtin_amdgcn_fmed3f(s - (float)(*hi)[e], -64.0f, 64.0f);
+  for (int e = 0; e < N; e += 2) {
+    const f2_t s = {v[e] * scale, v[e + 1] * scale};
+    const h2_t h = __builtin_convertvector(s, h2_t);
+    const f2_t d = {__builtin_amdgcn_fmed3f(fmaf((float)h[0], -1.0f, s[0]), -64.0f, 64.0f),
+                    __builtin_amdgcn_fmed3f(fmaf((float)h[1], -1.0f, s[1]), -64.0f, 64.0f)};
+    const h2_t l = __builtin_convertvector(d, h2_t);
+    (*hi)[e] = h[0];
+    (*hi)[e + 1] = h[1];
+    (*lo)[e] = l[0];
+    (*lo)[e + 1] = l[1];
   }
+}
+
+// The maximum with another lane's value: CTRL 0xB1, 0x4E: lanes ^ 1 and ^ 2; 0x120
+// + n: n lanes on within 16.
+template <int CTRL>
+__device__ __forceinline__ float max_lane(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)));
 }
 
 // The 16 bytes of lane 4 (lane % 16) + lane / 16: loads give each four lanes 64
@@ -77,37 +92,31 @@ __device__ __forceinline__ u4_t to_rows(u4_t v, int from) {
 typedef uint32_t u4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // ----------------------------------------------------------------------------
-// One wave's share of u[row][j] = sum over k of x[row][k] A[j][k]: 16 RT rows, 16
-// NT ranks, `steps` times 32 k, from the addresses x[r] and w on (row or rank lane / 4 of
+// One wave's share of u[row][j] = sum over k of x[row][k] A[j][k]: 16 rows, 16 NT
+// ranks, `steps` times 32 k, from the addresses x and w on (row or rank lane / 4 of
 // their tile, k 8 (lane % 4)), the loads of SEG steps on their way together.
 // v_mfma_f32_16x16x32_f16, whose products are exact; fp32 x as two fp16 parts
 // (split_scale), which costs two of these instructions where eight fp32 ones of
 // twice the time each would be needed.  The scale of a row follows the largest
 // value so far; the sums follow it where it changes.
-// acc[r][t][c]: row 16 r + 4 (lane / 16) + c, rank 16 t + lane % 16.
+// acc[t][c]: row 4 (lane / 16) + c, rank 16 t + lane % 16.
 // ----------------------------------------------------------------------------
-template <typename T, int RT, int NT, int SEG>
-__device__ __forceinline__ void lora_sum(const T* const* x, const _Float16* w, int steps, int k, int live, int lane, f4_t (*acc)[NT]) {
+template <typename T, int NT, int SEG>
+__device__ __forceinline__ void lora_sum(const T* x, const _Float16* w, int steps, int k, int live, int lane, f4_t* acc) {
   constexpr int kX = (int)sizeof(T) / 2;  // 16-byte loads of 8 values
   const int g = lane >> 4, from = 4 * (4 * (lane & 15) + g);
-  float scale[RT], inverse[RT];
+  float inverse, scale = split_scale(0.0f, &inverse);
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    scale[r] = split_scale(0.0f, &inverse[r]);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      acc[r][t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int t = 0; t < NT; ++t)
+    acc[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = 0; s0 < steps; s0 += SEG) {
-    u4_t wv[SEG][NT], xv[SEG][RT][kX];
+    u4_t wv[SEG][NT], xv[SEG][kX];
 #pragma unroll
     for (int s = 0; s < SEG; ++s)
       if (s0 + s < steps)
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < kX; ++h)
-            xv[s][r][h] = *reinterpret_cast<const u4_any_t*>(x[r] + 32 * (s0 + s) + 4 * h);
+        for (int h = 0; h < kX; ++h)
+          xv[s][h] = *reinterpret_cast<const u4_any_t*>(x + 32 * (s0 + s) + 4 * h);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -120,33 +129,29 @@ __device__ __forceinline__ void lora_sum(const T* const* x, const _Float16* w, i
             wv[s][t] = *reinterpret_cast<const u4_any_t*>(w + (size_t)(16 * t) * k + 32 * (s0 + s));
     }
     if constexpr (kX == 2) {
+      float m = 0.0f;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float m = 0.0f;
+      for (int s = 0; s < SEG; ++s)
+        if (s0 + s < steps)
 #pragma unroll
-        for (int s = 0; s < SEG; ++s)
-          if (s0 + s < steps)
+          for (int e = 0; e < 8; ++e)
+            m = fmaxf(m, fabsf(__builtin_bit_cast(float, (uint32_t)xv[s][e >> 2][e & 3])));
+      m = max_lane<0x4E>(max_lane<0xB1>(m));
+      // Lanes 4 i .. 4 i + 3 hold row i: its scale stays with them.
+      float undo;
+      const float now = split_scale(m, &undo);
+      if (__any(now < scale)) {
+        const float ratio = now < scale ? now * inverse : 1.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              m = fmaxf(m, fabsf(__builtin_bit_cast(float, (uint32_t)xv[s][r][e >> 2][e & 3])));
-        m = fmaxf(m, __shfl_xor(m, 1));
-        m = fmaxf(m, __shfl_xor(m, 2));
-        // Lanes 4 i .. 4 i + 3 hold row i: its scale stays with them.
-        float undo;
-        const float now = split_scale(m, &undo);
-        if (__any(now < scale[r])) {
-          const float ratio = now < scale[r] ? now * inverse[r] : 1.0f;
+        for (int c = 0; c < 4; ++c) {
+          const float q = __shfl(ratio, 4 * (4 * g + c));
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float q = __shfl(ratio, 4 * (4 * g + c));
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              acc[r][t][c] *= q;
-          }
-          if (now < scale[r]) {
-            scale[r] = now;
-            inverse[r] = undo;
-          }
+          for (int t = 0; t < NT; ++t)
+            acc[t][c] *= q;
+        }
+        if (now < scale) {
+          scale = now;
+          inverse = undo;
         }
       }
     }
@@ -157,41 +162,36 @@ __device__ __forceinline__ void lora_sum(const T* const* x, const _Float16* w, i
 #pragma unroll
         for (int t = 0; t < NT; ++t)
           a[t] = __builtin_bit_cast(h8_t, to_rows(wv[s][t], from));
+        if constexpr (kX == 1) {
+          const h8_t v = __builtin_bit_cast(h8_t, to_rows(xv[s][0], from));
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if constexpr (kX == 1) {
-            const h8_t v = __builtin_bit_cast(h8_t, to_rows(xv[s][r][0], from));
+          for (int t = 0; t < NT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, a[t], acc[t], 0, 0, 0);
+        } else {
+          float v[8];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, a[t], acc[r][t], 0, 0, 0);
-          } else {
-            float v[8];
+          for (int e = 0; e < 8; ++e)
+            v[e] = __builtin_bit_cast(float, (uint32_t)xv[s][e >> 2][e & 3]);
+          h8_t hi, lo;
+          split<8>(v, scale, &hi, &lo);
+          hi = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, hi), from));
+          lo = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, lo), from));
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[e] = __builtin_bit_cast(float, (uint32_t)xv[s][r][e >> 2][e & 3]);
-            h8_t hi, lo;
-            split8(v, scale[r], &hi, &lo);
-            hi = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, hi), from));
-            lo = __builtin_bit_cast(h8_t, to_rows(__builtin_bit_cast(u4_t, lo), from));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, a[t], acc[r][t], 0, 0, 0);
-              acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, a[t], acc[r][t], 0, 0, 0);
-            }
+          for (int t = 0; t < NT; ++t) {
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, a[t], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, a[t], acc[t], 0, 0, 0);
           }
         }
       }
   }
   if constexpr (kX == 2)
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int c = 0; c < 4; ++c) {
+      const float undo = __shfl(inverse, 4 * (4 * g + c));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float undo = __shfl(inverse[r], 4 * (4 * g + c));
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          acc[r][t][c] *= undo;
-      }
+      for (int t = 0; t < NT; ++t)
+        acc[t][c] *= undo;
+    }
 }
 
 // The waves' sums of one row and rank, added in pairs.
@@ -209,171 +209,35 @@ __device__ __forceinline__ float sum_waves(const float* p, int stride) {
   return v[0];
 }
 
-// K in slices: one workgroup per 16 RT rows, slice and 16 NT ranks; its WAVES
-// waves take a part of the slice each and add their sums in LDS.
-template <typename T, int RT, int NT, int WAVES, int SEG>
-__global__ __launch_bounds__(64 * WAVES, 4) void lora_shrink_kernel(LoraArgs a) {
-  constexpr int kSums = RT * NT * 256;
-  __shared__ float red[WAVES * kSums];
-  const LoraBlock b = lora_block(a, blockIdx.x, 16 * RT);
+// K in slices: one workgroup per 16 rows, slice and 16 NT ranks; its eight waves
+// take a part of the slice each and add their sums in LDS.
+template <typename T, int NT, int SEG>
+__global__ __launch_bounds__(512, 4) void lora_shrink_kernel(LoraArgs a) {
+  constexpr int kSums = NT * 256, kWaves = 8;
+  __shared__ float red[kWaves * kSums];
+  const LoraBlock b = lora_block(a, blockIdx.x, 16);
   const int j0 = (int)blockIdx.z * 16 * NT;
   if (b.adapter < 0 || j0 >= b.rank)
     return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
   // Units of 32 k per wave.
-  const int units = a.k / (32 * WAVES), u0 = (int)((int64_t)units * blockIdx.y / a.slices), u1 = (int)((int64_t)units * (blockIdx.y + 1) / a.slices);
-  const int k0 = 32 * (WAVES * u0 + wave * (u1 - u0)) + 8 * (lane & 3);
-  f4_t acc[RT][NT];
-  const T* x[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-    x[r] = static_cast<const T*>(a.x) + (size_t)(b.row + min(16 * r + (lane >> 2), b.rows - 1)) * a.k + k0;
-  lora_sum<T, RT, NT, SEG>(x, a.a + ((size_t)b.adapter * a.r + j0 + (lane >> 2)) * a.k + k0, u1 - u0, a.k, b.rank - j0, lane, acc);
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        red[wave * kSums + (16 * r + 4 * g + c) * (16 * NT) + 16 * t + i] = acc[r][t][c];
-  __syncthreads();
-  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row) * a.rpad + j0;
-  for (int o = tid; o < kSums; o += 64 * WAVES) {
-    const int row = o / (16 * NT), j = o % (16 * NT);
-    if (row < b.rows && j0 + j < b.rank)
-      part[(size_t)row * a.rpad + j] = sum_waves<WAVES>(red + o, kSums);
-  }
-}
-
-// The same for many rows: one workgroup of four waves per 64 rows, slice and 16 NT
-// ranks.  A wave reads, splits and multiplies its own 16 rows, 64 k at a time;
-// A's 64 k are shared through LDS, so that they cross from the L2 once per 64
-// rows.  The next 64 k are read while these are multiplied.
-template <typename T, int NT>
-__global__ __launch_bounds__(256) void lora_shrink_tall_kernel(LoraArgs a) {
-  constexpr int kPad = 72, kParts = sizeof(T) == 4 ? 2 : 1, kA = NT * 16 / 32;
-  __shared__ _Float16 as[2][NT * 16 * kPad], xs[4][kParts][16 * kPad];
-  const LoraBlock b = lora_block(a, blockIdx.x, 64);
-  const int j0 = (int)blockIdx.z * 16 * NT;
-  if (b.adapter < 0 || j0 >= b.rank)
-    return;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
-  const int chunks = a.k >> 6, c0 = (int)((int64_t)chunks * blockIdx.y / a.slices), c1 = (int)((int64_t)chunks * (blockIdx.y + 1) / a.slices);
-  // Register q of lane group g holds row 4 g + q of the wave: the rows whose sums
-  // acc[.][q] of the same lanes will be.
-  const T* x[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    x[q] = static_cast<const T*>(a.x) + (size_t)(b.row + min(16 * wave + 4 * g + q, b.rows - 1)) * a.k + 4 * i;
-  // Lane's share of A: rank tid / 8 (+ 32 h), 8 k from 8 (tid % 8) on.
-  const _Float16* w = a.a + ((size_t)b.adapter * a.r + j0) * a.k + 8 * (tid & 7);
-  typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  t4 xv[4];
-  u4_t wv[kA < 1 ? 1 : kA];
-  auto load = [&](int c) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      xv[q] = *reinterpret_cast<const t4*>(x[q] + 64 * c);
-#pragma unroll
-    for (int h = 0; h < (kA < 1 ? 1 : kA); ++h) {
-      const int j = (tid >> 3) + 32 * h;
-      wv[h] = u4_t{0u, 0u, 0u, 0u};
-      if (j < 16 * NT && j0 + j < b.rank)
-        wv[h] = *reinterpret_cast<const u4_any_t*>(w + (size_t)j * a.k + 64 * c);
-    }
-  };
+  const int units = a.k / (32 * kWaves), u0 = (int)((int64_t)units * blockIdx.y / a.slices), u1 = (int)((int64_t)units * (blockIdx.y + 1) / a.slices);
+  const int k0 = 32 * (kWaves * u0 + wave * (u1 - u0)) + 8 * (lane & 3);
   f4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-    acc[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  float scale[4], inverse[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    scale[q] = split_scale(0.0f, &inverse[q]);
-  load(c0);
-  for (int c = c0; c < c1; ++c) {
-    _Float16* at = as[c & 1];
-#pragma unroll
-    for (int h = 0; h < (kA < 1 ? 1 : kA); ++h) {
-      const int j = (tid >> 3) + 32 * h;
-      if (j < 16 * NT)
-        *reinterpret_cast<u4_t*>(at + j * kPad + 8 * (tid & 7)) = wv[h];
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      _Float16* to = &xs[wave][0][(4 * g + q) * kPad + 4 * i];
-      if constexpr (kParts == 1) {
-        *reinterpret_cast<h4_t*>(to) = __builtin_bit_cast(h4_t, xv[q]);
-      } else {
-        float m = fmaxf(fmaxf(fabsf(xv[q][0]), fabsf(xv[q][1])), fmaxf(fabsf(xv[q][2]), fabsf(xv[q][3])));
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1)
-          m = fmaxf(m, __shfl_xor(m, off));
-        float undo;
-        const float now = split_scale(m, &undo);
-        if (now < scale[q]) {
-          const float ratio = now * inverse[q];
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            acc[t][q] *= ratio;
-          scale[q] = now;
-          inverse[q] = undo;
-        }
-        h4_t hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = xv[q][e] * scale[q];
-          hi[e] = (_Float16)v;
-          lo[e] = (_Float16)__builtin_amdgcn_fmed3f(v - (float)hi[e], -64.0f, 64.0f);
-        }
-        *reinterpret_cast<h4_t*>(to) = hi;
-        *reinterpret_cast<h4_t*>(to + 16 * kPad) = lo;
-      }
-    }
-    if (c + 1 < c1)
-      load(c + 1);
-    // One barrier: A's other buffer is not written before every wave has left
-    // the previous round's reads of it; a wave's rows are its own.
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      h8_t av[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        av[t] = *reinterpret_cast<const h8_t*>(at + (16 * t + i) * kPad + 32 * s + 8 * g);
-#pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        const h8_t v = *reinterpret_cast<const h8_t*>(&xs[wave][part][i * kPad + 32 * s + 8 * g]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, av[t], acc[t], 0, 0, 0);
-      }
-    }
-  }
-  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row + 16 * wave) * a.rpad + j0;
+  lora_sum<T, NT, SEG>(static_cast<const T*>(a.x) + (size_t)(b.row + min(lane >> 2, b.rows - 1)) * a.k + k0,
+                       a.a + ((size_t)b.adapter * a.r + j0 + (lane >> 2)) * a.k + k0, u1 - u0, a.k, b.rank - j0, lane, acc);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (16 * wave + 4 * g + c < b.rows && j0 + 16 * t + i < b.rank)
-        part[(size_t)(4 * g + c) * a.rpad + 16 * t + i] = kParts == 2 ? acc[t][c] * inverse[c] : acc[t][c];
-}
-
-// The slices' sums, low slices first, into the first slice: four values per thread.
-__global__ __launch_bounds__(256) void lora_reduce_kernel(LoraArgs a) {
-  const size_t quads = (size_t)a.m * a.rpad / 4, q = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= quads)
-    return;
-  f4_t* p = reinterpret_cast<f4_t*>(a.part) + q;
-  f4_t v[kLoraTallSlices];
-#pragma unroll
-  for (int s = 0; s < kLoraTallSlices; ++s)
-    v[s] = s < a.slices ? p[s * quads] : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  f4_t sum = v[0];
-#pragma unroll
-  for (int s = 1; s < kLoraTallSlices; ++s)
-    sum += v[s];
-  *p = sum;
+      red[wave * kSums + (4 * g + c) * (16 * NT) + 16 * t + i] = acc[t][c];
+  __syncthreads();
+  float* part = a.part + ((size_t)blockIdx.y * a.m + b.row) * a.rpad + j0;
+  for (int o = tid; o < kSums; o += 64 * kWaves) {
+    const int row = o / (16 * NT), j = o % (16 * NT);
+    if (row < b.rows && j0 + j < b.rank)
+      part[(size_t)row * a.rpad + j] = sum_waves<kWaves>(red + o, kSums);
+  }
 }
 
 // ----------------------------------------------------------------------------
@@ -585,13 +449,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NC == 2 ? 3 : 4) void lora_e
       for (int h = 0; h < Q; ++h) {
         const int j = 4 * (q + (h << a.glog));
         if (j < width) {
+          const float x[4] = {v[h][0][0], v[h][0][1], v[h][0][2], v[h][0][3]};
           h4_t hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = v[h][0][e] * up;
-            hi[e] = (_Float16)x;
-            lo[e] = (_Float16)__builtin_amdgcn_fmed3f(x - (float)hi[e], -64.0f, 64.0f);
-          }
+          split<4>(x, up, &hi, &lo);
           *reinterpret_cast<h4_t*>(u.part[0] + row * u.pad + j) = hi;
           *reinterpret_cast<h4_t*>(u.part[1] + row * u.pad + j) = lo;
         }
@@ -602,6 +462,144 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NC == 2 ? 3 : 4) void lora_e
     __syncthreads();
   }
   cols.run(n0, u);
+}
+
+// The sum of a wave's lanes, in lane 63: within rows of 16 lanes, then across them.
+__device__ __forceinline__ float sum_lanes(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x111, 0xf, 0xf, true));  // row_shr:1
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x112, 0xf, 0xf, true));  // row_shr:2
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x114, 0xf, 0xf, true));  // row_shr:4
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x118, 0xf, 0xf, true));  // row_shr:8
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x142, 0xa, 0xf, true));  // row_bcast:15
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x143, 0xc, 0xf, true));  // row_bcast:31
+  return v;
+}
+
+// ----------------------------------------------------------------------------
+// Sequences of few rows and few ranks (decode) in one launch: every workgroup
+// forms u of its sequence's rows itself, on the vector units in fp32 (a wave
+// takes 512 k of one rank row in one contiguous load, 8 k per lane), and writes
+// a.span columns: 1 << a.glog lanes share a column's ranks, 8 each.  A second
+// launch would cost the caller more than reading A once per workgroup costs the L2.
+// ----------------------------------------------------------------------------
+template <typename T, int ROWS>
+__global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
+  __shared__ float red[8][ROWS][64], us[ROWS][64];
+  const LoraBlock b = lora_block(a, blockIdx.x, ROWS);
+  if (b.adapter < 0 && a.aux == a.y)
+    return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int share = lane & ((1 << a.glog) - 1), step = 512 >> a.glog;  // columns of a round of the workgroup
+  const int end = min((int)(blockIdx.y + 1) * a.span, a.n);
+  int n = (int)blockIdx.y * a.span + (tid >> a.glog);
+  const _Float16* bw = a.b + (size_t)max(b.adapter, 0) * a.n * a.r + 8 * share;
+  h8_t bv;
+  T x0[ROWS];
+  const auto load = [&](int col) {
+    bv = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    if (col >= end)
+      return;
+    const _Float16* src = bw + (size_t)col * a.r;
+    if (8 * share + 8 <= b.rank)
+      bv = *reinterpret_cast<const h8_any_t*>(src);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * share + e < b.rank)
+          bv[e] = src[e];
+    if (a.aux)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (r < b.rows && (r & ((1 << a.glog) - 1)) == share)
+          x0[r] = static_cast<const T*>(a.aux)[(size_t)(b.row + r) * a.n + col];
+  };
+  load(n);
+  float v[ROWS][8];
+  if (b.adapter >= 0) {
+    const float scale = a.scales ? a.scales[b.adapter] : 1.0f;
+    const T* x = static_cast<const T*>(a.x) + (size_t)b.row * a.k + 512 * wave + 8 * lane;
+    const _Float16* w = a.a + (size_t)b.adapter * a.r * a.k + 512 * wave + 8 * lane;
+    // Rounds of 8 ranks and 4096 k, the next one's ranks on their way.
+    const int segments = (a.k + 4095) >> 12, rounds = ((b.rank + 7) >> 3) * segments;
+    const int ke = 512 * wave + 8 * lane;
+    h8_t wv[8], wn[8];
+    const auto ranks = [&](int j0, int k0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        wn[j] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        if (k0 + ke < a.k && j0 + j < b.rank)
+          wn[j] = *reinterpret_cast<const h8_any_t*>(w + (size_t)(j0 + j) * a.k + k0);
+      }
+    };
+    float acc[ROWS][8];
+    ranks(0, 0);
+    for (int round = 0, j0 = 0, k0 = 0; round < rounds; ++round) {
+      if (segments > 1 || round == 0)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            v[r][e] = 0.0f;
+          if (k0 + ke < a.k && r < b.rows)
+            load8(x + (size_t)r * a.k + k0, v[r]);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        wv[j] = wn[j];
+      const bool last = k0 + 4096 >= a.k;
+      const int j1 = last ? j0 + 8 : j0, k1 = last ? 0 : k0 + 4096;
+      if (round + 1 < rounds)
+        ranks(j1, k1);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (r < b.rows)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float t = k0 == 0 ? 0.0f : acc[r][j];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              t = fmaf((float)wv[j][e], v[r][e], t);
+            acc[r][j] = t;
+            if (last) {
+              const float s = sum_lanes(t);
+              if (lane == 63)
+                red[wave][r][j0 + j] = s;
+            }
+          }
+      j0 = j1;
+      k0 = k1;
+    }
+    __syncthreads();
+    for (int o = tid; o < ROWS * 64; o += 512) {
+      const int r = o >> 6, j = o & 63;
+      us[r][j] = r < b.rows && j < b.rank ? sum_waves<8>(&red[0][r][j], ROWS * 64) * scale : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[r][e] = us[r][8 * share + e];
+  }
+  for (; n < end; n += step) {
+    float o[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      o[r] = 0.0f;
+      if (b.adapter >= 0 && r < b.rows) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          o[r] = fmaf((float)bv[e], v[r][e], o[r]);
+        for (int off = 1; off < 1 << a.glog; off <<= 1)
+          o[r] += __shfl_xor(o[r], off);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (r < b.rows && (r & ((1 << a.glog) - 1)) == share)
+        static_cast<T*>(a.y)[(size_t)(b.row + r) * a.n + n] = (T)(a.aux ? (float)x0[r] + o[r] : o[r]);
+    load(n + step);
+  }
 }
 
 // y = silu(aux) * t, 8 elements per thread.
@@ -637,39 +635,43 @@ int lora_lay_tiles(LoraArgs& a, int rows) {
   return t;
 }
 
-int lora_env(const char* n, int d) {
-  const char* v = getenv(n);
-  return v ? atoi(v) : d;
+template <typename T>
+hipError_t lora_token(hipStream_t s, LoraArgs a, int cus) {
+  int rows = 1;
+  for (int q = 0; q < a.nq; ++q)
+    rows = a.count[q] > rows ? a.count[q] : rows;
+  const int tile = rows <= 1 ? 1 : 2, tiles = lora_lay_tiles(a, tile);
+  a.glog = a.r <= 8 ? 0 : a.r <= 16 ? 1 : a.r <= 32 ? 2 : 3;
+  const int round = 512 >> a.glog, rounds = (a.n + round - 1) / round;
+  // One workgroup per CU: two took 8.1 us where one took 6.6.
+  const int64_t steps = ((int64_t)tiles * rounds + cus - 1) / cus;
+  a.span = round * (int)steps;
+  const dim3 grid(tiles, (a.n + a.span - 1) / a.span), block(512);
+  return tile == 1 ? dispatch(lora_token_kernel<T, 1>, grid, block, s, a) : dispatch(lora_token_kernel<T, 2>, grid, block, s, a);
 }
 
 template <typename T>
 hipError_t lora_shrink(hipStream_t s, LoraArgs a) {
   const int rt = (a.r + 15) / 16;
-  if (a.tall) {
-    const dim3 grid(lora_lay_tiles(a, 64), a.slices, (rt + 3) / 4), block(256);
-    hipError_t e = rt == 1   ? dispatch(lora_shrink_tall_kernel<T, 1>, grid, block, s, a)
-                   : rt == 2 ? dispatch(lora_shrink_tall_kernel<T, 2>, grid, block, s, a)
-                             : dispatch(lora_shrink_tall_kernel<T, 4>, grid, block, s, a);
-    return e;
-  }
   const dim3 grid(lora_lay_tiles(a, 16), a.slices, (rt + 3) / 4), block(512);
   if (rt == 1)
-    return dispatch(lora_shrink_kernel<T, 1, 1, 8, 4>, grid, block, s, a);
+    return dispatch(lora_shrink_kernel<T, 1, 4>, grid, block, s, a);
   if (rt == 2)
-    return dispatch(lora_shrink_kernel<T, 1, 2, 8, 2>, grid, block, s, a);
-  return dispatch(lora_shrink_kernel<T, 1, 4, 8, 2>, grid, block, s, a);
+    return dispatch(lora_shrink_kernel<T, 2, 2>, grid, block, s, a);
+  return dispatch(lora_shrink_kernel<T, 4, 2>, grid, block, s, a);
 }
 
 template <typename T>
 hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
-  // Row tiles that share a load of B: as many as the sequences' mean fills, up to four.
-  static const int cap = lora_env("LR", 4);
-  a.rt = a.r > 256 ? 1 : a.m / (16 * a.nq);
-  a.rt = a.rt < 1 ? 1 : a.rt > cap ? cap : a.rt;
+  // Row tiles that share a load of B and u's sums: two where the sequences fill
+  // them (64 rows of one sequence, 4096 -> 12288, rank 64, fp16: 11.4 us, with four
+  // 14.8), four where that still leaves four workgroups per CU (2048 rows, fp32: 60.5 us, with
+  // two 72.5); one for ranks beyond 256, whose parts fill the LDS.
+  const int64_t blocks = (int64_t)(a.m / 64) * ((a.n + 255) / 256);
+  a.rt = a.r > 256 || a.m < 32 * a.nq ? 1 : a.m >= 64 * a.nq && blocks >= 4 * (int64_t)cus ? 4 : 2;
   const int tiles = lora_lay_tiles(a, 16 * a.rt);
-  static const int per = lora_env("LX", 4);
-  // Columns of a workgroup: at least `per` workgroups per CU.
-  int steps = (int)(((int64_t)tiles * ((a.n + 255) / 256)) / ((int64_t)per * cus));
+  // Columns of a workgroup: at least four workgroups per CU.
+  int steps = (int)(((int64_t)tiles * ((a.n + 255) / 256)) / (4 * (int64_t)cus));
   steps = steps < 1 ? 1 : steps > 16 ? 16 : steps;
   a.span = 256 * steps;
   // Lanes of a row of u: four ranks each, twice beyond 256 ranks.
@@ -691,24 +693,30 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
 }  // namespace
 
 void lora_plan(LoraArgs& a, int cus) {
-  static const int tall = lora_env("LT", 64), per = lora_env("LS", 2);
-  a.tall = a.m >= tall * a.nq;
-  const int groups = (a.r + 63) / 64, tiles = lora_tiles(a, a.tall ? 64 : 16) * groups, units = a.k / (a.tall ? 64 : 256);
+  // Rounds of the one-launch kernel (8 ranks, 4096 k, one row).  Replayed back
+  // to back, fp16, 4096 -> 12288, 8 sequences: 1 round 4.1 us against 8.3 in two
+  // launches, 2 rounds 6.0 (7.3), 3 rounds (12288 -> 4096) 5.9 (8.8), 4 rounds 8.0
+  // (7.3) with two rows and 9.4 (7.6) with 32 ranks.
+  int rows = 0;
+  for (int q = 0; q < a.nq; ++q)
+    rows = a.count[q] > rows ? a.count[q] : rows;
+  a.one = rows <= 2 && rows * ((a.r + 7) / 8) * ((a.k + 4095) / 4096) <= 3;
+  if (a.one)
+    return;
   // Workgroups for every CU, each with at least 256 k.
-  int want = ((a.tall ? per : 1) * cus + tiles - 1) / (tiles > 0 ? tiles : 1);
-  want = want > (a.tall ? kLoraTallSlices : kLoraMaxSlices) ? (a.tall ? kLoraTallSlices : kLoraMaxSlices) : want;
+  const int tiles = lora_tiles(a, 16) * ((a.r + 63) / 64);
+  int want = (cus + tiles - 1) / (tiles > 0 ? tiles : 1);
+  want = want > kLoraMaxSlices ? kLoraMaxSlices : want;
   want = want > a.k / 256 ? a.k / 256 : want;
   a.slices = want < 1 ? 1 : want;
-  (void)units;
+}
+
+hipError_t launch_lora_token(hipStream_t s, const LoraArgs& a, int dtype, int cus) {
+  return dtype == kF32 ? lora_token<float>(s, a, cus) : lora_token<_Float16>(s, a, cus);
 }
 
 hipError_t launch_lora_shrink(hipStream_t s, const LoraArgs& a, int dtype) {
   return dtype == kF32 ? lora_shrink<float>(s, a) : lora_shrink<_Float16>(s, a);
-}
-
-hipError_t launch_lora_reduce(hipStream_t s, const LoraArgs& a) {
-  const size_t quads = (size_t)a.m * a.rpad / 4;
-  return dispatch(lora_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), s, a);
 }
 
 hipError_t launch_lora_expand(hipStream_t s, const LoraArgs& a, int dtype, int cus) {
