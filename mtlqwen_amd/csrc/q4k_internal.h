@@ -547,8 +547,11 @@ struct LoraArgs {
   int start[8] = {}, count[8] = {};  // rows of the sequences
   bool one = false;                  // few rows and ranks: one launch
   // Set by the launches: row tiles before a sequence and in a workgroup, columns
-  // per workgroup, log2 of the lanes of a row of u.
+  // per workgroup, log2 of the lanes of a row of u (of a column), the order of
+  // the expand's workgroups.
   int tile[8] = {}, rt = 1, span = 0, glog = 0;
+  uint32_t inner = 1;
+  bool by_rows = false;
 };
 // Sets one and slices.
 void lora_plan(LoraArgs& a, int cus);
