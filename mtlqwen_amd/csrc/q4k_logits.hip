@@ -203,7 +203,10 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
     for (int i = 0; i < V; ++i)
       y[i] = (T)((allowed[j] >> i) & 1u ? v[j][i] : -__builtin_inff());
     if (at + V <= left) {
-      *reinterpret_cast<vec_t*>(out + at) = y;
+      if constexpr (THREADS > 256)
+        __builtin_nontemporal_store(y, reinterpret_cast<vec_t*>(out + at));
+      else
+        *reinterpret_cast<vec_t*>(out + at) = y;
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
