@@ -35,18 +35,20 @@ except AttributeError:
         return torch.cuda.current_stream(device).cuda_stream
 
 
-def _stream_of(stream, device):
-    if stream is None:
-        return _raw_stream(device)
+def _stream_of(stream):
     return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else stream
+
+
+_rope, _qk_norm_rope, _lora, _linear_lora, _process_logits = (lib.q4k_rope, lib.q4k_qk_norm_rope, lib.q4k_lora, lib.q4k_linear_lora,
+                                                              lib.q4k_process_logits)
 
 
 def _activations(t, what):
     """(dtype code, device index) of an activation tensor."""
     code = _DTYPES.get(t.dtype)
+    device = t.get_device()
     if code is None:
         raise TypeError(f"{what} must be float32 or float16, got {t.dtype}")
-    device = t.get_device()
     if device < 0:
         raise ValueError(f"{what} must be a GPU tensor")
     return code, device
@@ -55,18 +57,18 @@ def _activations(t, what):
 def _address(t, dtype, numel, device, what):
     """The address of a contiguous tensor of ``dtype`` on ``device`` that holds
     at least ``numel`` elements (0 for None): the C ABI takes raw pointers, so
-    what does not fit is a ValueError here."""
+    what does not fit is refused here."""
     if t is None:
         return 0
-    if t.dtype != dtype:
+    if t.dtype is dtype and t.get_device() == device and t.numel() >= numel and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if t.get_device() != device:
         raise ValueError(f"{what} must be on cuda:{device}, is on {t.device}")
     if t.numel() < numel:
         raise ValueError(f"{what} holds {t.numel()} elements, needs {numel}")
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{what} must be contiguous")
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original_context=0, beta_slow=1.0, beta_fast=32.0, device="cuda"):
@@ -87,17 +89,18 @@ def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original
 
 def _heads(t, out, weight, what):
     """A q4k_heads of ``t`` and ``out`` [rows, heads, head_dim]."""
-    if t.dim() != 3 or out.shape != t.shape:
-        raise ValueError(f"{what} and its output must be [rows, heads, head_dim] alike, got {tuple(t.shape)} and {tuple(out.shape)}")
-    if out.dtype != t.dtype:
+    shape = t.shape
+    if len(shape) != 3 or out.shape != shape:
+        raise ValueError(f"{what} and its output must be [rows, heads, head_dim] alike, got {tuple(shape)} and {tuple(out.shape)}")
+    if out.dtype is not t.dtype:
         raise TypeError(f"{what} and its output must share a dtype")
     if out.get_device() != t.get_device():
         raise ValueError(f"{what} and its output must be on one GPU")
     ir, ih, ie = t.stride()
     orow, oh, oe = out.stride()
-    if (ie != 1 or oe != 1) and t.shape[2] > 1:
+    if (ie != 1 or oe != 1) and shape[2] > 1:
         raise ValueError(f"the elements of a head of {what} and its output must be contiguous")
-    return _HEADS(t.data_ptr(), out.data_ptr(), weight, ir, ih, orow, oh, t.shape[1])
+    return _HEADS(t.data_ptr(), out.data_ptr(), weight, ir, ih, orow, oh, shape[1])
 
 
 def _rotation(inv_freq, positions, rows, device, interleaved, scale):
@@ -117,8 +120,10 @@ def rope(x, inv_freq, positions, y, interleaved=False, scale=1.0, stream=None):
     code, device = _activations(x, "x")
     heads = _heads(x, y, 0, "x")
     rows, _, dim = x.shape
-    check(lib.q4k_rope(_stream_of(stream, device), device, heads, _rotation(inv_freq, positions, rows, device, interleaved, scale), rows, dim,
-                       code))
+    rc = _rope(_raw_stream(device) if stream is None else _stream_of(stream), device, heads,
+               _rotation(inv_freq, positions, rows, device, interleaved, scale), rows, dim, code)
+    if rc:
+        check(rc)
     return y
 
 
@@ -129,20 +134,22 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, q_out, k_out, in
     empty ``inv_freq`` norms only."""
     code, device = _activations(q, "q")
     rows, _, dim = q.shape
-    if k.dtype != q.dtype or k.get_device() != device or k.shape[0] != rows or k.shape[-1] != dim:
+    if k.dtype is not q.dtype or k.get_device() != device or k.shape[0] != rows or k.shape[-1] != dim:
         raise ValueError("q and k must share dtype, GPU, rows and head_dim")
     heads = _heads(q, q_out, _address(q_weight, torch.float32, dim, device, "q_weight"), "q")
     kv_heads = _heads(k, k_out, _address(k_weight, torch.float32, dim, device, "k_weight"), "k")
-    check(lib.q4k_qk_norm_rope(_stream_of(stream, device), device, heads, kv_heads,
-                               _rotation(inv_freq, positions, rows, device, interleaved, scale), rows, dim, eps, code))
+    rc = _qk_norm_rope(_raw_stream(device) if stream is None else _stream_of(stream), device, heads, kv_heads,
+                       _rotation(inv_freq, positions, rows, device, interleaved, scale), rows, dim, eps, code)
+    if rc:
+        check(rc)
     return q_out, k_out
 
 
 def _adapters(a, b, ids, ranks, scales, sequences, k, n, device):
     """A q4k_adapters of stacks a [slots, rank, k] and b [slots, n, rank]."""
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.shape[2] != k or b.shape[1] != n:
+    slots, rank, ak = a.shape
+    if ak != k or b.shape != (slots, n, rank):
         raise ValueError(f"adapters must be a [slots, rank, {k}] and b [slots, {n}, rank], got {tuple(a.shape)} and {tuple(b.shape)}")
-    slots, rank, _ = a.shape
     return _ADAPTERS(_address(a, torch.float16, 0, device, "a"), _address(b, torch.float16, 0, device, "b"),
                      _address(ids, torch.int32, sequences, device, "adapter_ids"), _address(ranks, torch.int32, slots, device, "ranks"),
                      _address(scales, torch.float32, slots, device, "scales"), slots, rank)
@@ -169,9 +176,11 @@ def lora(x, a, b, adapter_ids, count, output, auxiliary=None, query_counts=None,
     counts, sequences = _counts(query_counts, count)
     ad = _adapters(a, b, adapter_ids, ranks, scales, sequences, k, n, device)
     dtype = x.dtype
-    check(lib.q4k_lora(_stream_of(stream, device), device, ad, _address(x, dtype, count * k, device, "x"),
-                       _address(output, dtype, count * n, device, "output"), _address(auxiliary, dtype, count * n, device, "auxiliary"), count, k,
-                       n, counts, sequences, code))
+    rc = _lora(_raw_stream(device) if stream is None else _stream_of(stream), device, ad, _address(x, dtype, count * k, device, "x"),
+               _address(output, dtype, count * n, device, "output"), _address(auxiliary, dtype, count * n, device, "auxiliary"), count, k, n,
+               counts, sequences, code)
+    if rc:
+        check(rc)
     return output
 
 
@@ -179,15 +188,19 @@ def linear_lora(x, w, a, b, adapter_ids, count, output, auxiliary=None, gated=Fa
     """linear(x, w, ...) with the sequences' adapters added to the projection
     before its epilogue (arguments as linear's and lora's)."""
     code, device = _activations(x, "x")
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError("adapters must be a [slots, rank, k] and b [slots, n, rank]")
     if device != w.device:
         raise ValueError(f"x is on cuda:{device}, the weights on cuda:{w.device}")
     counts, sequences = _counts(query_counts, count)
     ad = _adapters(a, b, adapter_ids, ranks, scales, sequences, w.k, w.n, device)
     post = POST_GATE if gated else POST_ADD if auxiliary is not None else POST_STORE
     dtype = x.dtype
-    check(lib.q4k_linear_lora(_stream_of(stream, device), w.handle, ad, _address(x, dtype, count * w.k, device, "x"),
-                              _address(output, dtype, count * w.n, device, "output"),
-                              _address(auxiliary, dtype, count * w.n, device, "auxiliary"), count, counts, sequences, post, code))
+    rc = _linear_lora(_raw_stream(device) if stream is None else _stream_of(stream), w.handle, ad, _address(x, dtype, count * w.k, device, "x"),
+                      _address(output, dtype, count * w.n, device, "output"), _address(auxiliary, dtype, count * w.n, device, "auxiliary"),
+                      count, counts, sequences, post, code)
+    if rc:
+        check(rc)
     return output
 
 
@@ -209,7 +222,7 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
 
     Arguments left out leave their step out."""
     code, device = _activations(logits, "logits")
-    if logits.dim() != 2 or out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != device:
+    if logits.dim() != 2 or out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != device:
         raise ValueError("logits and out must be [rows, vocab] of one dtype on one GPU")
     rows, vocab = logits.shape
     in_stride, ie = logits.stride()
@@ -234,15 +247,23 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
         nmasks, words = mask.shape
         if mask.numel() == 0 and mask_rows is not None:  # no mask to take
             mask = mask_rows = None
-    params = _LOGITS(
-        _address(tokens, i32, 0, device, "tokens"), _address(slots, i32, rows, device, "slots"), _address(lengths, i32, rows, device, "lengths"),
-        _address(prompts, i32, rows, device, "prompts"), _address(repetition, f32, rows, device, "repetition"),
-        _address(frequency, f32, rows, device, "frequency"), _address(presence, f32, rows, device, "presence"),
-        _address(bias_offsets, i32, rows + 1, device, "bias_offsets"), _address(bias_tokens, i32, nbias, device, "bias_tokens"),
-        _address(bias_values, f32, nbias, device, "bias_values"), _address(mask, i32, 0, device, "mask"),
-        _address(mask_rows, i32, rows, device, "mask_rows"), nslots, capacity, nbias, nmasks, words)
-    check(lib.q4k_process_logits(_stream_of(stream, device), device, logits.data_ptr(), out.data_ptr(), rows, vocab, in_stride, out_stride,
-                                 params, code))
+    text = bias = (0, 0, 0)
+    given = (0, 0, 0, 0)
+    if tokens is not None or slots is not None or lengths is not None or prompts is not None:
+        given = (_address(tokens, i32, 0, device, "tokens"), _address(slots, i32, rows, device, "slots"),
+                 _address(lengths, i32, rows, device, "lengths"), _address(prompts, i32, rows, device, "prompts"))
+    if repetition is not None or frequency is not None or presence is not None:
+        text = (_address(repetition, f32, rows, device, "repetition"), _address(frequency, f32, rows, device, "frequency"),
+                _address(presence, f32, rows, device, "presence"))
+    if bias_offsets is not None or bias_tokens is not None or bias_values is not None:
+        bias = (_address(bias_offsets, i32, rows + 1, device, "bias_offsets"), _address(bias_tokens, i32, nbias, device, "bias_tokens"),
+                _address(bias_values, f32, nbias, device, "bias_values"))
+    params = _LOGITS(*given, *text, *bias, _address(mask, i32, 0, device, "mask"), _address(mask_rows, i32, rows, device, "mask_rows"), nslots,
+                     capacity, nbias, nmasks, words)
+    rc = _process_logits(_raw_stream(device) if stream is None else _stream_of(stream), device, logits.data_ptr(), out.data_ptr(), rows, vocab,
+                         in_stride, out_stride, params, code)
+    if rc:
+        check(rc)
     return out
 
 
