@@ -312,16 +312,22 @@ typedef struct q4k_adapters {
 /* y[m, n] = aux + scale * (x[m, k] A^T) B^T, row by row with the adapter of the
  * row's sequence (aux NULL: 0; aux may be y, which then keeps its bits in rows
  * without an adapter).  query_counts as for q4k_linear (NULL: one sequence);
- * k a multiple of 256, n of 16.  x, a and b are used as they are (x A^T sums
- * in fp32; fp32 x is not rounded), (x A^T) stays fp32, y is rounded once.
- * Elements of a and b past an adapter's rank are not used.  The sums of K-slices
- * live in the device's workspace. */
+ * k a multiple of 256, n of 16.  Products are exact and sums fp32; in batches
+ * beyond single rows fp32 x, and x A^T, enter them with 22 bits, scaled per row
+ * (values 2^-17 of a row's largest and below with an absolute error of 2^-40 of it).
+ * y is rounded once.  Elements of a and b past an adapter's rank are not used.
+ * The sums of K-slices live in the device's workspace (slices * m * rank floats,
+ * which the first projection's or adapter call's reservation holds up to 16 million of; single
+ * rows of few ranks need none). */
 int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m, uint32_t k, uint32_t n,
              const uint32_t* query_counts, uint32_t nqueries, uint32_t dtype);
 
 /* q4k_linear with adapters: y = post(x W^T + scale (x A^T) B^T, aux).  The
  * adapters' part is written first (post 0 and 1: into y with aux added, rounded to the
- * dtype; post 2: into a workspace buffer of m * n) and the projection adds to it. */
+ * dtype; post 2: into a workspace buffer of m * n) and the projection adds to it.  A
+ * call that needs more workspace while its stream captures fails with
+ * Q4K_ECAPTURE, as the projections' do (the adapters' launches may be enqueued by
+ * then). */
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);
 
