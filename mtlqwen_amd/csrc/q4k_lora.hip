@@ -13,9 +13,22 @@ constexpr int kLoraMaxSlices = 8;
 // sequence's adapter (-1: none) with its rank.
 struct LoraBlock {
   int row, rows, adapter, rank;
+  float scale;
 };
 
 __device__ __forceinline__ LoraBlock lora_block(const LoraArgs& a, int tile, int tile_rows) {
+  // Up to 64 slots: a wave reads all their ranks and scales while the sequence's
+  // adapter is on its way, not after it.
+  const int lane = threadIdx.x & 63;
+  const bool few = a.slots <= 64;
+  int ranks = a.r;
+  float scales = 1.0f;
+  if (few && lane < a.slots) {
+    if (a.ranks)
+      ranks = a.ranks[lane];
+    if (a.scales)
+      scales = a.scales[lane];
+  }
   // a.tile[q] = tiles before sequence q; constant indices, so that the tables
   // are read in one go.
   int q = 0, row = a.start[0], rows = a.count[0], first = 0;
@@ -30,10 +43,18 @@ __device__ __forceinline__ LoraBlock lora_block(const LoraArgs& a, int tile, int
   LoraBlock b;
   b.row = row + (tile - first) * tile_rows;
   b.rows = min(rows - (tile - first) * tile_rows, tile_rows);
-  b.adapter = a.ids[q];
+  b.adapter = __builtin_amdgcn_readfirstlane(a.ids[q]);
   if (b.adapter < 0 || b.adapter >= a.slots)
     b.adapter = -1;
-  b.rank = b.adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[b.adapter], 0), a.r) : a.r;
+  const int slot = max(b.adapter, 0);
+  if (few) {
+    b.rank = __builtin_amdgcn_readlane(ranks, slot);
+    b.scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scales), slot));
+  } else {
+    b.rank = a.ranks ? a.ranks[slot] : a.r;
+    b.scale = a.scales ? a.scales[slot] : 1.0f;
+  }
+  b.rank = b.adapter < 0 ? 0 : min(max(b.rank, 0), a.r);
   if (b.rank == 0)
     b.adapter = -1;
   return b;
@@ -398,8 +419,9 @@ __host__ __device__ inline size_t lora_ubytes(int rows, int r) {
 // The second launch: one workgroup per 16 a.rt rows of a sequence and a.span
 // columns.  2^a.glog lanes take one row of u, four ranks each (Q times), add the slices'
 // sums, low slices first, and split them.
-template <typename T, int NC>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && NC == 2 ? 3 : 4) void lora_expand_kernel(LoraArgs a) {
+// S slices at most; the loads of up to W rows per lane group are on their way together.
+template <typename T, int NC, int S>
+__global__ __launch_bounds__(256, S > 2 || (sizeof(T) == 4 && NC == 2) ? 3 : 4) void lora_expand_kernel(LoraArgs a) {
   extern __shared__ _Float16 lds[];
   const uint32_t outer = blockIdx.x / a.inner, inner = blockIdx.x - outer * a.inner;
   const uint32_t tile = a.by_rows ? outer : inner, piece = a.by_rows ? inner : outer;
@@ -416,50 +438,58 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && NC == 2 ? 3 : 4) void lora_e
   LoraColumns<T, NC, 4> cols(a, b, lane, min(start + a.span, a.n));
   cols.first(n0);
   if (b.adapter >= 0) {
-    constexpr int Q = NC == 3 ? 2 : 1;
-    const float scale = a.scales ? a.scales[b.adapter] : 1.0f;
-    const int q = tid & ((1 << a.glog) - 1), width = u.pad - 8;
-    for (int row = tid >> a.glog; row < ((b.rows + 15) & ~15); row += 256 >> a.glog) {
-      f4_t v[Q][kLoraMaxSlices];
+    constexpr int Q = NC == 3 ? 2 : 1, W = S > 2 ? 2 / Q : 4 / Q;
+    const float scale = b.scale;
+    const int q = tid & ((1 << a.glog) - 1), width = u.pad - 8, stride = 256 >> a.glog, rows16 = (b.rows + 15) & ~15;
+    for (int row0 = tid >> a.glog; row0 < rows16; row0 += W * stride) {
+      f4_t v[W][Q][S];
 #pragma unroll
-      for (int h = 0; h < Q; ++h)
+      for (int r = 0; r < W; ++r)
 #pragma unroll
-        for (int sl = 0; sl < kLoraMaxSlices; ++sl) {
+        for (int h = 0; h < Q; ++h)
+#pragma unroll
+          for (int sl = 0; sl < S; ++sl) {
+            const int row = row0 + r * stride, j = 4 * (q + (h << a.glog));
+            v[r][h][sl] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (row < b.rows && j < b.rank && sl < a.slices)
+              v[r][h][sl] = *reinterpret_cast<const f4_t*>(a.part + ((size_t)sl * a.m + b.row + row) * a.rpad + j);
+          }
+#pragma unroll
+      for (int r = 0; r < W; ++r) {
+        const int row = row0 + r * stride;
+        float m = 0.0f;
+#pragma unroll
+        for (int h = 0; h < Q; ++h) {
           const int j = 4 * (q + (h << a.glog));
-          v[h][sl] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-          if (row < b.rows && j < b.rank && sl < a.slices)
-            v[h][sl] = *reinterpret_cast<const f4_t*>(a.part + ((size_t)sl * a.m + b.row + row) * a.rpad + j);
+#pragma unroll
+          for (int sl = 1; sl < S; ++sl)
+            v[r][h][0] += v[r][h][sl];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[r][h][0][e] = j + e < b.rank ? v[r][h][0][e] * scale : 0.0f;
+            m = fmaxf(m, fabsf(v[r][h][0][e]));
+          }
         }
-      float m = 0.0f;
+        for (int off = (1 << a.glog) >> 1; off > 0; off >>= 1)
+          m = fmaxf(m, __shfl_xor(m, off));
+        float inverse;
+        const float up = split_scale(m, &inverse);
+        if (row >= rows16)
+          continue;
 #pragma unroll
-      for (int h = 0; h < Q; ++h) {
-        const int j = 4 * (q + (h << a.glog));
-#pragma unroll
-        for (int sl = 1; sl < kLoraMaxSlices; ++sl)
-          v[h][0] += v[h][sl];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[h][0][e] = j + e < b.rank ? v[h][0][e] * scale : 0.0f;
-          m = fmaxf(m, fabsf(v[h][0][e]));
+        for (int h = 0; h < Q; ++h) {
+          const int j = 4 * (q + (h << a.glog));
+          if (j < width) {
+            const float x[4] = {v[r][h][0][0], v[r][h][0][1], v[r][h][0][2], v[r][h][0][3]};
+            h4_t hi, lo;
+            split<4>(x, up, &hi, &lo);
+            *reinterpret_cast<h4_t*>(u.part[0] + row * u.pad + j) = hi;
+            *reinterpret_cast<h4_t*>(u.part[1] + row * u.pad + j) = lo;
+          }
         }
+        if (q == 0)
+          u.undo[row] = inverse;
       }
-      for (int off = (1 << a.glog) >> 1; off > 0; off >>= 1)
-        m = fmaxf(m, __shfl_xor(m, off));
-      float inverse;
-      const float up = split_scale(m, &inverse);
-#pragma unroll
-      for (int h = 0; h < Q; ++h) {
-        const int j = 4 * (q + (h << a.glog));
-        if (j < width) {
-          const float x[4] = {v[h][0][0], v[h][0][1], v[h][0][2], v[h][0][3]};
-          h4_t hi, lo;
-          split<4>(x, up, &hi, &lo);
-          *reinterpret_cast<h4_t*>(u.part[0] + row * u.pad + j) = hi;
-          *reinterpret_cast<h4_t*>(u.part[1] + row * u.pad + j) = lo;
-        }
-      }
-      if (q == 0)
-        u.undo[row] = inverse;
     }
     __syncthreads();
   }
@@ -518,7 +548,7 @@ __global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
   load(n);
   float v[ROWS][8];
   if (b.adapter >= 0) {
-    const float scale = a.scales ? a.scales[b.adapter] : 1.0f;
+    const float scale = b.scale;
     const T* x = static_cast<const T*>(a.x) + (size_t)b.row * a.k + 512 * wave + 8 * lane;
     const _Float16* w = a.a + (size_t)b.adapter * a.r * a.k + 512 * wave + 8 * lane;
     // Rounds of 8 ranks and 4096 k, the next one's ranks on their way.
@@ -663,6 +693,17 @@ hipError_t lora_shrink(hipStream_t s, LoraArgs a) {
   return dispatch(lora_shrink_kernel<T, 4, 2>, grid, block, s, a);
 }
 
+template <typename T, int S>
+hipError_t lora_expand_nc(hipStream_t s, const LoraArgs& a, dim3 grid, dim3 block, size_t lds) {
+  if (a.r <= 16)
+    return dispatch_lds(lora_expand_kernel<T, 0, S>, grid, block, lds, s, a);
+  if (a.r <= 32)
+    return dispatch_lds(lora_expand_kernel<T, 1, S>, grid, block, lds, s, a);
+  if (a.r <= 64)
+    return dispatch_lds(lora_expand_kernel<T, 2, S>, grid, block, lds, s, a);
+  return dispatch_lds(lora_expand_kernel<T, 3, S>, grid, block, lds, s, a);
+}
+
 template <typename T>
 hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   // Row tiles that share a load of B and u's sums: two where the sequences fill
@@ -690,13 +731,9 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   a.inner = a.by_rows ? cols : (uint32_t)tiles;
   const dim3 grid((uint32_t)tiles * cols), block(256);
   const size_t lds = lora_ubytes(16 * a.rt, a.r);
-  if (a.r <= 16)
-    return dispatch_lds(lora_expand_kernel<T, 0>, grid, block, lds, s, a);
-  if (a.r <= 32)
-    return dispatch_lds(lora_expand_kernel<T, 1>, grid, block, lds, s, a);
-  if (a.r <= 64)
-    return dispatch_lds(lora_expand_kernel<T, 2>, grid, block, lds, s, a);
-  return dispatch_lds(lora_expand_kernel<T, 3>, grid, block, lds, s, a);
+  if (a.slices <= 2)
+    return lora_expand_nc<T, 2>(s, a, grid, block, lds);
+  return lora_expand_nc<T, kLoraMaxSlices>(s, a, grid, block, lds);
 }
 
 }  // namespace

@@ -276,3 +276,13 @@ def test_pass_around_the_projections(q4k, oracle, gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(qkv, eager[0]) and torch.equal(logits, eager[1])
+
+
+@pytest.mark.parametrize("slots", [1, 63, 64, 65, 200])
+def test_lora_many_slots(q4k, gpu, slots):
+    """Stacks on both sides of the 64 slots whose ranks one wave reads at once,
+    the last slot in use, in every form (one launch, two)."""
+    rng = np.random.default_rng(slots)
+    for counts, r in (([1, 1], 8), ([1, 20], 24)):
+        ranks = [int(v) for v in rng.integers(1, r + 1, slots)]
+        _check(q4k, gpu, counts, [slots - 1, slots // 2], 256, 48, r, F32, slots=slots, ranks=ranks)
