@@ -231,7 +231,11 @@ __device__ __forceinline__ float sum_waves(const float* p, int stride) {
 }
 
 // K in slices: one workgroup per 16 rows, slice and 16 NT ranks; its eight waves
-// take a part of the slice each and add their sums in LDS.
+// take a part of the slice each and add their sums in LDS.  A is read once per 16
+// rows, from the L2.  8 rows of 8 sequences, rank 16, k = 4096: 3.6 us, launch
+// included; 2048 fp32 rows of rank 64: 19.6 us (x alone would take 6.7 at the rate
+// of a copy; sharing A between 64 rows through LDS, four slices of it on their way,
+// took 16.5 and 4.7 for adding twice the slices, and more for fewer rows).
 template <typename T, int NT, int SEG>
 __global__ __launch_bounds__(512, 4) void lora_shrink_kernel(LoraArgs a) {
   constexpr int kSums = NT * 256, kWaves = 8;
@@ -271,7 +275,10 @@ __global__ __launch_bounds__(512, 4) void lora_shrink_kernel(LoraArgs a) {
 // high part, 2, 3 the low, B given twice); NC = 1, 2: up to 32 NC ranks; NC = 3:
 // any number, B read anew for each row tile.  A wave takes every WAVES-th step of
 // the workgroup's columns; the loads of its first B and aux are on their way
-// before u is there, those of the next aux before its products.
+// before u is there, those of the next aux before its products.  2048 fp32 rows of
+// 12288, rank 64, with aux: 47.5 us, 4.2 TB/s of aux and y (a copy reaches 5.05); 333
+// ragged fp16 rows of 6144: 9.7 us, most of it the chain of loads from the
+// sequence's id to the sums and B.
 // ----------------------------------------------------------------------------
 struct LoraU {
   _Float16* part[2];  // [16 rt][pad] each
@@ -279,7 +286,7 @@ struct LoraU {
   int pad;
 };
 
-template <typename T, int NC, int WAVES>
+template <typename T, int NC, int WAVES, bool PAST>
 struct LoraColumns {
   static constexpr int kChunks = NC == 0 ? 1 : NC == 3 ? 1 : NC, P = 4;
   typedef T vec_t __attribute__((ext_vector_type(P), aligned(sizeof(T))));
@@ -324,7 +331,13 @@ struct LoraColumns {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         if (16 * t + 4 * g + c < b.rows)
-          x[c] = __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(static_cast<const T*>(a.aux) + at(n0, t, c)));
+          {
+            const vec_t* from = reinterpret_cast<const vec_t*>(static_cast<const T*>(a.aux) + at(n0, t, c));
+            if constexpr (PAST)
+              x[c] = __builtin_nontemporal_load(from);
+            else
+              x[c] = *from;
+          }
   }
 
   __device__ __forceinline__ void first(int n0) {
@@ -398,8 +411,13 @@ struct LoraColumns {
         if (n0 + P * i < a.n)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            if (16 * t + 4 * g + c < b.rows)
-              __builtin_nontemporal_store(y[c], reinterpret_cast<vec_t*>(static_cast<T*>(a.y) + at(n0, t, c)));
+            if (16 * t + 4 * g + c < b.rows) {
+              vec_t* to = reinterpret_cast<vec_t*>(static_cast<T*>(a.y) + at(n0, t, c));
+              if constexpr (PAST)
+                __builtin_nontemporal_store(y[c], to);
+              else
+                *to = y[c];
+            }
       }
       n0 += 16 * P * WAVES;
     }
@@ -435,7 +453,7 @@ __global__ __launch_bounds__(256, S > 2 || (sizeof(T) == 4 && NC == 2) ? 3 : 4) 
   u.part[0] = lds;
   u.part[1] = lds + 16 * a.rt * u.pad;
   u.undo = reinterpret_cast<float*>(lds + 32 * a.rt * u.pad);
-  LoraColumns<T, NC, 4> cols(a, b, lane, min(start + a.span, a.n));
+  LoraColumns<T, NC, 4, S <= 2> cols(a, b, lane, min(start + a.span, a.n));
   cols.first(n0);
   if (b.adapter >= 0) {
     constexpr int Q = NC == 3 ? 2 : 1, W = S > 2 ? 2 / Q : 4 / Q;
@@ -512,7 +530,9 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // forms u of its sequence's rows itself, on the vector units in fp32 (a wave
 // takes 512 k of one rank row in one contiguous load, 8 k per lane), and writes
 // a.span columns: 1 << a.glog lanes share a column's ranks, 8 each.  A second
-// launch would cost the caller more than reading A once per workgroup costs the L2.
+// launch would cost the caller more than reading A once per workgroup costs the L2:
+// 8 sequences of one fp16 row, rank 16, 4096 -> 12288: 5.9 us replayed and 6.7 a
+// call, in two launches 7.3 and 9.6; what bounds it is latency (launch, id, A, sum, B).
 // ----------------------------------------------------------------------------
 template <typename T, int ROWS>
 __global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
@@ -731,6 +751,9 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   a.inner = a.by_rows ? cols : (uint32_t)tiles;
   const dim3 grid((uint32_t)tiles * cols), block(256);
   const size_t lds = lora_ubytes(16 * a.rt, a.r);
+  // Batches of so many rows also write past the caches, which their output
+  // outgrows, and read aux past them (2048 rows, fp32: 79.9 -> 75.0 us); smaller
+  // outputs stay for the projection that adds to them.
   if (a.slices <= 2)
     return lora_expand_nc<T, 2>(s, a, grid, block, lds);
   return lora_expand_nc<T, kLoraMaxSlices>(s, a, grid, block, lds);
