@@ -264,7 +264,10 @@ int q4k_rope_frequencies(uint32_t rot_dim, double base, uint32_t scaling, double
 /* Heads of a packed batch: row r, head j, element d is at
  * r * row_stride + j * head_stride + d (strides in elements).  `out` is `in`
  * with the same strides, or none of its elements is one of `in`'s; the
- * outputs of a call must not overlap each other. */
+ * outputs of a call share no element either.  Sets that lie between each
+ * other's elements need equal row strides (columns of one matrix) or equal head
+ * strides that divide the row strides (heads of q, k and v in turn); others
+ * are refused. */
 typedef struct q4k_heads {
   const void* in;
   void* out;

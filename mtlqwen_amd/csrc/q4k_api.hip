@@ -1741,16 +1741,18 @@ struct DeviceScope {
   }
 };
 
-// The elements of a set of heads as two nested runs: `inner` contiguous values
-// from the base on, repeated `count` times every `step` values (the outer of
-// rows and heads).  False if two of its elements share a place, or a stride is
-// negative.
+// The elements of a set of heads: runs of `run` contiguous values, repeated
+// `inner` times every `inner_step` and all that `outer` times every `outer_step`
+// (the larger of the strides of rows and heads; bytes throughout).
 struct HeadSpan {
   uintptr_t base = 0;
-  uint64_t inner = 0, step = 0, count = 0;  // bytes, bytes, repetitions
-  uint64_t extent() const { return count ? (count - 1) * step + inner : 0; }
+  uint64_t run = 0, inner_step = 0, inner = 0, outer_step = 0, outer = 0;
+  uint64_t width() const { return inner ? (inner - 1) * inner_step + run : 0; }
+  uint64_t extent() const { return outer ? (outer - 1) * outer_step + width() : 0; }
 };
 
+// False if two of the elements share a place (or are not told apart: strides
+// that do not nest).
 bool head_span(const void* p, int64_t row_stride, int64_t head_stride, uint32_t rows, uint32_t heads, uint32_t dim, size_t es, HeadSpan* span) {
   uint64_t s[2] = {(uint64_t)row_stride, (uint64_t)head_stride}, c[2] = {rows, heads};
   if (c[0] <= 1)
@@ -1759,23 +1761,34 @@ bool head_span(const void* p, int64_t row_stride, int64_t head_stride, uint32_t 
     s[1] = 0;
   const int outer = c[1] <= 1 || (c[0] > 1 && s[0] >= s[1]) ? 0 : 1, in = 1 - outer;
   const bool apart = (c[in] <= 1 || s[in] >= dim) && (c[outer] <= 1 || s[outer] >= (c[in] - 1) * s[in] + dim);
-  span->base = (uintptr_t)p;
-  span->inner = ((c[in] - 1) * s[in] + dim) * es;
-  span->step = s[outer] * es;
-  span->count = c[outer];
+  *span = {(uintptr_t)p, dim * es, s[in] * es, c[in], s[outer] * es, c[outer]};
   return apart;
 }
 
-// Whether two sets may share an element: their runs are taken as solid, and
-// sets of one step (columns of one matrix) are compared within the step.
+// Whether a run of `na` bytes from a on and one of `nb` from b on, each repeated
+// every `step` bytes, never share a byte.
+bool repeats_apart(uintptr_t a, uint64_t na, uintptr_t b, uint64_t nb, uint64_t step) {
+  if (step == 0 || na > step || nb > step)
+    return false;
+  const uint64_t d = b >= a ? (b - a) % step : (step - (a - b) % step) % step;
+  return d >= na && d + nb <= step;
+}
+
+// Whether two sets may share an element.  They do not if their extents do not,
+// or if they have one outer step and lie in different parts of it (columns of
+// one matrix), or one inner step, which the outer ones are multiples of, and
+// lie in different parts of that (heads of queries and keys in turn).
 bool spans_meet(const HeadSpan& a, const HeadSpan& b) {
   if (!overlaps(reinterpret_cast<const void*>(a.base), a.extent(), reinterpret_cast<const void*>(b.base), b.extent()))
     return false;
-  const uint64_t step = a.count > 1 ? a.step : b.step;
-  if (step == 0 || (a.count > 1 && b.count > 1 && a.step != b.step) || a.inner > step || b.inner > step)
+  if (a.outer <= 1 || b.outer <= 1 || a.outer_step == b.outer_step)
+    if (repeats_apart(a.base, a.width(), b.base, b.width(), a.outer > 1 ? a.outer_step : b.outer_step))
+      return false;
+  const uint64_t step = a.inner > 1 ? a.inner_step : b.inner_step;
+  if (step == 0 || (a.inner > 1 && b.inner > 1 && a.inner_step != b.inner_step) || (a.outer > 1 && a.outer_step % step) ||
+      (b.outer > 1 && b.outer_step % step))
     return true;
-  const uint64_t d = b.base >= a.base ? (b.base - a.base) % step : (step - (a.base - b.base) % step) % step;
-  return d < a.inner || d + b.inner > step;
+  return !repeats_apart(a.base, a.run, b.base, b.run, step);
 }
 
 int check_heads(const char* what, const q4k_heads* h, uint32_t rows, uint32_t dim, size_t es, HeadSpan* in, HeadSpan* out) {

@@ -116,6 +116,27 @@ def test_heads_in_place_and_strided(q4k, gpu, dtype, norm):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_qk_heads_in_turn(q4k, gpu, rows, dtype):
+    """q, k and v heads in turn in the rows of one projection, in place and
+    into one buffer of the same form: the bits of separate tensors, v as it was."""
+    rng = np.random.default_rng(31)
+    qkv = _x(rng, rows, 6, 3, 64, dtype=dtype).to(gpu)
+    f, p = _freq(64).to(gpu), torch.arange(5, 5 + rows, dtype=torch.int32, device=gpu)
+    wq, wk = (torch.from_numpy(rng.uniform(0.5, 1.5, 64).astype(np.float32)).to(gpu) for _ in range(2))
+    q, k = qkv[:, :, 0].contiguous(), qkv[:, :, 1].contiguous()
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    q4k.qk_norm_rope(q, k, wq, wk, f, p, qo, ko)
+    other = torch.full_like(qkv, 7.0)
+    q4k.qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], wq, wk, f, p, other[:, :, 0], other[:, :, 1])
+    got = qkv.clone()
+    q4k.qk_norm_rope(got[:, :, 0], got[:, :, 1], wq, wk, f, p, got[:, :, 0], got[:, :, 1])
+    torch.cuda.synchronize()
+    for t, v in ((got, qkv[:, :, 2]), (other, torch.full_like(q, 7.0))):
+        assert torch.equal(t[:, :, 0], qo) and torch.equal(t[:, :, 1], ko) and torch.equal(t[:, :, 2], v)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("dim,rot,inter", [(128, 128, False), (256, 64, False), (64, 64, True), (80, 20, False), (96, 96, True), (112, 28, True),
                                           (65, 64, False), (128, 0, False), (1024, 1024, False), (7, 6, True), (576, 64, False), (1, 0, False)])
 def test_qk_norm_rope(q4k, gpu, dim, rot, inter, dtype):

@@ -89,6 +89,21 @@ def test_qk_refusals(q4k, a, b, kw, code):
     assert qk(q4k, a, b, rotation(), **kw) == code
 
 
+# q, k and v heads in turn: [rows, 4 heads, q k v, 128].
+TURNS = (1536, 384, 1536, 384)
+T1 = 128 * 4
+
+
+@pytest.mark.parametrize("a,b", [
+    (heads(o=X, strides=TURNS, n=4), heads(i=X + T1, o=X + T1 + 4, strides=TURNS, n=4)),  # k moves by one element
+    (heads(o=X, strides=TURNS, n=4), heads(i=X + T1, o=X + T1 - 4, strides=TURNS, n=4)),  # into q
+    (heads(o=X, strides=TURNS, n=4), heads(i=X + T1, o=X + T1, strides=(1600, 384, 1600, 384), n=4)),  # rows out of turn
+    (heads(o=X, strides=TURNS, n=4), heads(i=X + T1, o=X + T1, strides=(1536, 256, 1536, 256), n=4)),  # heads out of turn
+])
+def test_qk_in_turn_refusals(q4k, a, b):
+    assert qk(q4k, a, b, rotation()) == EALIAS
+
+
 def test_frequencies():
     rot, base, factor, ctx = 64, 10000.0, 8.0, 4096
     i = np.arange(rot // 2)
