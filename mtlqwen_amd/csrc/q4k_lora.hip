@@ -729,9 +729,10 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   // Row tiles that share a load of B and u's sums: two where the sequences fill
   // them (64 rows of one sequence, 4096 -> 12288, rank 64, fp16: 11.4 us, with four
   // 14.8), four where that still leaves four workgroups per CU (2048 rows, fp32: 60.5 us, with
-  // two 72.5); one for ranks beyond 256, whose parts fill the LDS.
+  // two 72.5) and u's parts take 64 KB at most, two workgroups to a CU's LDS (ranks up to
+  // 224); one for ranks beyond 256.
   const int64_t blocks = (int64_t)(a.m / 64) * ((a.n + 255) / 256);
-  a.rt = a.r > 256 || a.m < 32 * a.nq ? 1 : a.m >= 64 * a.nq && blocks >= 4 * (int64_t)cus ? 4 : 2;
+  a.rt = a.r > 256 || a.m < 32 * a.nq ? 1 : a.m >= 64 * a.nq && blocks >= 4 * (int64_t)cus && lora_ubytes(64, a.r) <= 65536 ? 4 : 2;
   const int tiles = lora_lay_tiles(a, 16 * a.rt);
   // Columns of a workgroup: at least four workgroups per CU.
   int steps = (int)(((int64_t)tiles * ((a.n + 255) / 256)) / (4 * (int64_t)cus));

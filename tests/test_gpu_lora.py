@@ -74,6 +74,14 @@ def test_lora_ranks(q4k, gpu, r, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("r", [128, 224, 225, 256, 257])
+def test_lora_large_ranks_of_many_rows(q4k, gpu, r, dtype):
+    """Enough rows and columns for the largest row tiles, at the ranks where
+    their shared memory decides."""
+    _check(q4k, gpu, [700, 868], [1, 0], 256, 12288, r, dtype, slots=2)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("ranks", [[1, 4, 20], [0, 20, 7], [20, 19, 18], [-5, 21, 3], [16, 1, 2**31 - 1]])
 def test_lora_mixed_ranks(q4k, gpu, ranks, dtype):
     """Ranks of 0 (and below) are no adapter, above the stack's all of it."""
