@@ -229,12 +229,16 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
     out_stride, oe = out.stride()
     if vocab > 1 and (ie != 1 or oe != 1):
         raise ValueError("the rows of logits and out must be contiguous")
+    if rows == 0:
+        return out
     nslots = capacity = nbias = nmasks = words = 0
     i32, f32 = torch.int32, torch.float32
     if tokens is not None:
         if tokens.dim() != 2:
             raise ValueError("tokens must be [slots, capacity]")
         nslots, capacity = tokens.shape
+        if nslots < rows and slots is None:
+            raise ValueError(f"without slots every row needs a text ({rows} rows, {nslots} texts)")
         if tokens.numel() == 0:  # a buffer of no tokens: every text is empty
             tokens = slots = lengths = prompts = repetition = frequency = presence = None
     if bias_tokens is not None and bias_values is not None:
@@ -245,7 +249,10 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
         if mask.dim() != 2:
             raise ValueError("mask must be [masks, words]")
         nmasks, words = mask.shape
-        if mask.numel() == 0 and mask_rows is not None:  # no mask to take
+        if words < (vocab + 31) // 32 or (nmasks < rows and mask_rows is None):
+            raise ValueError(f"a mask of {vocab} tokens needs {(vocab + 31) // 32} words a row, and without mask_rows every row a mask "
+                             f"(got {nmasks} masks of {words} for {rows} rows)")
+        if nmasks == 0:  # no mask to take
             mask = mask_rows = None
     text = bias = (0, 0, 0)
     given = (0, 0, 0, 0)

@@ -210,6 +210,22 @@ def test_empty_groups(q4k, gpu):
         q4k.process_logits(x, out, repetition=torch.ones(2, device=gpu))
 
 
+def test_masks_and_texts_too_few(q4k, gpu):
+    """Descriptions with nothing in them are refused where rows would need
+    them, never taken for a step left out; no rows need none."""
+    x = torch.randn((2, 50), device=gpu)
+    out = torch.empty_like(x)
+    none = torch.zeros(0, dtype=torch.int32, device=gpu)
+    rows = torch.zeros(2, dtype=torch.int32, device=gpu)
+    for bad in [{"mask": none.view(0, 2)}, {"mask": none.view(2, 0)}, {"mask": none.view(2, 0), "mask_rows": rows},
+                {"mask": rows.view(2, 1)}, {"mask": rows.view(1, 2)}, {"tokens": none.view(0, 5), "lengths": rows},
+                {"tokens": rows.view(1, 2), "lengths": rows}]:
+        with pytest.raises(ValueError):
+            q4k.process_logits(x, out, **bad)
+    got = q4k.process_logits(x[:0], out[:0], tokens=rows.view(1, 2), lengths=none, repetition=none.float(), mask=rows.view(1, 2), mask_rows=none)
+    assert got.shape == (0, 50)
+
+
 def test_captured_call_follows_its_descriptions(q4k, gpu):
     rng = np.random.default_rng(8)
     b = _batch(rng, 4, 5000, 200, 5, 10, 3, F32)
