@@ -1857,8 +1857,6 @@ int run_heads(void* stream, int device, const q4k_heads* sets, int nsets, const 
   }
   HeadsArgs a;
   for (int i = 0; i < nsets; ++i) {
-    a.in[i] = sets[i].in;
-    a.out[i] = sets[i].out;
     a.w[i] = sets[i].weight;
     a.heads[i] = sets[i].heads;
     a.row_in[i] = sets[i].in_row_stride;
@@ -1867,8 +1865,6 @@ int run_heads(void* stream, int device, const q4k_heads* sets, int nsets, const 
     a.head_out[i] = sets[i].out_head_stride;
   }
   a.inv_freq = rot->inv_freq;
-  a.positions = rot->positions;
-  a.rows = rows;
   a.dim = (int)dim;
   a.rot = (int)rot->rot_dim;
   a.scale = rot->scale;
@@ -1876,9 +1872,19 @@ int run_heads(void* stream, int device, const q4k_heads* sets, int nsets, const 
   DeviceScope scope(device);
   if (scope.rc)
     return scope.rc;
-  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
-  Q4K_TRY_HIP(launch_heads(static_cast<hipStream_t>(stream), a, norm, rot->layout == Q4K_ROPE_INTERLEAVED, (int)dtype, device_cus(device)),
-              "head rotation launch");
+  // A launch holds less than 2^32 threads: 2^24 workgroups, of one row or more.
+  constexpr uint32_t kRows = 1u << 23;
+  for (uint32_t row = 0; row < rows; row += kRows) {
+    for (int i = 0; i < nsets; ++i) {
+      a.in[i] = static_cast<const uint8_t*>(sets[i].in) + (size_t)row * sets[i].in_row_stride * es;
+      a.out[i] = static_cast<uint8_t*>(sets[i].out) + (size_t)row * sets[i].out_row_stride * es;
+    }
+    a.positions = rot->positions ? rot->positions + row : nullptr;
+    a.rows = rows - row < kRows ? rows - row : kRows;
+    LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_heads(static_cast<hipStream_t>(stream), a, norm, rot->layout == Q4K_ROPE_INTERLEAVED, (int)dtype, device_cus(device)),
+                "head rotation launch");
+  }
   return Q4K_OK;
 }
 

@@ -58,6 +58,24 @@ def test_rope_many_rows(q4k, gpu, rows, heads, dim, rot, dtype):
     _check_rope(q4k, gpu, rows, heads, dim, rot, False, dtype, np.arange(rows) + 100000, scale=1.2)
 
 
+def test_heads_of_millions_of_rows(q4k, gpu):
+    """More rows than one launch takes: around its end, and at both ends, the
+    bits of calls on those rows alone."""
+    rows, f = (1 << 23) + 70, _freq(2).to(gpu)
+    x = torch.randn((rows, 2, 2), device=gpu).half()
+    p = torch.arange(rows, dtype=torch.int32, device=gpu)
+    w = torch.tensor([0.5, 2.0], device=gpu)
+    y, q, k = torch.empty_like(x), torch.empty_like(x)[:, :1], torch.empty_like(x)[:, :1]
+    q4k.rope(x, f, p, y)
+    q4k.qk_norm_rope(x[:, :1], x[:, 1:], w, w, f, p, q, k)
+    for part in (slice(0, 100), slice((1 << 23) - 50, (1 << 23) + 50), slice(rows - 30, rows)):
+        want, wq, wk = torch.empty_like(x[part]), torch.empty_like(q[part]), torch.empty_like(k[part])
+        q4k.rope(x[part], f, p[part], want)
+        q4k.qk_norm_rope(x[part, :1], x[part, 1:], w, w, f, p[part], wq, wk)
+        torch.cuda.synchronize()
+        assert torch.equal(y[part], want) and torch.equal(q[part], wq) and torch.equal(k[part], wk)
+
+
 def test_rope_far_and_negative_positions(q4k, gpu):
     _check_rope(q4k, gpu, 7, 3, 128, 128, False, F32, [2**31 - 1, -(2**31), 2**30 + 7, -1, 0, 1 << 24, 12345678], far=True)
     # Up to 2^20 the near bound holds.
