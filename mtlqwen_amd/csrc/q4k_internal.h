@@ -580,8 +580,9 @@ struct LogitsArgs {
   const uint32_t* mask = nullptr;  // [nmasks, mask_stride] words or nullptr
   const int32_t* mask_rows = nullptr;  // [rows] or nullptr: row r takes mask r
   uint32_t rows = 0, vocab = 0, nslots = 0, capacity = 0, nbias = 0, nmasks = 0, mask_stride = 0;
-  uint32_t stagger = 1;
-  uint32_t count_bits = 0;  // set by the launch: the bits that hold a count of up to `capacity`
+  // Set by the launch: the workgroups of a round of the CUs, and the bits that
+  // hold a count of up to `capacity`.
+  uint32_t stagger = 1, count_bits = 0;
 };
 hipError_t launch_logits(hipStream_t s, LogitsArgs a, int dtype, int cus);
 

@@ -14,21 +14,21 @@ namespace {
 //   out = masked ? -inf : l3
 //
 // One read and one write of the row, bound by memory: 64 rows of 248320 fp32 take
-// 19.1 us with nothing else to do (6.7 TB/s, the inputs in the memory-side cache), 36.2
-// with texts of 32768 to 65536 tokens, 300 biases and masks, whose counting
-// overlaps the copy in part.  A workgroup owns
-// THREADS * E consecutive tokens, held in registers while it counts, in LDS,
-// those of the row's text and biases that fall into its range.  One word per
-// token: bit 31 = seen in the prompt; below it 31 - s bits with the number of the last
-// bias entry (0: none); s low bits with c, s enough for the token buffer's
-// capacity.  Integer counts and maxima, so the order of the atomics does not
-// matter, and no count of the whole vocabulary is cleared, written or read.  A
-// row of more biases than fit into 31 - s bits takes a second round through the
-// words.  Workgroups of every other round of the CUs read their logits after
-// the text, so that not all of them leave the memory idle while they count (the case
-// above: 46.9 -> 45.6 us when it took that long).  The text is read once per workgroup; the workgroups of a row sit
-// a multiple of the row count apart, with 8 rows and their multiples on one
-// XCD, whose L2 then serves every reading after the first.
+// 19.1 us with nothing else to do (6.7 TB/s, the inputs in the memory-side
+// cache), 36.2 with texts of 32768 to 65536 tokens, 300 biases and masks, whose
+// counting overlaps the copy in part.  A workgroup owns THREADS * E consecutive
+// tokens, held in registers while it counts, in LDS, those of the row's text and
+// biases that fall into its range.  One word per token: bit 31 = seen in the
+// prompt; below it 31 - s bits with the number of the last bias entry (0: none);
+// s low bits with c, s enough for the token buffer's capacity.  Integer counts
+// and maxima, so the order of the atomics does not matter, and no count of the
+// whole vocabulary is cleared, written or read.  A row of more biases than fit
+// into 31 - s bits takes a second round through the words.  Workgroups of every
+// other round of the CUs read their logits after the text, so that not all of
+// them leave the memory idle while they count (the case above: 46.9 -> 45.6 us
+// when it took that long).  The text is read once per workgroup; the workgroups
+// of a row sit a multiple of the row count apart, with 8 rows and their multiples
+// on one XCD, whose L2 then serves every reading after the first.
 // ----------------------------------------------------------------------------
 typedef int32_t i4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 

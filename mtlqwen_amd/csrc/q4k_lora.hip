@@ -330,14 +330,13 @@ struct LoraColumns {
     if (a.aux && n0 + P * i < a.n)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (16 * t + 4 * g + c < b.rows)
-          {
-            const vec_t* from = reinterpret_cast<const vec_t*>(static_cast<const T*>(a.aux) + at(n0, t, c));
-            if constexpr (PAST)
-              x[c] = __builtin_nontemporal_load(from);
-            else
-              x[c] = *from;
-          }
+        if (16 * t + 4 * g + c < b.rows) {
+          const vec_t* from = reinterpret_cast<const vec_t*>(static_cast<const T*>(a.aux) + at(n0, t, c));
+          if constexpr (PAST)
+            x[c] = __builtin_nontemporal_load(from);
+          else
+            x[c] = *from;
+        }
   }
 
   __device__ __forceinline__ void first(int n0) {
