@@ -328,9 +328,8 @@ int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void*
 /* q4k_linear with adapters: y = post(x W^T + scale (x A^T) B^T, aux).  The
  * adapters' part is written first (post 0 and 1: into y with aux added, rounded to the
  * dtype; post 2: into a workspace buffer of m * n) and the projection adds to it.  A
- * call that needs more workspace while its stream captures fails with
- * Q4K_ECAPTURE, as the projections' do (the adapters' launches may be enqueued by
- * then). */
+ * call that needs more workspace than there is (Q4K_ENOMEM, or Q4K_ECAPTURE while
+ * its stream captures) enqueues nothing and leaves y as it was. */
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);
 

@@ -91,6 +91,15 @@ struct Workspace {
   // that needs more fails (ensure_buffer).
   bool fixed = false;
   bool reserved = false;  // reserve_workspace has run
+  // While set, a projection grows its buffers and launches nothing (SizingScope):
+  // every path takes all its buffers before its first launch.
+  bool sizing = false;
+};
+
+struct SizingScope {
+  Workspace& ws;
+  explicit SizingScope(Workspace& w) : ws(w) { ws.sizing = true; }
+  ~SizingScope() { ws.sizing = false; }
 };
 
 Workspace g_ws[64];
@@ -475,7 +484,7 @@ int gemm2_split_buffers(hipStream_t stream, Workspace& ws, int device, GemmArgs&
 int stage_pack(hipStream_t stream, Workspace& ws, int device, const void* x, uint32_t dtype, uint32_t m, uint32_t k, DecodePack* pk) {
   const size_t nb = k / 256;
   int rc = ensure_buffer(stream, ws, device, ws.pack, ws.pack_bytes, nb * kPackBytesPerBlock, "decode pack");
-  if (rc)
+  if (rc || ws.sizing)
     return rc;
   pk->frag = reinterpret_cast<u4_t*>(ws.pack);
   pk->xs = reinterpret_cast<h4_t*>(ws.pack + nb * 8 * 64 * 16);
@@ -533,13 +542,13 @@ int set_device(int device) {
 }
 
 // A prefill GEMM of the middle row counts (mid_plan): x staged as for the
-// other GEMMs, the K-slices' sums in the split-K workspace.
+// other GEMMs, the K-slices' sums in the split-K workspace (mid_buffers, before
+// the staging).
+int mid_buffers(hipStream_t stream, Workspace& ws, int device, const MidPlan& plan) {
+  return plan.slices > 1 ? ensure_buffer(stream, ws, device, ws.part, ws.part_elems, plan.part_floats, "split-K workspace") : Q4K_OK;
+}
+
 int run_mid(hipStream_t stream, Workspace& ws, q4k_weight* w, const GemmArgs& g, uint32_t dtype, const MidPlan& plan, bool gated) {
-  if (plan.slices > 1) {
-    int rc = ensure_buffer(stream, ws, w->device, ws.part, ws.part_elems, plan.part_floats, "split-K workspace");
-    if (rc)
-      return rc;
-  }
   MidArgs a;
   a.w = g.w;
   a.wu = g.wu;
@@ -577,8 +586,11 @@ constexpr uint32_t kTypedGemmRows = 64;
 int run_typed_gemm_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, const void* x, void* y, const void* aux, uint32_t m, uint32_t post,
                           uint32_t dtype, const float* norm_w, float eps) {
   const size_t rows = (size_t)gemm2_rows((int)m);
+  const MidPlan mid = mid_plan((int)m, (int)w->n, (int)(w->k / 256), device_cus(w->device));
   int rc = ensure_workspace(stream, ws, w->device, rows * w->k, rows);
-  if (rc)
+  if (!rc)
+    rc = mid_buffers(stream, ws, w->device, mid);
+  if (rc || ws.sizing)
     return rc;
   {
     LaunchTimer timer(stream, Q4K_KERNEL_STAGE);
@@ -595,7 +607,6 @@ int run_typed_gemm_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, cons
   a.k = (int)w->k;
   a.nb = (int)(w->k / 256);
   a.post = (int)post;
-  const MidPlan mid = mid_plan(a.m, a.n, a.nb, device_cus(w->device));
   if (mid.rt)
     return run_mid(stream, ws, w, a, dtype, mid, false);
   LaunchTimer timer(stream, Q4K_KERNEL_GEMM);
@@ -613,7 +624,7 @@ int prenorm(hipStream_t stream, Workspace& ws, int device, const void*& x, const
     return Q4K_OK;
   const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2;
   int rc = ensure_buffer(stream, ws, device, ws.normed, ws.normed_bytes, (size_t)m * k * es, "normalised-activation buffer");
-  if (rc)
+  if (rc || ws.sizing)
     return rc;
   LaunchTimer timer(stream, Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_rms_norm(stream, x, norm_w, ws.normed, (int)m, (int)k, eps, (int)dtype, nullptr), "rms_norm launch");
@@ -633,7 +644,7 @@ int run_gemv_groups_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, con
     const void* xg = static_cast<const uint8_t*>(x) + (size_t)r0 * w->k * es;
     GemvArgs a{};
     int rc = stage_pack(stream, ws, w->device, xg, dtype, mg, w->k, &a.pack);
-    if (rc)
+    if (rc || ws.sizing)
       return rc;
     a.w = w->data;
     a.x = xg;
@@ -679,7 +690,7 @@ int run_rows_gemm_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_w
   int rc = ensure_workspace(stream, ws, w->device, rows_gemm_halves(w->k), 64);
   if (!rc && part)
     rc = ensure_buffer(stream, ws, w->device, ws.part, ws.part_elems, part, "split-K workspace");
-  if (rc)
+  if (rc || ws.sizing)
     return rc;
   _Float16* const xs = ws.x + (size_t)128 * w->k;
   {
@@ -722,8 +733,10 @@ bool rows_gemm_takes(const q4k_weight* w, bool gated, uint32_t m, bool norm) {
 
 // Up to 8 rows with K = 4096, plain or (wu) a gate/up pair of one type: one
 // launch that packs (and normalises) x itself.
-int run_decode_gemv(hipStream_t stream, q4k_weight* w, q4k_weight* wu, const void* x, void* y, const void* aux, uint32_t m, uint32_t post,
+int run_decode_gemv(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weight* wu, const void* x, void* y, const void* aux, uint32_t m, uint32_t post,
                     uint32_t dtype, const float* norm_w, float eps) {
+  if (ws.sizing)  // no buffer of the workspace
+    return Q4K_OK;
   GemvArgs a{};
   a.w = w->data;
   a.wu = wu ? wu->data : nullptr;
@@ -753,7 +766,7 @@ int run_typed_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, const voi
   if (rows_gemm_takes(w, false, m, norm_w != nullptr))
     return run_rows_gemm_locked(stream, ws, w, nullptr, x, y, aux, m, post, dtype, norm_w, eps);
   if (decode_gemv_supported((int)m, (int)(w->k / 256), (int)w->n, false, device_cus(w->device)))
-    return run_decode_gemv(stream, w, nullptr, x, y, aux, m, post, dtype, norm_w, eps);
+    return run_decode_gemv(stream, ws, w, nullptr, x, y, aux, m, post, dtype, norm_w, eps);
   int rc = prenorm(stream, ws, w->device, x, norm_w, eps, m, w->k, dtype);
   if (rc)
     return rc;
@@ -788,7 +801,7 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     return run_gemv_groups_locked(stream, ws, w, x, y, aux, m, post, dtype);
   }
   if (!wu && decode_gemv_supported((int)m, (int)(w->k / 256), (int)w->n, false, device_cus(w->device)))
-    return run_decode_gemv(stream, w, nullptr, x, y, aux, m, post, dtype, norm_w, eps);
+    return run_decode_gemv(stream, ws, w, nullptr, x, y, aux, m, post, dtype, norm_w, eps);
   const bool gemv = kern.kind != kGemm || m <= 16u * kGemvMaxRowTiles;
   const bool split = gemv && gemv_split((int)m);
   const int rows = split ? 2 * (int)m : (int)m;
@@ -799,7 +812,7 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     int rc = prenorm(stream, ws, w->device, x, norm_w, eps, m, w->k, dtype);
     if (!rc)
       rc = ensure_splitk_workspace(stream, ws, w->device, gemv_splitk_part_floats(plan), (size_t)plan.groups);
-    if (rc)
+    if (rc || ws.sizing)
       return rc;
     if (ws.fixed)  // the scratch's counters start at zero for this launch (a fill kernel: capture-safe)
       Q4K_TRY_HIP(launch_fill_u32(stream, reinterpret_cast<uint32_t*>(ws.counters), 0u, (uint32_t)plan.groups), "counter fill launch");
@@ -831,7 +844,7 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     return run_gemv_groups_locked(stream, ws, w, x, y, aux, m, post, dtype);
   }
   if (gemv && wu && decode_gemv_supported((int)m, (int)(w->k / 256), (int)w->n, true, device_cus(w->device)))
-    return run_decode_gemv(stream, w, wu, x, y, nullptr, m, post, dtype, norm_w, eps);
+    return run_decode_gemv(stream, ws, w, wu, x, y, nullptr, m, post, dtype, norm_w, eps);
   if (gemv && !wu && q4k_persistent_supported((int)m, (int)(w->k / 256), (int)w->n, device_cus(w->device))) {
     // Wide plain projections (the LM head): the persistent GEMV, x fragments
     // resident in registers.
@@ -839,7 +852,7 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     int rc = prenorm(stream, ws, w->device, x, norm_w, eps, m, w->k, dtype);
     if (!rc)
       rc = stage_pack(stream, ws, w->device, x, dtype, m, w->k, &a.pack);
-    if (rc)
+    if (rc || ws.sizing)
       return rc;
     a.w = w->data;
     a.x = x;
@@ -860,8 +873,28 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
   // xs (and, for single fp16 fragments, the residual plane after it) is
   // read 32 lanes at a time from its start; +128 halves of slack.
   const size_t xs_halves = gemv ? 2 * gemv_xs_halves(rows, (int)w->k) + 128 : 0;
+  const int nb = (int)(w->k / 256), cus = device_cus(w->device);
+  const RowsPlan rows_plan = gemv ? gemv_rows_plan(rows, nb, (int)w->n, wu != nullptr, cus) : RowsPlan();
+  const MidPlan mid = gemv ? MidPlan() : mid_plan((int)m, (int)w->n, nb, cus);
+  GemmArgs g;
+  g.w = w->data;
+  g.y = y;
+  g.aux = aux;
+  g.m = (int)m;
+  g.n = (int)w->n;
+  g.k = (int)w->k;
+  g.nb = nb;
+  g.post = (int)post;
   int rc = ensure_workspace(stream, ws, w->device, ws_rows * w->k + xs_halves, ws_rows);
-  if (rc)
+  if (!rc && rows_plan.slices > 1) {
+    const size_t groups = (size_t)(w->n / (16 * rows_plan.tiles));
+    rc = ensure_splitk_workspace(stream, ws, w->device, gemv_rows_part_floats(rows_plan, (int)w->n), groups);
+    if (!rc && ws.fixed)  // the scratch's counters start at zero for this launch (a fill kernel: capture-safe)
+      Q4K_TRY_HIP(launch_fill_u32(stream, reinterpret_cast<uint32_t*>(ws.counters), 0u, (uint32_t)groups), "counter fill launch");
+  } else if (!rc && !gemv) {
+    rc = mid.rt ? mid_buffers(stream, ws, w->device, mid) : gemm2_split_buffers(stream, ws, w->device, g, false);
+  }
+  if (rc || ws.sizing)
     return rc;
   _Float16* xs = ws.x + ws_rows * w->k;
   if (restage) {
@@ -870,15 +903,6 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     Q4K_TRY_HIP(launch_stage_x(stream, x, (int)dtype, ws.x, xs, ws.scale, (int)m, (int)w->k, mode, norm_w, eps), "stage_x launch");
   }
   if (gemv) {
-    const RowsPlan rows_plan = gemv_rows_plan(rows, (int)(w->k / 256), (int)w->n, wu != nullptr, device_cus(w->device));
-    if (rows_plan.slices > 1) {
-      const size_t groups = (size_t)(w->n / (16 * rows_plan.tiles));
-      rc = ensure_splitk_workspace(stream, ws, w->device, gemv_rows_part_floats(rows_plan, (int)w->n), groups);
-      if (rc)
-        return rc;
-      if (ws.fixed)  // the scratch's counters start at zero for this launch (a fill kernel: capture-safe)
-        Q4K_TRY_HIP(launch_fill_u32(stream, reinterpret_cast<uint32_t*>(ws.counters), 0u, (uint32_t)groups), "counter fill launch");
-    }
     GemvArgs a;
     a.w = w->data;
     a.wu = wu ? wu->data : w->data;
@@ -890,7 +914,7 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     a.m = (int)m;
     a.n = (int)w->n;
     a.k = (int)w->k;
-    a.nb = (int)(w->k / 256);
+    a.nb = nb;
     a.post = (int)post;
     a.rows = rows;
     a.split = split ? 1 : 0;
@@ -902,28 +926,14 @@ int run_linear_locked(hipStream_t stream, Workspace& ws, q4k_weight* w, q4k_weig
     if (rows_plan.tiles > 0)
       Q4K_TRY_HIP(launch_gemv_rows(stream, a, (int)dtype, rows_plan, wu != nullptr), "gemv rows launch");
     else
-      Q4K_TRY_HIP(launch_gemv(stream, a, (int)dtype, gemv_shape(rows, (int)w->n, a.nb, wu != nullptr, device_cus(w->device)), wu != nullptr),
-                  "gemv launch");
+      Q4K_TRY_HIP(launch_gemv(stream, a, (int)dtype, gemv_shape(rows, (int)w->n, nb, wu != nullptr, cus), wu != nullptr), "gemv launch");
   } else {
-    GemmArgs a;
-    a.w = w->data;
-    a.xh = ws.x;
-    a.rowscale = ws.scale;
-    a.y = y;
-    a.aux = aux;
-    a.m = (int)m;
-    a.n = (int)w->n;
-    a.k = (int)w->k;
-    a.nb = (int)(w->k / 256);
-    a.post = (int)post;
-    const MidPlan mid = mid_plan(a.m, a.n, a.nb, device_cus(w->device));
+    g.xh = ws.x;
+    g.rowscale = ws.scale;
     if (mid.rt)
-      return run_mid(stream, ws, w, a, dtype, mid, false);
-    rc = gemm2_split_buffers(stream, ws, w->device, a, false);
-    if (rc)
-      return rc;
+      return run_mid(stream, ws, w, g, dtype, mid, false);
     LaunchTimer timer(stream, Q4K_KERNEL_GEMM);
-    Q4K_TRY_HIP(launch_gemm2(stream, a, (int)dtype, device_cus(w->device)), "gemm launch");
+    Q4K_TRY_HIP(launch_gemm2(stream, g, (int)dtype, cus), "gemm launch");
   }
   return Q4K_OK;
 }
@@ -1341,7 +1351,7 @@ int mlp_gate_up_impl(void* stream, q4k_weight* wg, q4k_weight* wu, const void* x
     reserve_workspace(s, ws, wg->device);
     resolve(wg, phase);
     resolve(wu, phase);
-    return run_decode_gemv(s, wg, wu, x, y, nullptr, m, Q4K_POST_STORE, dtype, norm_w, eps);
+    return run_decode_gemv(s, ws, wg, wu, x, y, nullptr, m, Q4K_POST_STORE, dtype, norm_w, eps);
   }
   Workspace& ws = workspace(wg->device);
   std::lock_guard<std::mutex> lock(ws.mu);
@@ -1357,18 +1367,9 @@ int mlp_gate_up_impl(void* stream, q4k_weight* wg, q4k_weight* wu, const void* x
     // same buffer bit for bit), without storing the gate and reading it back.
     resolve(wu, phase);
     const size_t rows = (size_t)gemm2_rows((int)m);
-    rc = ensure_workspace(s, ws, wg->device, rows * wg->k, rows);
-    if (rc)
-      return rc;
-    {
-      LaunchTimer timer(s, Q4K_KERNEL_STAGE);
-      Q4K_TRY_HIP(launch_stage_x(s, x, (int)dtype, ws.x, nullptr, ws.scale, (int)m, (int)wg->k, kStageGemm, norm_w, eps), "stage_x launch");
-    }
     GemmArgs a;
     a.w = wg->data;
     a.wu = wu->data;
-    a.xh = ws.x;
-    a.rowscale = ws.scale;
     a.y = y;
     a.aux = nullptr;
     a.m = (int)m;
@@ -1377,11 +1378,19 @@ int mlp_gate_up_impl(void* stream, q4k_weight* wg, q4k_weight* wu, const void* x
     a.nb = (int)(wg->k / 256);
     a.post = Q4K_POST_GATE;
     const MidPlan mid = mid_plan(a.m, a.n, a.nb, device_cus(wg->device));
-    if (mid.rt)
-      return run_mid(s, ws, wg, a, dtype, mid, true);
-    rc = gemm2_split_buffers(s, ws, wg->device, a, true);
+    rc = ensure_workspace(s, ws, wg->device, rows * wg->k, rows);
+    if (!rc)
+      rc = mid.rt ? mid_buffers(s, ws, wg->device, mid) : gemm2_split_buffers(s, ws, wg->device, a, true);
     if (rc)
       return rc;
+    {
+      LaunchTimer timer(s, Q4K_KERNEL_STAGE);
+      Q4K_TRY_HIP(launch_stage_x(s, x, (int)dtype, ws.x, nullptr, ws.scale, (int)m, (int)wg->k, kStageGemm, norm_w, eps), "stage_x launch");
+    }
+    a.xh = ws.x;
+    a.rowscale = ws.scale;
+    if (mid.rt)
+      return run_mid(s, ws, wg, a, dtype, mid, true);
     LaunchTimer timer(s, Q4K_KERNEL_GEMM);
     Q4K_TRY_HIP(launch_gemm2_gated(s, a, (int)dtype, device_cus(wg->device)), "gated gemm launch");
     return Q4K_OK;
@@ -1921,9 +1930,10 @@ int check_lora(const q4k_adapters* ad, const void* x, const void* y, const void*
   return Q4K_OK;
 }
 
-// The adapters' part of a projection, with the device's workspace lock held.
-int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_adapters* ad, const void* x, void* y, const void* aux, uint32_t m,
-                    uint32_t k, uint32_t n, const uint32_t* counts, uint32_t nq, uint32_t dtype) {
+// The adapters' part of a projection: its arguments and plan, its buffer, and
+// its launches (with the device's workspace lock held).
+LoraArgs lora_args(int device, const q4k_adapters* ad, const void* x, void* y, const void* aux, uint32_t m, uint32_t k, uint32_t n,
+                   const uint32_t* counts, uint32_t nq) {
   LoraArgs a;
   a.x = x;
   a.y = y;
@@ -1947,14 +1957,19 @@ int run_lora_locked(hipStream_t stream, Workspace& ws, int device, const q4k_ada
     start += (uint32_t)a.count[q];
   }
   lora_plan(a, device_cus(device));
+  return a;
+}
+
+int lora_buffers(hipStream_t stream, Workspace& ws, int device, const LoraArgs& a) {
+  return a.one ? Q4K_OK : ensure_buffer(stream, ws, device, ws.part, ws.part_elems, (size_t)a.slices * a.m * a.rpad, "split-K workspace");
+}
+
+int launch_lora_locked(hipStream_t stream, Workspace& ws, int device, LoraArgs& a, uint32_t dtype) {
   if (a.one) {
     LaunchTimer timer(stream, Q4K_KERNEL_AUX);
     Q4K_TRY_HIP(launch_lora_token(stream, a, (int)dtype, device_cus(device)), "adapter launch");
     return Q4K_OK;
   }
-  int rc = ensure_buffer(stream, ws, device, ws.part, ws.part_elems, (size_t)a.slices * a.m * a.rpad, "split-K workspace");
-  if (rc)
-    return rc;
   a.part = ws.part;
   {
     LaunchTimer timer(stream, Q4K_KERNEL_AUX);
@@ -2028,7 +2043,9 @@ int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void*
   Workspace& ws = workspace(device);
   std::lock_guard<std::mutex> lock(ws.mu);
   reserve_workspace(s, ws, device);
-  return run_lora_locked(s, ws, device, adapters, x, y, aux, m, k, n, query_counts, nqueries, dtype);
+  LoraArgs a = lora_args(device, adapters, x, y, aux, m, k, n, query_counts, nqueries);
+  rc = lora_buffers(s, ws, device, a);
+  return rc ? rc : launch_lora_locked(s, ws, device, a, dtype);
 }
 
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
@@ -2056,7 +2073,16 @@ int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, c
       return rc;
     sum = ws.adapted;
   }
-  rc = run_lora_locked(s, ws, w->device, adapters, x, sum, post == Q4K_POST_ADD ? aux : nullptr, m, w->k, w->n, query_counts, nqueries, dtype);
+  // All buffers first: a call that is refused has enqueued nothing, and left y
+  // (which may be aux) as it was.
+  LoraArgs a = lora_args(w->device, adapters, x, sum, post == Q4K_POST_ADD ? aux : nullptr, m, w->k, w->n, query_counts, nqueries);
+  rc = lora_buffers(s, ws, w->device, a);
+  if (!rc) {
+    SizingScope sizing(ws);
+    rc = run_linear_locked(s, ws, w, nullptr, x, sum, sum, m, Q4K_POST_ADD, dtype, phase, true);
+  }
+  if (!rc)
+    rc = launch_lora_locked(s, ws, w->device, a, dtype);
   if (rc)
     return rc;
   rc = run_linear_locked(s, ws, w, nullptr, x, sum, sum, m, Q4K_POST_ADD, dtype, phase, true);

@@ -1,0 +1,92 @@
+"""q4k_linear_lora in a process whose workspace is as small as the case makes it.
+
+What a call finds in the workspace depends on every call before it, so these
+cases need a fresh process: the parent test (test_gpu_adapter_workspace.py) runs
+``python adapter_child.py CASE``.  Exit status 0 means every check passed.
+"""
+import os
+import sys
+
+import numpy as np
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+import mtlqwen_amd as q4k  # noqa: E402
+from q4k_ref import TYPE_Q4_K, TYPE_Q6_K, make_weight, make_x  # noqa: E402
+
+dev = torch.device("cuda:0")
+rng = np.random.default_rng(9600)
+
+
+class Call:
+    """A linear_lora call over one stack of two adapters."""
+
+    def __init__(self, t, counts, n, k, r, post, dtype=torch.float32):
+        m = sum(counts)
+        self.name = f"type {t} {m}x{k}->{n} rank {r} post {post} {dtype}"
+        print(self.name, flush=True)
+        self.W = q4k.Weight(make_weight(rng, n, k, t), n, k, ggml_type=t)
+        self.x = torch.from_numpy(make_x(rng, m, k, 0.25)).to(dev).to(dtype)
+        self.aux = torch.from_numpy(make_x(rng, m, n, 0.5)).to(dev).to(dtype)
+        self.a = torch.from_numpy((rng.standard_normal((2, r, k)) / np.sqrt(k)).astype(np.float16)).to(dev)
+        self.b = torch.from_numpy((rng.standard_normal((2, n, r)) / np.sqrt(r)).astype(np.float16)).to(dev)
+        self.ids = torch.ones(len(counts), dtype=torch.int32, device=dev)
+        self.m, self.counts, self.post = m, counts, post
+
+    def __call__(self, y, aux=None):
+        q4k.linear_lora(self.x, self.W, self.a, self.b, self.ids, self.m, y, auxiliary=aux if self.post else None, gated=self.post == 2,
+                        query_counts=self.counts)
+
+
+def refused(call):
+    """In a capture that needs more workspace, in place over the auxiliary: the
+    error, and a graph that holds nothing of the call."""
+    y, count = call.aux.clone(), torch.zeros(1, device=dev)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        count.add_(1)
+        try:
+            call(y, y)
+            code = 0
+        except q4k.Q4KError as e:
+            code = e.code
+    assert code == q4k.ECAPTURE, (call.name, code)
+    for i in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert count.item() == i + 1 and torch.equal(y, call.aux), call.name
+
+
+def eager(call):
+    """The call out of place, and in place over the auxiliary."""
+    y, z = torch.empty_like(call.aux), call.aux.clone()
+    call(y, call.aux)
+    call(z, z)
+    torch.cuda.synchronize()
+    assert torch.isfinite(y).all() and (call.post == 0 or torch.equal(y, z)), call.name
+    return y
+
+
+case = sys.argv[1]
+if case == "refused":
+    # No workspace at all: adapters of a single launch, which need none, beside
+    # projections that do (split-K, staged, persistent, packed).
+    ones = [1] * 8
+    for post in (1, 2):
+        for t, n, k in ((TYPE_Q4_K, 4096, 12288), (TYPE_Q4_K, 512, 1024), (TYPE_Q4_K, 65536, 2048), (TYPE_Q6_K, 512, 1024), (TYPE_Q6_K, 1024, 8192)):
+            refused(Call(t, ones, n, k, 8, post))
+    # Adapters that fit what a small call reserved, beside a projection that stages more.
+    small = Call(TYPE_Q4_K, [3], 512, 1024, 8, 1)
+    eager(small)
+    for t in (TYPE_Q4_K, TYPE_Q6_K):
+        for post in (1, 2):
+            large = Call(t, [8000, 192], 256, 8192, 16, post)
+            refused(large)
+            if (t, post) == (TYPE_Q6_K, 2):
+                eager(large)
+else:
+    raise SystemExit(f"no case {case}")
+print("ok", flush=True)
