@@ -18,9 +18,9 @@
  *    from one submitter / one stream at a time, as the reference engine does
  *    (single worker thread, one command buffer per pass).
  *  - The workspace lives until the process ends.  The first projection on a
- *    device, of any shape, reserves about 93 MB (hipMalloc); a call that
+ *    device, of any shape, reserves 94 MB (hipMalloc); a call that
  *    needs more (mostly by staging more activations: m * k above 4.3 million,
- *    m rounded up to 128) grows it.  Which kernel a call takes depends on its
+ *    m rounded up to 128, or m above 1024) grows it.  Which kernel a call takes depends on its
  *    shape alone, so a captured call gives the bits of the eager one.  A call
  *    made while its stream captures a HIP graph must not need growth: the
  *    launch that would need it fails with Q4K_ECAPTURE before allocating
@@ -327,8 +327,9 @@ int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void*
 
 /* q4k_linear with adapters: y = post(x W^T + scale (x A^T) B^T, aux).  The
  * adapters' part is written first (post 0 and 1: into y with aux added, rounded to the
- * dtype; post 2: into a workspace buffer of m * n) and the projection adds to it.  A
- * call that needs more workspace than there is (Q4K_ENOMEM, or Q4K_ECAPTURE while
+ * dtype; post 2: into a workspace buffer of m * n, of which the first
+ * projection's or adapter call's reservation holds 64 rows of 32768 fp32 outputs) and
+ * the projection adds to it.  A call that needs more workspace than there is (Q4K_ENOMEM, or Q4K_ECAPTURE while
  * its stream captures) enqueues nothing and leaves y as it was. */
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);

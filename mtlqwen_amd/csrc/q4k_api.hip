@@ -69,7 +69,8 @@ struct Kernel {
 
 // Per-device staging workspace for activations (fp16 copy + row scales).
 // Outgrown buffers are retired, not freed: a HIP graph captured earlier may
-// still name them.  Growth is bounded by the largest m * k staged.
+// still name them.  Growth is bounded by the largest m * k staged (and m * n of
+// the gated sums beside adapters).
 struct Workspace {
   std::mutex mu;
   _Float16* x = nullptr;  // staged activations, then the sub-block sums
@@ -427,6 +428,21 @@ int ensure_splitk_workspace(hipStream_t stream, Workspace& ws, int device, size_
   return Q4K_OK;
 }
 
+// The gated sums beside adapters, m * n values and no less than twice what there
+// was (where the card has room): a slow rise of m retires less than the last
+// buffer holds.
+int ensure_adapted(hipStream_t stream, Workspace& ws, int device, size_t bytes) {
+  const size_t twice = 2 * ws.adapted_bytes;
+  if (ws.adapted_bytes < bytes && bytes < twice && !stream_capturing(stream)) {
+    const std::string last = g_error;
+    if (!ensure_buffer(stream, ws, device, ws.adapted, ws.adapted_bytes, twice, "adapted-projection buffer"))
+      return Q4K_OK;
+    (void)hipGetLastError();
+    g_error = last;
+  }
+  return ensure_buffer(stream, ws, device, ws.adapted, ws.adapted_bytes, bytes, "adapted-projection buffer");
+}
+
 // Longest row of the rows GEMM, and the fp16 values it stages: 128 rows, then
 // the sub-block sums, 256 values per block and row tile.
 constexpr uint32_t kRowsGemmMaxK = 32768;
@@ -439,9 +455,11 @@ constexpr size_t rows_gemm_halves(size_t k) {
 // Kernels differ in the buffers they need (a prefill of 512 rows may sum no
 // K-slices where one of 64 sums sixteen), so a device's first call outside a
 // capture reserves what any call of up to 63 rows and any K-sliced one can need
-// (about 93 MB, once): a capture then grows nothing unless it stages more
-// activations than any call before it.  A card too full for it is not an
-// error here: the calls grow what they need themselves.
+// (94 MB, once; gated outputs beside adapters up to kReservedOutputs wide): a
+// capture then grows nothing unless it stages more activations, or sums of
+// adapters, than any call before it.  A card too full for it is not an error
+// here: the calls grow what they need themselves.
+constexpr size_t kReservedOutputs = 32768;
 void reserve_workspace(hipStream_t stream, Workspace& ws, int device) {
   if (ws.reserved || ws.fixed || stream_capturing(stream))
     return;
@@ -454,6 +472,8 @@ void reserve_workspace(hipStream_t stream, Workspace& ws, int device) {
     rc = ensure_buffer(stream, ws, device, ws.pack, ws.pack_bytes, kRowsGemmMaxK / 256 * kPackBytesPerBlock, "decode pack");
   if (!rc)
     rc = ensure_buffer(stream, ws, device, ws.normed, ws.normed_bytes, (size_t)64 * kRowsGemmMaxK * sizeof(float), "normalised-activation buffer");
+  if (!rc)
+    rc = ensure_adapted(stream, ws, device, (size_t)64 * kReservedOutputs * sizeof(float));
   if (rc) {
     (void)hipGetLastError();
     g_error = last;
@@ -2068,7 +2088,7 @@ int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, c
   void* sum = y;
   if (post == Q4K_POST_GATE) {
     const size_t bytes = (size_t)m * w->n * (dtype == Q4K_DTYPE_F32 ? 4 : 2);
-    rc = ensure_buffer(s, ws, w->device, ws.adapted, ws.adapted_bytes, bytes, "adapted-projection buffer");
+    rc = ensure_adapted(s, ws, w->device, bytes);
     if (rc)
       return rc;
     sum = ws.adapted;

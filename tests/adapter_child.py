@@ -4,6 +4,7 @@ What a call finds in the workspace depends on every call before it, so these
 cases need a fresh process: the parent test (test_gpu_adapter_workspace.py) runs
 ``python adapter_child.py CASE``.  Exit status 0 means every check passed.
 """
+import ctypes
 import os
 import sys
 
@@ -87,6 +88,47 @@ if case == "refused":
             refused(large)
             if (t, post) == (TYPE_Q6_K, 2):
                 eager(large)
+elif case == "captured":
+    # Any first call reserves what gated calls of few rows need.
+    q4k.linear(torch.zeros((3, 1024), device=dev), q4k.Weight(make_weight(rng, 512, 1024, TYPE_Q4_K), 512, 1024), 3, torch.empty((3, 512), device=dev))
+    for t, counts, n, k, r, dtype in ((TYPE_Q4_K, [1] * 8, 12288, 4096, 8, torch.float32), (TYPE_Q4_K, [5] * 8, 32768, 512, 64, torch.float32),
+                                      (TYPE_Q6_K, [60, 3], 1024, 1024, 16, torch.float16)):
+        call = Call(t, counts, n, k, r, 2, dtype)
+        y = call.aux.clone()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+            call(y, y)
+        want = eager(call)
+        for _ in range(3):
+            y.copy_(call.aux)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), call.name
+            eager(call)
+elif case == "growth":
+    # Rising row counts: the sums' buffer at least doubles, from 8.4 MB to 16.8
+    # at 528 rows and 33.5 at 1040.  Two more allocations are the row scales of the
+    # projection's staging (1024 rows reserved; rows in steps of 128): 1152 and 1280.
+    def allocations():
+        c = ctypes.c_uint64()
+        assert q4k.lib.q4k_workspace_allocations(ctypes.byref(c)) == 0
+        return c.value
+
+    call = Call(TYPE_Q4_K, [1200], 4096, 256, 8, 2)
+    every = call.x, call.aux
+    call.x, call.aux, call.m, call.counts = every[0][:8], every[1][:8], 8, [8]
+    eager(call)
+    before = allocations()
+    for m in range(528, 1201, 16):  # from 8.7 to 19.7 MB of sums
+        call.x, call.aux, call.m, call.counts = every[0][:m], every[1][:m], m, [m]
+        y = eager(call)
+        base, delta = torch.empty_like(y), torch.empty_like(y)
+        q4k.linear(call.x, call.W, m, base, query_counts=[m])
+        q4k.lora(call.x, call.a, call.b, call.ids, m, delta)
+        want = torch.nn.functional.silu(call.aux) * (base + delta)
+        assert ((y - want).norm(dim=1) <= 1e-5 * want.norm(dim=1)).all(), m
+    assert allocations() - before <= 4, allocations() - before
 else:
     raise SystemExit(f"no case {case}")
 print("ok", flush=True)
