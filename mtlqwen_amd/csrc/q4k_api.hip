@@ -47,7 +47,10 @@ int q4k_internal_fail(int code, const char* msg) {
 
 namespace {
 
+// The runtime's own record of the error is cleared: it is reported here, and the
+// next launch's check would report it again.
 int hip_fail(hipError_t e, const char* what) {
+  (void)hipGetLastError();
   return fail(Q4K_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
 
@@ -368,6 +371,7 @@ int ws_alloc(hipStream_t stream, int device, void** p, size_t bytes, const char*
                 what, bytes, device);
   if (hipMalloc(p, bytes) != hipSuccess) {
     *p = nullptr;
+    (void)hipGetLastError();  // reported here, not by the next launch
     return fail(Q4K_ENOMEM, "cannot allocate %zu-byte %s on device %d", bytes, what, device);
   }
   g_ws_allocations.fetch_add(1, std::memory_order_relaxed);
@@ -437,7 +441,6 @@ int ensure_adapted(hipStream_t stream, Workspace& ws, int device, size_t bytes) 
     const std::string last = g_error;
     if (!ensure_buffer(stream, ws, device, ws.adapted, ws.adapted_bytes, twice, "adapted-projection buffer"))
       return Q4K_OK;
-    (void)hipGetLastError();
     g_error = last;
   }
   return ensure_buffer(stream, ws, device, ws.adapted, ws.adapted_bytes, bytes, "adapted-projection buffer");
@@ -474,10 +477,8 @@ void reserve_workspace(hipStream_t stream, Workspace& ws, int device) {
     rc = ensure_buffer(stream, ws, device, ws.normed, ws.normed_bytes, (size_t)64 * kRowsGemmMaxK * sizeof(float), "normalised-activation buffer");
   if (!rc)
     rc = ensure_adapted(stream, ws, device, (size_t)64 * kReservedOutputs * sizeof(float));
-  if (rc) {
-    (void)hipGetLastError();
+  if (rc)
     g_error = last;
-  }
 }
 
 // The pipelined GEMM of a shape with fewer tiles than CUs runs two
@@ -1052,6 +1053,7 @@ int q4k_weight_create(const void* gguf_bytes, size_t bytes, uint32_t n, uint32_t
   w->bytes = bytes;
   if (hipMalloc(&w->data, bytes) != hipSuccess) {
     delete w;
+    (void)hipGetLastError();
     return fail(Q4K_ENOMEM, "cannot allocate %zu bytes of weights on device %d", bytes, device);
   }
   hipError_t e = hipMemcpy(w->data, tiled.data(), bytes, hipMemcpyHostToDevice);
@@ -1089,6 +1091,7 @@ int q4k_weight_create_from_device(const void* gguf_device_bytes, size_t bytes, u
   w->bytes = bytes;
   if (hipMalloc(&w->data, bytes) != hipSuccess) {
     delete w;
+    (void)hipGetLastError();
     return fail(Q4K_ENOMEM, "cannot allocate %zu bytes of weights on device %d", bytes, device);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);

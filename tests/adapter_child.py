@@ -15,6 +15,8 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import mtlqwen_amd as q4k  # noqa: E402
+from mtlqwen_amd import operators as ops  # noqa: E402
+from mtlqwen_amd._lib import EHIP  # noqa: E402
 from q4k_ref import TYPE_Q4_K, TYPE_Q6_K, make_weight, make_x  # noqa: E402
 
 dev = torch.device("cuda:0")
@@ -129,6 +131,25 @@ elif case == "growth":
         want = torch.nn.functional.silu(call.aux) * (base + delta)
         assert ((y - want).norm(dim=1) <= 1e-5 * want.norm(dim=1)).all(), m
     assert allocations() - before <= 4, allocations() - before
+elif case == "errors":
+    # A call that the runtime refuses reports that once: the next calls, the
+    # library's and torch's, run.  The first asks for 2.2 TB of sums, before
+    # anything is launched; its addresses are only compared.
+    call = Call(TYPE_Q4_K, [3], 32768, 256, 8, 2)
+    want = eager(call)
+    m, address = 1 << 24, 1 << 40
+    ad = ops._ADAPTERS(address, 2 * address, 3 * address, 0, 0, 1, 8)
+    rc = q4k.lib.q4k_linear_lora(None, call.W.handle, ad, 4 * address, 8 * address, 8 * address, m, ops._COUNTS[1](m), 1, 2, 0)
+    assert rc == q4k.ENOMEM, rc
+    assert torch.equal(eager(call), want)
+    # A device that is not there.
+    x, y = torch.randn((2, 4, 64), device=dev), torch.empty((2, 4, 64), device=dev)
+    f, p = torch.ones(32, device=dev, dtype=torch.float64), torch.zeros(2, device=dev, dtype=torch.int32)
+    heads = ops._HEADS(x.data_ptr(), y.data_ptr(), 0, 256, 64, 256, 64, 4)
+    rc = q4k.lib.q4k_rope(None, torch.cuda.device_count(), heads, ops._ROTATION(f.data_ptr(), p.data_ptr(), 64, 0, 1.0), 2, 64, 0)
+    assert rc == EHIP, rc
+    q4k.rope(x, f, p, y)
+    assert torch.equal(x + 0, y) and torch.cuda.current_device() == 0
 else:
     raise SystemExit(f"no case {case}")
 print("ok", flush=True)

@@ -1,7 +1,7 @@
 """The workspace of q4k_linear_lora, each case in a process of its own
 (adapter_child.py): a call that is refused for want of it has done nothing, gated
-calls of few rows are captured after any first call, and a slow rise of their rows
-allocates seldom."""
+calls of few rows are captured after any first call, a slow rise of their rows
+allocates seldom, and a call refused by the runtime does not fail the next."""
 import os
 import subprocess
 import sys
@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("case", ["refused", "captured", "growth"])
+@pytest.mark.parametrize("case", ["refused", "captured", "growth", "errors"])
 def test_adapter_workspace(case, gpu):
     env = {k: v for k, v in os.environ.items() if not k.startswith(("Q4K_", "Q6K_"))}
     r = subprocess.run([sys.executable, "-u", os.path.join(HERE, "adapter_child.py"), case], env=env, capture_output=True, text=True, timeout=110)
