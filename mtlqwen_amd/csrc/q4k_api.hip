@@ -2099,6 +2099,7 @@ int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, c
   // All buffers first: a call that is refused has enqueued nothing, and left y
   // (which may be aux) as it was.
   LoraArgs a = lora_args(w->device, adapters, x, sum, post == Q4K_POST_ADD ? aux : nullptr, m, w->k, w->n, query_counts, nqueries);
+  a.reread = true;
   rc = lora_buffers(s, ws, w->device, a);
   if (!rc) {
     SizingScope sizing(ws);

@@ -545,6 +545,7 @@ struct LoraArgs {
   float* part = nullptr;           // [slices, m, rpad]
   int m = 0, k = 0, n = 0, r = 0, rpad = 0, slots = 0, nq = 0, slices = 1;
   int start[8] = {}, count[8] = {};  // rows of the sequences
+  bool reread = false;               // the caller's next launch reads y
   bool one = false;                  // few rows and ranks: one launch
   // Set by the launches: row tiles before a sequence and in a workgroup, columns
   // per workgroup, log2 of the lanes of a row of u (of a column), the order of

@@ -437,7 +437,8 @@ __host__ __device__ inline size_t lora_ubytes(int rows, int r) {
 // columns.  2^a.glog lanes take one row of u, four ranks each (Q times), add the slices'
 // sums, low slices first, and split them.
 // S slices at most; the loads of up to W rows per lane group are on their way together.
-template <typename T, int NC, int S>
+// PAST: aux and y past the caches (lora_expand).
+template <typename T, int NC, int S, bool PAST>
 __global__ __launch_bounds__(256, S > 2 || (sizeof(T) == 4 && NC == 2) ? 3 : 4) void lora_expand_kernel(LoraArgs a) {
   extern __shared__ _Float16 lds[];
   const uint32_t outer = blockIdx.x / a.inner, inner = blockIdx.x - outer * a.inner;
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(256, S > 2 || (sizeof(T) == 4 && NC == 2) ? 3 : 4) 
   u.part[0] = lds;
   u.part[1] = lds + 16 * a.rt * u.pad;
   u.undo = reinterpret_cast<float*>(lds + 32 * a.rt * u.pad);
-  LoraColumns<T, NC, 4, S <= 2> cols(a, b, lane, min(start + a.span, a.n));
+  LoraColumns<T, NC, 4, PAST> cols(a, b, lane, min(start + a.span, a.n));
   cols.first(n0);
   if (b.adapter >= 0) {
     constexpr int Q = NC == 3 ? 2 : 1, W = S > 2 ? 2 / Q : 4 / Q;
@@ -712,15 +713,15 @@ hipError_t lora_shrink(hipStream_t s, LoraArgs a) {
   return dispatch(lora_shrink_kernel<T, 4, 2>, grid, block, s, a);
 }
 
-template <typename T, int S>
+template <typename T, int S, bool PAST>
 hipError_t lora_expand_nc(hipStream_t s, const LoraArgs& a, dim3 grid, dim3 block, size_t lds) {
   if (a.r <= 16)
-    return dispatch_lds(lora_expand_kernel<T, 0, S>, grid, block, lds, s, a);
+    return dispatch_lds(lora_expand_kernel<T, 0, S, PAST>, grid, block, lds, s, a);
   if (a.r <= 32)
-    return dispatch_lds(lora_expand_kernel<T, 1, S>, grid, block, lds, s, a);
+    return dispatch_lds(lora_expand_kernel<T, 1, S, PAST>, grid, block, lds, s, a);
   if (a.r <= 64)
-    return dispatch_lds(lora_expand_kernel<T, 2, S>, grid, block, lds, s, a);
-  return dispatch_lds(lora_expand_kernel<T, 3, S>, grid, block, lds, s, a);
+    return dispatch_lds(lora_expand_kernel<T, 2, S, PAST>, grid, block, lds, s, a);
+  return dispatch_lds(lora_expand_kernel<T, 3, S, PAST>, grid, block, lds, s, a);
 }
 
 template <typename T>
@@ -751,12 +752,18 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   a.inner = a.by_rows ? cols : (uint32_t)tiles;
   const dim3 grid((uint32_t)tiles * cols), block(256);
   const size_t lds = lora_ubytes(16 * a.rt, a.r);
-  // Batches of so many rows also write past the caches, which their output
-  // outgrows, and read aux past them (2048 rows, fp32: 79.9 -> 75.0 us); smaller
-  // outputs stay for the projection that adds to them.
+  // Outputs that outgrow the caches are written past them, and aux read past
+  // them: from 64 MB of both on, where nothing reads y next; of y alone where aux
+  // is y or a projection reads y next.  Calls back to back, 4096 inputs, rank 64,
+  // past / through the caches: with aux, 25 MB each 29.3 / 26.9 us, 34 MB 40.4 /
+  // 43.3, 50 MB 41.7 / 44.7, 101 MB 66.3 / 71.0; in place, 50 MB 41.4 / 38.4, 101 MB
+  // 65.8 / 71.4; linear_lora, 50 MB 148 / 144, 101 MB 273 / 278.
+  const size_t y_bytes = (size_t)a.m * a.n * sizeof(T);
+  const bool past = (a.aux && a.aux != a.y && !a.reread ? 2 : 1) * y_bytes >= 64u << 20;
   if (a.slices <= 2)
-    return lora_expand_nc<T, 2>(s, a, grid, block, lds);
-  return lora_expand_nc<T, kLoraMaxSlices>(s, a, grid, block, lds);
+    return past ? lora_expand_nc<T, 2, true>(s, a, grid, block, lds) : lora_expand_nc<T, 2, false>(s, a, grid, block, lds);
+  return past ? lora_expand_nc<T, kLoraMaxSlices, true>(s, a, grid, block, lds)
+              : lora_expand_nc<T, kLoraMaxSlices, false>(s, a, grid, block, lds);
 }
 
 }  // namespace
