@@ -532,7 +532,6 @@ hipError_t launch_heads(hipStream_t s, const HeadsArgs& a, bool norm, bool inter
 
 // Low-rank adapters of a packed batch (q4k_lora.hip): y = aux + s u B^T with u =
 // x A^T, the sums of u's K-slices in `part`.
-constexpr uint32_t kLoraMaxRank = 512;
 struct LoraArgs {
   const void* x = nullptr;
   const void* aux = nullptr;  // nullptr: zero; may be y

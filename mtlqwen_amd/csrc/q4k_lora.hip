@@ -8,6 +8,10 @@ namespace q4k {
 namespace {
 
 constexpr int kLoraMaxSlices = 8;
+// The one-launch kernel's rounds of 8 ranks and 4096 k, times rows (lora_plan), and
+// the ranks that this leaves it, in powers of two: four lanes' eight.
+constexpr int kTokenRounds = 3, kTokenRanks = 32;
+static_assert(8 * kTokenRounds <= kTokenRanks, "ranks of the one-launch kernel");
 
 // Up to 16 RT rows that lie in one sequence: the first row, the rows, and the
 // sequence's adapter (-1: none) with its rank.
@@ -536,7 +540,7 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // ----------------------------------------------------------------------------
 template <typename T, int ROWS>
 __global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
-  __shared__ float red[8][ROWS][64], us[ROWS][64];
+  __shared__ float red[8][ROWS][kTokenRanks], us[ROWS][kTokenRanks];
   const LoraBlock b = lora_block(a, blockIdx.x, ROWS);
   if (b.adapter < 0 && a.aux == a.y)
     return;
@@ -622,9 +626,9 @@ __global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
       k0 = k1;
     }
     __syncthreads();
-    for (int o = tid; o < ROWS * 64; o += 512) {
-      const int r = o >> 6, j = o & 63;
-      us[r][j] = r < b.rows && j < b.rank ? sum_waves<8>(&red[0][r][j], ROWS * 64) * scale : 0.0f;
+    if (tid < ROWS * kTokenRanks) {
+      const int r = tid / kTokenRanks, j = tid % kTokenRanks;
+      us[r][j] = r < b.rows && j < b.rank ? sum_waves<8>(&red[0][r][j], ROWS * kTokenRanks) * scale : 0.0f;
     }
     __syncthreads();
 #pragma unroll
@@ -693,7 +697,7 @@ hipError_t lora_token(hipStream_t s, LoraArgs a, int cus) {
   for (int q = 0; q < a.nq; ++q)
     rows = a.count[q] > rows ? a.count[q] : rows;
   const int tile = rows <= 1 ? 1 : 2, tiles = lora_lay_tiles(a, tile);
-  a.glog = a.r <= 8 ? 0 : a.r <= 16 ? 1 : a.r <= 32 ? 2 : 3;
+  a.glog = a.r <= 8 ? 0 : a.r <= 16 ? 1 : 2;
   const int round = 512 >> a.glog, rounds = (a.n + round - 1) / round;
   // One workgroup per CU: two took 8.1 us where one took 6.6.
   const int64_t steps = ((int64_t)tiles * rounds + cus - 1) / cus;
@@ -776,7 +780,7 @@ void lora_plan(LoraArgs& a, int cus) {
   int rows = 0;
   for (int q = 0; q < a.nq; ++q)
     rows = a.count[q] > rows ? a.count[q] : rows;
-  a.one = rows <= 2 && rows * ((a.r + 7) / 8) * ((a.k + 4095) / 4096) <= 3;
+  a.one = rows <= 2 && rows * ((a.r + 7) / 8) * ((a.k + 4095) / 4096) <= kTokenRounds;
   if (a.one)
     return;
   // Workgroups for every CU, each with at least 256 k.
