@@ -43,6 +43,11 @@ _rope, _qk_norm_rope, _lora, _linear_lora, _process_logits = (lib.q4k_rope, lib.
                                                               lib.q4k_process_logits)
 
 
+def _cut(*sizes):
+    """The C ABI's sizes have 32 bits, to which ctypes would cut what it is given."""
+    return ValueError(f"sizes must be 0 to 2^32 - 1, got {', '.join(map(str, sizes))}")
+
+
 def _activations(t, what):
     """(dtype code, device index) of an activation tensor."""
     code = _DTYPES.get(t.dtype)
@@ -80,7 +85,9 @@ def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original
     ``factor``, those of more than ``beta_fast`` kept, a ramp between)."""
     if scaling not in ROPE_SCALINGS:
         raise ValueError(f"scaling must be one of {', '.join(ROPE_SCALINGS)}, got {scaling!r}")
-    values = (ctypes.c_double * max(1, rot_dim // 2))()
+    if (rot_dim | original_context) >> 32:
+        raise _cut(rot_dim, original_context)
+    values = (ctypes.c_double * min(max(1, rot_dim // 2), 1 << 16))()
     scale = ctypes.c_float()
     check(lib.q4k_rope_frequencies(rot_dim, float(base), ROPE_SCALINGS[scaling], float(factor), original_context, float(beta_slow),
                                    float(beta_fast), values, ctypes.byref(scale)))
@@ -120,6 +127,8 @@ def rope(x, inv_freq, positions, y, interleaved=False, scale=1.0, stream=None):
     code, device = _activations(x, "x")
     heads = _heads(x, y, 0, "x")
     rows, _, dim = x.shape
+    if (rows | dim) >> 32:
+        raise _cut(rows, dim)
     rc = _rope(_raw_stream(device) if stream is None else _stream_of(stream), device, heads,
                _rotation(inv_freq, positions, rows, device, interleaved, scale), rows, dim, code)
     if rc:
@@ -134,6 +143,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, q_out, k_out, in
     empty ``inv_freq`` norms only."""
     code, device = _activations(q, "q")
     rows, _, dim = q.shape
+    if (rows | dim) >> 32:
+        raise _cut(rows, dim)
     if k.dtype is not q.dtype or k.get_device() != device or k.shape[0] != rows or k.shape[-1] != dim:
         raise ValueError("q and k must share dtype, GPU, rows and head_dim")
     heads = _heads(q, q_out, _address(q_weight, torch.float32, dim, device, "q_weight"), "q")
@@ -173,6 +184,8 @@ def lora(x, a, b, adapter_ids, count, output, auxiliary=None, query_counts=None,
     if a.dim() != 3 or b.dim() != 3:
         raise ValueError("adapters must be a [slots, rank, k] and b [slots, n, rank]")
     k, n = a.shape[2], b.shape[1]
+    if (count | k | n) >> 32:
+        raise _cut(count, k, n)
     counts, sequences = _counts(query_counts, count)
     ad = _adapters(a, b, adapter_ids, ranks, scales, sequences, k, n, device)
     dtype = x.dtype
@@ -192,6 +205,8 @@ def linear_lora(x, w, a, b, adapter_ids, count, output, auxiliary=None, gated=Fa
         raise ValueError("adapters must be a [slots, rank, k] and b [slots, n, rank]")
     if device != w.device:
         raise ValueError(f"x is on cuda:{device}, the weights on cuda:{w.device}")
+    if count >> 32:
+        raise _cut(count)
     counts, sequences = _counts(query_counts, count)
     ad = _adapters(a, b, adapter_ids, ranks, scales, sequences, w.k, w.n, device)
     post = POST_GATE if gated else POST_ADD if auxiliary is not None else POST_STORE
@@ -225,6 +240,8 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
     if logits.dim() != 2 or out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != device:
         raise ValueError("logits and out must be [rows, vocab] of one dtype on one GPU")
     rows, vocab = logits.shape
+    if (rows | vocab) >> 32:
+        raise _cut(rows, vocab)
     in_stride, ie = logits.stride()
     out_stride, oe = out.stride()
     if vocab > 1 and (ie != 1 or oe != 1):
