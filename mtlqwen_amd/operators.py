@@ -199,7 +199,10 @@ def lora(x, a, b, adapter_ids, count, output, auxiliary=None, query_counts=None,
 
 def linear_lora(x, w, a, b, adapter_ids, count, output, auxiliary=None, gated=False, query_counts=None, ranks=None, scales=None, stream=None):
     """linear(x, w, ...) with the sequences' adapters added to the projection
-    before its epilogue (arguments as linear's and lora's)."""
+    before its epilogue (arguments as linear's and lora's, but ``auxiliary`` is a
+    tensor: the fused gate/up pair takes no adapters)."""
+    if auxiliary is not None and not isinstance(auxiliary, torch.Tensor):
+        raise TypeError(f"auxiliary must be a tensor, got {type(auxiliary).__name__}: the fused gate/up pair takes no adapters")
     code, device = _activations(x, "x")
     if a.dim() != 3 or b.dim() != 3:
         raise ValueError("adapters must be a [slots, rank, k] and b [slots, n, rank]")
