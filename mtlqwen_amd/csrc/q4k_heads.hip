@@ -24,9 +24,11 @@ namespace {
 // A workgroup takes U rows per lane and every gridDim.y-th group of hb heads of
 // them: its angles are made once, in LDS, for all those heads, and the values of
 // the next group are asked for before the present one's are used.
-// Angles are 64-bit products of the position and the frequency in turns, whose
-// fraction is rounded to 32 bits: at position 2^20 a product in 32 bits would
-// be off by 0.06 rad, at any position below 2^31 this one is by 5e-7.
+// Angles are 64-bit products of the position and the frequency in turns: at
+// position 2^20 a product in 32 bits would be off by 0.06 rad, at any position
+// below 2^31 this one is by 5e-7.  The fraction enters the function in 32 bits, and
+// what that rounding left, d rad, as c - n d and n + c d (d^2 < 1e-14): without it
+// (9.4e-8 rad) a value near zero would keep few of its bits.
 // ----------------------------------------------------------------------------
 template <typename T, int V>
 struct VecOf {
@@ -102,10 +104,12 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsArgs a) {
     const uint32_t row = blockIdx.x * (uint32_t)(rb * U) + (uint32_t)r;
     if (row < a.rows) {
       const double turns = (double)a.positions[row] * (a.inv_freq[f] * 0.15915494309189533577);
+      const double part = turns - rint(turns);
+      const float near = (float)part, d = 6.2831853f * (float)(part - (double)near);
       float s, c;
-      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-      cs[(2 * r) * h + f] = a.scale * c;
-      cs[(2 * r + 1) * h + f] = a.scale * s;
+      sincospif(2.0f * near, &s, &c);
+      cs[(2 * r) * h + f] = a.scale * fmaf(-s, d, c);
+      cs[(2 * r + 1) * h + f] = a.scale * fmaf(c, d, s);
     }
   }
   __syncthreads();
