@@ -250,6 +250,10 @@ int q4k_rms_norm_gather(void* stream, const void* x, const float* w, void* out, 
 #define Q4K_ROPE_SCALING_LINEAR 1u /* f_i / factor: positions interpolated */
 #define Q4K_ROPE_SCALING_NTK 2u    /* base * factor^(rot_dim / (rot_dim - 2)) */
 #define Q4K_ROPE_SCALING_YARN 3u   /* f_i / factor below beta_slow turns in the original context, f_i above beta_fast, a ramp between */
+/* YARN's ramp is linear in the turns, as the method's paper writes it.  Models
+ * whose code ramps over the pair index i instead differ in the middle pairs, by up
+ * to twice a frequency and more: take those from the model's code and pass them as
+ * inv_freq, which holds any frequencies. */
 
 #define Q4K_MAX_HEAD_DIM 1024u
 
@@ -317,7 +321,9 @@ typedef struct q4k_adapters {
  * without an adapter).  query_counts as for q4k_linear (NULL: one sequence);
  * k a multiple of 256, n of 16.  Products are exact and sums fp32; in batches
  * beyond single rows fp32 x, and x A^T, enter them with 22 bits, scaled per row
- * (values 2^-17 of a row's largest and below with an absolute error of 2^-40 of it).
+ * (values 2^-17 of a row's largest and below with an absolute error of 2^-39 of it).
+ * An infinity or NaN in the ranks in use of a or b makes the elements of y that it
+ * reaches infinite or NaN (not always the one that fp32 products would give).
  * y is rounded once.  Elements of a and b past an adapter's rank are not used.
  * The sums of K-slices live in the device's workspace (slices * m * rank floats,
  * which the first projection's or adapter call's reservation holds up to 16 million of; single
@@ -329,7 +335,9 @@ int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void*
  * adapters' part is written first (post 0 and 1: into y with aux added, rounded to the
  * dtype; post 2: into a workspace buffer of m * n, of which the first
  * projection's or adapter call's reservation holds 64 rows of 32768 fp32 outputs) and
- * the projection adds to it.  A call that needs more workspace than there is (Q4K_ENOMEM, or Q4K_ECAPTURE while
+ * the projection adds to it.  So in fp16 the adapters' part (post 1: with aux) is
+ * rounded before the projection is added, and for post 2 their sum before the gate:
+ * where one of these passes 65504 the result is infinite.  A call that needs more workspace than there is (Q4K_ENOMEM, or Q4K_ECAPTURE while
  * its stream captures) enqueues nothing and leaves y as it was. */
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);

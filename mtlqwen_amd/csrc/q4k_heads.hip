@@ -43,10 +43,11 @@ struct VecOf<T, 1> {
   static __device__ __forceinline__ void set(type& v, int, float x) { v = (T)x; }
 };
 
-// The calls that fill the card write past the caches: what they write outgrows
-// them (norm and rotation of 8192 rows of 40 heads of 128, fp16: 41.3 -> 34.7 us,
-// 4.84 TB/s; rotation alone, fp32: 66.8 -> 63.8 us, 5.26 TB/s, where a copy of 1
-// GiB reaches 5.05).
+// The calls that fill the card (two rows per lane) write past the caches: what they
+// write outgrows them.  Replayed back to back, through the caches -> past them: norm
+// and rotation of 8192 rows of 40 heads of 128, fp16, 38.2 -> 33.9 us, 4.95 TB/s
+// (2048 rows 10.2 -> 9.0); rotation alone, fp32, 66.9 -> 63.9 us, 5.25 TB/s, where a
+// copy of 1 GiB reaches 5.05.
 template <int U, typename V>
 __device__ __forceinline__ void put(V* p, V v) {
   if constexpr (U > 1)
@@ -256,8 +257,12 @@ hipError_t heads_launch(hipStream_t s, HeadsArgs a, int cus) {
     --a.hblog;
   const uint32_t rb = 256u >> (a.glog + a.hblog), groups = (heads + (1u << a.hblog) - 1) >> a.hblog;
   // Two rows per lane, and as many head groups per workgroup, as leave every CU
-  // four workgroups (821 rows of 20 heads of 256, fp16: 5.9 us, with two 6.7; 8192
-  // rows of 40 heads of 128: 41.3 us, with eight 44.7, before the stores below).
+  // four workgroups.  Replayed, with norms, fp16, stores through the caches: 821
+  // rows of 20 heads of 256 5.8 us, with two 6.6, with eight 5.8; 8192 rows of 40
+  // heads of 128 38.2 us, with two 38.2, with eight 40.7, and 38.1 with one row per
+  // lane, whose stores stay in the caches.  Heads that 16 bytes do not divide take
+  // four- and two-byte accesses and one row: 8192 fp16 rows of 40 heads of 80 with 40
+  // rotated 65 us, with 80 rotated (16 bytes) 23.
   const uint64_t want = 4ull * (uint32_t)cus;
   const bool deep = v == kWide && (uint64_t)((a.rows + kDeep * rb - 1) / (kDeep * rb)) * groups >= want &&
                     (size_t)rb * kDeep * a.rot * sizeof(float) <= 32768;

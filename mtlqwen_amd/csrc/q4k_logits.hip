@@ -13,9 +13,9 @@ namespace {
 //   l3 = l2 + the row's last bias entry for v (if any)
 //   out = masked ? -inf : l3
 //
-// One read and one write of the row, bound by memory: 64 rows of 248320 fp32 take
-// 19.1 us with nothing else to do (6.7 TB/s, the inputs in the memory-side
-// cache), 36.2 with texts of 32768 to 65536 tokens, 300 biases and masks, whose
+// One read and one write of the row, bound by memory: 64 rows of 248320 fp32 take,
+// replayed, 19.3 us with nothing else to do (6.6 TB/s, the inputs in the memory-side
+// cache), 36.1 with texts of 32768 to 65536 tokens, 300 biases and masks, whose
 // counting overlaps the copy in part.  A workgroup owns THREADS * E consecutive
 // tokens, held in registers while it counts, in LDS, those of the row's text and
 // biases that fall into its range.  One word per token: bit 31 = seen in the
@@ -25,8 +25,8 @@ namespace {
 // whole vocabulary is cleared, written or read.  A row of more biases than fit
 // into 31 - s bits takes a second round through the words.  Workgroups of every
 // other round of the CUs read their logits after the text, so that not all of
-// them leave the memory idle while they count (the case above: 46.9 -> 45.6 us
-// when it took that long).  The text is read once per workgroup; the workgroups
+// them leave the memory idle while they count (the case above 36.6 -> 36.0 us, and
+// 46.7 -> 44.6 with stores through the caches).  The text is read once per workgroup; the workgroups
 // of a row sit a multiple of the row count apart, with 8 rows and their multiples
 // on one XCD, whose L2 then serves every reading after the first.
 // ----------------------------------------------------------------------------
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitsArgs a) {
     for (int i = 0; i < V; ++i)
       y[i] = (T)((allowed[j] >> i) & 1u ? v[j][i] : -__builtin_inff());
     if (at + V <= left) {
-      if constexpr (THREADS > 512)  // past the caches, which such outputs outgrow: 45.6 -> 36.6 us
+      if constexpr (THREADS > 512)  // past the caches, which such outputs outgrow: 44.6 -> 36.1 us
         __builtin_nontemporal_store(y, reinterpret_cast<vec_t*>(out + at));
       else
         *reinterpret_cast<vec_t*>(out + at) = y;
@@ -229,8 +229,9 @@ template <typename T>
 hipError_t logits_launch(hipStream_t s, const LogitsArgs& a, int cus) {
   // Large ranges read the text fewer times, small ones fill the card: 4096 tokens
   // to a workgroup, or 16384 once every CU has one of those, or half of them where
-  // texts may be long.  fp32, 248320 tokens, texts up to 65536 / 4000: 1 row 9.3 / 6.2 us (16384:
-  // 11.8 / 8.9), 16 rows 20.2 / 10.9 (15.2 / 12.1), 32 rows 33.5 / 18.7 (20.8 / 14.6).
+  // texts may be long.  Replayed, fp32, 248320 tokens, texts up to 65536 / 4000: 1 row
+  // 9.0 / 5.9 us (16384: 11.3 / 8.5), 8 rows 13.0 / 7.5 (11.9 / 9.0), 16 rows 19.8 /
+  // 11.5 (13.7 / 11.1), 32 rows 32.1 / 17.7 (18.8 / 13.3).
   const uint64_t logits = (uint64_t)a.rows * a.vocab, fill = (uint64_t)cus * 16384;
   if (logits >= fill || (a.tokens && a.capacity > 32768 && logits >= fill / 2))
     return logits_dispatch<T, 1024, 16>(s, a);

@@ -66,8 +66,8 @@ __device__ __forceinline__ LoraBlock lora_block(const LoraArgs& a, int tile, int
 
 // Power of two that brings a largest magnitude m to [2^14, 2^15), and its
 // inverse: values scaled by it split into two fp16 parts, hi = fp16(v) and lo =
-// fp16(v - hi), that keep 22 of v's bits down to 2^-17 of the largest, and every
-// bit above 2^-25 of 1 below that.  (m below 2^-112, infinities and NaN: the
+// fp16(v - hi), that keep 22 of v's bits down to 2^-17 of the largest, and all but
+// 2^-25 of a scaled value (2^-39 of the largest) below that.  (m below 2^-112, infinities and NaN: the
 // nearest such power.)
 __device__ __forceinline__ float split_scale(float m, float* inverse) {
   const int e = min(max((int)(__builtin_bit_cast(uint32_t, m) >> 23), 15), 254);
@@ -236,8 +236,8 @@ __device__ __forceinline__ float sum_waves(const float* p, int stride) {
 
 // K in slices: one workgroup per 16 rows, slice and 16 NT ranks; its eight waves
 // take a part of the slice each and add their sums in LDS.  A is read once per 16
-// rows, from the L2.  8 rows of 8 sequences, rank 16, k = 4096: 3.6 us, launch
-// included; 2048 fp32 rows of rank 64: 19.6 us (x alone would take 6.7 at the rate
+// rows, from the L2.  The kernel's own time: 333 ragged fp16 rows of rank 64, k =
+// 4096, 5.0 us; 2048 fp32 rows of rank 64 19.2 (x alone would take 6.7 at the rate
 // of a copy; sharing A between 64 rows through LDS, four slices of it on their way,
 // took 16.5 and 4.7 for adding twice the slices, and more for fewer rows).
 template <typename T, int NT, int SEG>
@@ -279,10 +279,11 @@ __global__ __launch_bounds__(512, 4) void lora_shrink_kernel(LoraArgs a) {
 // high part, 2, 3 the low, B given twice); NC = 1, 2: up to 32 NC ranks; NC = 3:
 // any number, B read anew for each row tile.  A wave takes every WAVES-th step of
 // the workgroup's columns; the loads of its first B and aux are on their way
-// before u is there, those of the next aux before its products.  2048 fp32 rows of
-// 12288, rank 64, with aux: 47.5 us, 4.2 TB/s of aux and y (a copy reaches 5.05); 333
-// ragged fp16 rows of 6144: 9.7 us, most of it the chain of loads from the
-// sequence's id to the sums and B.
+// before u is there, those of the next aux before its products.  The kernel's own
+// time: 2048 fp32 rows of 12288, rank 64, with aux 48.1 us, 4.2 TB/s of aux and y (a
+// copy reaches 5.05); 333 ragged fp16 rows of 6144 10.4 us: the chain of loads from
+// the sequence's id to the sums and B, and the sums themselves, which every workgroup
+// adds up anew from its rows' slices (8 here, 64 KB to a workgroup).
 // ----------------------------------------------------------------------------
 struct LoraU {
   _Float16* part[2];  // [16 rt][pad] each
@@ -535,8 +536,8 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // takes 512 k of one rank row in one contiguous load, 8 k per lane), and writes
 // a.span columns: 1 << a.glog lanes share a column's ranks, 8 each.  A second
 // launch would cost the caller more than reading A once per workgroup costs the L2:
-// 8 sequences of one fp16 row, rank 16, 4096 -> 12288: 5.9 us replayed and 6.7 a
-// call, in two launches 7.3 and 9.6; what bounds it is latency (launch, id, A, sum, B).
+// 8 sequences of one fp16 row, rank 16, 4096 -> 12288: 5.9 us replayed and 7.0 a
+// call, in two launches 8.1 and 9.5; what bounds it is latency (launch, id, A, sum, B).
 // ----------------------------------------------------------------------------
 template <typename T, int ROWS>
 __global__ __launch_bounds__(512) void lora_token_kernel(LoraArgs a) {
@@ -699,7 +700,7 @@ hipError_t lora_token(hipStream_t s, LoraArgs a, int cus) {
   const int tile = rows <= 1 ? 1 : 2, tiles = lora_lay_tiles(a, tile);
   a.glog = a.r <= 8 ? 0 : a.r <= 16 ? 1 : 2;
   const int round = 512 >> a.glog, rounds = (a.n + round - 1) / round;
-  // One workgroup per CU: two took 8.1 us where one took 6.6.
+  // One workgroup per CU: replayed 5.9 us (rank 16, above), with two 7.4.
   const int64_t steps = ((int64_t)tiles * rounds + cus - 1) / cus;
   a.span = round * (int)steps;
   const dim3 grid(tiles, (a.n + a.span - 1) / a.span), block(512);
@@ -731,10 +732,12 @@ hipError_t lora_expand_nc(hipStream_t s, const LoraArgs& a, dim3 grid, dim3 bloc
 template <typename T>
 hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   // Row tiles that share a load of B and u's sums: two where the sequences fill
-  // them (64 rows of one sequence, 4096 -> 12288, rank 64, fp16: 11.4 us, with four
-  // 14.8), four where that still leaves four workgroups per CU (2048 rows, fp32: 60.5 us, with
-  // two 72.5) and u's parts take 64 KB at most, two workgroups to a CU's LDS (ranks up to
-  // 224); one for ranks beyond 256.
+  // them, four where that still leaves four workgroups per CU and u's parts take 64
+  // KB at most, two workgroups to a CU's LDS (ranks up to 224); one for ranks beyond
+  // 256.  Calls back to back, both launches, 4096 inputs, rank 64, with aux, one / two
+  // / four tiles: 64 fp16 rows of one sequence, 12288 outputs, 10.3 / 11.2 / 14.4 us;
+  // 333 ragged ones, 6144 outputs, 15.8 / 15.7 / 17.6; 2048 ragged ones, 12288
+  // outputs, 68.9 / 60.5 / 49.4, fp32 81.5 / 77.7 / 66.3.
   const int64_t blocks = (int64_t)(a.m / 64) * ((a.n + 255) / 256);
   a.rt = a.r > 256 || a.m < 32 * a.nq ? 1 : a.m >= 64 * a.nq && blocks >= 4 * (int64_t)cus && lora_ubytes(64, a.r) <= 65536 ? 4 : 2;
   const int tiles = lora_lay_tiles(a, 16 * a.rt);
@@ -747,10 +750,10 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
   a.glog = 2;
   while ((1 << a.glog) < quads && a.glog < 6)
     ++a.glog;
-  // Workgroups side by side continue each other's rows, for the memory's sake (2048
-  // rows, fp32: 69.1 us, column by column 74.4); with few rows they take the
-  // sequences in turn, so that each XCD's L2 holds the B of its own (20 rows of 4
-  // sequences, rank 64: 9.0 us, row by row 10.1).
+  // Workgroups side by side continue each other's rows, for the memory's sake (calls
+  // as above, 2048 rows, fp32: 66.2 us, column by column 71.4; 128 fp16 rows 14.5 and
+  // 15.0); with few rows they take the sequences in turn, so that each XCD's L2 holds
+  // the B of its own (20 rows of 4 sequences: 9.95 us, row by row 10.2).
   const uint32_t cols = (uint32_t)((a.n + a.span - 1) / a.span);
   a.by_rows = a.m > 64;
   a.inner = a.by_rows ? cols : (uint32_t)tiles;
@@ -773,10 +776,11 @@ hipError_t lora_expand(hipStream_t s, LoraArgs a, int cus) {
 }  // namespace
 
 void lora_plan(LoraArgs& a, int cus) {
-  // Rounds of the one-launch kernel (8 ranks, 4096 k, one row).  Replayed back
-  // to back, fp16, 4096 -> 12288, 8 sequences: 1 round 4.1 us against 8.3 in two
-  // launches, 2 rounds 6.0 (7.3), 3 rounds (12288 -> 4096) 5.9 (8.8), 4 rounds 8.0
-  // (7.3) with two rows and 9.4 (7.6) with 32 ranks.
+  // Rounds of the one-launch kernel (8 ranks of the stack, 4096 k, one row; the
+  // ranks in use are on the device).  Replayed back to back, fp16, 4096 -> 12288, 8
+  // sequences: 1 round 4.1 us against 8.8 in two launches, 2 rounds 5.9 (8.1), with
+  // two rows 5.2 (8.9), 3 rounds 8.5 (9.1), 12288 -> 4096 6.0 (9.1), 4 rounds 7.9 (8.2)
+  // with two rows and 9.1 (8.0) with 32 ranks.
   int rows = 0;
   for (int q = 0; q < a.nq; ++q)
     rows = a.count[q] > rows ? a.count[q] : rows;

@@ -82,7 +82,11 @@ def rope_frequencies(rot_dim, base=10000.0, scaling="none", factor=1.0, original
     values.  ``scaling``: "none"; "linear" (positions divided by ``factor``);
     "ntk" (base * factor^(rot_dim / (rot_dim - 2))); "yarn" (frequencies of
     fewer than ``beta_slow`` turns in ``original_context`` divided by
-    ``factor``, those of more than ``beta_fast`` kept, a ramp between)."""
+    ``factor``, those of more than ``beta_fast`` kept, a ramp between that is
+    linear in the turns, as the method's paper writes it).  Models whose code
+    ramps over the pair index instead differ in the middle pairs, by up to twice a
+    frequency and more: pass theirs as ``inv_freq``, a float64 tensor of any
+    frequencies."""
     if scaling not in ROPE_SCALINGS:
         raise ValueError(f"scaling must be one of {', '.join(ROPE_SCALINGS)}, got {scaling!r}")
     if (rot_dim | original_context) >> 32:
@@ -200,7 +204,8 @@ def lora(x, a, b, adapter_ids, count, output, auxiliary=None, query_counts=None,
 def linear_lora(x, w, a, b, adapter_ids, count, output, auxiliary=None, gated=False, query_counts=None, ranks=None, scales=None, stream=None):
     """linear(x, w, ...) with the sequences' adapters added to the projection
     before its epilogue (arguments as linear's and lora's, but ``auxiliary`` is a
-    tensor: the fused gate/up pair takes no adapters)."""
+    tensor: the fused gate/up pair takes no adapters).  In float16 the adapters'
+    part is rounded before the projection is added, and the sum before the gate."""
     if auxiliary is not None and not isinstance(auxiliary, torch.Tensor):
         raise TypeError(f"auxiliary must be a tensor, got {type(auxiliary).__name__}: the fused gate/up pair takes no adapters")
     code, device = _activations(x, "x")
