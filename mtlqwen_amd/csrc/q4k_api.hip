@@ -95,8 +95,8 @@ struct Workspace {
   // that needs more fails (ensure_buffer).
   bool fixed = false;
   bool reserved = false;  // reserve_workspace has run
-  // While set, a projection grows its buffers and launches nothing (SizingScope):
-  // every path takes all its buffers before its first launch.
+  // While set, a projection (without a norm) grows its buffers and launches nothing
+  // (SizingScope): every path takes all its buffers before its first launch.
   bool sizing = false;
 };
 
