@@ -342,6 +342,93 @@ int q4k_lora(void* stream, int device, const q4k_adapters* adapters, const void*
 int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, const void* x, void* y, const void* aux, uint32_t m,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t post, uint32_t dtype);
 
+/* ---- Paged keys and values -------------------------------------------------
+ * Between the rotation and the output projection: the reference's attention
+ * over its sparse key/value pages (attention.metal:104-216, device.cpp:147-198),
+ * here for any number of heads and of pages, and what a server does with the
+ * pages.  A cache is fp16 pages in device memory: element d of token t of head
+ * h of page p is at p * page_stride + h * head_stride + t * token_stride + d of
+ * k and of v alike (strides in elements, multiples of 8; k and v 16-byte
+ * aligned).  Tokens 0, 1, ... of a sequence lie in the pages that its row of
+ * `tables` lists; a number outside [0, pages) means that the page is not there.
+ * Tables, slots, positions and all that follows them are device memory, read
+ * when the call runs, so a captured call follows them from replay to replay;
+ * the counts of new rows are host values, as for q4k_linear. */
+#define Q4K_MAX_SEQUENCES 64u  /* sequences of a call */
+#define Q4K_MAX_PAGE_SIZE 1024u
+typedef struct q4k_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, token_stride;
+  const int32_t* tables; /* [table_rows, width] */
+  const int32_t* slots;  /* [nqueries]: each sequence's row of tables, outside it: no pages; NULL: row q */
+  uint32_t pages, page_size; /* page_size: a power of two, 16..1024 */
+  uint32_t heads, head_dim;  /* head_dim: a multiple of 8 up to 256 */
+  uint32_t table_rows, width; /* width * page_size up to 2^30 */
+} q4k_cache;
+
+/* Keys and values of the new tokens into their pages: row t of sequence q
+ * (query_counts[q] rows, packed; NULL: nqueries 0 and one sequence of `rows`) goes to
+ * position positions[q] + t.  `in` and the input strides of k and v are used,
+ * their heads are the cache's.  Values are rounded to fp16.  A row whose
+ * position is negative, behind the table or in a page that is not there is not
+ * written; of rows with one place, one's values stay there. */
+int q4k_cache_write(void* stream, int device, const q4k_cache* cache, const q4k_heads* k, const q4k_heads* v, const int32_t* positions,
+                    const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype);
+
+typedef struct q4k_attention_params {
+  float scale;         /* of q.k */
+  float softcap;       /* above 0: x becomes softcap * tanh(x / softcap) */
+  const float* slopes; /* [heads] or NULL: slopes[h] * (key's position - row's) is added */
+  uint32_t window;     /* above 0: a row sees its own position and the window - 1 before it */
+} q4k_attention_params;
+
+/* Row t of sequence q stands at position p = positions[q] + t and sees keys
+ * 0..p that its table holds (those of the new tokens among them: write them
+ * first), each head of q->heads the cache head h / (q->heads / cache->heads):
+ *   out = sum_j exp(x_j) v_j / sum_j exp(x_j),   x_j = scale (q . k_j), capped, then biased.
+ * A row that sees no key (a position below 0, pages that are not there) becomes
+ * zero; what a row does not see does not reach it, infinities and NaN included.
+ * Scores, statistics and sums are fp32.  fp16 q are multiplied as they are and
+ * weights enter the products with v as fp16; fp32 q, and their weights, with 22 bits.  q and out as in q4k_rope, but they must not overlap.  Positions lie
+ * in [-2^30, 2^30].  Work is split by the lengths that the device holds; sums
+ * of the parts live in the device's workspace, as the projections' do. */
+int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache* cache, const q4k_attention_params* params,
+                  const int32_t* positions, const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype);
+
+/* A pool of pages of any content: page p is `blocks` runs of page_size *
+ * token_bytes from p * blocks * page_size * token_bytes on (all layers' keys
+ * and values of a page, say).  data and token_bytes are multiples of 16. */
+#define Q4K_MAX_POOL_PAGES 262144u
+#define Q4K_MAX_SLOTS 1024u
+typedef struct q4k_pool {
+  void* data;
+  uint32_t pages, blocks, page_size, token_bytes;
+} q4k_pool;
+
+/* All slots at once take over their parents' states: slot s holds the first
+ * lengths[p] tokens of p = parents[s] (outside [0, slots): none, the slot is
+ * free; parents NULL: p = s), and has pages for counts[s] more (NULL: none).
+ * Full pages are shared.  A last page that is not full stays with the lowest
+ * slot that holds it (if no other holds it as a full one), the others get a
+ * page with a copy of its tokens.  New pages are the lowest that no slot's new
+ * tokens lie in, in the order of the slots.  Entries without a page are -1;
+ * *missing (may be NULL) is the number of pages asked for and not given.  A page
+ * counts as held where it lies below a slot's length (clamped to its table), so
+ * the caller adds the tokens it has written to the lengths.  tables and lengths are
+ * read, new_tables and new_lengths written; none may overlap.  Forks, beams in
+ * a new order, sequences that end and pages for the next tokens are all this
+ * call. */
+int q4k_cache_assign(void* stream, int device, const q4k_pool* pool, const int32_t* tables, const int32_t* lengths, uint32_t slots, uint32_t width,
+                     const int32_t* parents, const int32_t* counts, int32_t* new_tables, int32_t* new_lengths, int32_t* missing);
+
+/* Moves pages so that the n that slots hold are pages 0..n - 1: the i-th held
+ * one behind them, by number, to the i-th free one among them.  new_tables
+ * lists them; entries behind a slot's length are -1.  *used (may be NULL) = n.
+ * The list of moves lives in the device's workspace. */
+int q4k_cache_compact(void* stream, int device, const q4k_pool* pool, const int32_t* tables, const int32_t* lengths, uint32_t slots,
+                      uint32_t width, int32_t* new_tables, int32_t* used);
+
 /* ---- Logits -----------------------------------------------------------------
  * No counterpart in the reference (its sample_logits, native_ops.metal:122,
  * takes them as they are).  Every pointer is a device pointer, read when the
@@ -434,7 +521,7 @@ int q4k_workspace_allocations(uint64_t* count);
 #define Q4K_KERNEL_GEMV 1u       /* MFMA GEMV, phases 0/2 and small prefill */
 #define Q4K_KERNEL_GEMV_GATED 2u /* fused gate/up GEMV, phase 3 */
 #define Q4K_KERNEL_GEMM 3u       /* LDS-tiled MFMA GEMM, phase 1 */
-#define Q4K_KERNEL_AUX 4u        /* token embedding, RMS norm, rms_norm_gather, rotary positions, adapters, logits */
+#define Q4K_KERNEL_AUX 4u        /* token embedding, RMS norm, rms_norm_gather, rotary positions, adapters, logits, attention and its cache */
 
 /* Event timing of every kernel launch (no counterpart in the reference, whose
  * method is paired A/B timing, agents/KERNELS.md:13-21).  While enabled, each

@@ -82,6 +82,10 @@ def _load():
         "q4k_lora": (c_int, [p, c_int, p, p, p, p, u32, u32, u32, p, u32, u32]),
         "q4k_linear_lora": (c_int, [p, p, p, p, p, p, u32, p, u32, u32, u32]),
         "q4k_process_logits": (c_int, [p, c_int, p, p, u32, u32, ctypes.c_int64, ctypes.c_int64, p, u32]),
+        "q4k_cache_write": (c_int, [p, c_int, p, p, p, p, p, u32, u32, u32]),
+        "q4k_attention": (c_int, [p, c_int, p, p, p, p, p, u32, u32, u32]),
+        "q4k_cache_assign": (c_int, [p, c_int, p, p, p, u32, u32, p, p, p, p, p]),
+        "q4k_cache_compact": (c_int, [p, c_int, p, p, p, u32, u32, p, p]),
         "q4k_profile_enable": (c_int, [c_int]),
         "q4k_profile_query": (c_int, [u32, pu32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),
                                       ctypes.POINTER(ctypes.c_double)]),

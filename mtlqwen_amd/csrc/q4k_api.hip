@@ -14,6 +14,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 
@@ -2003,6 +2004,162 @@ int launch_lora_locked(hipStream_t stream, Workspace& ws, int device, LoraArgs& 
   return Q4K_OK;
 }
 
+// ---- paged keys and values ---------------------------------------------------
+
+constexpr int64_t kMaxCacheStride = 1ll << 40;
+
+// Packed rows of up to kMaxSequences sequences.
+int check_sequences(const uint32_t* counts, uint32_t nq, uint32_t rows) {
+  if (rows > (1u << 24))
+    return fail(Q4K_ESHAPE, "at most 2^24 rows (got %u)", rows);
+  if (!counts)
+    return nq == 0 ? Q4K_OK : fail(Q4K_EINVAL, "query_counts is NULL but nqueries=%u", nq);
+  if (nq == 0 || nq > Q4K_MAX_SEQUENCES)
+    return fail(Q4K_EINVAL, "nqueries must be in [1, %u] (got %u)", Q4K_MAX_SEQUENCES, nq);
+  uint64_t sum = 0;
+  for (uint32_t i = 0; i < nq; ++i)
+    sum += counts[i];
+  return sum == rows ? Q4K_OK : fail(Q4K_EINVAL, "query counts sum to %llu but rows=%u", (unsigned long long)sum, rows);
+}
+
+size_t cache_extent(const q4k_cache* c) {
+  return c->pages == 0 ? 0
+                       : ((size_t)(c->pages - 1) * c->page_stride + (size_t)(c->heads - 1) * c->head_stride +
+                          (size_t)(c->page_size - 1) * c->token_stride + c->head_dim) * 2;
+}
+
+int check_cache(const q4k_cache* c, const int32_t* positions, uint32_t nq) {
+  if (c->page_size < 16 || c->page_size > Q4K_MAX_PAGE_SIZE || (c->page_size & (c->page_size - 1)))
+    return fail(Q4K_ESHAPE, "page_size must be a power of two, 16..%u (got %u)", Q4K_MAX_PAGE_SIZE, c->page_size);
+  if (c->head_dim == 0 || c->head_dim % 8 != 0 || c->head_dim > 256)
+    return fail(Q4K_ESHAPE, "head_dim must be a multiple of 8 up to 256 (got %u)", c->head_dim);
+  if (c->heads == 0 || c->heads > 65535)
+    return fail(Q4K_ESHAPE, "the cache's heads must be 1..65535 (got %u)", c->heads);
+  if (c->pages > 0x7fffffffu || c->table_rows > 0x7fffffffu || (uint64_t)c->width * c->page_size > (1u << 30))
+    return fail(Q4K_ESHAPE, "a cache has up to 2^31 - 1 pages and tables, a table up to 2^30 tokens (got %u, %u, %u pages of %u)", c->pages,
+                c->table_rows, c->width, c->page_size);
+  const int64_t strides[3] = {c->page_stride, c->head_stride, c->token_stride};
+  for (int64_t s : strides)
+    if (s < 0 || s > kMaxCacheStride || s % 8 != 0)
+      return fail(Q4K_ESHAPE, "strides of the cache must be multiples of 8, 0..2^40 elements (got %lld)", (long long)s);
+  if ((c->pages && (!c->k || !c->v)) || !positions)
+    return fail(Q4K_EINVAL, "k, v and positions must be non-NULL");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 != 0)
+    return fail(Q4K_EINVAL, "k and v must be 16-byte aligned");
+  if (!c->tables && c->table_rows && c->width)
+    return fail(Q4K_EINVAL, "tables is NULL");
+  if (!c->slots && c->table_rows < nq)
+    return fail(Q4K_ESHAPE, "without slots every sequence needs a table (%u sequences, %u tables)", nq, c->table_rows);
+  return Q4K_OK;
+}
+
+// Whether two elements of the cache share a place.  k and v are one more axis, of
+// two: places differ where each axis's step, in the order of the steps, spans
+// all that lies below it.
+bool cache_places_meet(const q4k_cache* c) {
+  const uint64_t apart = (uint64_t)((uintptr_t)c->k > (uintptr_t)c->v ? (uintptr_t)c->k - (uintptr_t)c->v : (uintptr_t)c->v - (uintptr_t)c->k);
+  struct {
+    uint64_t step, count;
+  } axis[4] = {{(uint64_t)c->page_stride * 2, c->pages}, {(uint64_t)c->head_stride * 2, c->heads}, {(uint64_t)c->token_stride * 2, c->page_size}, {apart, 2}};
+  for (int i = 1; i < 4; ++i)
+    for (int j = i; j > 0 && (axis[j].count <= 1 ? 0 : axis[j].step) < (axis[j - 1].count <= 1 ? 0 : axis[j - 1].step); --j)
+      std::swap(axis[j], axis[j - 1]);
+  uint64_t span = (uint64_t)c->head_dim * 2;
+  for (const auto& x : axis) {
+    if (x.count <= 1)
+      continue;
+    if (x.step < span)
+      return true;
+    span += x.step * (x.count - 1);
+  }
+  return false;
+}
+
+CacheArgs cache_args(const q4k_cache* c, const int32_t* positions, const uint32_t* counts, uint32_t nq, uint32_t rows) {
+  CacheArgs a;
+  a.k = c->k;
+  a.v = c->v;
+  a.page_stride = c->page_stride;
+  a.head_stride = c->head_stride;
+  a.token_stride = c->token_stride;
+  a.tables = c->tables;
+  a.slots = c->slots;
+  a.positions = positions;
+  a.pages = c->pages;
+  a.heads = c->heads;
+  a.page_log = __builtin_ctz(c->page_size);
+  a.dim = (int)c->head_dim;
+  a.table_rows = c->width ? (int)c->table_rows : 0;
+  a.width = (int)c->width;
+  a.nq = counts ? (int)nq : 1;
+  int at = 0;
+  for (int i = 0; i < a.nq; ++i) {
+    a.start[i] = at;
+    a.count[i] = (int)(counts ? counts[i] : rows);
+    at += a.count[i];
+  }
+  return a;
+}
+
+// Whether `out` meets the tables, slots or positions of a call.
+bool meets_tables(const HeadSpan& out, const q4k_cache* c, const int32_t* positions, uint32_t nq) {
+  return span_meets(out, c->tables, (size_t)c->table_rows * c->width * 4) || span_meets(out, c->slots, (size_t)nq * 4) ||
+         span_meets(out, positions, (size_t)nq * 4);
+}
+
+int check_pool(const q4k_pool* p, const int32_t* tables, const int32_t* lengths, uint32_t slots, uint32_t width, const int32_t* new_tables) {
+  if (p->pages == 0 || p->pages > Q4K_MAX_POOL_PAGES)
+    return fail(Q4K_ESHAPE, "a pool has 1..%u pages (got %u)", Q4K_MAX_POOL_PAGES, p->pages);
+  if (p->page_size == 0 || p->page_size > (1u << 20) || (p->page_size & (p->page_size - 1)))
+    return fail(Q4K_ESHAPE, "page_size must be a power of two up to 2^20 (got %u)", p->page_size);
+  if (p->blocks == 0 || p->token_bytes == 0 || p->token_bytes % 16 != 0 || (uint64_t)p->page_size * p->token_bytes > (1u << 30) ||
+      (uint64_t)p->blocks * p->page_size * p->token_bytes > (1ull << 34))
+    return fail(Q4K_ESHAPE, "pages must be of 1 or more blocks of up to 2^30 bytes, 2^34 in all, token_bytes a multiple of 16 (got %u blocks of %u x %u)",
+                p->blocks, p->page_size, p->token_bytes);
+  if (slots > Q4K_MAX_SLOTS || (uint64_t)width * p->page_size > (1u << 30))
+    return fail(Q4K_ESHAPE, "up to %u slots of up to 2^30 tokens (got %u of %u pages of %u)", Q4K_MAX_SLOTS, slots, width, p->page_size);
+  if (!p->data || (slots && (!lengths || (width && (!tables || !new_tables)))))
+    return fail(Q4K_EINVAL, "data, tables, lengths and new_tables must be non-NULL");
+  if ((uintptr_t)p->data % 16 != 0)
+    return fail(Q4K_EINVAL, "the pool must be 16-byte aligned");
+  return Q4K_OK;
+}
+
+struct Bytes {
+  const void* p;
+  size_t bytes;
+};
+
+// Whether one of the first `written` ranges meets another of the n.
+bool any_meet(const Bytes* r, int n, int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = 0; j < n; ++j)
+      if (j != i && r[i].p && r[j].p && r[i].bytes && r[j].bytes && overlaps(r[i].p, r[i].bytes, r[j].p, r[j].bytes))
+        return true;
+  return false;
+}
+
+TableArgs table_args(const q4k_pool* p, const int32_t* tables, const int32_t* lengths, uint32_t slots, uint32_t width, int32_t* new_tables) {
+  TableArgs a;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.new_tables = new_tables;
+  a.pages = p->pages;
+  a.slots = (int)slots;
+  a.width = (int)width;
+  a.page_log = __builtin_ctz(p->page_size);
+  return a;
+}
+
+PoolArgs pool_args(const q4k_pool* p) {
+  PoolArgs a;
+  a.data = static_cast<uint8_t*>(p->data);
+  a.blocks = p->blocks;
+  a.block_bytes = p->page_size * p->token_bytes;
+  a.token_bytes = p->token_bytes;
+  return a;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2192,6 +2349,177 @@ int q4k_process_logits(void* stream, int device, const void* logits, void* out, 
     return scope.rc;
   LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_logits(static_cast<hipStream_t>(stream), a, (int)dtype, device_cus(device)), "logits launch");
+  return Q4K_OK;
+}
+
+int q4k_cache_write(void* stream, int device, const q4k_cache* cache, const q4k_heads* k, const q4k_heads* v, const int32_t* positions,
+                    const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype) {
+  if (!cache || !k || !v)
+    return fail(Q4K_EINVAL, "null argument");
+  if (dtype > Q4K_DTYPE_F16)
+    return fail(Q4K_EINVAL, "bad dtype %u", dtype);
+  int rc = check_sequences(query_counts, nqueries, rows);
+  if (!rc)
+    rc = check_cache(cache, positions, query_counts ? nqueries : 1);
+  if (rc)
+    return rc;
+  if (cache->pages && cache_places_meet(cache))
+    return fail(Q4K_ESHAPE, "places of the cache meet (strides %lld, %lld, %lld, k and v %lld bytes apart)", (long long)cache->page_stride,
+                (long long)cache->head_stride, (long long)cache->token_stride, (long long)((intptr_t)cache->v - (intptr_t)cache->k));
+  const int64_t strides[4] = {k->in_row_stride, k->in_head_stride, v->in_row_stride, v->in_head_stride};
+  for (int64_t s : strides)
+    if (s < 0 || s > kMaxCacheStride)
+      return fail(Q4K_ESHAPE, "strides must be 0..2^40 elements (got %lld)", (long long)s);
+  if ((uint64_t)rows * cache->heads * cache->head_dim > (1ull << 33))
+    return fail(Q4K_ESHAPE, "at most 2^33 values (got %u rows of %u heads of %u)", rows, cache->heads, cache->head_dim);
+  if (rows == 0 || cache->pages == 0 || cache->width == 0)
+    return Q4K_OK;
+  if (!k->in || !v->in)
+    return fail(Q4K_EINVAL, "k and v must be non-NULL");
+  const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2, extent = cache_extent(cache), nq = query_counts ? nqueries : 1;
+  const Bytes ranges[] = {{cache->k, extent}, {cache->v, extent},
+                          {k->in, ((size_t)(rows - 1) * k->in_row_stride + (size_t)(cache->heads - 1) * k->in_head_stride + cache->head_dim) * es},
+                          {v->in, ((size_t)(rows - 1) * v->in_row_stride + (size_t)(cache->heads - 1) * v->in_head_stride + cache->head_dim) * es},
+                          {cache->tables, (size_t)cache->table_rows * cache->width * 4}, {cache->slots, nq * 4}, {positions, nq * 4}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 2; j < 7; ++j)
+      if (ranges[j].p && ranges[j].bytes && overlaps(ranges[i].p, ranges[i].bytes, ranges[j].p, ranges[j].bytes))
+        return fail(Q4K_EALIAS, "the cache must not overlap the rows, tables, slots or positions");
+  const CacheArgs a = cache_args(cache, positions, query_counts, nqueries, rows);
+  CacheRows in;
+  in.k = k->in;
+  in.v = v->in;
+  in.k_row = k->in_row_stride;
+  in.k_head = k->in_head_stride;
+  in.v_row = v->in_row_stride;
+  in.v_head = v->in_head_stride;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_cache_write(static_cast<hipStream_t>(stream), a, in, rows, (int)dtype), "cache write launch");
+  return Q4K_OK;
+}
+
+int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache* cache, const q4k_attention_params* params,
+                  const int32_t* positions, const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype) {
+  if (!q || !cache || !params)
+    return fail(Q4K_EINVAL, "null argument");
+  if (dtype > Q4K_DTYPE_F16)
+    return fail(Q4K_EINVAL, "bad dtype %u", dtype);
+  const uint32_t nq = query_counts ? nqueries : 1;
+  int rc = check_sequences(query_counts, nqueries, rows);
+  if (!rc)
+    rc = check_cache(cache, positions, nq);
+  if (rc)
+    return rc;
+  if (q->heads % cache->heads != 0)
+    return fail(Q4K_ESHAPE, "the heads of q must be a multiple of the cache's (got %u and %u)", q->heads, cache->heads);
+  if (!std::isfinite(params->scale) || !std::isfinite(params->softcap) || params->softcap < 0.0f || params->window > 0x7fffffffu)
+    return fail(Q4K_EINVAL, "scale must be finite, softcap finite and not negative, window below 2^31");
+  const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2;
+  HeadSpan in, out;
+  rc = check_heads("q", q, rows, cache->head_dim, es, &in, &out);
+  if (rc || rows == 0)
+    return rc;
+  if (spans_meet(in, out) || q->in == q->out)
+    return fail(Q4K_EALIAS, "out must not overlap q");
+  const size_t extent = cache_extent(cache);
+  if (span_meets(out, cache->k, extent) || span_meets(out, cache->v, extent) || meets_tables(out, cache, positions, nq) ||
+      span_meets(out, params->slopes, (size_t)q->heads * 4))
+    return fail(Q4K_EALIAS, "out must not overlap the cache, tables, slots, positions or slopes");
+  AttentionArgs a;
+  a.cache = cache_args(cache, positions, query_counts, nqueries, rows);
+  a.q = q->in;
+  a.out = q->out;
+  a.q_row = q->in_row_stride;
+  a.q_head = q->in_head_stride;
+  a.out_row = q->out_row_stride;
+  a.out_head = q->out_head_stride;
+  a.slopes = params->slopes;
+  a.scale = params->scale;
+  a.softcap = params->softcap;
+  a.heads = (int)q->heads;
+  a.group = (int)(q->heads / cache->heads);
+  a.rows = (int)rows;
+  a.window = (int)params->window;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_attention(static_cast<hipStream_t>(stream), a, (int)dtype, device_cus(device)), "attention launch");
+  return Q4K_OK;
+}
+
+int q4k_cache_assign(void* stream, int device, const q4k_pool* pool, const int32_t* tables, const int32_t* lengths, uint32_t slots, uint32_t width,
+                     const int32_t* parents, const int32_t* counts, int32_t* new_tables, int32_t* new_lengths, int32_t* missing) {
+  if (!pool)
+    return fail(Q4K_EINVAL, "pool is NULL");
+  int rc = check_pool(pool, tables, lengths, slots, width, new_tables);
+  if (rc)
+    return rc;
+  if (slots && !new_lengths)
+    return fail(Q4K_EINVAL, "new_lengths must be non-NULL");
+  const uint64_t page = (uint64_t)pool->blocks * pool->page_size * pool->token_bytes;
+  const size_t t = (size_t)slots * width * 4, n = (size_t)slots * 4;
+  const Bytes ranges[] = {{new_tables, t}, {new_lengths, n}, {missing, 4}, {pool->data, page * pool->pages}, {tables, t}, {lengths, n}, {parents, n}, {counts, n}};
+  if (any_meet(ranges, 8, 4))
+    return fail(Q4K_EALIAS, "new_tables, new_lengths, missing and the pool must not overlap each other or what is read");
+  if (slots == 0 && !missing)
+    return Q4K_OK;
+  TableArgs a = table_args(pool, tables, lengths, slots, width, new_tables);
+  a.parents = parents;
+  a.counts = counts;
+  a.new_lengths = new_lengths;
+  a.missing = missing;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  {
+    LaunchTimer timer(s, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_cache_assign(s, a), "cache assign launch");
+  }
+  if (slots < 2 || width == 0 || pool->page_size == 1)  // no page can have two holders, or none is filled in part
+    return Q4K_OK;
+  LaunchTimer timer(s, Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_page_fork(s, a, pool_args(pool)), "page fork launch");
+  return Q4K_OK;
+}
+
+int q4k_cache_compact(void* stream, int device, const q4k_pool* pool, const int32_t* tables, const int32_t* lengths, uint32_t slots,
+                      uint32_t width, int32_t* new_tables, int32_t* used) {
+  if (!pool)
+    return fail(Q4K_EINVAL, "pool is NULL");
+  int rc = check_pool(pool, tables, lengths, slots, width, new_tables);
+  if (rc)
+    return rc;
+  const uint64_t page = (uint64_t)pool->blocks * pool->page_size * pool->token_bytes;
+  const size_t t = (size_t)slots * width * 4, n = (size_t)slots * 4;
+  const Bytes ranges[] = {{new_tables, t}, {used, 4}, {pool->data, page * pool->pages}, {tables, t}, {lengths, n}};
+  if (any_meet(ranges, 5, 3))
+    return fail(Q4K_EALIAS, "new_tables, used and the pool must not overlap each other or what is read");
+  if (slots == 0 && !used)
+    return Q4K_OK;
+  TableArgs a = table_args(pool, tables, lengths, slots, width, new_tables);
+  a.missing = used;
+  DeviceScope scope(device);
+  if (scope.rc)
+    return scope.rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Workspace& ws = workspace(device);
+  std::lock_guard<std::mutex> lock(ws.mu);
+  reserve_workspace(s, ws, device);
+  rc = ensure_buffer(s, ws, device, ws.part, ws.part_elems, (size_t)pool->pages + 2, "split-K workspace");
+  if (rc)
+    return rc;
+  int32_t* moves = reinterpret_cast<int32_t*>(ws.part);
+  {
+    LaunchTimer timer(s, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_cache_compact(s, a, moves), "cache compact launch");
+  }
+  LaunchTimer timer(s, Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_page_move(s, moves, pool_args(pool), pool->pages, device_cus(device)), "page move launch");
   return Q4K_OK;
 }
 

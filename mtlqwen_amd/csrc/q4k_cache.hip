@@ -1,0 +1,339 @@
+// The paged key/value cache besides the attention that reads it: keys and
+// values of new tokens into their pages (cache_write_kernel), slots that take
+// over the states of others (cache_assign_kernel), pages moved to the front of
+// the pool (cache_compact_kernel), and the copies that the last two ask for.
+#include "q4k_device.h"
+
+namespace q4k {
+namespace {
+
+// ----------------------------------------------------------------------------
+// Row t of sequence q goes to position p = positions[q] + t: token p % page_size
+// of page tables[slot of q][p / page_size], rounded to fp16 (the cache's type;
+// half a step, 2^-11 of the value).  A lane moves 8 values of one head; keys and
+// values of a row are 2 * heads * dim / 8 lanes next to each other.  Bound by
+// memory: every value is read and written once.
+// ----------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs c, CacheRows in, uint32_t per_row, uint32_t rows) {
+  const uint32_t chunks = (uint32_t)c.dim >> 3;
+  const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t row = (uint32_t)(item / per_row);
+  if (row >= rows)
+    return;
+  uint32_t at = (uint32_t)(item - (uint64_t)row * per_row);
+  const bool value = at >= (per_row >> 1);
+  at -= value ? per_row >> 1 : 0;
+  const uint32_t head = at / chunks, d = (at - head * chunks) << 3;
+  const T* x = static_cast<const T*>(value ? in.v : in.k) + (int64_t)row * (value ? in.v_row : in.k_row) + (int64_t)head * (value ? in.v_head : in.k_head) + d;
+  float f[8];
+  load8(x, f);
+  int q = 0;
+  while (q + 1 < c.nq && row >= (uint32_t)c.start[q + 1])
+    ++q;
+  const int64_t pos = (int64_t)c.positions[q] + (row - (uint32_t)c.start[q]);
+  const int slot = c.slots ? c.slots[q] : q;
+  if (pos < 0 || pos >> c.page_log >= c.width || (uint32_t)slot >= (uint32_t)c.table_rows)
+    return;
+  const int32_t page = c.tables[(int64_t)slot * c.width + (pos >> c.page_log)];
+  if ((uint32_t)page >= c.pages)
+    return;
+  _Float16* y = static_cast<_Float16*>(value ? c.v : c.k) + (int64_t)page * c.page_stride + (int64_t)head * c.head_stride +
+                (pos & ((1 << c.page_log) - 1)) * c.token_stride + d;
+  h8_t h;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    h[i] = (_Float16)f[i];
+  *reinterpret_cast<h8_t*>(y) = h;
+}
+
+// ----------------------------------------------------------------------------
+// Tables.  One workgroup of 1024 threads per call: which pages are held is a
+// bit per page in LDS (up to 2^18 pages, 32 KB), so nothing about the pool is
+// kept between calls, and the lowest free pages are found by counting bits.
+// ----------------------------------------------------------------------------
+constexpr int kTableThreads = 1024;
+
+// Sum over the threads before this one, and over all of them.  `sums` holds 17
+// words; free for the next call behind the caller's next barrier.
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* sums, uint32_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t s = v;
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t o = __shfl_up(s, off);
+    s += lane >= off ? o : 0;
+  }
+  if (lane == 63)
+    sums[wave] = s;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (int w = 0; w < kTableThreads / 64; ++w) {
+    before += w < wave ? sums[w] : 0;
+    all += sums[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + s - v;
+}
+
+__device__ __forceinline__ bool bit_of(const uint32_t* bits, uint32_t p) {
+  return (bits[p >> 5] >> (p & 31)) & 1;
+}
+
+// Bits of the words past the last page are set: no page there is free.
+__device__ __forceinline__ void clear_bits(uint32_t* bits, uint32_t pages) {
+  for (uint32_t w = threadIdx.x; w < kMaxPages / 32; w += kTableThreads)
+    bits[w] = 32 * w >= pages ? ~0u : pages - 32 * w < 32 ? ~0u << (pages - 32 * w) : 0u;
+}
+
+// A slot's tokens: not negative, no more than its table holds.
+__device__ __forceinline__ int32_t tokens_of(int32_t length, const TableArgs& a) {
+  const int64_t most = (int64_t)a.width << a.page_log;
+  return length < 0 ? 0 : length > most ? (int32_t)most : length;
+}
+
+// Slot s takes the first lengths[p] tokens of its parent p.  Pages full of tokens are
+// shared.  A page that is not full will be written on, so it can stay with one
+// slot only: with the lowest of those that hold it, unless another holds it as a
+// full page; the others get a page of their own and a copy (page_fork_kernel).
+// Then, slot by slot, the lowest free pages for counts[s] more tokens.
+__global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a) {
+  __shared__ uint32_t bits[kMaxPages / 32], sums[17], before[kMaxSlots + 1];
+  __shared__ int32_t parent[kMaxSlots], last[kMaxSlots], full[kMaxSlots], first[kMaxSlots], kept[kMaxSlots];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  clear_bits(bits, a.pages);
+  int32_t length = 0;
+  if (tid < a.slots) {
+    const int32_t p = a.parents ? a.parents[tid] : tid;
+    const bool live = (uint32_t)p < (uint32_t)a.slots;
+    length = live ? tokens_of(a.lengths[p], a) : 0;
+    parent[tid] = live ? p : 0;
+    full[tid] = length >> a.page_log;
+  }
+  __syncthreads();
+  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
+    const int32_t* t = a.tables + (int64_t)parent[s] * a.width;
+    for (int e = lane; e < full[s]; e += 64) {
+      const uint32_t p = (uint32_t)t[e];
+      if (p < a.pages)
+        atomicOr(&bits[p >> 5], 1u << (p & 31));
+    }
+  }
+  const bool part = length & ((1 << a.page_log) - 1);
+  if (tid < a.slots) {
+    const int32_t p = part ? a.tables[(int64_t)parent[tid] * a.width + full[tid]] : -1;
+    last[tid] = (uint32_t)p < a.pages ? p : -1;
+  }
+  __syncthreads();
+  bool keep = false;
+  if (tid < a.slots && last[tid] >= 0) {
+    keep = !bit_of(bits, (uint32_t)last[tid]);
+    for (int s = 0; s < tid && keep; ++s)
+      keep = last[s] != last[tid];
+  }
+  __syncthreads();
+  uint32_t wants = 0, beyond = 0;
+  if (tid < a.slots) {
+    if (keep)
+      atomicOr(&bits[last[tid] >> 5], 1u << (last[tid] & 31));
+    // A page that the parent's table lacks stays lacking.
+    const int32_t from = full[tid] + (part && (keep || last[tid] < 0));
+    const int32_t count = a.counts ? a.counts[tid] : 0;
+    const int64_t need = ((int64_t)length + (count > 0 ? count : 0) + (1 << a.page_log) - 1) >> a.page_log;
+    const int64_t most = need < a.width ? need : a.width;
+    wants = most > from ? (uint32_t)(most - from) : 0;
+    beyond = (uint32_t)(need - most);
+    first[tid] = from;
+    kept[tid] = keep;
+    a.new_lengths[tid] = length;
+  }
+  uint32_t asked, lacking, there;
+  const uint32_t mine = scan_before(wants, sums, &asked);
+  if (tid < a.slots)
+    before[tid] = mine;
+  if (tid == 0)
+    before[a.slots] = asked;
+  (void)scan_before(beyond, sums, &lacking);
+  constexpr int kWords = kMaxPages / 32 / kTableThreads;
+  uint32_t n = 0;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    n += 32 - __popc(bits[tid * kWords + w]);
+  uint32_t rank = scan_before(n, sums, &there);
+  if (tid == 0 && a.missing)
+    *a.missing = (int32_t)(lacking + (asked > there ? asked - there : 0));
+  // Request r of slot s (before[s] <= r < before[s + 1]) takes the r-th free page.
+  for (int w = 0; w < kWords && rank < asked; ++w) {
+    uint32_t open = ~bits[tid * kWords + w];
+    for (; open && rank < asked; open &= open - 1, ++rank) {
+      int lo = 0, hi = a.slots;  // before[lo] <= rank < before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (before[mid] <= rank ? lo : hi) = mid;
+      }
+      a.new_tables[(int64_t)lo * a.width + first[lo] + (rank - before[lo])] = 32 * (tid * kWords + w) + __ffs(open) - 1;
+    }
+  }
+  const uint32_t given = asked < there ? asked : there;
+  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
+    const int32_t* t = a.tables + (int64_t)parent[s] * a.width;
+    int32_t* y = a.new_tables + (int64_t)s * a.width;
+    const int64_t to = first[s] + (before[s] >= given ? 0 : (int64_t)(before[s + 1] < given ? before[s + 1] : given) - before[s]);
+    for (int e = lane; e < a.width; e += 64) {
+      if (e >= first[s] && e < to)
+        continue;  // given above
+      const bool old = e < full[s] || (e == full[s] && kept[s]);
+      const int32_t p = old ? t[e] : -1;
+      y[e] = (uint32_t)p < a.pages ? p : -1;
+    }
+  }
+}
+
+// The pages that cache_assign_kernel gave in place of ones that are shared: what
+// their slots hold of them, `part` tokens of every block.  A workgroup copies up
+// to kCopyBytes of a block.
+constexpr uint32_t kCopyBytes = 16384;
+
+__device__ __forceinline__ void copy_bytes(const uint8_t* from, uint8_t* to, uint32_t bytes) {
+  constexpr int kDeep = 4;
+  u4_t v[kDeep];
+  for (uint32_t at = threadIdx.x * 16; at < bytes; at += 256 * 16 * kDeep) {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (at + i * 4096 < bytes)
+        v[i] = *reinterpret_cast<const u4_t*>(from + at + i * 4096);
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (at + i * 4096 < bytes)
+        *reinterpret_cast<u4_t*>(to + at + i * 4096) = v[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void page_fork_kernel(TableArgs a, PoolArgs p) {
+  const uint32_t s = blockIdx.y;
+  const int32_t from = a.parents ? a.parents[s] : (int32_t)s;
+  if ((uint32_t)from >= (uint32_t)a.slots)
+    return;
+  const int32_t length = tokens_of(a.lengths[from], a), full = length >> a.page_log;
+  const uint32_t tokens = (uint32_t)length & ((1u << a.page_log) - 1);
+  if (!tokens)
+    return;
+  const int32_t src = a.tables[(int64_t)from * a.width + full], dst = a.new_tables[(int64_t)s * a.width + full];
+  if ((uint32_t)src >= a.pages || (uint32_t)dst >= a.pages || src == dst)
+    return;
+  const uint64_t bytes = (uint64_t)tokens * p.token_bytes;
+  const uint32_t block = blockIdx.x / p.parts;
+  const uint64_t at = (uint64_t)(blockIdx.x - block * p.parts) * kCopyBytes;
+  if (at >= bytes)
+    return;
+  const uint64_t off = (uint64_t)block * p.block_bytes + at, page = (uint64_t)p.blocks * p.block_bytes;
+  copy_bytes(p.data + (uint64_t)src * page + off, p.data + (uint64_t)dst * page + off, (uint32_t)(bytes - at < kCopyBytes ? bytes - at : kCopyBytes));
+}
+
+// Of the n pages held by any slot, the i-th at or behind page n moves to the i-th
+// free one before it: no page is read that another is written over.  moves[0]
+// = their number, then the pairs.
+__global__ __launch_bounds__(kTableThreads) void cache_compact_kernel(TableArgs a, int32_t* moves) {
+  __shared__ uint32_t bits[kMaxPages / 32], sums[17], chunk[kTableThreads];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int w = tid; w < (int)(kMaxPages / 32); w += kTableThreads)
+    bits[w] = 0;
+  __syncthreads();
+  const int round = (1 << a.page_log) - 1;
+  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
+    const int held = (int)(((int64_t)tokens_of(a.lengths[s], a) + round) >> a.page_log);
+    for (int e = lane; e < held; e += 64) {
+      const uint32_t p = (uint32_t)a.tables[(int64_t)s * a.width + e];
+      if (p < a.pages)
+        atomicOr(&bits[p >> 5], 1u << (p & 31));
+    }
+  }
+  __syncthreads();
+  constexpr int kWords = kMaxPages / 32 / kTableThreads;
+  uint32_t n = 0, used;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    n += __popc(bits[tid * kWords + w]);
+  const uint32_t mine = scan_before(n, sums, &used);
+  chunk[tid] = mine;
+  __syncthreads();
+  const auto held_before = [&](uint32_t p) {
+    uint32_t r = chunk[p / (32 * kWords)];
+    for (uint32_t w = p / (32 * kWords) * kWords; w < (p >> 5); ++w)
+      r += __popc(bits[w]);
+    return r + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1));
+  };
+  const uint32_t low = used < kMaxPages ? held_before(used) : used;  // pages that stay
+  if (tid == 0) {
+    moves[0] = (int32_t)(used - low);
+    if (a.missing)
+      *a.missing = (int32_t)used;
+  }
+  uint32_t rank = mine;  // held pages before the present one
+  for (int w = 0; w < kWords; ++w) {
+    const uint32_t word = bits[tid * kWords + w], p0 = 32 * (tid * kWords + w);
+    if (p0 < used)  // holes before page `used`
+      for (uint32_t open = ~word; open; open &= open - 1) {
+        const uint32_t b = (uint32_t)__ffs(open) - 1, p = p0 + b;
+        if (p < used)
+          moves[2 + 2 * (p - rank - __popc(word & ((1u << b) - 1)))] = (int32_t)p;
+      }
+    if (p0 + 31 >= used)  // pages to move
+      for (uint32_t held = word; held; held &= held - 1) {
+        const uint32_t b = (uint32_t)__ffs(held) - 1, p = p0 + b;
+        if (p >= used)
+          moves[1 + 2 * (rank + __popc(word & ((1u << b) - 1)) - low)] = (int32_t)p;
+      }
+    rank += __popc(word);
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
+    const int held = (int)(((int64_t)tokens_of(a.lengths[s], a) + round) >> a.page_log);
+    for (int e = lane; e < a.width; e += 64) {
+      const uint32_t p = e < held ? (uint32_t)a.tables[(int64_t)s * a.width + e] : ~0u;
+      int32_t to = p < a.pages ? (int32_t)p : -1;
+      if (p < a.pages && p >= used)
+        to = moves[2 + 2 * (held_before(p) - low)];
+      a.new_tables[(int64_t)s * a.width + e] = to;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void page_move_kernel(const int32_t* moves, PoolArgs p) {
+  const uint64_t page = (uint64_t)p.blocks * p.block_bytes, at = (uint64_t)blockIdx.x * kCopyBytes;
+  const uint32_t bytes = (uint32_t)(page - at < kCopyBytes ? page - at : kCopyBytes);
+  const int n = moves[0];
+  for (int i = blockIdx.y; i < n; i += gridDim.y)
+    copy_bytes(p.data + (uint64_t)moves[1 + 2 * i] * page + at, p.data + (uint64_t)moves[2 + 2 * i] * page + at, bytes);
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(hipStream_t s, const CacheArgs& c, const CacheRows& in, uint32_t rows, int dtype) {
+  const uint32_t per_row = 2 * c.heads * (uint32_t)c.dim / 8;
+  const dim3 grid((uint32_t)(((uint64_t)rows * per_row + 255) / 256)), block(256);
+  return dtype == kF32 ? dispatch(cache_write_kernel<float>, grid, block, s, c, in, per_row, rows)
+                       : dispatch(cache_write_kernel<_Float16>, grid, block, s, c, in, per_row, rows);
+}
+
+hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a) {
+  return dispatch(cache_assign_kernel, dim3(1), dim3(kTableThreads), s, a);
+}
+
+hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p) {
+  p.parts = (p.block_bytes + kCopyBytes - 1) / kCopyBytes;
+  return dispatch(page_fork_kernel, dim3(p.blocks * p.parts, a.slots), dim3(256), s, a, p);
+}
+
+hipError_t launch_cache_compact(hipStream_t s, const TableArgs& a, int32_t* moves) {
+  return dispatch(cache_compact_kernel, dim3(1), dim3(kTableThreads), s, a, moves);
+}
+
+hipError_t launch_page_move(hipStream_t s, const int32_t* moves, const PoolArgs& p, uint32_t pages, int cus) {
+  const uint32_t parts = (uint32_t)(((uint64_t)p.blocks * p.block_bytes + kCopyBytes - 1) / kCopyBytes);
+  const uint32_t want = (16u * (uint32_t)cus + parts - 1) / parts, most = pages / 2 > 0 ? pages / 2 : 1;
+  return dispatch(page_move_kernel, dim3(parts, want < most ? want : most), dim3(256), s, moves, p);
+}
+
+}  // namespace q4k

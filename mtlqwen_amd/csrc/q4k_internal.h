@@ -586,6 +586,67 @@ struct LogitsArgs {
 };
 hipError_t launch_logits(hipStream_t s, LogitsArgs a, int dtype, int cus);
 
+// A layer's keys and values in pages (q4k_cache.hip, q4k_attention.hip): element d
+// of token t of head h of a page is at page * page_stride + h * head_stride + t *
+// token_stride + d of k and of v.  Strides count elements and are multiples of 8.
+constexpr int kMaxSequences = 64;
+struct CacheArgs {
+  void* k = nullptr;
+  void* v = nullptr;
+  int64_t page_stride = 0, head_stride = 0, token_stride = 0;
+  const int32_t* tables = nullptr;     // [table_rows, width] pages, others than 0 .. pages - 1: none
+  const int32_t* slots = nullptr;      // [nq] the table row of each sequence, or nullptr: q
+  const int32_t* positions = nullptr;  // [nq] of the first new token
+  uint32_t pages = 0, heads = 0;
+  int page_log = 0, dim = 0, table_rows = 0, width = 0, nq = 0;
+  int start[kMaxSequences] = {}, count[kMaxSequences] = {};  // rows of the sequences
+};
+// Keys and values of the new tokens.
+struct CacheRows {
+  const void* k = nullptr;
+  const void* v = nullptr;
+  int64_t k_row = 0, k_head = 0, v_row = 0, v_head = 0;
+};
+hipError_t launch_cache_write(hipStream_t s, const CacheArgs& c, const CacheRows& in, uint32_t rows, int dtype);
+
+struct AttentionArgs {
+  CacheArgs cache;
+  const void* q = nullptr;
+  void* out = nullptr;
+  int64_t q_row = 0, q_head = 0, out_row = 0, out_head = 0;
+  const float* slopes = nullptr;  // [heads] or nullptr
+  float scale = 1.0f, softcap = 0.0f;
+  int heads = 0, group = 1, rows = 0;
+  int window = 0;  // keys that a row sees, its own the last; 0: all before it
+};
+hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype, int cus);
+
+// Tables of all slots, as they are and as they become.
+constexpr uint32_t kMaxPages = 1u << 18;
+constexpr int kMaxSlots = 1024;
+struct TableArgs {
+  const int32_t* tables = nullptr;   // [slots, width]
+  const int32_t* lengths = nullptr;  // [slots] tokens held
+  const int32_t* parents = nullptr;  // [slots] or nullptr: each its own
+  const int32_t* counts = nullptr;   // [slots] or nullptr: no tokens to come
+  int32_t* new_tables = nullptr;
+  int32_t* new_lengths = nullptr;
+  int32_t* missing = nullptr;  // pages asked for and not given (assign), pages held (compact); or nullptr
+  uint32_t pages = 0;
+  int slots = 0, width = 0, page_log = 0;
+};
+// A page is `blocks` runs of block_bytes = page size * token_bytes.
+struct PoolArgs {
+  uint8_t* data = nullptr;
+  uint32_t blocks = 0, block_bytes = 0, token_bytes = 0;
+  uint32_t parts = 0;  // set by the launch: workgroups of a block
+};
+hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a);
+hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p);
+// moves: 1 + pages + pages % 2 values.
+hipError_t launch_cache_compact(hipStream_t s, const TableArgs& a, int32_t* moves);
+hipError_t launch_page_move(hipStream_t s, const int32_t* moves, const PoolArgs& p, uint32_t pages, int cus);
+
 // Device-side GGUF -> tiled re-layout (src and dst are device buffers).
 hipError_t launch_relayout(hipStream_t s, const uint8_t* src, uint8_t* dst, uint32_t n, uint32_t k);
 

@@ -1,13 +1,16 @@
 """The operators of a decoder pass around its projections: rotary positions
 and head norms (``rope``, ``qk_norm_rope``; the reference's attention_prepare,
 attention.metal:15), low-rank adapters beside a projection (``lora``,
-``linear_lora``) and penalties, biases and grammar masks on logits
-(``process_logits``).
+``linear_lora``), attention over a paged key/value cache and what a server does
+with its pages (``attention``, ``cache_write``, ``cache_assign``,
+``cache_compact``; the reference's attention_scan and attention_reduce,
+attention.metal:104-216, over its sparse pages, device.cpp:147-198) and
+penalties, biases and grammar masks on logits (``process_logits``).
 
 All work is done by libq4k.so through its C ABI.  Tensors are torch tensors on
 one GPU; every call launches on ``stream`` (default: the current stream of that
 GPU) and returns without waiting.  What describes a batch on the device
-(positions, adapter ids, texts, biases, masks) is read when the call runs, so
+(positions, adapter ids, page tables, texts, biases, masks) is read when the call runs, so
 a captured call follows it from replay to replay.
 """
 import ctypes
@@ -26,6 +29,9 @@ _HEADS = struct.Struct("=3Q4qI4x").pack
 _ROTATION = struct.Struct("=2Q2If4x").pack
 _ADAPTERS = struct.Struct("=5Q2I").pack
 _LOGITS = struct.Struct("=12Q5I4x").pack
+_CACHE = struct.Struct("=2Q3q2Q6I").pack
+_ATTENTION = struct.Struct("=2fQI4x").pack
+_POOL = struct.Struct("=Q4I").pack
 _COUNTS = [struct.Struct(f"={n}I").pack for n in range(65)]
 
 try:
@@ -41,6 +47,7 @@ def _stream_of(stream):
 
 _rope, _qk_norm_rope, _lora, _linear_lora, _process_logits = (lib.q4k_rope, lib.q4k_qk_norm_rope, lib.q4k_lora, lib.q4k_linear_lora,
                                                               lib.q4k_process_logits)
+_attention, _cache_write, _cache_assign, _cache_compact = lib.q4k_attention, lib.q4k_cache_write, lib.q4k_cache_assign, lib.q4k_cache_compact
 
 
 def _cut(*sizes):
@@ -227,6 +234,166 @@ def linear_lora(x, w, a, b, adapter_ids, count, output, auxiliary=None, gated=Fa
     return output
 
 
+def _sequences(query_counts, rows):
+    """(packed counts, sequences, rows that they cover) of up to ``rows`` rows."""
+    if query_counts is None:
+        return _COUNTS[1](rows), 1, rows
+    n = len(query_counts)
+    covered = sum(query_counts)
+    if covered > rows:
+        raise ValueError(f"query_counts cover {covered} rows, there are {rows}")
+    return (_COUNTS[n] if n < len(_COUNTS) else struct.Struct(f"={n}I").pack)(*query_counts), n, covered
+
+
+def _cache(k_cache, v_cache, tables, slots, positions, sequences, device):
+    """A q4k_cache, and the address of the positions."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache and v_cache must be [pages, heads, page_size, head_dim] alike, got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    if k_cache.dtype is not torch.float16 or v_cache.dtype is not torch.float16:
+        raise TypeError(f"k_cache and v_cache must be float16, got {k_cache.dtype} and {v_cache.dtype}")
+    if k_cache.get_device() != device or v_cache.get_device() != device:
+        raise ValueError(f"k_cache and v_cache must be on cuda:{device}")
+    pages, heads, size, dim = k_cache.shape
+    strides = k_cache.stride()
+    if strides != v_cache.stride() or (strides[3] != 1 and dim > 1):
+        raise ValueError("k_cache and v_cache must have the same strides and contiguous tokens")
+    if tables.dim() != 2:
+        raise ValueError("tables must be [table rows, width]")
+    rows, width = tables.shape
+    if (pages | heads | size | dim | rows | width) >> 32:
+        raise _cut(pages, heads, size, dim, rows, width)
+    i32 = torch.int32
+    return (_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], _address(tables, i32, 0, device, "tables"),
+                   _address(slots, i32, sequences, device, "slots"), pages, size, heads, dim, rows, width),
+            _address(positions, i32, sequences, device, "positions"))
+
+
+def _rows_of(t, like, what):
+    """A q4k_heads of ``t``, read only, of the dtype, GPU, rows and head_dim of ``like``."""
+    if t.dim() != 3 or t.dtype is not like.dtype or t.get_device() != like.get_device() or t.shape[0] != like.shape[0]:
+        raise ValueError(f"{what} must be [rows, heads, head_dim], of k's dtype, GPU and rows")
+    row, head, element = t.stride()
+    if element != 1 and t.shape[2] > 1:
+        raise ValueError(f"the elements of a head of {what} must be contiguous")
+    return _HEADS(t.data_ptr(), 0, 0, row, head, 0, 0, t.shape[1])
+
+
+def cache_write(k, v, k_cache, v_cache, tables, positions, query_counts=None, slots=None, stream=None):
+    """Keys and values of new tokens into their pages: row t of sequence q of
+    ``k`` and ``v`` [rows, heads, head_dim] (float32 or float16, any row and head
+    strides; ``query_counts`` as linear's, up to 64 sequences, default one) goes to
+    position positions[q] + t, rounded to float16.  ``k_cache`` and ``v_cache`` are
+    [pages, heads, page_size, head_dim], views of any page, head and token strides
+    (multiples of 8; page_size a power of two from 16, head_dim a multiple of 8 up to 256).
+    ``tables`` (int32 [table rows, width]) lists the pages of a sequence's tokens 0,
+    1, ... in row ``slots``[q] (int32, default: q); numbers outside the cache are
+    pages that are not there.  Rows behind the last sequence, and rows whose place
+    is not there, are not written."""
+    code, device = _activations(k, "k")
+    if k.dim() != 3 or k_cache.dim() != 4 or k.shape[1] != k_cache.shape[1] or k.shape[2] != k_cache.shape[3] or v.shape != k.shape:
+        raise ValueError(f"k and v must be [rows, heads, head_dim] of the cache's heads, got {tuple(k.shape)} and {tuple(v.shape)} for a cache of "
+                         f"{tuple(k_cache.shape)}")
+    counts, sequences, rows = _sequences(query_counts, k.shape[0])
+    if rows >> 32:
+        raise _cut(rows)
+    cache, at = _cache(k_cache, v_cache, tables, slots, positions, sequences, device)
+    rc = _cache_write(_raw_stream(device) if stream is None else _stream_of(stream), device, cache, _rows_of(k, k, "k"), _rows_of(v, k, "v"), at,
+                      counts, sequences, rows, code)
+    if rc:
+        check(rc)
+    return k_cache, v_cache
+
+
+def attention(q, k_cache, v_cache, tables, positions, out, query_counts=None, slots=None, scale=None, softcap=0.0, window=0, slopes=None,
+              stream=None):
+    """Causal attention of new tokens over their sequences' pages (cache_write's,
+    the new tokens' own keys and values among them): row t of sequence q of ``q``
+    [rows, heads, head_dim] stands at positions[q] + t and sees the keys up to
+    there, head h those of cache head h // (heads / cache heads).  Scores are
+    ``scale`` (default 1 / sqrt(head_dim)) times the products; above 0,
+    ``softcap`` bounds them (softcap * tanh(score / softcap)) and ``window`` is the
+    number of keys that a row sees, its own the last; ``slopes`` (float32 [heads])
+    times the (negative) distance to the key is added.  ``out`` is like ``q``, of
+    any row and head strides, and must not overlap it.  A row that sees no key
+    becomes zero; rows behind the last sequence are left as they were."""
+    code, device = _activations(q, "q")
+    heads = _heads(q, out, 0, "q")
+    if k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3]:
+        raise ValueError(f"q must have the cache's head_dim, got {tuple(q.shape)} for a cache of {tuple(k_cache.shape)}")
+    counts, sequences, rows = _sequences(query_counts, q.shape[0])
+    if rows >> 32 or window >> 32:
+        raise _cut(rows, window)
+    cache, at = _cache(k_cache, v_cache, tables, slots, positions, sequences, device)
+    params = _ATTENTION(q.shape[2] ** -0.5 if scale is None else scale, softcap, _address(slopes, torch.float32, q.shape[1], device, "slopes"),
+                        window)
+    rc = _attention(_raw_stream(device) if stream is None else _stream_of(stream), device, heads, cache, params, at, counts, sequences, rows, code)
+    if rc:
+        check(rc)
+    return out
+
+
+def _pool(pool, tables, lengths, new_tables):
+    """(q4k_pool, device, slots, width) of a pool [pages, ..., page_size, token]."""
+    device = pool.get_device()
+    if device < 0:
+        raise ValueError("pool must be a GPU tensor")
+    if pool.dim() < 3 or not pool.is_contiguous():
+        raise ValueError("pool must be contiguous, [pages, ..., page_size, elements of a token]")
+    pages, size = pool.shape[0], pool.shape[-2]
+    token = pool.shape[-1] * pool.element_size()
+    blocks = pool.numel() // max(1, pages * size * pool.shape[-1])
+    if tables.dim() != 2 or new_tables.shape != tables.shape:
+        raise ValueError(f"tables and new_tables must be [slots, width] alike, got {tuple(tables.shape)} and {tuple(new_tables.shape)}")
+    slots, width = tables.shape
+    if (pages | blocks | size | token | slots | width) >> 32:
+        raise _cut(pages, blocks, size, token, slots, width)
+    i32 = torch.int32
+    return (_POOL(pool.data_ptr(), pages, blocks, size, token), device, slots, width, _address(tables, i32, 0, device, "tables"),
+            _address(lengths, i32, slots, device, "lengths"), _address(new_tables, i32, 0, device, "new_tables"))
+
+
+def cache_assign(pool, tables, lengths, parents, new_tables, new_lengths, counts=None, missing=None, stream=None):
+    """The slots take over the states of their parents, all at once: slot s holds
+    the ``lengths``[p] tokens of p = ``parents``[s] (outside the slots: none, it is
+    free; None: p = s) and has pages for ``counts``[s] more (default: none).  Forks,
+    beams in a new order, sequences that end and pages for the next tokens are all
+    this call.
+
+    ``pool`` [pages, ..., page_size, elements of a token] holds the pages, of all
+    layers, keys and values, say; its parts are what cache_write and attention take
+    (pool[:, layer, 0] of a pool [pages, layers, 2, heads, page_size, head_dim]).
+    Full pages are shared.  A last page that is not full stays with the lowest slot
+    that holds it, the others get a page with a copy of its tokens.  New pages are
+    the lowest that no slot's new tokens lie in, in the order of the slots; entries
+    of ``new_tables`` [slots, width] without a page are -1, and ``missing`` (int32
+    [1]) becomes the number of pages asked for and not given.  A page counts as held
+    where it lies below a slot's length: add the tokens that were written to the
+    lengths before the next call.  Whole numbers are int32; tables and lengths are
+    read, the new ones must not overlap them."""
+    p, device, slots, width, old, held, new = _pool(pool, tables, lengths, new_tables)
+    i32 = torch.int32
+    rc = _cache_assign(_raw_stream(device) if stream is None else _stream_of(stream), device, p, old, held, slots, width,
+                       _address(parents, i32, slots, device, "parents"), _address(counts, i32, slots, device, "counts"), new,
+                       _address(new_lengths, i32, slots, device, "new_lengths"), _address(missing, i32, 1, device, "missing"))
+    if rc:
+        check(rc)
+    return new_tables, new_lengths
+
+
+def cache_compact(pool, tables, lengths, new_tables, used=None, stream=None):
+    """Moves the n pages that slots hold tokens in to the front of ``pool``: the
+    i-th held one, by number, behind page n - 1 to the i-th free one before page n.
+    ``new_tables`` lists them (entries behind a slot's length are -1), ``used`` (int32
+    [1]) becomes n.  Arguments as cache_assign's."""
+    p, device, slots, width, old, held, new = _pool(pool, tables, lengths, new_tables)
+    rc = _cache_compact(_raw_stream(device) if stream is None else _stream_of(stream), device, p, old, held, slots, width, new,
+                        _address(used, torch.int32, 1, device, "used"))
+    if rc:
+        check(rc)
+    return new_tables
+
+
 def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=None, repetition=None, frequency=None, presence=None,
                    bias_offsets=None, bias_tokens=None, bias_values=None, mask=None, mask_rows=None, stream=None):
     """``logits`` [rows, vocab] into ``out`` (which may be ``logits``), row r
@@ -299,4 +466,5 @@ def process_logits(logits, out, tokens=None, slots=None, lengths=None, prompts=N
     return out
 
 
-__all__ = ["rope", "qk_norm_rope", "rope_frequencies", "lora", "linear_lora", "process_logits", "ROPE_SCALINGS"]
+__all__ = ["rope", "qk_norm_rope", "rope_frequencies", "lora", "linear_lora", "attention", "cache_write", "cache_assign", "cache_compact",
+           "process_logits", "ROPE_SCALINGS"]
