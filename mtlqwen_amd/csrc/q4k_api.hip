@@ -2038,6 +2038,8 @@ int check_cache(const q4k_cache* c, const int32_t* positions, uint32_t nq) {
   if (c->pages > 0x7fffffffu || c->table_rows > 0x7fffffffu || (uint64_t)c->width * c->page_size > (1u << 30))
     return fail(Q4K_ESHAPE, "a cache has up to 2^31 - 1 pages and tables, a table up to 2^30 tokens (got %u, %u, %u pages of %u)", c->pages,
                 c->table_rows, c->width, c->page_size);
+  if (c->token_stride > (1ll << 26))
+    return fail(Q4K_ESHAPE, "token_stride must be up to 2^26 elements (got %lld)", (long long)c->token_stride);
   const int64_t strides[3] = {c->page_stride, c->head_stride, c->token_stride};
   for (int64_t s : strides)
     if (s < 0 || s > kMaxCacheStride || s % 8 != 0)
@@ -2437,7 +2439,8 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
   a.out_row = q->out_row_stride;
   a.out_head = q->out_head_stride;
   a.slopes = params->slopes;
-  a.scale = params->scale;
+  a.sign = params->scale > 0.0f ? 1.0f : params->scale < 0.0f ? -1.0f : 0.0f;
+  a.scale = params->scale == 0.0f ? 1.0f : std::fabs(params->scale);
   a.softcap = params->softcap;
   a.heads = (int)q->heads;
   a.group = (int)(q->heads / cache->heads);
@@ -2446,8 +2449,16 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
   DeviceScope scope(device);
   if (scope.rc)
     return scope.rc;
-  LaunchTimer timer(static_cast<hipStream_t>(stream), Q4K_KERNEL_AUX);
-  Q4K_TRY_HIP(launch_attention(static_cast<hipStream_t>(stream), a, (int)dtype, device_cus(device)), "attention launch");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Workspace& ws = workspace(device);
+  std::lock_guard<std::mutex> lock(ws.mu);
+  reserve_workspace(s, ws, device);
+  rc = ensure_buffer(s, ws, device, ws.part, ws.part_elems, attention_plan(a, (int)dtype, device_cus(device)), "split-K workspace");
+  if (rc)
+    return rc;
+  a.part = ws.part;
+  LaunchTimer timer(s, Q4K_KERNEL_AUX);
+  Q4K_TRY_HIP(launch_attention(s, a, (int)dtype), "attention launch");
   return Q4K_OK;
 }
 

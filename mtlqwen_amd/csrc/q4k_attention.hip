@@ -1,76 +1,1080 @@
 // Attention of a packed batch's new tokens over a paged key/value cache.
+//
+// For a row and head, x_j = scale q.k_j (capped, biased) over the keys that the row
+// sees and o = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m), t = x log2(e), in one pass
+// over the keys with the running maximum m: the sums of a part of the keys are
+// rescaled by 2^(m - m') where the maximum rises, and parts of the keys that were
+// summed apart join the same way.
+//
+// The query rows of a sequence and a cache head are its tokens' rows times the
+// `group` heads that share the cache head: row u = token u / group, head u %
+// group.  Both products run on the matrix units, transposed, so that a query row
+// is a lane's column throughout and neither the maxima nor the rescaling move
+// between lanes:
+//   S^T [16 keys x 16 rows] = K [keys x d] Q^T,  O^T [16 d x 16 rows] = V^T P^T
+// Lane 16 g + i of S^T holds keys 4 g + 0..3 of row i, which is what the second
+// product wants of P^T for the key order (4 g + e, 16 + 4 g + e) of 32 keys; V is
+// read from LDS in that order with the transposing read.
+//
+// Work is a line of key tiles: cache heads, their units (blocks of query rows of a
+// sequence), their tiles.  Lengths are on the device, so a launch has a fixed
+// number of workgroups and each takes an equal stretch of that line (locate());
+// a unit that several share leaves its sums, one per stretch, in the workspace,
+// and attention_join_kernel adds them.
 #include "q4k_device.h"
 
 namespace q4k {
 namespace {
 
-// One row and head: x_j = scale q.k_j, capped and biased, over the keys that the
-// row sees, o = sum_j exp(x_j) v_j / sum_j exp(x_j), in one pass over the keys with
-// the running maximum and sum.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
-  __shared__ float so[4][256], sm[4], sl[4];
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+
+// Weights are 2^(t - m + kTop), so that fp16 holds those down to 2^-22 of the
+// largest with all its bits; the maximum is raised where a score passes it by kSlack
+// (2^(kTop + kSlack) is still finite), which is rare after the first tiles.
+constexpr float kTop = 8.0f, kSlack = 7.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// tanh within 2^-21 of the value: the odd series below 1/4 (its next term is
+// 2^-26 of the value there), 1 - 2 / (e^2x + 1) above, whose error is 2^-23.
+__device__ __forceinline__ float tanh_score(float x) {
+  const float y = x * x;
+  const float small = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  const float e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e));
+  const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+  return fabsf(x) < 0.25f ? small : large;
+}
+
+// Maximum over the four lanes of a query row (lane ^ 16, lane ^ 32).
+__device__ __forceinline__ float row_max(float v) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto h = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const float w = fmaxf(__builtin_bit_cast(float, (uint32_t)h[0]), __builtin_bit_cast(float, (uint32_t)h[1]));
+  const uint32_t b = __builtin_bit_cast(uint32_t, w);
+  const auto q = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
+}
+
+__device__ __forceinline__ float row_sum(float v) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto h = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const float w = __builtin_bit_cast(float, (uint32_t)h[0]) + __builtin_bit_cast(float, (uint32_t)h[1]);
+  const uint32_t b = __builtin_bit_cast(uint32_t, w);
+  const auto q = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
+}
+
+__device__ __forceinline__ int lane_value(int v, int lane) {
+  return __builtin_amdgcn_readlane(v, lane);
+}
+
+// ---- the line of work --------------------------------------------------------
+
+// One sequence per lane: the position of its first row, the keys that its table
+// holds, its query rows per cache head, the units before it, its table.
+struct Sequences {
+  int first, cap, rows, unit, slot;
+};
+
+__device__ __forceinline__ Sequences load_sequences(const AttentionArgs& a) {
   const CacheArgs& c = a.cache;
-  const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int q = 0;
-  while (q + 1 < c.nq && row >= c.start[q + 1])
-    ++q;
-  const int64_t pos = (int64_t)c.positions[q] + (row - c.start[q]);
-  const int slot = c.slots ? c.slots[q] : q;
-  const int64_t cap = (uint32_t)slot < (uint32_t)c.table_rows ? (int64_t)c.width << c.page_log : 0;
-  const int64_t hi = pos + 1 < cap ? pos + 1 : cap, lo = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0;
-  const int kvh = head / a.group;
-  float x[4], o[4] = {};
-  for (int i = 0; i < 4; ++i)
-    x[i] = lane + 64 * i < c.dim ? (float)(static_cast<const T*>(a.q) + (int64_t)row * a.q_row + (int64_t)head * a.q_head)[lane + 64 * i] : 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = lo + wave; j < hi; j += 4) {
-    const int32_t page = c.tables[(int64_t)slot * c.width + (j >> c.page_log)];
-    if ((uint32_t)page >= c.pages)
-      continue;
-    const int64_t at = (int64_t)page * c.page_stride + (int64_t)kvh * c.head_stride + (j & ((1 << c.page_log) - 1)) * c.token_stride;
-    float s = 0.0f;
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < c.dim)
-        s = fmaf(x[i], (float)static_cast<const _Float16*>(c.k)[at + lane + 64 * i], s);
+  const int s = threadIdx.x & 63;
+  Sequences q{0, 0, 0, a.units, 0};
+  if (s < c.nq) {
+    const int p = c.positions[s];
+    q.first = p < -(1 << 30) ? -(1 << 30) : p > (1 << 30) ? 1 << 30 : p;
+    q.slot = c.slots ? c.slots[s] : s;
+    q.cap = (uint32_t)q.slot < (uint32_t)c.table_rows && c.pages ? c.width << c.page_log : 0;
+    q.rows = c.count[s] * a.group;
+    q.unit = a.unit[s];
+  }
+  return q;
+}
+
+// A unit: its sequence, query rows [row, row_end), the first key tile's first key,
+// the key past the last row's, its tiles (one at least, so that rows that see nothing
+// are written too).
+struct Unit {
+  int seq, row, row_end, lo, hi, tiles;
+};
+
+template <int QB, int TK>
+__device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const Sequences& q, int u) {
+  Unit x{0, 0, 0, 0, 0, 0};
+  int first = 0, cap = 0, rows = 0;
+  for (int s = 0; s < a.cache.nq; ++s) {
+    const int from = lane_value(q.unit, s);
+    if (u >= from) {
+      x.seq = s;
+      x.row = (u - from) * QB;
+      first = lane_value(q.first, s);
+      cap = lane_value(q.cap, s);
+      rows = lane_value(q.rows, s);
+    }
+  }
+  if (u >= a.units)
+    return x;
+  x.row_end = x.row + QB < rows ? x.row + QB : rows;
+  const int t0 = x.row / a.group, t1 = (x.row_end - 1) / a.group;
+  x.hi = first + t1 + 1 < cap ? first + t1 + 1 : cap;
+  x.hi = x.hi < 0 ? 0 : x.hi;
+  x.lo = a.window && first + t0 + 1 > a.window ? (first + t0 + 1 - a.window) & -TK : 0;
+  x.tiles = x.hi > x.lo ? (x.hi - x.lo + TK - 1) / TK : 1;
+  return x;
+}
+
+// All tiles of one cache head.
+template <int QB, int TK>
+__device__ __forceinline__ int64_t tiles_of_head(const AttentionArgs& a, const Sequences& q) {
+  int64_t all = 0;
+  for (int u0 = 0; u0 < a.units; u0 += 64) {
+    int t = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63)).tiles;  // up to 64 * 2^26
+    uint32_t n = (uint32_t)t;
     for (int off = 32; off; off >>= 1)
-      s += __shfl_xor(s, off);
-    s *= a.scale;
-    if (a.softcap > 0.0f)
-      s = a.softcap * tanhf(s / a.softcap);
-    if (a.slopes)
-      s = fmaf(a.slopes[head], (float)(j - pos), s);
-    // fmaxf leaves a NaN out; the weight, and with it the sums, takes it up.
-    const float n = fmaxf(m, s), top = n == -INFINITY ? 0.0f : n, r = m == n ? 1.0f : expf(m - n), p = expf(s - top);
-    l = l * r + p;
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < c.dim)
-        o[i] = fmaf(p, (float)static_cast<const _Float16*>(c.v)[at + lane + 64 * i], o[i] * r);
-    m = n;
+      n += __shfl_xor(n, off);
+    all += n;
   }
-  for (int i = 0; i < 4; ++i)
-    so[wave][lane + 64 * i] = o[i];
-  sm[wave] = m;
-  sl[wave] = l;
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= c.dim)
+  return ((int64_t)__builtin_amdgcn_readfirstlane((uint32_t)(all >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)all);
+}
+
+// The unit that holds place x of the line, and the place of its first tile (wave-uniform).
+struct Place {
+  Unit unit;
+  int head;
+  int64_t at;
+};
+
+template <int QB, int TK>
+__device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, int64_t per_head, int64_t x) {
+  Place p;
+  p.head = (int)(x / per_head);
+  const int64_t y = x - p.head * per_head;
+  int64_t before = 0;
+  p.at = x;
+  p.unit = Unit{0, 0, 0, 0, 0, 1};
+  for (int u0 = 0; u0 < a.units; u0 += 64) {
+    const Unit u = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63));
+    uint32_t n = (uint32_t)u.tiles;
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t o = __shfl_up(n, off);
+      n += (int)(threadIdx.x & 63) >= off ? o : 0;
+    }
+    const uint32_t all = __builtin_amdgcn_readlane(n, 63);
+    if (y < before + all) {
+      const int lane = __ffsll((unsigned long long)__ballot((uint64_t)n > (uint64_t)(y - before))) - 1;
+      p.unit.seq = lane_value(u.seq, lane);
+      p.unit.row = lane_value(u.row, lane);
+      p.unit.row_end = lane_value(u.row_end, lane);
+      p.unit.lo = lane_value(u.lo, lane);
+      p.unit.hi = lane_value(u.hi, lane);
+      p.unit.tiles = lane_value(u.tiles, lane);
+      p.at = p.head * per_head + before + (int64_t)((uint32_t)__builtin_amdgcn_readlane(n, lane) - (uint32_t)p.unit.tiles);
+      break;
+    }
+    before += all;
+  }
+  return p;
+}
+
+// Stretch r of n: [total r / n, total (r + 1) / n).
+__device__ __forceinline__ int64_t stretch(int64_t total, int r, int n) {
+  return total / n * r + total % n * r / n;
+}
+
+// ---- query rows ----------------------------------------------------------------
+
+// NQ column tiles of 16 query rows: their fragments (fp32 rows as two fp16 parts
+// under a power of two, 22 bits), what turns a product into t, and where the rows
+// stand (-1: no row; it sees nothing).
+template <typename T, int DP, int NQ>
+struct Rows {
+  static constexpr bool kParts = sizeof(T) == 4;
+  h8_t q[NQ][DP / 32], ql[kParts ? NQ : 1][DP / 32];
+  float c[kParts ? NQ : 1], slope[NQ];
+  int pos[NQ], cap;
+
+  __device__ __forceinline__ float factor(int n) const { return c[kParts ? n : 0]; }
+
+  // The row of tile n sees key j + x for low < x <= high.
+  __device__ __forceinline__ void seen(const AttentionArgs& a, int n, int j, int& low, int& high) const {
+    high = (pos[n] < cap ? pos[n] : cap - 1) - j;
+    low = a.window && pos[n] >= a.window ? pos[n] - a.window - j : -j - 1;
+  }
+
+  __device__ __forceinline__ void load(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row) {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int first = lane_value(s.first, u.seq), start = a.cache.start[u.seq];
+    cap = lane_value(s.cap, u.seq);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int r = row + 16 * n + i;
+      const bool live = r < u.row_end;
+      const int t = r / a.group, h = head * a.group + (r - t * a.group);
+      const T* x = static_cast<const T*>(a.q) + (int64_t)(start + t) * a.q_row + (int64_t)h * a.q_head + 8 * g;
+      c[kParts ? n : 0] = a.scale * kLog2e;
+      if constexpr (kParts) {
+        // Read twice, for the row's largest value and for its parts: 8 values at a
+        // time in registers.
+        const auto part = [&](int d, float (&f)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            f[e] = 0.0f;
+          if (live && 32 * d + 8 * g < a.cache.dim)
+            load8(x + 32 * d, f);
+          asm volatile("" ::: "memory");
+        };
+        float mx = 0.0f, up, down;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          float f[8];
+          part(d, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            mx = fmaxf(mx, fabsf(f[e]));
+        }
+        pow2_scale(row_max(mx), up, down);
+        c[n] *= down;
+        up *= a.sign;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          float f[8];
+          part(d, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = f[e] * up;
+            q[n][d][e] = (_Float16)v;
+            ql[n][d][e] = (_Float16)(v - (float)q[n][d][e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          h8_t v = {};
+          if (live && 32 * d + 8 * g < a.cache.dim)
+            v = *reinterpret_cast<const h8_any_t*>(x + 32 * d);
+          q[n][d] = v * (_Float16)a.sign;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      slope[n] = live && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+      pos[n] = live ? first + t : -1;
+    }
+  }
+};
+
+// ---- one tile of keys --------------------------------------------------------------
+// K lies in LDS as the fragments of the first product: 16 keys x 32 d, 1 KB, lane
+// 16 g + i at 16 (16 g + i): key i, d = 8 g + 0..7.  V lies row by row, 16-byte
+// chunks swizzled so that the rows of a transposing read meet no bank twice.
+
+template <int DP>
+__device__ __forceinline__ int v_swizzle(int row) {
+  // Rows that start in the same banks: every one (512 and 256 bytes), every second
+  // (384 and 128), every fourth (192).
+  return DP % 128 == 0 ? 2 * (row & 7) : DP % 64 == 0 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1);
+}
+
+template <typename T, int DP, int NQ, int NA>
+__device__ __forceinline__ void scores(const uint8_t* k, const Rows<T, DP, NQ>& r, f4_t (&s)[NA][NQ]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int a = 0; a < NA; ++a)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+      s[a][n] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  // The fragments of the next 32 d are asked for under the products of these, and
+  // no earlier: more of them would not fit the registers beside O.
+  h8_t f[2][NA];
+  const auto read = [&](int d) {
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+      f[d & 1][a] = *reinterpret_cast<const h8_t*>(k + (a * (DP / 32) + d) * 1024 + lane * 16);
+    asm volatile("" ::: "memory");
+  };
+  read(0);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) {
+    if (d + 1 < DP / 32)
+      read(d + 1);
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        s[a][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d & 1][a], r.q[n][d], s[a][n], 0, 0, 0);
+        if constexpr (Rows<T, DP, NQ>::kParts)
+          s[a][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d & 1][a], r.ql[n][d], s[a][n], 0, 0, 0);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Products become t: capped, biased and, in a tile that not every row sees whole,
+// -inf for the keys that a row does not see.  `there`: a bit per 16 keys whose page
+// is there.  With neither cap nor bias products stay as they are (c turns them into
+// t where the weights are formed).
+template <typename T, int DP, int NQ, int NA>
+__device__ __forceinline__ void finish_scores(const AttentionArgs& a, const Rows<T, DP, NQ>& r, int key, bool whole, uint32_t there, bool formed,
+                                              f4_t (&s)[NA][NQ]) {
+  const int g = (threadIdx.x & 63) >> 4;
+  if (formed) {
+    const float in = a.softcap > 0.0f ? 1.0f / (a.softcap * kLog2e) : 0.0f, out = a.softcap * kLog2e;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float away = (float)(key + 4 * g - r.pos[n]);
+#pragma unroll
+      for (int b = 0; b < NA; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float t = s[b][n][e] * r.factor(n);
+          if (a.softcap > 0.0f)
+            t = out * tanh_score(t * in);
+          s[b][n][e] = fmaf(r.slope[n], away + (float)(16 * b + e), t);
+        }
+    }
+  }
+  if (!whole) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      int low, high;
+      r.seen(a, n, key + 4 * g, low, high);
+#pragma unroll
+      for (int b = 0; b < NA; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((there >> b) & 1) || 16 * b + e <= low || 16 * b + e > high)
+            s[b][n][e] = -INFINITY;
+    }
+  }
+}
+
+// The running sums of NQ column tiles: O^T, the maximum that its weights refer to
+// and this lane's part of their sum.
+template <int DP, int NQ>
+struct Sums {
+  f4_t o[NQ][DP / 16];
+  float m[NQ], l[NQ];
+  uint32_t up[NQ][(DP + 127) / 128], down[NQ][(DP + 127) / 128];  // sums that infinities and NaN reach: bit 4 d + e
+
+  // They reach them: infinity, -infinity, or both, a NaN.
+  __device__ __forceinline__ void settle() {
+    uint32_t any = 0;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < (DP + 127) / 128; ++i)
+        any |= up[n][i] | down[n][i];
+    if (__any(any != 0)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[n][d][e] += ((up[n][d / 8] >> (4 * (d % 8) + e)) & 1 ? INFINITY : 0.0f) - ((down[n][d / 8] >> (4 * (d % 8) + e)) & 1 ? INFINITY : 0.0f);
+    }
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        o[n][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < (DP + 127) / 128; ++i)
+        up[n][i] = down[n][i] = 0;
+    }
+  }
+
+  // Scores to weights (in place), the sums rescaled where a maximum rises.
+  template <int NA, typename F>
+  __device__ __forceinline__ void weigh(f4_t (&s)[NA][NQ], const F& c) {
+    float top[NQ];
+    bool rise = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float v = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NA; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v = fmaxf(v, s[b][n][e]);
+      top[n] = row_max(v) * c(n);
+      rise = rise || top[n] > m[n] + kSlack;
+    }
+    if (__any(rise)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const float now = fmaxf(m[n], top[n]);
+        const float f = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
+        m[n] = now;
+        l[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+          o[n][d] *= f;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      // No score yet: weights of -inf become 0, of a NaN NaN.
+      const float ref = (m[n] == -INFINITY ? 0.0f : m[n]) - kTop;
+#pragma unroll
+      for (int b = 0; b < NA; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[b][n][e] = __builtin_amdgcn_exp2f(fmaf(s[b][n][e], c(n), -ref));
+          l[n] += s[b][n][e];
+        }
+    }
+  }
+};
+
+__device__ __forceinline__ h8_t pack_weights(f4_t a, f4_t b) {
+  return h8_t{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3], (_Float16)b[0], (_Float16)b[1], (_Float16)b[2], (_Float16)b[3]};
+}
+
+__device__ __forceinline__ h8_t pack_rest(f4_t a, f4_t b, h8_t p) {
+  return h8_t{(_Float16)(a[0] - (float)p[0]), (_Float16)(a[1] - (float)p[1]), (_Float16)(a[2] - (float)p[2]), (_Float16)(a[3] - (float)p[3]),
+              (_Float16)(b[0] - (float)p[4]), (_Float16)(b[1] - (float)p[5]), (_Float16)(b[2] - (float)p[6]), (_Float16)(b[3] - (float)p[7])};
+}
+
+// A V^T fragment of 16 d x 32 keys: lane 16 g + i, d = 16 dt + i, keys 4 g + e
+// and 16 + 4 g + e.  The swizzle is an exclusive or with bits of the row, so the
+// fragments of a row differ by one with bits of dt.
+template <int DP>
+__device__ __forceinline__ uint32_t v_base(const uint8_t* v) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int row = 4 * g + (i >> 2);
+  return lds_addr(v) + row * (DP * 2) + (v_swizzle<DP>(row) + ((i & 3) >> 1)) * 16 + (i & 1) * 8;
+}
+
+template <int DP>
+__device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
+  constexpr int kBits = DP % 128 == 0 ? 3 : DP % 64 == 0 ? 2 : 1;
+  const uint32_t at = (base ^ ((dt & ((1 << kBits) - 1)) << 5)) + (dt >> kBits) * (32 << kBits);
+  const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(uintptr_t)at);
+  const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(uintptr_t)(at + 16 * DP * 2));
+  typedef short s8_t __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(h8_t, s8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+}
+
+// Halves of f that are infinite or NaN become zero.
+__device__ __forceinline__ h8_t finite_part(h8_t f) {
+  h8_t y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    y[e] = __builtin_fabsf16(f[e]) < (_Float16)INFINITY ? f[e] : (_Float16)0.0f;
+  return y;
+}
+
+// O^T += V^T P^T of 32 keys.  A weight of zero does not keep an infinity or NaN of V
+// out of the product, so where not every row sees every key (whole = false) they
+// are taken out of V, and a product of the places that hold them with who sees them
+// says which sums they reach (Sums::up, down: a bit per sum, for settle()).
+template <typename T, int DP, int NQ>
+__device__ __forceinline__ void add_values(const AttentionArgs& a, const uint8_t* v, const Rows<T, DP, NQ>& r, const f4_t (&p0)[NQ], const f4_t (&p1)[NQ],
+                                           int key, bool whole, uint32_t there, Sums<DP, NQ>& sums) {
+  constexpr bool kParts = Rows<T, DP, NQ>::kParts;
+  h8_t w[NQ], wl[kParts ? NQ : 1];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    w[n] = pack_weights(p0[n], p1[n]);
+    if constexpr (kParts)
+      wl[n] = pack_rest(p0[n], p1[n], w[n]);
+  }
+  uint32_t base = v_base<DP>(v);
+  asm volatile("" : "+v"(base));  // one register, not one per fragment
+  bool odd = false;
+  if (!whole) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      asm volatile("" : "+v"(base)::"memory");  // V is read anew below, not kept in registers
+      const u4_t f = __builtin_bit_cast(u4_t, v_fragment<DP>(base, d));
+      // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
+      bits |= ((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
+              ((f.w & 0x7fff7fffu) + 0x04000400u);
+    }
+    odd = __any((bits & 0x80008000u) != 0);
+    if (odd) {
+      const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        int low, high;
+        r.seen(a, n, key + 4 * g, low, high);
+        h8_t one;  // who sees which key
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = 16 * (e >> 2) + (e & 3);
+          one[e] = ((there >> (e >> 2)) & 1) && k > low && k <= high ? (_Float16)1.0f : (_Float16)0.0f;
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+#pragma unroll
+          for (int sign = 0; sign < 2; ++sign) {
+            asm volatile("" : "+v"(base)::"memory");
+            h8_t f = v_fragment<DP>(base, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)  // infinity and NaN, -infinity and NaN
+              f[e] = (sign ? f[e] >= (_Float16)-65504.0f : f[e] <= (_Float16)65504.0f) ? (_Float16)0.0f : (_Float16)1.0f;
+            const f4_t many = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              (sign ? sums.down : sums.up)[n][d / 8] |= many[e] > 0.0f ? 1u << (4 * (d % 8) + e) : 0u;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+    asm volatile("" : "+v"(base)::"memory");
+  }
+  constexpr int kAhead = kParts && DP == 256 ? 1 : 2;
+  h8_t f[kAhead + 1];
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d)
+    f[d] = v_fragment<DP>(base, d);
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) {
+    if (d + kAhead < DP / 16)
+      f[(d + kAhead) % (kAhead + 1)] = v_fragment<DP>(base, d + kAhead);
+    asm volatile("" ::: "memory");
+    h8_t& x = f[d % (kAhead + 1)];
+    if (odd)
+      x = finite_part(x);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[n], sums.o[n][d], 0, 0, 0);
+      if constexpr (kParts)
+        sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wl[n], sums.o[n][d], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// ---- keys and values into LDS --------------------------------------------------------
+
+// The pages of a sequence: 64 table entries at a time, one per lane, from entry
+// `base` on.
+struct Pages {
+  const int32_t* table;
+  int width, base, mine;
+
+  __device__ __forceinline__ void open(const AttentionArgs& a, const Sequences& s, int seq) {
+    const int slot = lane_value(s.slot, seq);
+    const bool there = (uint32_t)slot < (uint32_t)a.cache.table_rows;
+    table = a.cache.tables + (there ? (int64_t)slot * a.cache.width : 0);
+    width = there ? a.cache.width : 0;
+    base = -64;
+    mine = -1;
+  }
+  // The page of entry e (wave-uniform), -1 if it is not there.
+  __device__ __forceinline__ int page(const AttentionArgs& a, int e) {
+    if (e < base || e >= base + 64) {
+      base = e;
+      const int at = e + (int)(threadIdx.x & 63);
+      const int p = at < width ? table[at] : -1;
+      mine = (uint32_t)p < a.cache.pages ? p : -1;
+    }
+    return lane_value(mine, e - base);
+  }
+};
+
+// Where this lane's 16 bytes of each 1 KB transfer come from, relative to the
+// first of 16 tokens.  K: key i, d = 8 g + 0..7 of a fragment.  V: transfer x holds
+// rows kRows x on, whose swizzle differs from the first one's by bits of x alone
+// (heads of 96 and 192, whose rows no transfer ends with: an offset each).  Heads
+// shorter than DP: chunks past them are not loaded (their LDS is zero).
+template <int DP>
+struct Lanes {
+  static constexpr bool kEven = 512 % DP == 0;
+  static constexpr int kRows = 512 / DP, kVs = kEven ? 1 : DP / 32;
+  uint32_t k, row, chunk[kVs];
+
+  __device__ __forceinline__ void set(const CacheArgs& c) {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    k = (uint32_t)(i * (int)c.token_stride) * 2 + g * 16;
+    row = (uint32_t)((lane / (DP / 8)) * (int)c.token_stride) * 2;
+#pragma unroll
+    for (int x = 0; x < kVs; ++x) {
+      const int n = x * 64 + lane, r = n / (DP / 8);
+      chunk[x] = ((n - r * (DP / 8)) ^ v_swizzle<DP>(r)) * 16 + (kEven ? 0u : (uint32_t)(r * (int)c.token_stride) * 2);
+    }
+  }
+  // Bytes of the first chunk past the head that transfer x would load, or more.
+  __device__ __forceinline__ bool in_head(const CacheArgs& c, int x) const {
+    const int lane = threadIdx.x & 63, n = x * 64 + lane, r = n / (DP / 8);
+    return 8 * ((n - r * (DP / 8)) ^ v_swizzle<DP>(r)) < c.dim;
+  }
+};
+
+template <int DP, int D = 0>
+__device__ __forceinline__ void dma_k(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+  if constexpr (D < DP / 32) {
+    // The instruction's offset moves both addresses.
+    if (c.dim == DP || 32 * D + 8 * (int)((threadIdx.x & 63) >> 4) < c.dim)
+      lds_dma16<64 * D>(from, l.k, __builtin_amdgcn_readfirstlane(lds + (1024 - 64) * D));
+    dma_k<DP, D + 1>(c, l, from, lds);
+  }
+}
+
+template <int DP>
+__device__ __forceinline__ void dma_v(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+  using L = Lanes<DP>;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x)
+    if (c.dim == DP || l.in_head(c, x)) {
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds + 1024 * x);
+      if constexpr (L::kEven)
+        lds_dma16<0>(from + (int64_t)(x * L::kRows) * c.token_stride * 2, (l.chunk[0] ^ (v_swizzle<DP>(x * L::kRows) * 16)) + l.row, to);
+      else
+        lds_dma16<0>(from, l.chunk[x], to);
+    }
+}
+
+// The first of 16 tokens from key j on in `page` (one that is not there: page 0,
+// whose tokens nothing sees).
+__device__ __forceinline__ const uint8_t* tokens_at(const CacheArgs& c, const void* base, int head, int page, int j) {
+  const int64_t at = (int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)head * c.head_stride + (int64_t)(j & ((1 << c.page_log) - 1)) * c.token_stride;
+  return uniform_ptr(static_cast<const uint8_t*>(base) + 2 * at);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Every read of LDS so far is done (a transfer may overwrite what it read).
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f4_t v) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  vec y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e] = (T)v[e];
+  *reinterpret_cast<vec*>(p) = y;
+}
+
+template <typename T>
+__device__ __forceinline__ T* out_row(const AttentionArgs& a, int start, int head, int u) {
+  const int t = u / a.group, h = head * a.group + (u - t * a.group);
+  return static_cast<T*>(a.out) + (int64_t)(start + t) * a.out_row + (int64_t)h * a.out_head;
+}
+
+// ----------------------------------------------------------------------------
+// Chunks of tokens: four waves of 16 NQ query rows each over the same key tiles,
+// two buffers of K and V in LDS, the next tile's transfers under the present
+// tile's products.
+// ----------------------------------------------------------------------------
+template <typename T, int DP, int NQ, int TK, bool FORM>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionShape::chunk_waves(DP, sizeof(T) == 4)))) void attention_chunk_kernel(
+    AttentionArgs a) {
+  constexpr int QB = 64 * NQ, NA = TK / 16, kTile = TK * DP * 2;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // K, V of two tiles
+  const CacheArgs& c = a.cache;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+  const int64_t per_head = tiles_of_head<QB, TK>(a, load_sequences(a)), total = per_head * c.heads;
+  // Neighbouring stretches read the same keys: they go to one XCD.
+  const int n8 = a.stretches / 8, wg = n8 * 8 == a.stretches ? ((int)blockIdx.x & 7) * n8 + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
+  int64_t x = stretch(total, wg, a.stretches);
+  const int64_t end = stretch(total, wg + 1, a.stretches);
+  if (x >= end)
     return;
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float sum = 0.0f, y = 0.0f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = sm[w] == top ? 1.0f : expf(sm[w] - top);
-    sum += f * sl[w];
-    y += f * so[w][d];
+  if (c.dim != DP) {
+    for (int i = tid; i < 4 * kTile / 16; i += 256)
+      reinterpret_cast<u4_t*>(lds)[i] = u4_t{0, 0, 0, 0};
+    __syncthreads();
   }
-  (static_cast<T*>(a.out) + (int64_t)row * a.out_row + (int64_t)head * a.out_head)[d] = (T)(sum == 0.0f ? 0.0f : y / sum);
+  Lanes<DP> from;
+  from.set(c);
+  bool leading = true;  // the stretch's first unit
+  while (x < end) {
+    const Sequences seqs = load_sequences(a);  // anew for each unit: no registers under its products
+    const Place p = locate<QB, TK>(a, seqs, per_head, x);
+    const Unit& u = p.unit;
+    const int start = c.start[u.seq];
+    const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
+    Rows<T, DP, NQ> rows;
+    const int row = u.row + wave * 16 * NQ;
+    rows.load(a, seqs, u, p.head, row);
+    Sums<DP, NQ> sums;
+    sums.clear();
+    // What the wave's rows see, at most and at least.
+    const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
+    const int last = (row + 16 * NQ < u.row_end ? row + 16 * NQ : u.row_end) - 1;
+    const bool active = row < u.row_end;
+    const int ta = first + row / a.group + 1, tb = first + (active ? last : row) / a.group + 1;
+    const int hi_least = ta < cap ? ta : cap, hi_most = tb < cap ? tb : cap;
+    const int lo_least = a.window && ta > a.window ? ta - a.window : 0, lo_most = a.window && tb > a.window ? tb - a.window : 0;
+    const bool none = u.hi <= u.lo;
+    Pages pages;
+    pages.open(a, seqs, u.seq);
+    uint32_t there = 0;
+    const auto fetch = [&](int t, int buffer) {
+      const int key = u.lo + t * TK;
+      int page[NA];
+      there = 0;
+#pragma unroll
+      for (int b = 0; b < NA; ++b) {
+        page[b] = pages.page(a, (key + 16 * b) >> c.page_log);
+        there |= page[b] >= 0 ? 1u << b : 0u;
+      }
+      const uint32_t at = lds_addr(lds) + buffer * 2 * kTile;
+      constexpr int kSteps = 2 * NA;  // K and V of 16 tokens each, dealt to the waves
+#pragma unroll
+      for (int s = 0; s < kSteps / 4; ++s) {
+        const int step = s * 4 + wave, b = step % NA;
+        int pg = page[0];
+#pragma unroll
+        for (int y = 1; y < NA; ++y)
+          pg = b == y ? page[y] : pg;
+        if (step < NA)
+          dma_k<DP>(c, from, tokens_at(c, c.k, p.head, pg, key + 16 * b), at + b * (DP / 32) * 1024);
+        else
+          dma_v<DP>(c, from, tokens_at(c, c.v, p.head, pg, key + 16 * b), at + kTile + b * (DP / 32) * 1024);
+      }
+    };
+    if (!none) {
+      __syncthreads();  // the buffers' last readers are done
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(t0, 0);
+      for (int t = 0; t < n; ++t) {
+        const uint32_t here = there;
+        wait_loads<0>();
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + 1 < n)
+          fetch(t0 + t + 1, (t + 1) & 1);
+        const int key = u.lo + (t0 + t) * TK;
+        if (!active || key >= hi_most || key + TK <= lo_least)
+          continue;
+        const bool whole = key + TK <= hi_least && key >= lo_most && here == (1u << NA) - 1;
+        const uint8_t* k = lds + (t & 1) * 2 * kTile;
+        f4_t s[NA][NQ];
+        scores<T, DP, NQ, NA>(k, rows, s);
+        finish_scores<T, DP, NQ, NA>(a, rows, key, whole, here, FORM, s);
+        sums.weigh(s, [&](int y) { return FORM ? 1.0f : rows.factor(y); });
+#pragma unroll
+        for (int h = 0; h < NA / 2; ++h) {
+          add_values<T, DP, NQ>(a, k + kTile + h * 32 * DP * 2, rows, s[2 * h], s[2 * h + 1], key + 32 * h, whole, here >> (2 * h), sums);
+        }
+      }
+    }
+    sums.settle();
+    // Whole units are done; of others the sums go to the workspace.
+    const bool done = n == u.tiles;
+    const int64_t slot = 2 * (int64_t)wg + (leading ? 0 : 1);
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      const float l = row_sum(sums.l[y]);
+      const int r = row + 16 * y + (lane & 15);
+      if (r >= u.row_end)
+        continue;
+      if (done) {
+        T* o = out_row<T>(a, start, p.head, r);
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+          if (16 * d + 4 * g < c.dim)
+            store4(o + 16 * d + 4 * g, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : sums.o[y][d] * f);
+      } else {
+        float* o = a.part + (slot * QB + (r - u.row)) * DP;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+          *reinterpret_cast<f4_t*>(o + 16 * d + 4 * g) = sums.o[y][d];
+        if (g == 0) {
+          float* ml = a.part + 2 * (int64_t)a.stretches * QB * DP + (slot * QB + (r - u.row)) * 2;
+          ml[0] = sums.m[y];
+          ml[1] = l;
+        }
+      }
+    }
+    x += n;
+    leading = false;
+  }
+}
+
+// ----------------------------------------------------------------------------
+// Few query rows: every wave takes every NW-th tile of 32 keys of its workgroup's
+// stretch, with a buffer for K and one for V of its own, refilled as soon as each
+// has been read; the waves' sums join in LDS at the end of a unit.  Bound by the
+// reading of K and V.
+// ----------------------------------------------------------------------------
+template <typename T, int DP, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a) {
+  constexpr int QB = 16 * NQ, TK = 32, kTile = TK * DP * 2, kLoads = DP / 16;
+  static_assert(NW * 16 * DP * 4 <= NW * 2 * kTile, "the waves' sums fit into the buffers");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * 2 * kTile];
+  __shared__ float sm[NW][QB], sl[NW][QB];
+  const CacheArgs& c = a.cache;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+  const int64_t per_head = tiles_of_head<QB, TK>(a, load_sequences(a)), total = per_head * c.heads;
+  const int wg = (int)blockIdx.x;
+  int64_t x = stretch(total, wg, a.stretches);
+  const int64_t end = stretch(total, wg + 1, a.stretches);
+  if (x >= end)
+    return;
+  Lanes<DP> from;
+  from.set(c);
+  uint8_t* const mine = lds + wave * 2 * kTile;
+  const uint32_t at = lds_addr(mine);
+  const bool formed = a.softcap > 0.0f || a.slopes;
+  bool leading = true;
+  while (x < end) {
+    const Sequences seqs = load_sequences(a);  // anew for each unit: no registers under its products
+    const Place p = locate<QB, TK>(a, seqs, per_head, x);
+    const Unit& u = p.unit;
+    const int start = c.start[u.seq];
+    const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
+    Rows<T, DP, NQ> rows;
+    rows.load(a, seqs, u, p.head, u.row);
+    Sums<DP, NQ> sums;
+    sums.clear();
+    const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
+    const int ta = first + u.row / a.group + 1, tb = first + (u.row_end - 1) / a.group + 1;
+    const int hi_least = ta < cap ? ta : cap, lo_most = a.window && tb > a.window ? tb - a.window : 0;
+    Pages pages;
+    pages.open(a, seqs, u.seq);
+    if (c.dim != DP)  // chunks that are not loaded are zero (the buffers held sums before)
+      for (int i = lane; i < 2 * kTile / 16; i += 64)
+        reinterpret_cast<u4_t*>(mine)[i] = u4_t{0, 0, 0, 0};
+    wait_lds();
+    int pg[2];
+    const auto open = [&](int t) {
+      const int key = u.lo + t * TK;
+      pg[0] = pages.page(a, key >> c.page_log);
+      pg[1] = pages.page(a, (key + 16) >> c.page_log);
+    };
+    const auto fetch_k = [&](int t) {
+      const int key = u.lo + t * TK;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        dma_k<DP>(c, from, tokens_at(c, c.k, p.head, pg[b], key + 16 * b), at + b * (DP / 32) * 1024);
+    };
+    const auto fetch_v = [&](int t) {
+      const int key = u.lo + t * TK;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        dma_v<DP>(c, from, tokens_at(c, c.v, p.head, pg[b], key + 16 * b), at + kTile + b * (DP / 32) * 1024);
+    };
+    if (u.hi > u.lo && wave < n) {
+      open(t0 + wave);
+      fetch_k(t0 + wave);
+      fetch_v(t0 + wave);
+      for (int t = wave; t < n; t += NW) {
+        const int key = u.lo + (t0 + t) * TK;
+        const uint32_t there = (pg[0] >= 0 ? 1u : 0u) | (pg[1] >= 0 ? 2u : 0u);
+        const bool whole = key + TK <= hi_least && key >= lo_most && there == 3u, more = t + NW < n;
+        wait_loads<kLoads>();  // K is here, V may be on its way
+        f4_t s[2][NQ];
+        scores<T, DP, NQ, 2>(mine, rows, s);
+        wait_lds();
+        if (more) {
+          open(t0 + t + NW);
+          fetch_k(t0 + t + NW);
+        }
+        finish_scores<T, DP, NQ, 2>(a, rows, key, whole, there, formed, s);
+        sums.weigh(s, [&](int y) { return formed ? 1.0f : rows.factor(y); });
+        if (more)
+          wait_loads<kLoads>();
+        else
+          wait_loads<0>();
+        add_values<T, DP, NQ>(a, mine + kTile, rows, s[0], s[1], key, whole, there, sums);
+        wait_lds();
+        if (more)
+          fetch_v(t0 + t + NW);
+      }
+    }
+    sums.settle();
+    // The waves' sums of each 16 rows, joined by all threads.
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      const float l = row_sum(sums.l[y]);
+      if (g == 0) {
+        sm[wave][16 * y + (lane & 15)] = sums.m[y];
+        sl[wave][16 * y + (lane & 15)] = l;
+      }
+    }
+    const bool done = n == u.tiles;
+    const int64_t slot = 2 * (int64_t)wg + (leading ? 0 : 1);
+    float* const buffer = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int y = 0; y < NQ; ++y) {
+      __syncthreads();  // every wave's products are done, and the rows before these are out
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        *reinterpret_cast<f4_t*>(buffer + (wave * 16 + (lane & 15)) * DP + 16 * d + 4 * g) = sums.o[y][d];
+      __syncthreads();
+      for (int i = tid; i < 16 * DP / 4; i += 64 * NW) {
+        const int rr = i / (DP / 4), d = 4 * (i - rr * (DP / 4)), r = u.row + 16 * y + rr;
+        if (r >= u.row_end || d >= c.dim)
+          continue;
+        float top = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+          top = fmaxf(top, sm[w][16 * y + rr]);
+        f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float m = sm[w][16 * y + rr], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+          l = fmaf(f, sl[w][16 * y + rr], l);
+          o += f * *reinterpret_cast<const f4_t*>(buffer + (w * 16 + rr) * DP + d);
+        }
+        if (done) {
+          store4(out_row<T>(a, start, p.head, r) + d, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / l));
+        } else {
+          *reinterpret_cast<f4_t*>(a.part + (slot * QB + 16 * y + rr) * DP + d) = o;
+          if (d == 0) {
+            float* ml = a.part + 2 * (int64_t)a.stretches * QB * DP + (slot * QB + 16 * y + rr) * 2;
+            ml[0] = top;
+            ml[1] = l;
+          }
+        }
+      }
+    }
+    __syncthreads();  // before the buffers and statistics are used again
+    x += n;
+    leading = false;
+  }
+}
+
+// ----------------------------------------------------------------------------
+// Joins the sums of a unit that several stretches share.  Workgroup (b, part)
+// stands for the border before stretch b + 1: if it is the first within its
+// unit, the workgroup adds 16 of the unit's rows up, in the order of the
+// stretches.
+// ----------------------------------------------------------------------------
+template <typename T, int DP, int QB, int TK>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
+  const CacheArgs& c = a.cache;
+  const Sequences seqs = load_sequences(a);
+  const int64_t per_head = tiles_of_head<QB, TK>(a, seqs), total = per_head * c.heads;
+  const int b = (int)blockIdx.x + 1;
+  const int64_t x = stretch(total, b, a.stretches), before = stretch(total, b - 1, a.stretches);
+  if (x >= total || x == before)
+    return;
+  const Place p = locate<QB, TK>(a, seqs, per_head, x);
+  if (p.at == x || before > p.at)
+    return;
+  const Unit& u = p.unit;
+  const int64_t last = p.at + u.tiles;
+  const int rr = 16 * (int)blockIdx.y + (int)(threadIdx.x >> 4), r = u.row + rr, d0 = 4 * (int)(threadIdx.x & 15);
+  if (r >= u.row_end)
+    return;
+  const float* const ml = a.part + 2 * (int64_t)a.stretches * QB * DP;
+  // Stretch b - 1 ends within the unit: its sums are its last ones (slot 1), unless
+  // it began there too.
+  const int64_t lead = 2 * (int64_t)(b - 1) + (before == p.at ? 0 : stretch(total, b - 1, a.stretches) < p.at ? 1 : 0);
+  float top = ml[(lead * QB + rr) * 2];
+  int to = b;
+  for (; to < a.stretches && stretch(total, to, a.stretches) < last; ++to)
+    if (stretch(total, to + 1, a.stretches) > stretch(total, to, a.stretches))
+      top = fmaxf(top, ml[(2 * (int64_t)to * QB + rr) * 2]);
+  f4_t o[DP / 64 + (DP % 64 != 0)];
+  constexpr int kSteps = sizeof(o) / sizeof(o[0]);
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    o[i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = b - 1; s < to; ++s) {
+    if (s >= b && stretch(total, s + 1, a.stretches) == stretch(total, s, a.stretches))
+      continue;
+    const int64_t at = (s < b ? lead : 2 * (int64_t)s) * QB + rr;
+    const float m = ml[at * 2], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    l = fmaf(f, ml[at * 2 + 1], l);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if (d0 + 64 * i < c.dim)
+        o[i] += f * *reinterpret_cast<const f4_t*>(a.part + at * DP + d0 + 64 * i);
+  }
+  T* y = out_row<T>(a, c.start[u.seq], p.head, r);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    if (d0 + 64 * i < c.dim)
+      store4(y + d0 + 64 * i, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[i] * (1.0f / l));
+}
+
+template <typename T, int DP, int QB, int TK>
+hipError_t launch_join(hipStream_t s, const AttentionArgs& a) {
+  return dispatch(attention_join_kernel<T, DP, QB, TK>, dim3(a.stretches - 1, (QB + 15) / 16), dim3(256), s, a);
+}
+
+template <typename T, int DP>
+hipError_t launch_t(hipStream_t s, const AttentionArgs& a) {
+  if (a.row_tiles) {
+    hipError_t e;
+    if (a.row_tiles == 1)
+      e = dispatch(attention_rows_kernel<T, DP, 1, DP <= 128 ? 8 : 4>, dim3(a.stretches), dim3(DP <= 128 ? 512 : 256), s, a);
+    else if (a.row_tiles == 2)
+      e = dispatch(attention_rows_kernel<T, DP, 2, 4>, dim3(a.stretches), dim3(256), s, a);
+    else if constexpr (DP <= 128)
+      e = dispatch(attention_rows_kernel<T, DP, 3, 4>, dim3(a.stretches), dim3(256), s, a);
+    else
+      e = hipErrorInvalidValue;
+    if (e != hipSuccess || a.stretches == 1)
+      return e;
+    return a.row_tiles == 1 ? launch_join<T, DP, 16, 32>(s, a) : a.row_tiles == 2 ? launch_join<T, DP, 32, 32>(s, a) : launch_join<T, DP, 48, 32>(s, a);
+  }
+  constexpr int NQ = AttentionShape::chunk_tiles(DP, sizeof(T) == 4), TK = AttentionShape::chunk_keys(DP);
+  hipError_t e = a.softcap > 0.0f || a.slopes ? dispatch(attention_chunk_kernel<T, DP, NQ, TK, true>, dim3(a.stretches), dim3(256), s, a)
+                                              : dispatch(attention_chunk_kernel<T, DP, NQ, TK, false>, dim3(a.stretches), dim3(256), s, a);
+  if (e != hipSuccess || a.stretches == 1)
+    return e;
+  return launch_join<T, DP, 64 * NQ, TK>(s, a);
+}
+
+template <typename T>
+hipError_t launch_d(hipStream_t s, const AttentionArgs& a) {
+  switch (AttentionShape::padded(a.cache.dim)) {
+    case 64:
+      return launch_t<T, 64>(s, a);
+    case 96:
+      return launch_t<T, 96>(s, a);
+    case 128:
+      return launch_t<T, 128>(s, a);
+    case 192:
+      return launch_t<T, 192>(s, a);
+    default:
+      return launch_t<T, 256>(s, a);
+  }
 }
 
 }  // namespace
 
-hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype, int cus) {
-  const dim3 grid(a.rows, a.heads);
-  return dtype == kF32 ? dispatch(attention_kernel<float>, grid, dim3(256), s, a) : dispatch(attention_kernel<_Float16>, grid, dim3(256), s, a);
+// Which kernel, how many query rows a unit has, how many workgroups: by the
+// counts of new rows, the heads and the head size, which the host knows.
+size_t attention_plan(AttentionArgs& a, int dtype, int cus) {
+  const CacheArgs& c = a.cache;
+  int most = 0;
+  for (int s = 0; s < c.nq; ++s)
+    most = c.count[s] > most ? c.count[s] : most;
+  const int64_t rows = (int64_t)most * a.group;
+  const int dp = AttentionShape::padded(c.dim);
+  a.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && dp <= 128 ? 3 : 0;
+  const int qb = a.row_tiles ? 16 * a.row_tiles : 64 * AttentionShape::chunk_tiles(dp, dtype == kF32);
+  const int tk = a.row_tiles ? 32 : AttentionShape::chunk_keys(dp);
+  a.units = 0;
+  for (int s = 0; s < c.nq; ++s) {
+    a.unit[s] = a.units;
+    a.units += (int)(((int64_t)c.count[s] * a.group + qb - 1) / qb);
+  }
+  // No more workgroups than tiles: as many as a table holds, for every unit.
+  const int64_t tiles = (int64_t)a.units * c.heads * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1);
+  const int wgs = a.row_tiles ? cus : 2 * cus;
+  a.stretches = tiles < wgs ? (int)tiles : wgs;
+  return 2 * (size_t)a.stretches * qb * (dp + 2);
+}
+
+hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype) {
+  return dtype == kF32 ? launch_d<float>(s, a) : launch_d<_Float16>(s, a);
 }
 
 }  // namespace q4k

@@ -615,11 +615,27 @@ struct AttentionArgs {
   void* out = nullptr;
   int64_t q_row = 0, q_head = 0, out_row = 0, out_head = 0;
   const float* slopes = nullptr;  // [heads] or nullptr
-  float scale = 1.0f, softcap = 0.0f;
+  float scale = 1.0f, sign = 1.0f;  // of q.k; scale is positive, q is taken times sign (1, -1 or 0)
+  float softcap = 0.0f;
   int heads = 0, group = 1, rows = 0;
   int window = 0;  // keys that a row sees, its own the last; 0: all before it
+  // Set by attention_plan: the 16-row tiles of a unit (0: a chunk's), the units and
+  // those before each sequence, the workgroups.
+  int row_tiles = 0, units = 0, stretches = 1;
+  int unit[kMaxSequences] = {};
+  float* part = nullptr;  // the plan's floats: sums of units that workgroups share
 };
-hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype, int cus);
+// Head sizes, as the kernels are built for them, and their chunks: 16-row tiles of
+// a wave, keys of a tile.
+struct AttentionShape {
+  static constexpr int padded(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+  static constexpr int chunk_tiles(int dp, bool f32) { return f32 && dp == 256 ? 1 : 2; }
+  static constexpr int chunk_waves(int dp, bool f32) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
+  static constexpr int chunk_keys(int dp) { return dp > 128 ? 32 : 64; }
+};
+// Sets the plan; the floats of `part`.
+size_t attention_plan(AttentionArgs& a, int dtype, int cus);
+hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype);
 
 // Tables of all slots, as they are and as they become.
 constexpr uint32_t kMaxPages = 1u << 18;
