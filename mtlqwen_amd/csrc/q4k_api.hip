@@ -2453,10 +2453,12 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
   Workspace& ws = workspace(device);
   std::lock_guard<std::mutex> lock(ws.mu);
   reserve_workspace(s, ws, device);
-  rc = ensure_buffer(s, ws, device, ws.part, ws.part_elems, attention_plan(a, (int)dtype, device_cus(device)), "split-K workspace");
+  const size_t floats = attention_plan(a, (int)dtype, device_cus(device));
+  rc = ensure_splitk_workspace(s, ws, device, floats, (size_t)a.stretches);
   if (rc)
     return rc;
   a.part = ws.part;
+  a.counters = ws.counters;
   LaunchTimer timer(s, Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_attention(s, a, (int)dtype), "attention launch");
   return Q4K_OK;

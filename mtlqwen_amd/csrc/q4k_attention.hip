@@ -20,7 +20,7 @@
 // sequence), their tiles.  Lengths are on the device, so a launch has a fixed
 // number of workgroups and each takes an equal stretch of that line (locate());
 // a unit that several share leaves its sums, one per stretch, in the workspace,
-// and attention_join_kernel adds them.
+// and the workgroup that comes last adds them, in the order of the stretches.
 #include "q4k_device.h"
 
 namespace q4k {
@@ -71,24 +71,38 @@ __device__ __forceinline__ int lane_value(int v, int lane) {
 // ---- the line of work --------------------------------------------------------
 
 // One sequence per lane: the position of its first row, the keys that its table
-// holds, its query rows per cache head, the units before it, its table.
+// holds, its query rows per cache head, the units before it, its table, its first
+// row in the batch.  Read from the arguments and the device's arrays once (the
+// arguments lie in host memory: a reading there takes microseconds), then kept in LDS.
 struct Sequences {
-  int first, cap, rows, unit, slot;
+  int first, cap, rows, unit, slot, start;
 };
+constexpr int kSequenceInts = 6 * 64;
 
 __device__ __forceinline__ Sequences load_sequences(const AttentionArgs& a) {
   const CacheArgs& c = a.cache;
   const int s = threadIdx.x & 63;
-  Sequences q{0, 0, 0, a.units, 0};
+  Sequences q{0, 0, 0, a.units, 0, 0};
   if (s < c.nq) {
     const int p = c.positions[s];
-    q.first = p < -(1 << 30) ? -(1 << 30) : p > (1 << 30) ? 1 << 30 : p;
     q.slot = c.slots ? c.slots[s] : s;
-    q.cap = (uint32_t)q.slot < (uint32_t)c.table_rows && c.pages ? c.width << c.page_log : 0;
     q.rows = c.count[s] * a.group;
     q.unit = a.unit[s];
+    q.start = c.start[s];
+    q.first = p < -(1 << 30) ? -(1 << 30) : p > (1 << 30) ? 1 << 30 : p;
+    q.cap = (uint32_t)q.slot < (uint32_t)c.table_rows && c.pages ? c.width << c.page_log : 0;
   }
   return q;
+}
+
+__device__ __forceinline__ void keep_sequences(const Sequences& q, int* lds) {
+  const int s = threadIdx.x & 63;
+  lds[s] = q.first, lds[64 + s] = q.cap, lds[128 + s] = q.rows, lds[192 + s] = q.unit, lds[256 + s] = q.slot, lds[320 + s] = q.start;
+}
+
+__device__ __forceinline__ Sequences kept_sequences(const int* lds) {
+  const int s = threadIdx.x & 63;
+  return Sequences{lds[s], lds[64 + s], lds[128 + s], lds[192 + s], lds[256 + s], lds[320 + s]};
 }
 
 // A unit: its sequence, query rows [row, row_end), the first key tile's first key,
@@ -123,18 +137,54 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const Sequences&
   return x;
 }
 
-// All tiles of one cache head.
-template <int QB, int TK>
-__device__ __forceinline__ int64_t tiles_of_head(const AttentionArgs& a, const Sequences& q) {
-  int64_t all = 0;
+// The line: tiles of one cache head and in all, and its n stretches, stretch r from
+// start(r) on.  No more of them than leaves LEAST tiles to each.  Wave-uniform.
+struct Line {
+  int64_t per_head, total, step;
+  int n, rest;  // total = n step + rest
+  float per_n;
+  double per_tiles;  // 1 / per_head
+
+  // n step r / n + floor(rest r / n): rest r < 2^20 and n <= 1024, so that half a
+  // unit keeps the rounded quotient off the next whole number.
+  __device__ __forceinline__ int64_t start(int r) const { return step * r + (int)(((float)(rest * r) + 0.5f) * per_n); }
+
+  // The stretch that holds place x.
+  __device__ __forceinline__ int of(int64_t x) const {
+    int r = __builtin_amdgcn_readfirstlane((int)((double)x / (double)step));
+    r = r < n - 1 ? r : n - 1;
+    while (start(r) > x)
+      --r;
+    return r;
+  }
+};
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)v));
+}
+
+template <int QB, int TK, int LEAST>
+__device__ __forceinline__ Line make_line(const AttentionArgs& a, const Sequences& q) {
+  Line x;
+  x.per_head = 0;
   for (int u0 = 0; u0 < a.units; u0 += 64) {
-    int t = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63)).tiles;  // up to 64 * 2^26
-    uint32_t n = (uint32_t)t;
+    uint32_t n = (uint32_t)unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63)).tiles;  // up to 64 * 2^26
     for (int off = 32; off; off >>= 1)
       n += __shfl_xor(n, off);
-    all += n;
+    x.per_head += n;
   }
-  return ((int64_t)__builtin_amdgcn_readfirstlane((uint32_t)(all >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)all);
+  x.per_head = uniform(x.per_head);
+  x.total = x.per_head * a.cache.heads;
+  x.n = x.total >= (int64_t)a.stretches * LEAST ? a.stretches : (int)((uint32_t)(x.total + LEAST - 1) / LEAST);
+  x.step = uniform((int64_t)((double)x.total / (double)x.n));
+  x.rest = (int)(x.total - x.step * x.n);
+  if (x.rest < 0 || x.rest >= x.n) {  // the quotient rounded over a whole number
+    x.step += x.rest < 0 ? -1 : 1;
+    x.rest = (int)(x.total - x.step * x.n);
+  }
+  x.per_n = 1.0f / (float)x.n;
+  x.per_tiles = 1.0 / (double)x.per_head;
+  return x;
 }
 
 // The unit that holds place x of the line, and the place of its first tile (wave-uniform).
@@ -145,10 +195,14 @@ struct Place {
 };
 
 template <int QB, int TK>
-__device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, int64_t per_head, int64_t x) {
+__device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, const Line& line, int64_t x) {
   Place p;
-  p.head = (int)(x / per_head);
-  const int64_t y = x - p.head * per_head;
+  p.head = __builtin_amdgcn_readfirstlane((int)((double)x * line.per_tiles));
+  int64_t y = x - p.head * line.per_head;
+  if (y < 0 || y >= line.per_head) {
+    p.head += y < 0 ? -1 : 1;
+    y = x - p.head * line.per_head;
+  }
   int64_t before = 0;
   p.at = x;
   p.unit = Unit{0, 0, 0, 0, 0, 1};
@@ -168,17 +222,12 @@ __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences&
       p.unit.lo = lane_value(u.lo, lane);
       p.unit.hi = lane_value(u.hi, lane);
       p.unit.tiles = lane_value(u.tiles, lane);
-      p.at = p.head * per_head + before + (int64_t)((uint32_t)__builtin_amdgcn_readlane(n, lane) - (uint32_t)p.unit.tiles);
+      p.at = p.head * line.per_head + before + (int64_t)((uint32_t)__builtin_amdgcn_readlane(n, lane) - (uint32_t)p.unit.tiles);
       break;
     }
     before += all;
   }
   return p;
-}
-
-// Stretch r of n: [total r / n, total (r + 1) / n).
-__device__ __forceinline__ int64_t stretch(int64_t total, int r, int n) {
-  return total / n * r + total % n * r / n;
 }
 
 // ---- query rows ----------------------------------------------------------------
@@ -203,7 +252,7 @@ struct Rows {
 
   __device__ __forceinline__ void load(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int first = lane_value(s.first, u.seq), start = a.cache.start[u.seq];
+    const int first = lane_value(s.first, u.seq), start = lane_value(s.start, u.seq);
     cap = lane_value(s.cap, u.seq);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -461,23 +510,85 @@ __device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
   return __builtin_bit_cast(h8_t, s8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
 }
 
-// Halves of f that are infinite or NaN become zero.
-__device__ __forceinline__ h8_t finite_part(h8_t f) {
-  h8_t y;
+// A weight of zero does not keep an infinity or NaN of V out of a product, so a
+// tile that some row does not see whole is looked over first (odd_values, by
+// THREADS threads together).  If it holds one, a product of the places of infinities and
+// NaN with who sees them says which sums they reach (mark_values: a bit per sum,
+// for settle()), and they become zero in LDS (clear_values).
+template <int THREADS, int BYTES>
+__device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
+  uint32_t bits = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    y[e] = __builtin_fabsf16(f[e]) < (_Float16)INFINITY ? f[e] : (_Float16)0.0f;
-  return y;
+  for (int i = 0; i < BYTES / 16 / THREADS; ++i) {
+    const u4_t f = *reinterpret_cast<const u4_t*>(v + (i * THREADS + thread) * 16);
+    // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
+    bits |= ((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
+            ((f.w & 0x7fff7fffu) + 0x04000400u);
+  }
+  return (bits & 0x80008000u) != 0;
 }
 
-// O^T += V^T P^T of 32 keys.  A weight of zero does not keep an infinity or NaN of V
-// out of the product, so where not every row sees every key (whole = false) they
-// are taken out of V, and a product of the places that hold them with who sees them
-// says which sums they reach (Sums::up, down: a bit per sum, for settle()).
+template <int THREADS, int BYTES>
+__device__ __forceinline__ void clear_values(uint8_t* v, int thread) {
+#pragma unroll 1
+  for (int i = 0; i < BYTES / 16 / THREADS; ++i) {
+    h8_t f = *reinterpret_cast<const h8_t*>(v + (i * THREADS + thread) * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      f[e] = __builtin_fabsf16(f[e]) <= (_Float16)65504.0f ? f[e] : (_Float16)0.0f;
+    *reinterpret_cast<h8_t*>(v + (i * THREADS + thread) * 16) = f;
+  }
+}
+
 template <typename T, int DP, int NQ>
-__device__ __forceinline__ void add_values(const AttentionArgs& a, const uint8_t* v, const Rows<T, DP, NQ>& r, const f4_t (&p0)[NQ], const f4_t (&p1)[NQ],
-                                           int key, bool whole, uint32_t there, Sums<DP, NQ>& sums) {
+__device__ __forceinline__ void mark_values(const AttentionArgs& a, const uint8_t* v, const Rows<T, DP, NQ>& r, int key, uint32_t there,
+                                            Sums<DP, NQ>& sums) {
+  const int g = (threadIdx.x & 63) >> 4;
+  const uint32_t base = v_base<DP>(v);
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    int low, high;
+    r.seen(a, n, key + 4 * g, low, high);
+    h8_t one;  // who sees which key
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = 16 * (e >> 2) + (e & 3);
+      one[e] = ((there >> (e >> 2)) & 1) && k > low && k <= high ? (_Float16)1.0f : (_Float16)0.0f;
+    }
+#pragma unroll 1
+    for (int step = 0; step < DP / 8; ++step) {  // d and sign: a fragment at a time in registers
+      const int d = step >> 1;
+      const bool below = step & 1;
+      h8_t f = v_fragment<DP>(base, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // infinity and NaN, -infinity and NaN
+        f[e] = (below ? -f[e] : f[e]) <= (_Float16)65504.0f ? (_Float16)0.0f : (_Float16)1.0f;
+      const f4_t many = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        bits |= many[e] > 0.0f ? 1u << e : 0u;
+      bits <<= 4 * (d & 7);
+#pragma unroll
+      for (int i = 0; i < (DP + 127) / 128; ++i) {
+        sums.up[n][i] |= !below && d >> 3 == i ? bits : 0u;
+        sums.down[n][i] |= below && d >> 3 == i ? bits : 0u;
+      }
+    }
+  }
+}
+
+// O^T += V^T P^T of 32 keys.
+template <typename T, int DP, int NQ>
+__device__ __forceinline__ void add_values(const uint8_t* v, const f4_t (&p0)[NQ], const f4_t (&p1)[NQ], Sums<DP, NQ>& sums) {
   constexpr bool kParts = Rows<T, DP, NQ>::kParts;
+  constexpr int kAhead = kParts && DP == 256 ? 1 : 4;
+  uint32_t base = v_base<DP>(v);
+  asm volatile("" : "+v"(base));  // one register, not one per fragment
+  h8_t f[kAhead + 1];
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d)
+    f[d] = v_fragment<DP>(base, d);
   h8_t w[NQ], wl[kParts ? NQ : 1];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -485,70 +596,16 @@ __device__ __forceinline__ void add_values(const AttentionArgs& a, const uint8_t
     if constexpr (kParts)
       wl[n] = pack_rest(p0[n], p1[n], w[n]);
   }
-  uint32_t base = v_base<DP>(v);
-  asm volatile("" : "+v"(base));  // one register, not one per fragment
-  bool odd = false;
-  if (!whole) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) {
-      asm volatile("" : "+v"(base)::"memory");  // V is read anew below, not kept in registers
-      const u4_t f = __builtin_bit_cast(u4_t, v_fragment<DP>(base, d));
-      // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
-      bits |= ((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
-              ((f.w & 0x7fff7fffu) + 0x04000400u);
-    }
-    odd = __any((bits & 0x80008000u) != 0);
-    if (odd) {
-      const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        int low, high;
-        r.seen(a, n, key + 4 * g, low, high);
-        h8_t one;  // who sees which key
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = 16 * (e >> 2) + (e & 3);
-          one[e] = ((there >> (e >> 2)) & 1) && k > low && k <= high ? (_Float16)1.0f : (_Float16)0.0f;
-        }
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-#pragma unroll
-          for (int sign = 0; sign < 2; ++sign) {
-            asm volatile("" : "+v"(base)::"memory");
-            h8_t f = v_fragment<DP>(base, d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)  // infinity and NaN, -infinity and NaN
-              f[e] = (sign ? f[e] >= (_Float16)-65504.0f : f[e] <= (_Float16)65504.0f) ? (_Float16)0.0f : (_Float16)1.0f;
-            const f4_t many = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              (sign ? sums.down : sums.up)[n][d / 8] |= many[e] > 0.0f ? 1u << (4 * (d % 8) + e) : 0u;
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-      }
-    }
-    asm volatile("" : "+v"(base)::"memory");
-  }
-  constexpr int kAhead = kParts && DP == 256 ? 1 : 2;
-  h8_t f[kAhead + 1];
-#pragma unroll
-  for (int d = 0; d < kAhead; ++d)
-    f[d] = v_fragment<DP>(base, d);
 #pragma unroll
   for (int d = 0; d < DP / 16; ++d) {
     if (d + kAhead < DP / 16)
       f[(d + kAhead) % (kAhead + 1)] = v_fragment<DP>(base, d + kAhead);
     asm volatile("" ::: "memory");
-    h8_t& x = f[d % (kAhead + 1)];
-    if (odd)
-      x = finite_part(x);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[n], sums.o[n][d], 0, 0, 0);
+      sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d % (kAhead + 1)], w[n], sums.o[n][d], 0, 0, 0);
       if constexpr (kParts)
-        sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, wl[n], sums.o[n][d], 0, 0, 0);
+        sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d % (kAhead + 1)], wl[n], sums.o[n][d], 0, 0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -669,6 +726,95 @@ __device__ __forceinline__ T* out_row(const AttentionArgs& a, int start, int hea
   return static_cast<T*>(a.out) + (int64_t)(start + t) * a.out_row + (int64_t)h * a.out_head;
 }
 
+// ---- units that stretches share ------------------------------------------------------
+// The sums of stretch r's first unit are in slot 2 r of the workspace, those of its
+// last one in slot 2 r + 1: QB rows of DP values, and behind all slots each row's
+// maximum and sum of weights.  They are written and read past the caches, which
+// workgroups on different XCDs do not share.
+
+template <int DP, int QB>
+__device__ __forceinline__ float* part_row(const AttentionArgs& a, int64_t slot, int row) {
+  return a.part + (slot * QB + row) * DP;
+}
+
+template <int DP, int QB>
+__device__ __forceinline__ float* part_weights(const AttentionArgs& a, int64_t slot, int row) {
+  return a.part + 2 * (int64_t)a.stretches * QB * DP + (slot * QB + row) * 2;
+}
+
+__device__ __forceinline__ float2 load_part(const float* p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM));
+}
+
+// Called by all threads once their sums are stored: the last workgroup of the unit
+// joins them.  A lane holds 4 values of a row; what bounds it is the way to memory,
+// so the loads of RU rows and PU stretches are on their way at once.
+template <typename T, int DP, int QB, int NW, int RU, int PU>
+__device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& line, const Place& p, int start, int wave) {
+  constexpr int kLanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kRows = NW * (64 / kLanes);  // lanes of a row, rows at once
+  __shared__ int arrived;
+  const int lane = threadIdx.x & 63, d = 4 * (lane & (kLanes - 1)), row = wave * (64 / kLanes) + lane / kLanes;
+  const Unit& u = p.unit;
+  const int r0 = line.of(p.at), parts = line.of(p.at + u.tiles - 1) - r0 + 1, rows = u.row_end - u.row;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    arrived = count_arrival(a.counters + r0);
+  __syncthreads();
+  if (arrived != parts - 1)
+    return;
+  if (threadIdx.x == 0)
+    reset_counter(a.counters + r0);
+  // Stretch r0 began before the unit, or with it; the others within it.
+  const int late = line.start(r0) < p.at ? 1 : 0;
+#pragma unroll 1
+  for (int first = row; first - row < rows; first += RU * kRows) {
+    float m[RU], l[RU];
+    f4_t o[RU];
+#pragma unroll
+    for (int y = 0; y < RU; ++y) {
+      m[y] = -INFINITY;
+      l[y] = 0.0f;
+      o[y] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll 1
+    for (int s0 = 0; s0 < parts; s0 += PU) {
+      float2 w[RU][PU], lo[RU][PU], hi[RU][PU];
+#pragma unroll
+      for (int s = 0; s < PU; ++s) {
+        // Past the last stretch, row or value: the last one again, left out below.
+        const int at = s0 + s < parts ? s0 + s : parts - 1;
+        const int64_t slot = 2 * (int64_t)(r0 + at) + (at == 0 ? late : 0);
+#pragma unroll
+        for (int y = 0; y < RU; ++y) {
+          const int r = first + y * kRows < rows ? first + y * kRows : rows - 1;
+          const float* v = part_row<DP, QB>(a, slot, r) + (d < DP ? d : 0);
+          w[y][s] = load_part(part_weights<DP, QB>(a, slot, r));
+          lo[y][s] = load_part(v);
+          hi[y][s] = load_part(v + 2);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < PU; ++s)
+#pragma unroll
+        for (int y = 0; y < RU; ++y) {
+          const float in = s0 + s < parts ? w[y][s].x : -INFINITY, top = fmaxf(m[y], in);
+          const float old = m[y] == top ? 1.0f : __builtin_amdgcn_exp2f(m[y] - top);
+          const float f = s0 + s < parts ? (in == top ? 1.0f : __builtin_amdgcn_exp2f(in - top)) : 0.0f;
+          m[y] = top;
+          if (s0 + s < parts) {
+            l[y] = l[y] * old + f * w[y][s].y;
+            o[y] = o[y] * old + f * f4_t{lo[y][s].x, lo[y][s].y, hi[y][s].x, hi[y][s].y};
+          }
+        }
+    }
+#pragma unroll
+    for (int y = 0; y < RU; ++y)
+      if (first + y * kRows < rows && d < a.cache.dim)
+        store4(out_row<T>(a, start, p.head, u.row + first + y * kRows) + d, l[y] == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[y] * (1.0f / l[y]));
+  }
+}
+
 // ----------------------------------------------------------------------------
 // Chunks of tokens: four waves of 16 NQ query rows each over the same key tiles,
 // two buffers of K and V in LDS, the next tile's transfers under the present
@@ -681,13 +827,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // K, V of two tiles
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int64_t per_head = tiles_of_head<QB, TK>(a, load_sequences(a)), total = per_head * c.heads;
-  // Neighbouring stretches read the same keys: they go to one XCD.
-  const int n8 = a.stretches / 8, wg = n8 * 8 == a.stretches ? ((int)blockIdx.x & 7) * n8 + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
-  int64_t x = stretch(total, wg, a.stretches);
-  const int64_t end = stretch(total, wg + 1, a.stretches);
-  if (x >= end)
+  __shared__ int kept[kSequenceInts];
+  const Sequences loaded = load_sequences(a);
+  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded);
+  if ((int)blockIdx.x >= line.n)
     return;
+  if (wave == 0)
+    keep_sequences(loaded, kept);
+  __syncthreads();
+  // Neighbouring stretches read the same keys: they go to one XCD (workgroup L runs
+  // on XCD L % 8).
+  const int xcd = (int)blockIdx.x & 7, more = line.n & 7;
+  const int wg = xcd * (line.n >> 3) + (xcd < more ? xcd : more) + ((int)blockIdx.x >> 3);
+  int64_t x = line.start(wg);
+  const int64_t end = line.start(wg + 1);
   if (c.dim != DP) {
     for (int i = tid; i < 4 * kTile / 16; i += 256)
       reinterpret_cast<u4_t*>(lds)[i] = u4_t{0, 0, 0, 0};
@@ -697,10 +850,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
   from.set(c);
   bool leading = true;  // the stretch's first unit
   while (x < end) {
-    const Sequences seqs = load_sequences(a);  // anew for each unit: no registers under its products
-    const Place p = locate<QB, TK>(a, seqs, per_head, x);
+    const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
+    const Place p = locate<QB, TK>(a, seqs, line, x);
     const Unit& u = p.unit;
-    const int start = c.start[u.seq];
+    const int start = lane_value(seqs.start, u.seq);
     const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
     Rows<T, DP, NQ> rows;
     const int row = u.row + wave * 16 * NQ;
@@ -715,6 +868,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
     const int hi_least = ta < cap ? ta : cap, hi_most = tb < cap ? tb : cap;
     const int lo_least = a.window && ta > a.window ? ta - a.window : 0, lo_most = a.window && tb > a.window ? tb - a.window : 0;
     const bool none = u.hi <= u.lo;
+    // What all rows of the unit see.
+    const int ua = first + u.row / a.group + 1, ub = first + (u.row_end - 1) / a.group + 1;
+    const int unit_hi = ua < cap ? ua : cap, unit_lo = a.window && ub > a.window ? ub - a.window : 0;
     Pages pages;
     pages.open(a, seqs, u.seq);
     uint32_t there = 0;
@@ -754,17 +910,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
         if (t + 1 < n)
           fetch(t0 + t + 1, (t + 1) & 1);
         const int key = u.lo + (t0 + t) * TK;
-        if (!active || key >= hi_most || key + TK <= lo_least)
+        uint8_t* const k = lds + (t & 1) * 2 * kTile;
+        const bool most = active && key < hi_most && key + TK > lo_least;
+        if (key + TK > unit_hi || key < unit_lo || here != (1u << NA) - 1) {
+          if (__syncthreads_or(odd_values<256, kTile>(k + kTile, tid))) {
+            if (most)
+#pragma unroll
+              for (int h = 0; h < NA / 2; ++h)
+                mark_values<T, DP, NQ>(a, k + kTile + h * 32 * DP * 2, rows, key + 32 * h, here >> (2 * h), sums);
+            __syncthreads();
+            clear_values<256, kTile>(k + kTile, tid);
+            __syncthreads();
+          }
+        }
+        if (!most)
           continue;
         const bool whole = key + TK <= hi_least && key >= lo_most && here == (1u << NA) - 1;
-        const uint8_t* k = lds + (t & 1) * 2 * kTile;
         f4_t s[NA][NQ];
         scores<T, DP, NQ, NA>(k, rows, s);
         finish_scores<T, DP, NQ, NA>(a, rows, key, whole, here, FORM, s);
         sums.weigh(s, [&](int y) { return FORM ? 1.0f : rows.factor(y); });
 #pragma unroll
         for (int h = 0; h < NA / 2; ++h) {
-          add_values<T, DP, NQ>(a, k + kTile + h * 32 * DP * 2, rows, s[2 * h], s[2 * h + 1], key + 32 * h, whole, here >> (2 * h), sums);
+          add_values<T, DP, NQ>(k + kTile + h * 32 * DP * 2, s[2 * h], s[2 * h + 1], sums);
         }
       }
     }
@@ -786,17 +954,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
           if (16 * d + 4 * g < c.dim)
             store4(o + 16 * d + 4 * g, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : sums.o[y][d] * f);
       } else {
-        float* o = a.part + (slot * QB + (r - u.row)) * DP;
+        float* o = part_row<DP, QB>(a, slot, r - u.row);
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
-          *reinterpret_cast<f4_t*>(o + 16 * d + 4 * g) = sums.o[y][d];
+          store_coherent4(o + 16 * d + 4 * g, sums.o[y][d]);
         if (g == 0) {
-          float* ml = a.part + 2 * (int64_t)a.stretches * QB * DP + (slot * QB + (r - u.row)) * 2;
-          ml[0] = sums.m[y];
-          ml[1] = l;
+          float* ml = part_weights<DP, QB>(a, slot, r - u.row);
+          store_coherent(ml, sums.m[y]);
+          store_coherent(ml + 1, l);
         }
       }
     }
+    if (!done)
+      join_unit<T, DP, QB, 4, 8, 2>(a, line, p, start, wave);
     x += n;
     leading = false;
   }
@@ -816,12 +986,17 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   __shared__ float sm[NW][QB], sl[NW][QB];
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int64_t per_head = tiles_of_head<QB, TK>(a, load_sequences(a)), total = per_head * c.heads;
+  __shared__ int kept[kSequenceInts];
+  const Sequences loaded = load_sequences(a);
+  const Line line = make_line<QB, TK, NW>(a, loaded);
   const int wg = (int)blockIdx.x;
-  int64_t x = stretch(total, wg, a.stretches);
-  const int64_t end = stretch(total, wg + 1, a.stretches);
-  if (x >= end)
+  if (wg >= line.n)
     return;
+  if (wave == 0)
+    keep_sequences(loaded, kept);
+  __syncthreads();
+  int64_t x = line.start(wg);
+  const int64_t end = line.start(wg + 1);
   Lanes<DP> from;
   from.set(c);
   uint8_t* const mine = lds + wave * 2 * kTile;
@@ -829,10 +1004,10 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   const bool formed = a.softcap > 0.0f || a.slopes;
   bool leading = true;
   while (x < end) {
-    const Sequences seqs = load_sequences(a);  // anew for each unit: no registers under its products
-    const Place p = locate<QB, TK>(a, seqs, per_head, x);
+    const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
+    const Place p = locate<QB, TK>(a, seqs, line, x);
     const Unit& u = p.unit;
-    const int start = c.start[u.seq];
+    const int start = lane_value(seqs.start, u.seq);
     const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
     Rows<T, DP, NQ> rows;
     rows.load(a, seqs, u, p.head, u.row);
@@ -887,7 +1062,13 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
           wait_loads<kLoads>();
         else
           wait_loads<0>();
-        add_values<T, DP, NQ>(a, mine + kTile, rows, s[0], s[1], key, whole, there, sums);
+        if (!whole && __any(odd_values<64, kTile>(mine + kTile, lane))) {
+          mark_values<T, DP, NQ>(a, mine + kTile, rows, key, there, sums);
+          wait_lds();
+          clear_values<64, kTile>(mine + kTile, lane);
+          wait_lds();
+        }
+        add_values<T, DP, NQ>(mine + kTile, s[0], s[1], sums);
         wait_lds();
         if (more)
           fetch_v(t0 + t + NW);
@@ -931,80 +1112,21 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         if (done) {
           store4(out_row<T>(a, start, p.head, r) + d, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / l));
         } else {
-          *reinterpret_cast<f4_t*>(a.part + (slot * QB + 16 * y + rr) * DP + d) = o;
+          store_coherent4(part_row<DP, QB>(a, slot, 16 * y + rr) + d, o);
           if (d == 0) {
-            float* ml = a.part + 2 * (int64_t)a.stretches * QB * DP + (slot * QB + 16 * y + rr) * 2;
-            ml[0] = top;
-            ml[1] = l;
+            float* ml = part_weights<DP, QB>(a, slot, 16 * y + rr);
+            store_coherent(ml, top);
+            store_coherent(ml + 1, l);
           }
         }
       }
     }
+    if (!done)
+      join_unit<T, DP, QB, NW, 1, 8>(a, line, p, start, wave);
     __syncthreads();  // before the buffers and statistics are used again
     x += n;
     leading = false;
   }
-}
-
-// ----------------------------------------------------------------------------
-// Joins the sums of a unit that several stretches share.  Workgroup (b, part)
-// stands for the border before stretch b + 1: if it is the first within its
-// unit, the workgroup adds 16 of the unit's rows up, in the order of the
-// stretches.
-// ----------------------------------------------------------------------------
-template <typename T, int DP, int QB, int TK>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
-  const CacheArgs& c = a.cache;
-  const Sequences seqs = load_sequences(a);
-  const int64_t per_head = tiles_of_head<QB, TK>(a, seqs), total = per_head * c.heads;
-  const int b = (int)blockIdx.x + 1;
-  const int64_t x = stretch(total, b, a.stretches), before = stretch(total, b - 1, a.stretches);
-  if (x >= total || x == before)
-    return;
-  const Place p = locate<QB, TK>(a, seqs, per_head, x);
-  if (p.at == x || before > p.at)
-    return;
-  const Unit& u = p.unit;
-  const int64_t last = p.at + u.tiles;
-  const int rr = 16 * (int)blockIdx.y + (int)(threadIdx.x >> 4), r = u.row + rr, d0 = 4 * (int)(threadIdx.x & 15);
-  if (r >= u.row_end)
-    return;
-  const float* const ml = a.part + 2 * (int64_t)a.stretches * QB * DP;
-  // Stretch b - 1 ends within the unit: its sums are its last ones (slot 1), unless
-  // it began there too.
-  const int64_t lead = 2 * (int64_t)(b - 1) + (before == p.at ? 0 : stretch(total, b - 1, a.stretches) < p.at ? 1 : 0);
-  float top = ml[(lead * QB + rr) * 2];
-  int to = b;
-  for (; to < a.stretches && stretch(total, to, a.stretches) < last; ++to)
-    if (stretch(total, to + 1, a.stretches) > stretch(total, to, a.stretches))
-      top = fmaxf(top, ml[(2 * (int64_t)to * QB + rr) * 2]);
-  f4_t o[DP / 64 + (DP % 64 != 0)];
-  constexpr int kSteps = sizeof(o) / sizeof(o[0]);
-  float l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    o[i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = b - 1; s < to; ++s) {
-    if (s >= b && stretch(total, s + 1, a.stretches) == stretch(total, s, a.stretches))
-      continue;
-    const int64_t at = (s < b ? lead : 2 * (int64_t)s) * QB + rr;
-    const float m = ml[at * 2], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-    l = fmaf(f, ml[at * 2 + 1], l);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-      if (d0 + 64 * i < c.dim)
-        o[i] += f * *reinterpret_cast<const f4_t*>(a.part + at * DP + d0 + 64 * i);
-  }
-  T* y = out_row<T>(a, c.start[u.seq], p.head, r);
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (d0 + 64 * i < c.dim)
-      store4(y + d0 + 64 * i, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[i] * (1.0f / l));
-}
-
-template <typename T, int DP, int QB, int TK>
-hipError_t launch_join(hipStream_t s, const AttentionArgs& a) {
-  return dispatch(attention_join_kernel<T, DP, QB, TK>, dim3(a.stretches - 1, (QB + 15) / 16), dim3(256), s, a);
 }
 
 template <typename T, int DP>
@@ -1019,16 +1141,11 @@ hipError_t launch_t(hipStream_t s, const AttentionArgs& a) {
       e = dispatch(attention_rows_kernel<T, DP, 3, 4>, dim3(a.stretches), dim3(256), s, a);
     else
       e = hipErrorInvalidValue;
-    if (e != hipSuccess || a.stretches == 1)
-      return e;
-    return a.row_tiles == 1 ? launch_join<T, DP, 16, 32>(s, a) : a.row_tiles == 2 ? launch_join<T, DP, 32, 32>(s, a) : launch_join<T, DP, 48, 32>(s, a);
+    return e;
   }
   constexpr int NQ = AttentionShape::chunk_tiles(DP, sizeof(T) == 4), TK = AttentionShape::chunk_keys(DP);
-  hipError_t e = a.softcap > 0.0f || a.slopes ? dispatch(attention_chunk_kernel<T, DP, NQ, TK, true>, dim3(a.stretches), dim3(256), s, a)
-                                              : dispatch(attention_chunk_kernel<T, DP, NQ, TK, false>, dim3(a.stretches), dim3(256), s, a);
-  if (e != hipSuccess || a.stretches == 1)
-    return e;
-  return launch_join<T, DP, 64 * NQ, TK>(s, a);
+  return a.softcap > 0.0f || a.slopes ? dispatch(attention_chunk_kernel<T, DP, NQ, TK, true>, dim3(a.stretches), dim3(256), s, a)
+                                      : dispatch(attention_chunk_kernel<T, DP, NQ, TK, false>, dim3(a.stretches), dim3(256), s, a);
 }
 
 template <typename T>

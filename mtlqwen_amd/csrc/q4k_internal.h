@@ -623,7 +623,8 @@ struct AttentionArgs {
   // those before each sequence, the workgroups.
   int row_tiles = 0, units = 0, stretches = 1;
   int unit[kMaxSequences] = {};
-  float* part = nullptr;  // the plan's floats: sums of units that workgroups share
+  float* part = nullptr;     // the plan's floats: sums of units that workgroups share
+  int* counters = nullptr;   // [stretches], zero between launches
 };
 // Head sizes, as the kernels are built for them, and their chunks: 16-row tiles of
 // a wave, keys of a tile.
@@ -631,6 +632,7 @@ struct AttentionShape {
   static constexpr int padded(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
   static constexpr int chunk_tiles(int dp, bool f32) { return f32 && dp == 256 ? 1 : 2; }
   static constexpr int chunk_waves(int dp, bool f32) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
+  static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
   static constexpr int chunk_keys(int dp) { return dp > 128 ? 32 : 64; }
 };
 // Sets the plan; the floats of `part`.
