@@ -2415,6 +2415,8 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
     rc = check_cache(cache, positions, nq);
   if (rc)
     return rc;
+  if ((uint64_t)rows * q->heads > 0x7fffffffu)
+    return fail(Q4K_ESHAPE, "at most 2^31 - 1 rows of heads (got %u of %u)", rows, q->heads);
   if (q->heads % cache->heads != 0)
     return fail(Q4K_ESHAPE, "the heads of q must be a multiple of the cache's (got %u and %u)", q->heads, cache->heads);
   if (!std::isfinite(params->scale) || !std::isfinite(params->softcap) || params->softcap < 0.0f || params->window > 0x7fffffffu)
@@ -2453,14 +2455,28 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
   Workspace& ws = workspace(device);
   std::lock_guard<std::mutex> lock(ws.mu);
   reserve_workspace(s, ws, device);
-  const size_t floats = attention_plan(a, (int)dtype, device_cus(device));
+  size_t floats = 0;
+  const uint32_t heads = (uint32_t)attention_plan(a, (int)dtype, device_cus(device), &floats);
+  if (heads == 0)
+    return fail(Q4K_ESHAPE, "%u rows of %u heads over tables of %u pages of %u tokens are more than one call takes", rows, q->heads, cache->width,
+                cache->page_size);
   rc = ensure_splitk_workspace(s, ws, device, floats, (size_t)a.stretches);
   if (rc)
     return rc;
   a.part = ws.part;
   a.counters = ws.counters;
-  LaunchTimer timer(s, Q4K_KERNEL_AUX);
-  Q4K_TRY_HIP(launch_attention(s, a, (int)dtype), "attention launch");
+  const AttentionArgs all = a;
+  for (uint32_t h = 0; h < cache->heads; h += heads) {
+    const uint32_t first = h * (uint32_t)all.group;
+    a.cache.heads = cache->heads - h < heads ? cache->heads - h : heads;
+    a.cache.k = static_cast<uint8_t*>(all.cache.k) + (size_t)h * cache->head_stride * 2;
+    a.cache.v = static_cast<uint8_t*>(all.cache.v) + (size_t)h * cache->head_stride * 2;
+    a.q = static_cast<const uint8_t*>(all.q) + (size_t)first * q->in_head_stride * es;
+    a.out = static_cast<uint8_t*>(all.out) + (size_t)first * q->out_head_stride * es;
+    a.slopes = all.slopes ? all.slopes + first : nullptr;
+    LaunchTimer timer(s, Q4K_KERNEL_AUX);
+    Q4K_TRY_HIP(launch_attention(s, a, (int)dtype), "attention launch");
+  }
   return Q4K_OK;
 }
 

@@ -69,11 +69,25 @@ __device__ __forceinline__ int lane_value(int v, int lane) {
 }
 
 // ---- the line of work --------------------------------------------------------
+// Whole numbers of 32 bits throughout (attention_plan bounds the line): what is
+// computed once per launch or unit is computed by code that was never fetched
+// before, at about 140 clocks for every 64 bytes of it.
+
+// x / y for any x, m = 2^32 / y rounded down (2^32 - 1 for y = 1): the product is
+// one too small at most.
+__device__ __forceinline__ uint32_t divided(uint32_t x, uint32_t y, uint32_t m) {
+  const uint32_t q = __umulhi(x, m);
+  return q + ((uint64_t)(q + 1) * y <= x ? 1u : 0u);
+}
+
+// The token of query row u of a sequence.
+__device__ __forceinline__ int token_of(const AttentionArgs& a, int u) {
+  return (int)divided((uint32_t)u, (uint32_t)a.group, a.group_inverse);
+}
 
 // One sequence per lane: the position of its first row, the keys that its table
 // holds, its query rows per cache head, the units before it, its table, its first
-// row in the batch.  Read from the arguments and the device's arrays once (the
-// arguments lie in host memory: a reading there takes microseconds), then kept in LDS.
+// row in the batch.
 struct Sequences {
   int first, cap, rows, unit, slot, start;
 };
@@ -129,7 +143,7 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const Sequences&
   if (u >= a.units)
     return x;
   x.row_end = x.row + QB < rows ? x.row + QB : rows;
-  const int t0 = x.row / a.group, t1 = (x.row_end - 1) / a.group;
+  const int t0 = token_of(a, x.row), t1 = token_of(a, x.row_end - 1);
   x.hi = first + t1 + 1 < cap ? first + t1 + 1 : cap;
   x.hi = x.hi < 0 ? 0 : x.hi;
   x.lo = a.window && first + t0 + 1 > a.window ? (first + t0 + 1 - a.window) & -TK : 0;
@@ -137,96 +151,88 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const Sequences&
   return x;
 }
 
-// The line: tiles of one cache head and in all, and its n stretches, stretch r from
-// start(r) on.  No more of them than leaves LEAST tiles to each.  Wave-uniform.
-struct Line {
-  int64_t per_head, total, step;
-  int n, rest;  // total = n step + rest
-  float per_n;
-  double per_tiles;  // 1 / per_head
-
-  // n step r / n + floor(rest r / n): rest r < 2^20 and n <= 1024, so that half a
-  // unit keeps the rounded quotient off the next whole number.
-  __device__ __forceinline__ int64_t start(int r) const { return step * r + (int)(((float)(rest * r) + 0.5f) * per_n); }
-
-  // The stretch that holds place x.
-  __device__ __forceinline__ int of(int64_t x) const {
-    int r = __builtin_amdgcn_readfirstlane((int)((double)x / (double)step));
-    r = r < n - 1 ? r : n - 1;
-    while (start(r) > x)
-      --r;
-    return r;
-  }
-};
-
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return (int64_t)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)v));
+// Sum over this lane and those before it.
+__device__ __forceinline__ int scan_lanes(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
 }
 
+// 64 units from u0 on, one per lane, and the tiles up to each.
+struct Units {
+  Unit unit;
+  int upto;
+};
+
+template <int QB, int TK>
+__device__ __forceinline__ Units units_from(const AttentionArgs& a, const Sequences& q, int u0) {
+  Units x;
+  x.unit = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63));
+  x.upto = scan_lanes(x.unit.tiles);
+  return x;
+}
+
+// The line: tiles of one cache head and in all, and the tiles of a stretch: a
+// multiple of LEAST, so that the line makes no more stretches than workgroups.
+// Wave-uniform.
+struct Line {
+  int per_head, total, step;
+
+  // x / y where the quotient is small beside 2^23: the rounded one is one off at most.
+  static __device__ __forceinline__ int quotient(int x, int y) {
+    const int q = __builtin_amdgcn_readfirstlane((int)((float)x * __builtin_amdgcn_rcpf((float)y)));
+    const int rest = (int)((uint32_t)x - (uint32_t)q * (uint32_t)y);
+    return q + (rest >= y ? 1 : 0) - (rest < 0 ? 1 : 0);
+  }
+  __device__ __forceinline__ int stretches() const { return quotient(total - 1, step) + 1; }
+  __device__ __forceinline__ int start(int r) const { return r * step; }
+  __device__ __forceinline__ int end(int r) const { return r * step < total - step ? r * step + step : total; }
+  // The stretch that holds place x.
+  __device__ __forceinline__ int of(int x) const { return quotient(x, step); }
+};
+
+// `near`: the first 64 units.
 template <int QB, int TK, int LEAST>
-__device__ __forceinline__ Line make_line(const AttentionArgs& a, const Sequences& q) {
+__device__ __forceinline__ Line make_line(const AttentionArgs& a, const Sequences& q, const Units& near) {
   Line x;
-  x.per_head = 0;
-  for (int u0 = 0; u0 < a.units; u0 += 64) {
-    uint32_t n = (uint32_t)unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63)).tiles;  // up to 64 * 2^26
-    for (int off = 32; off; off >>= 1)
-      n += __shfl_xor(n, off);
-    x.per_head += n;
-  }
-  x.per_head = uniform(x.per_head);
-  x.total = x.per_head * a.cache.heads;
-  x.n = x.total >= (int64_t)a.stretches * LEAST ? a.stretches : (int)((uint32_t)(x.total + LEAST - 1) / LEAST);
-  x.step = uniform((int64_t)((double)x.total / (double)x.n));
-  x.rest = (int)(x.total - x.step * x.n);
-  if (x.rest < 0 || x.rest >= x.n) {  // the quotient rounded over a whole number
-    x.step += x.rest < 0 ? -1 : 1;
-    x.rest = (int)(x.total - x.step * x.n);
-  }
-  x.per_n = 1.0f / (float)x.n;
-  x.per_tiles = 1.0 / (double)x.per_head;
+  x.per_head = lane_value(near.upto, 63);
+  for (int u0 = 64; u0 < a.units; u0 += 64)
+    x.per_head += lane_value(units_from<QB, TK>(a, q, u0).upto, 63);
+  x.total = x.per_head * (int)a.cache.heads;
+  const int each = (int)divided((uint32_t)(x.total + a.stretches - 1), (uint32_t)a.stretches, a.stretches_inverse);
+  x.step = (each + LEAST - 1) & -LEAST;
   return x;
 }
 
 // The unit that holds place x of the line, and the place of its first tile (wave-uniform).
 struct Place {
   Unit unit;
-  int head;
-  int64_t at;
+  int head, at;
 };
 
 template <int QB, int TK>
-__device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, const Line& line, int64_t x) {
+__device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, const Line& line, const Units& near, int x) {
   Place p;
-  p.head = __builtin_amdgcn_readfirstlane((int)((double)x * line.per_tiles));
-  int64_t y = x - p.head * line.per_head;
-  if (y < 0 || y >= line.per_head) {
-    p.head += y < 0 ? -1 : 1;
-    y = x - p.head * line.per_head;
+  p.head = Line::quotient(x, line.per_head);
+  const int y = x - p.head * line.per_head;
+  Units here = near;
+  int before = 0;
+  for (int u0 = 64; y >= before + lane_value(here.upto, 63); u0 += 64) {  // ends: y < per_head
+    before += lane_value(here.upto, 63);
+    here = units_from<QB, TK>(a, q, u0);
   }
-  int64_t before = 0;
-  p.at = x;
-  p.unit = Unit{0, 0, 0, 0, 0, 1};
-  for (int u0 = 0; u0 < a.units; u0 += 64) {
-    const Unit u = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63));
-    uint32_t n = (uint32_t)u.tiles;
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = __shfl_up(n, off);
-      n += (int)(threadIdx.x & 63) >= off ? o : 0;
-    }
-    const uint32_t all = __builtin_amdgcn_readlane(n, 63);
-    if (y < before + all) {
-      const int lane = __ffsll((unsigned long long)__ballot((uint64_t)n > (uint64_t)(y - before))) - 1;
-      p.unit.seq = lane_value(u.seq, lane);
-      p.unit.row = lane_value(u.row, lane);
-      p.unit.row_end = lane_value(u.row_end, lane);
-      p.unit.lo = lane_value(u.lo, lane);
-      p.unit.hi = lane_value(u.hi, lane);
-      p.unit.tiles = lane_value(u.tiles, lane);
-      p.at = p.head * line.per_head + before + (int64_t)((uint32_t)__builtin_amdgcn_readlane(n, lane) - (uint32_t)p.unit.tiles);
-      break;
-    }
-    before += all;
-  }
+  const int lane = __ffsll((unsigned long long)__ballot(here.upto > y - before)) - 1;
+  p.unit.seq = lane_value(here.unit.seq, lane);
+  p.unit.row = lane_value(here.unit.row, lane);
+  p.unit.row_end = lane_value(here.unit.row_end, lane);
+  p.unit.lo = lane_value(here.unit.lo, lane);
+  p.unit.hi = lane_value(here.unit.hi, lane);
+  p.unit.tiles = lane_value(here.unit.tiles, lane);
+  p.at = p.head * line.per_head + before + lane_value(here.upto, lane) - p.unit.tiles;
   return p;
 }
 
@@ -258,7 +264,7 @@ struct Rows {
     for (int n = 0; n < NQ; ++n) {
       const int r = row + 16 * n + i;
       const bool live = r < u.row_end;
-      const int t = r / a.group, h = head * a.group + (r - t * a.group);
+      const int t = token_of(a, r), h = head * a.group + (r - t * a.group);
       const T* x = static_cast<const T*>(a.q) + (int64_t)(start + t) * a.q_row + (int64_t)h * a.q_head + 8 * g;
       c[kParts ? n : 0] = a.scale * kLog2e;
       if constexpr (kParts) {
@@ -722,7 +728,7 @@ __device__ __forceinline__ void store4(T* p, f4_t v) {
 
 template <typename T>
 __device__ __forceinline__ T* out_row(const AttentionArgs& a, int start, int head, int u) {
-  const int t = u / a.group, h = head * a.group + (u - t * a.group);
+  const int t = token_of(a, u), h = head * a.group + (u - t * a.group);
   return static_cast<T*>(a.out) + (int64_t)(start + t) * a.out_row + (int64_t)h * a.out_head;
 }
 
@@ -829,18 +835,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   __shared__ int kept[kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded);
-  if ((int)blockIdx.x >= line.n)
+  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded, units_from<QB, TK>(a, loaded, 0));
+  const int stretches = line.stretches();
+  if ((int)blockIdx.x >= stretches)
     return;
   if (wave == 0)
     keep_sequences(loaded, kept);
   __syncthreads();
   // Neighbouring stretches read the same keys: they go to one XCD (workgroup L runs
   // on XCD L % 8).
-  const int xcd = (int)blockIdx.x & 7, more = line.n & 7;
-  const int wg = xcd * (line.n >> 3) + (xcd < more ? xcd : more) + ((int)blockIdx.x >> 3);
-  int64_t x = line.start(wg);
-  const int64_t end = line.start(wg + 1);
+  const int xcd = (int)blockIdx.x & 7, more = stretches & 7;
+  const int wg = xcd * (stretches >> 3) + (xcd < more ? xcd : more) + ((int)blockIdx.x >> 3);
+  int x = line.start(wg);
+  const int end = line.end(wg);
   if (c.dim != DP) {
     for (int i = tid; i < 4 * kTile / 16; i += 256)
       reinterpret_cast<u4_t*>(lds)[i] = u4_t{0, 0, 0, 0};
@@ -851,10 +858,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
   bool leading = true;  // the stretch's first unit
   while (x < end) {
     const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
-    const Place p = locate<QB, TK>(a, seqs, line, x);
+    const Place p = locate<QB, TK>(a, seqs, line, units_from<QB, TK>(a, seqs, 0), x);
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
-    const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
+    const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
     Rows<T, DP, NQ> rows;
     const int row = u.row + wave * 16 * NQ;
     rows.load(a, seqs, u, p.head, row);
@@ -864,12 +871,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
     const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
     const int last = (row + 16 * NQ < u.row_end ? row + 16 * NQ : u.row_end) - 1;
     const bool active = row < u.row_end;
-    const int ta = first + row / a.group + 1, tb = first + (active ? last : row) / a.group + 1;
+    const int ta = first + token_of(a, row) + 1, tb = first + token_of(a, active ? last : row) + 1;
     const int hi_least = ta < cap ? ta : cap, hi_most = tb < cap ? tb : cap;
     const int lo_least = a.window && ta > a.window ? ta - a.window : 0, lo_most = a.window && tb > a.window ? tb - a.window : 0;
     const bool none = u.hi <= u.lo;
     // What all rows of the unit see.
-    const int ua = first + u.row / a.group + 1, ub = first + (u.row_end - 1) / a.group + 1;
+    const int ua = first + token_of(a, u.row) + 1, ub = first + token_of(a, u.row_end - 1) + 1;
     const int unit_hi = ua < cap ? ua : cap, unit_lo = a.window && ub > a.window ? ub - a.window : 0;
     Pages pages;
     pages.open(a, seqs, u.seq);
@@ -986,17 +993,22 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   __shared__ float sm[NW][QB], sl[NW][QB];
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  __shared__ int kept[kSequenceInts];
+  // With one row tile they stay in registers; with more they would not fit beside O.
+  constexpr bool kKeep = NQ == 1;
+  __shared__ int kept[kKeep ? 1 : kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Line line = make_line<QB, TK, NW>(a, loaded);
+  const Units first_units = units_from<QB, TK>(a, loaded, 0);
+  const Line line = make_line<QB, TK, NW>(a, loaded, first_units);
   const int wg = (int)blockIdx.x;
-  if (wg >= line.n)
+  if (wg >= line.stretches())
     return;
-  if (wave == 0)
-    keep_sequences(loaded, kept);
-  __syncthreads();
-  int64_t x = line.start(wg);
-  const int64_t end = line.start(wg + 1);
+  if constexpr (!kKeep) {
+    if (wave == 0)
+      keep_sequences(loaded, kept);
+    __syncthreads();
+  }
+  int x = line.start(wg);
+  const int end = line.end(wg);
   Lanes<DP> from;
   from.set(c);
   uint8_t* const mine = lds + wave * 2 * kTile;
@@ -1004,17 +1016,18 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   const bool formed = a.softcap > 0.0f || a.slopes;
   bool leading = true;
   while (x < end) {
-    const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
-    const Place p = locate<QB, TK>(a, seqs, line, x);
+    Sequences seqs = loaded;
+    Units near = first_units;
+    if constexpr (!kKeep) {
+      seqs = kept_sequences(kept);
+      near = units_from<QB, TK>(a, seqs, 0);
+    }
+    const Place p = locate<QB, TK>(a, seqs, line, near, x);
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
-    const int t0 = (int)(x - p.at), left = u.tiles - t0, n = end - x < left ? (int)(end - x) : left;
-    Rows<T, DP, NQ> rows;
-    rows.load(a, seqs, u, p.head, u.row);
-    Sums<DP, NQ> sums;
-    sums.clear();
+    const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
     const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
-    const int ta = first + u.row / a.group + 1, tb = first + (u.row_end - 1) / a.group + 1;
+    const int ta = first + token_of(a, u.row) + 1, tb = first + token_of(a, u.row_end - 1) + 1;
     const int hi_least = ta < cap ? ta : cap, lo_most = a.window && tb > a.window ? tb - a.window : 0;
     Pages pages;
     pages.open(a, seqs, u.seq);
@@ -1040,10 +1053,17 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
       for (int b = 0; b < 2; ++b)
         dma_v<DP>(c, from, tokens_at(c, c.v, p.head, pg[b], key + 16 * b), at + kTile + b * (DP / 32) * 1024);
     };
-    if (u.hi > u.lo && wave < n) {
+    const bool busy = u.hi > u.lo && wave < n;
+    if (busy) {
       open(t0 + wave);
       fetch_k(t0 + wave);
       fetch_v(t0 + wave);
+    }
+    Rows<T, DP, NQ> rows;  // on their way with the first keys
+    rows.load(a, seqs, u, p.head, u.row);
+    Sums<DP, NQ> sums;
+    sums.clear();
+    if (busy) {
       for (int t = wave; t < n; t += NW) {
         const int key = u.lo + (t0 + t) * TK;
         const uint32_t there = (pg[0] >= 0 ? 1u : 0u) | (pg[1] >= 0 ? 2u : 0u);
@@ -1167,13 +1187,14 @@ hipError_t launch_d(hipStream_t s, const AttentionArgs& a) {
 }  // namespace
 
 // Which kernel, how many query rows a unit has, how many workgroups: by the
-// counts of new rows, the heads and the head size, which the host knows.
-size_t attention_plan(AttentionArgs& a, int dtype, int cus) {
+// counts of new rows, the heads and the head size, which the host knows.  Returns the
+// cache heads that a launch may take (the line's places have 32 bits; 0: not one).
+int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats) {
   const CacheArgs& c = a.cache;
   int most = 0;
   for (int s = 0; s < c.nq; ++s)
     most = c.count[s] > most ? c.count[s] : most;
-  const int64_t rows = (int64_t)most * a.group;
+  const int rows = most * a.group;
   const int dp = AttentionShape::padded(c.dim);
   a.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && dp <= 128 ? 3 : 0;
   const int qb = a.row_tiles ? 16 * a.row_tiles : 64 * AttentionShape::chunk_tiles(dp, dtype == kF32);
@@ -1184,10 +1205,16 @@ size_t attention_plan(AttentionArgs& a, int dtype, int cus) {
     a.units += (int)(((int64_t)c.count[s] * a.group + qb - 1) / qb);
   }
   // No more workgroups than tiles: as many as a table holds, for every unit.
-  const int64_t tiles = (int64_t)a.units * c.heads * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1);
-  const int wgs = a.row_tiles ? cus : 2 * cus;
-  a.stretches = tiles < wgs ? (int)tiles : wgs;
-  return 2 * (size_t)a.stretches * qb * (dp + 2);
+  const int64_t tiles = (int64_t)a.units * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1);
+  const int wgs = a.row_tiles ? cus : AttentionShape::chunk_waves(dp, dtype == kF32) * cus;
+  a.stretches = tiles * c.heads < wgs ? (int)(tiles * c.heads) : wgs;
+  const auto inverse = [](int y) { return y == 1 ? ~0u : (uint32_t)((1ull << 32) / (uint32_t)y); };
+  a.group_inverse = inverse(a.group);
+  a.stretches_inverse = inverse(a.stretches);
+  *floats = 2 * (size_t)a.stretches * qb * (dp + 2);
+  // Stretches of up to 8 tiles more than their share, 32-bit places.
+  const int64_t places = (1ll << 31) - 1 - 16ll * wgs;
+  return tiles > places ? 0 : (int)(places / tiles < (int64_t)c.heads ? places / tiles : c.heads);
 }
 
 hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype) {

@@ -622,6 +622,7 @@ struct AttentionArgs {
   // Set by attention_plan: the 16-row tiles of a unit (0: a chunk's), the units and
   // those before each sequence, the workgroups.
   int row_tiles = 0, units = 0, stretches = 1;
+  uint32_t group_inverse = 0, stretches_inverse = 0;  // 2^32 / y, rounded down
   int unit[kMaxSequences] = {};
   float* part = nullptr;     // the plan's floats: sums of units that workgroups share
   int* counters = nullptr;   // [stretches], zero between launches
@@ -635,8 +636,8 @@ struct AttentionShape {
   static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
   static constexpr int chunk_keys(int dp) { return dp > 128 ? 32 : 64; }
 };
-// Sets the plan; the floats of `part`.
-size_t attention_plan(AttentionArgs& a, int dtype, int cus);
+// Sets the plan and the floats of `part`; the cache heads that a launch may take.
+int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats);
 hipError_t launch_attention(hipStream_t s, const AttentionArgs& a, int dtype);
 
 // Tables of all slots, as they are and as they become.
