@@ -524,7 +524,7 @@ __device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
 template <int THREADS, int BYTES>
 __device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
   uint32_t bits = 0;
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < BYTES / 16 / THREADS; ++i) {
     const u4_t f = *reinterpret_cast<const u4_t*>(v + (i * THREADS + thread) * 16);
     // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
@@ -673,28 +673,44 @@ struct Lanes {
   }
 };
 
-template <int DP, int D = 0>
-__device__ __forceinline__ void dma_k(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+template <int DP, bool WHOLE, int D = 0>
+__device__ __forceinline__ void dma_k_from(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
   if constexpr (D < DP / 32) {
     // The instruction's offset moves both addresses.
-    if (c.dim == DP || 32 * D + 8 * (int)((threadIdx.x & 63) >> 4) < c.dim)
+    if (WHOLE || 32 * D + 8 * (int)((threadIdx.x & 63) >> 4) < c.dim)
       lds_dma16<64 * D>(from, l.k, __builtin_amdgcn_readfirstlane(lds + (1024 - 64) * D));
-    dma_k<DP, D + 1>(c, l, from, lds);
+    dma_k_from<DP, WHOLE, D + 1>(c, l, from, lds);
   }
 }
 
-template <int DP>
-__device__ __forceinline__ void dma_v(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+template <int DP, bool WHOLE>
+__device__ __forceinline__ void dma_v_from(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
   using L = Lanes<DP>;
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x)
-    if (c.dim == DP || l.in_head(c, x)) {
+    if (WHOLE || l.in_head(c, x)) {
       const uint32_t to = __builtin_amdgcn_readfirstlane(lds + 1024 * x);
       if constexpr (L::kEven)
         lds_dma16<0>(from + (int64_t)(x * L::kRows) * c.token_stride * 2, (l.chunk[0] ^ (v_swizzle<DP>(x * L::kRows) * 16)) + l.row, to);
       else
         lds_dma16<0>(from, l.chunk[x], to);
     }
+}
+
+template <int DP>
+__device__ __forceinline__ void dma_k(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+  if (c.dim == DP)
+    dma_k_from<DP, true>(c, l, from, lds);
+  else
+    dma_k_from<DP, false>(c, l, from, lds);
+}
+
+template <int DP>
+__device__ __forceinline__ void dma_v(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
+  if (c.dim == DP)
+    dma_v_from<DP, true>(c, l, from, lds);
+  else
+    dma_v_from<DP, false>(c, l, from, lds);
 }
 
 // The first of 16 tokens from key j on in `page` (one that is not there: page 0,
@@ -822,14 +838,13 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
 }
 
 // ----------------------------------------------------------------------------
-// Chunks of tokens: four waves of 16 NQ query rows each over the same key tiles,
+// Chunks of tokens: NW waves of 16 NQ query rows each over the same key tiles,
 // two buffers of K and V in LDS, the next tile's transfers under the present
 // tile's products.
 // ----------------------------------------------------------------------------
-template <typename T, int DP, int NQ, int TK, bool FORM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionShape::chunk_waves(DP, sizeof(T) == 4)))) void attention_chunk_kernel(
-    AttentionArgs a) {
-  constexpr int QB = 64 * NQ, NA = TK / 16, kTile = TK * DP * 2;
+template <typename T, int DP, int NQ, int NW, int TK, bool FORM>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void attention_chunk_kernel(AttentionArgs a) {
+  constexpr int QB = 16 * NW * NQ, NA = TK / 16, kTile = TK * DP * 2;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // K, V of two tiles
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
@@ -849,7 +864,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
   int x = line.start(wg);
   const int end = line.end(wg);
   if (c.dim != DP) {
-    for (int i = tid; i < 4 * kTile / 16; i += 256)
+    for (int i = tid; i < 4 * kTile / 16; i += 64 * NW)
       reinterpret_cast<u4_t*>(lds)[i] = u4_t{0, 0, 0, 0};
     __syncthreads();
   }
@@ -893,8 +908,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
       const uint32_t at = lds_addr(lds) + buffer * 2 * kTile;
       constexpr int kSteps = 2 * NA;  // K and V of 16 tokens each, dealt to the waves
 #pragma unroll
-      for (int s = 0; s < kSteps / 4; ++s) {
-        const int step = s * 4 + wave, b = step % NA;
+      for (int s = 0; s < (kSteps + NW - 1) / NW; ++s) {
+        const int step = s * NW + wave, b = step % NA;
+        if (step >= kSteps)
+          break;
         int pg = page[0];
 #pragma unroll
         for (int y = 1; y < NA; ++y)
@@ -920,13 +937,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
         uint8_t* const k = lds + (t & 1) * 2 * kTile;
         const bool most = active && key < hi_most && key + TK > lo_least;
         if (key + TK > unit_hi || key < unit_lo || here != (1u << NA) - 1) {
-          if (__syncthreads_or(odd_values<256, kTile>(k + kTile, tid))) {
+          if (__syncthreads_or(odd_values<64 * NW, kTile>(k + kTile, tid))) {
             if (most)
 #pragma unroll
               for (int h = 0; h < NA / 2; ++h)
                 mark_values<T, DP, NQ>(a, k + kTile + h * 32 * DP * 2, rows, key + 32 * h, here >> (2 * h), sums);
             __syncthreads();
-            clear_values<256, kTile>(k + kTile, tid);
+            clear_values<64 * NW, kTile>(k + kTile, tid);
             __syncthreads();
           }
         }
@@ -973,7 +990,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AttentionSh
       }
     }
     if (!done)
-      join_unit<T, DP, QB, 4, 8, 2>(a, line, p, start, wave);
+      join_unit<T, DP, QB, NW, 8, 2>(a, line, p, start, wave);
     x += n;
     leading = false;
   }
@@ -1163,9 +1180,10 @@ hipError_t launch_t(hipStream_t s, const AttentionArgs& a) {
       e = hipErrorInvalidValue;
     return e;
   }
-  constexpr int NQ = AttentionShape::chunk_tiles(DP, sizeof(T) == 4), TK = AttentionShape::chunk_keys(DP);
-  return a.softcap > 0.0f || a.slopes ? dispatch(attention_chunk_kernel<T, DP, NQ, TK, true>, dim3(a.stretches), dim3(256), s, a)
-                                      : dispatch(attention_chunk_kernel<T, DP, NQ, TK, false>, dim3(a.stretches), dim3(256), s, a);
+  constexpr bool kF = sizeof(T) == 4;
+  constexpr int NQ = AttentionShape::chunk_tiles(DP, kF), NW = AttentionShape::chunk_waves(DP, kF), TK = AttentionShape::chunk_keys(DP, kF);
+  return a.softcap > 0.0f || a.slopes ? dispatch(attention_chunk_kernel<T, DP, NQ, NW, TK, true>, dim3(a.stretches), dim3(64 * NW), s, a)
+                                      : dispatch(attention_chunk_kernel<T, DP, NQ, NW, TK, false>, dim3(a.stretches), dim3(64 * NW), s, a);
 }
 
 template <typename T>
@@ -1197,8 +1215,9 @@ int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats) {
   const int rows = most * a.group;
   const int dp = AttentionShape::padded(c.dim);
   a.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && dp <= 128 ? 3 : 0;
-  const int qb = a.row_tiles ? 16 * a.row_tiles : 64 * AttentionShape::chunk_tiles(dp, dtype == kF32);
-  const int tk = a.row_tiles ? 32 : AttentionShape::chunk_keys(dp);
+  const bool f32 = dtype == kF32;
+  const int qb = a.row_tiles ? 16 * a.row_tiles : 16 * AttentionShape::chunk_waves(dp, f32) * AttentionShape::chunk_tiles(dp, f32);
+  const int tk = a.row_tiles ? 32 : AttentionShape::chunk_keys(dp, f32);
   a.units = 0;
   for (int s = 0; s < c.nq; ++s) {
     a.unit[s] = a.units;
@@ -1206,7 +1225,7 @@ int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats) {
   }
   // No more workgroups than tiles: as many as a table holds, for every unit.
   const int64_t tiles = (int64_t)a.units * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1);
-  const int wgs = a.row_tiles ? cus : AttentionShape::chunk_waves(dp, dtype == kF32) * cus;
+  const int wgs = a.row_tiles ? cus : 8 / AttentionShape::chunk_waves(dp, f32) * cus;
   a.stretches = tiles * c.heads < wgs ? (int)(tiles * c.heads) : wgs;
   const auto inverse = [](int y) { return y == 1 ? ~0u : (uint32_t)((1ull << 32) / (uint32_t)y); };
   a.group_inverse = inverse(a.group);

@@ -631,10 +631,10 @@ struct AttentionArgs {
 // a wave, keys of a tile.
 struct AttentionShape {
   static constexpr int padded(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
-  static constexpr int chunk_tiles(int dp, bool f32) { return f32 && dp == 256 ? 1 : 2; }
-  static constexpr int chunk_waves(int dp, bool f32) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
+  static constexpr int chunk_tiles(int dp, bool f32) { return dp > (f32 ? 128 : 192) ? 1 : 2; }
+  static constexpr int chunk_waves(int dp, bool f32) { return dp > (f32 ? 128 : 192) ? 8 : 4; }
+  static constexpr int chunk_keys(int dp, bool f32) { return dp > (f32 ? 64 : 128) && chunk_waves(dp, f32) == 4 ? 32 : 64; }
   static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
-  static constexpr int chunk_keys(int dp) { return dp > 128 ? 32 : 64; }
 };
 // Sets the plan and the floats of `part`; the cache heads that a launch may take.
 int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats);
