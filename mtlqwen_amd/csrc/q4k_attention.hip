@@ -211,7 +211,7 @@ __device__ __forceinline__ Line make_line(const AttentionArgs& a, const Sequence
 // The unit that holds place x of the line, and the place of its first tile (wave-uniform).
 struct Place {
   Unit unit;
-  int head, at;
+  int head, at, index;
 };
 
 template <int QB, int TK>
@@ -220,10 +220,11 @@ __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences&
   p.head = Line::quotient(x, line.per_head);
   const int y = x - p.head * line.per_head;
   Units here = near;
-  int before = 0;
-  for (int u0 = 64; y >= before + lane_value(here.upto, 63); u0 += 64) {  // ends: y < per_head
+  int before = 0, start = 0;
+  while (y >= before + lane_value(here.upto, 63)) {  // ends: y < per_head
     before += lane_value(here.upto, 63);
-    here = units_from<QB, TK>(a, q, u0);
+    start += 64;
+    here = units_from<QB, TK>(a, q, start);
   }
   const int lane = __ffsll((unsigned long long)__ballot(here.upto > y - before)) - 1;
   p.unit.seq = lane_value(here.unit.seq, lane);
@@ -233,6 +234,24 @@ __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences&
   p.unit.hi = lane_value(here.unit.hi, lane);
   p.unit.tiles = lane_value(here.unit.tiles, lane);
   p.at = p.head * line.per_head + before + lane_value(here.upto, lane) - p.unit.tiles;
+  p.index = start + lane;
+  return p;
+}
+
+// The unit behind p's on the line.
+template <int QB, int TK>
+__device__ __forceinline__ Place behind(const AttentionArgs& a, const Sequences& q, Place p) {
+  p.at += p.unit.tiles;
+  const bool last = p.index + 1 == a.units;
+  p.index = last ? 0 : p.index + 1;
+  p.head += last ? 1 : 0;
+  const Unit u = unit_of<QB, TK>(a, q, p.index);
+  p.unit.seq = __builtin_amdgcn_readfirstlane(u.seq);
+  p.unit.row = __builtin_amdgcn_readfirstlane(u.row);
+  p.unit.row_end = __builtin_amdgcn_readfirstlane(u.row_end);
+  p.unit.lo = __builtin_amdgcn_readfirstlane(u.lo);
+  p.unit.hi = __builtin_amdgcn_readfirstlane(u.hi);
+  p.unit.tiles = __builtin_amdgcn_readfirstlane(u.tiles);
   return p;
 }
 
@@ -633,70 +652,68 @@ struct Pages {
     base = -64;
     mine = -1;
   }
-  // The page of entry e (wave-uniform), -1 if it is not there.
-  __device__ __forceinline__ int page(const AttentionArgs& a, int e) {
-    if (e < base || e >= base + 64) {
+  // Entries e .. e + 7 are at hand.
+  __device__ __forceinline__ void reach(const AttentionArgs& a, int e) {
+    if (e < base || e + 7 >= base + 64) {
       base = e;
       const int at = e + (int)(threadIdx.x & 63);
       const int p = at < width ? table[at] : -1;
       mine = (uint32_t)p < a.cache.pages ? p : -1;
     }
-    return lane_value(mine, e - base);
+  }
+  // The page of entry e (wave-uniform), -1 if it is not there.
+  __device__ __forceinline__ int page(int e) const { return lane_value(mine, e - base); }
+
+  // Bytes from a head's first page to key j in `page` (one that is not there: page 0,
+  // whose tokens nothing sees).
+  static __device__ __forceinline__ int64_t bytes(const CacheArgs& c, int page, int j) {
+    return (int64_t)(page < 0 ? 0 : page) * (c.page_stride * 2) + (int64_t)(j & ((1 << c.page_log) - 1)) * (c.token_stride * 2);
   }
 };
 
 // Where this lane's 16 bytes of each 1 KB transfer come from, relative to the
-// first of 16 tokens.  K: key i, d = 8 g + 0..7 of a fragment.  V: transfer x holds
-// rows kRows x on, whose swizzle differs from the first one's by bits of x alone
-// (heads of 96 and 192, whose rows no transfer ends with: an offset each).  Heads
-// shorter than DP: chunks past them are not loaded (their LDS is zero).
+// first of 16 tokens.  K: key i, d = 8 g + 0..7 of a fragment.  V: chunk 64 x +
+// lane of the rows.  Heads shorter than DP: chunks past them are not loaded (their
+// LDS is zero).
 template <int DP>
 struct Lanes {
-  static constexpr bool kEven = 512 % DP == 0;
-  static constexpr int kRows = 512 / DP, kVs = kEven ? 1 : DP / 32;
-  uint32_t k, row, chunk[kVs];
+  uint32_t k, v[DP / 32];
 
   __device__ __forceinline__ void set(const CacheArgs& c) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     k = (uint32_t)(i * (int)c.token_stride) * 2 + g * 16;
-    row = (uint32_t)((lane / (DP / 8)) * (int)c.token_stride) * 2;
 #pragma unroll
-    for (int x = 0; x < kVs; ++x) {
-      const int n = x * 64 + lane, r = n / (DP / 8);
-      chunk[x] = ((n - r * (DP / 8)) ^ v_swizzle<DP>(r)) * 16 + (kEven ? 0u : (uint32_t)(r * (int)c.token_stride) * 2);
+    for (int x = 0; x < DP / 32; ++x) {
+      const int n = x * 64 + lane, row = n / (DP / 8), chunk = (n - row * (DP / 8)) ^ v_swizzle<DP>(row);
+      v[x] = (uint32_t)(row * (int)c.token_stride) * 2 + chunk * 16;
     }
   }
-  // Bytes of the first chunk past the head that transfer x would load, or more.
-  __device__ __forceinline__ bool in_head(const CacheArgs& c, int x) const {
-    const int lane = threadIdx.x & 63, n = x * 64 + lane, r = n / (DP / 8);
-    return 8 * ((n - r * (DP / 8)) ^ v_swizzle<DP>(r)) < c.dim;
+  __device__ __forceinline__ bool k_in_head(const CacheArgs& c, int d) const { return 32 * d + 8 * (int)((threadIdx.x & 63) >> 4) < c.dim; }
+  __device__ __forceinline__ bool v_in_head(const CacheArgs& c, int x) const {
+    const int n = x * 64 + (int)(threadIdx.x & 63), row = n / (DP / 8);
+    return 8 * ((n - row * (DP / 8)) ^ v_swizzle<DP>(row)) < c.dim;
   }
 };
 
 template <int DP, bool WHOLE, int D = 0>
 __device__ __forceinline__ void dma_k_from(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
   if constexpr (D < DP / 32) {
-    // The instruction's offset moves both addresses.
-    if (WHOLE || 32 * D + 8 * (int)((threadIdx.x & 63) >> 4) < c.dim)
-      lds_dma16<64 * D>(from, l.k, __builtin_amdgcn_readfirstlane(lds + (1024 - 64) * D));
+    if (WHOLE || l.k_in_head(c, D))
+      lds_dma16_at<64 * D, (1024 - 64) * D>(from, l.k, lds);  // the instruction's offset moves both addresses
     dma_k_from<DP, WHOLE, D + 1>(c, l, from, lds);
   }
 }
 
-template <int DP, bool WHOLE>
+template <int DP, bool WHOLE, int X = 0>
 __device__ __forceinline__ void dma_v_from(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
-  using L = Lanes<DP>;
-#pragma unroll
-  for (int x = 0; x < DP / 32; ++x)
-    if (WHOLE || l.in_head(c, x)) {
-      const uint32_t to = __builtin_amdgcn_readfirstlane(lds + 1024 * x);
-      if constexpr (L::kEven)
-        lds_dma16<0>(from + (int64_t)(x * L::kRows) * c.token_stride * 2, (l.chunk[0] ^ (v_swizzle<DP>(x * L::kRows) * 16)) + l.row, to);
-      else
-        lds_dma16<0>(from, l.chunk[x], to);
-    }
+  if constexpr (X < DP / 32) {
+    if (WHOLE || l.v_in_head(c, X))
+      lds_dma16_at<0, 1024 * X>(from, l.v[X], lds);
+    dma_v_from<DP, WHOLE, X + 1>(c, l, from, lds);
+  }
 }
 
+// K and V of 16 tokens, `lds` and `from` wave-uniform.
 template <int DP>
 __device__ __forceinline__ void dma_k(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
   if (c.dim == DP)
@@ -711,13 +728,6 @@ __device__ __forceinline__ void dma_v(const CacheArgs& c, const Lanes<DP>& l, co
     dma_v_from<DP, true>(c, l, from, lds);
   else
     dma_v_from<DP, false>(c, l, from, lds);
-}
-
-// The first of 16 tokens from key j on in `page` (one that is not there: page 0,
-// whose tokens nothing sees).
-__device__ __forceinline__ const uint8_t* tokens_at(const CacheArgs& c, const void* base, int head, int page, int j) {
-  const int64_t at = (int64_t)(page < 0 ? 0 : page) * c.page_stride + (int64_t)head * c.head_stride + (int64_t)(j & ((1 << c.page_log) - 1)) * c.token_stride;
-  return uniform_ptr(static_cast<const uint8_t*>(base) + 2 * at);
 }
 
 template <int N>
@@ -850,7 +860,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   __shared__ int kept[kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded, units_from<QB, TK>(a, loaded, 0));
+  const Units near = units_from<QB, TK>(a, loaded, 0);
+  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded, near);
   const int stretches = line.stretches();
   if ((int)blockIdx.x >= stretches)
     return;
@@ -870,10 +881,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   }
   Lanes<DP> from;
   from.set(c);
+  Place p = locate<QB, TK>(a, loaded, line, near, x);
   bool leading = true;  // the stretch's first unit
-  while (x < end) {
+  while (true) {
     const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
-    const Place p = locate<QB, TK>(a, seqs, line, units_from<QB, TK>(a, seqs, 0), x);
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
     const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
@@ -896,31 +907,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     Pages pages;
     pages.open(a, seqs, u.seq);
     uint32_t there = 0;
+    // A wave transfers K, V or both of 16 of the tile's tokens.
+    static_assert(NW == NA || NW == 2 * NA, "16 tokens to a wave");
+    const int group = wave % NA;
+    const uint8_t* const k_head = uniform_ptr(static_cast<const uint8_t*>(c.k) + (int64_t)p.head * c.head_stride * 2);
+    const uint8_t* const v_head = uniform_ptr(static_cast<const uint8_t*>(c.v) + (int64_t)p.head * c.head_stride * 2);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + group * (DP / 32) * 1024);
     const auto fetch = [&](int t, int buffer) {
-      const int key = u.lo + t * TK;
-      int page[NA];
-      there = 0;
+      const int key = u.lo + t * TK, mine = key + 16 * group;
+      pages.reach(a, key >> c.page_log);
+      const int page = pages.page(mine >> c.page_log);
+      if (c.page_log >= (TK == 64 ? 6 : 5)) {
+        there = page >= 0 ? (1u << NA) - 1 : 0u;
+      } else {
+        there = 0;
 #pragma unroll
-      for (int b = 0; b < NA; ++b) {
-        page[b] = pages.page(a, (key + 16 * b) >> c.page_log);
-        there |= page[b] >= 0 ? 1u << b : 0u;
+        for (int b = 0; b < NA; ++b)
+          there |= pages.page((key + 16 * b) >> c.page_log) >= 0 ? 1u << b : 0u;
       }
-      const uint32_t at = lds_addr(lds) + buffer * 2 * kTile;
-      constexpr int kSteps = 2 * NA;  // K and V of 16 tokens each, dealt to the waves
-#pragma unroll
-      for (int s = 0; s < (kSteps + NW - 1) / NW; ++s) {
-        const int step = s * NW + wave, b = step % NA;
-        if (step >= kSteps)
-          break;
-        int pg = page[0];
-#pragma unroll
-        for (int y = 1; y < NA; ++y)
-          pg = b == y ? page[y] : pg;
-        if (step < NA)
-          dma_k<DP>(c, from, tokens_at(c, c.k, p.head, pg, key + 16 * b), at + b * (DP / 32) * 1024);
-        else
-          dma_v<DP>(c, from, tokens_at(c, c.v, p.head, pg, key + 16 * b), at + kTile + b * (DP / 32) * 1024);
-      }
+      const int64_t at = Pages::bytes(c, page, mine);
+      const uint32_t here = to + buffer * 2 * kTile;
+      if (NW == NA || wave < NA)
+        dma_k<DP>(c, from, k_head + at, here);
+      if (NW == NA || wave >= NA)
+        dma_v<DP>(c, from, v_head + at, here + kTile);
     };
     if (!none) {
       __syncthreads();  // the buffers' last readers are done
@@ -992,7 +1002,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     if (!done)
       join_unit<T, DP, QB, NW, 8, 2>(a, line, p, start, wave);
     x += n;
+    if (x >= end)
+      return;
     leading = false;
+    p = behind<QB, TK>(a, kept_sequences(kept), p);
   }
 }
 
@@ -1010,36 +1023,27 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   __shared__ float sm[NW][QB], sl[NW][QB];
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  // With one row tile they stay in registers; with more they would not fit beside O.
-  constexpr bool kKeep = NQ == 1;
-  __shared__ int kept[kKeep ? 1 : kSequenceInts];
+  __shared__ int kept[kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Units first_units = units_from<QB, TK>(a, loaded, 0);
-  const Line line = make_line<QB, TK, NW>(a, loaded, first_units);
+  const Units near = units_from<QB, TK>(a, loaded, 0);
+  const Line line = make_line<QB, TK, NW>(a, loaded, near);
   const int wg = (int)blockIdx.x;
   if (wg >= line.stretches())
     return;
-  if constexpr (!kKeep) {
-    if (wave == 0)
-      keep_sequences(loaded, kept);
-    __syncthreads();
-  }
+  if (wave == 0)
+    keep_sequences(loaded, kept);
+  __syncthreads();
   int x = line.start(wg);
   const int end = line.end(wg);
   Lanes<DP> from;
   from.set(c);
   uint8_t* const mine = lds + wave * 2 * kTile;
-  const uint32_t at = lds_addr(mine);
+  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_addr(mine));
   const bool formed = a.softcap > 0.0f || a.slopes;
+  Place p = locate<QB, TK>(a, loaded, line, near, x);
   bool leading = true;
-  while (x < end) {
-    Sequences seqs = loaded;
-    Units near = first_units;
-    if constexpr (!kKeep) {
-      seqs = kept_sequences(kept);
-      near = units_from<QB, TK>(a, seqs, 0);
-    }
-    const Place p = locate<QB, TK>(a, seqs, line, near, x);
+  while (true) {
+    const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
     const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
@@ -1052,29 +1056,33 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
       for (int i = lane; i < 2 * kTile / 16; i += 64)
         reinterpret_cast<u4_t*>(mine)[i] = u4_t{0, 0, 0, 0};
     wait_lds();
-    int pg[2];
+    uint32_t there = 0;
+    int64_t from_page[2] = {0, 0};
+    const uint8_t* const k_head = uniform_ptr(static_cast<const uint8_t*>(c.k) + (int64_t)p.head * c.head_stride * 2);
+    const uint8_t* const v_head = uniform_ptr(static_cast<const uint8_t*>(c.v) + (int64_t)p.head * c.head_stride * 2);
     const auto open = [&](int t) {
       const int key = u.lo + t * TK;
-      pg[0] = pages.page(a, key >> c.page_log);
-      pg[1] = pages.page(a, (key + 16) >> c.page_log);
+      pages.reach(a, key >> c.page_log);
+      const int first_page = pages.page(key >> c.page_log), second_page = pages.page((key + 16) >> c.page_log);
+      from_page[0] = Pages::bytes(c, first_page, key);
+      from_page[1] = Pages::bytes(c, second_page, key + 16);
+      there = (first_page >= 0 ? 1u : 0u) | (second_page >= 0 ? 2u : 0u);
     };
-    const auto fetch_k = [&](int t) {
-      const int key = u.lo + t * TK;
+    const auto fetch_k = [&]() {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        dma_k<DP>(c, from, tokens_at(c, c.k, p.head, pg[b], key + 16 * b), at + b * (DP / 32) * 1024);
+        dma_k<DP>(c, from, k_head + from_page[b], at + b * (DP / 32) * 1024);
     };
-    const auto fetch_v = [&](int t) {
-      const int key = u.lo + t * TK;
+    const auto fetch_v = [&]() {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        dma_v<DP>(c, from, tokens_at(c, c.v, p.head, pg[b], key + 16 * b), at + kTile + b * (DP / 32) * 1024);
+        dma_v<DP>(c, from, v_head + from_page[b], at + kTile + b * (DP / 32) * 1024);
     };
     const bool busy = u.hi > u.lo && wave < n;
     if (busy) {
       open(t0 + wave);
-      fetch_k(t0 + wave);
-      fetch_v(t0 + wave);
+      fetch_k();
+      fetch_v();
     }
     Rows<T, DP, NQ> rows;  // on their way with the first keys
     rows.load(a, seqs, u, p.head, u.row);
@@ -1083,24 +1091,24 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
     if (busy) {
       for (int t = wave; t < n; t += NW) {
         const int key = u.lo + (t0 + t) * TK;
-        const uint32_t there = (pg[0] >= 0 ? 1u : 0u) | (pg[1] >= 0 ? 2u : 0u);
-        const bool whole = key + TK <= hi_least && key >= lo_most && there == 3u, more = t + NW < n;
+        const uint32_t here = there;
+        const bool whole = key + TK <= hi_least && key >= lo_most && here == 3u, more = t + NW < n;
         wait_loads<kLoads>();  // K is here, V may be on its way
         f4_t s[2][NQ];
         scores<T, DP, NQ, 2>(mine, rows, s);
         wait_lds();
         if (more) {
           open(t0 + t + NW);
-          fetch_k(t0 + t + NW);
+          fetch_k();
         }
-        finish_scores<T, DP, NQ, 2>(a, rows, key, whole, there, formed, s);
+        finish_scores<T, DP, NQ, 2>(a, rows, key, whole, here, formed, s);
         sums.weigh(s, [&](int y) { return formed ? 1.0f : rows.factor(y); });
         if (more)
           wait_loads<kLoads>();
         else
           wait_loads<0>();
         if (!whole && __any(odd_values<64, kTile>(mine + kTile, lane))) {
-          mark_values<T, DP, NQ>(a, mine + kTile, rows, key, there, sums);
+          mark_values<T, DP, NQ>(a, mine + kTile, rows, key, here, sums);
           wait_lds();
           clear_values<64, kTile>(mine + kTile, lane);
           wait_lds();
@@ -1108,7 +1116,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         add_values<T, DP, NQ>(mine + kTile, s[0], s[1], sums);
         wait_lds();
         if (more)
-          fetch_v(t0 + t + NW);
+          fetch_v();
       }
     }
     sums.settle();
@@ -1160,9 +1168,12 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
     }
     if (!done)
       join_unit<T, DP, QB, NW, 1, 8>(a, line, p, start, wave);
-    __syncthreads();  // before the buffers and statistics are used again
     x += n;
+    if (x >= end)
+      return;
     leading = false;
+    p = behind<QB, TK>(a, kept_sequences(kept), p);
+    __syncthreads();  // before the buffers and statistics are used again
   }
 }
 

@@ -256,6 +256,12 @@ __device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint3
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET) : "m0");
 }
 
+// The same with a constant added to the LDS address.
+template <int OFFSET, int LDS>
+__device__ __forceinline__ void lds_dma16_at(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %4\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET), "n"(LDS) : "m0", "scc");
+}
+
 // Stores and loads that bypass every cache level (sc0 sc1: system
 // coherence), for data exchanged between workgroups on different XCDs.  The
 // loads return through vmcnt like the others: wait before use.
