@@ -349,8 +349,9 @@ __device__ __forceinline__ int v_swizzle(int row) {
   return DP % 128 == 0 ? 2 * (row & 7) : DP % 64 == 0 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1);
 }
 
-template <typename T, int DP, int NQ, int NA>
-__device__ __forceinline__ void scores(const uint8_t* k, const Rows<T, DP, NQ>& r, f4_t (&s)[NA][NQ]) {
+// `between`: called with every d / 32 behind the products of 32 d.
+template <typename T, int DP, int NQ, int NA, typename F>
+__device__ __forceinline__ void scores(const uint8_t* k, const Rows<T, DP, NQ>& r, f4_t (&s)[NA][NQ], const F& between) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int a = 0; a < NA; ++a)
@@ -380,6 +381,7 @@ __device__ __forceinline__ void scores(const uint8_t* k, const Rows<T, DP, NQ>& 
           s[a][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d & 1][a], r.ql[n][d], s[a][n], 0, 0, 0);
       }
     __builtin_amdgcn_sched_barrier(0);
+    between(d);
   }
 }
 
@@ -695,12 +697,18 @@ struct Lanes {
   }
 };
 
-template <int DP, bool WHOLE, int D = 0>
+// Transfer X of K or V of 16 tokens.
+template <int X>
+__device__ __forceinline__ void dma_k_one(uint32_t lane, const uint8_t* from, uint32_t lds) {
+  lds_dma16_at<64 * X, (1024 - 64) * X>(from, lane, lds);  // the instruction's offset moves both addresses
+}
+
+template <int DP, bool WHOLE, int X = 0>
 __device__ __forceinline__ void dma_k_from(const CacheArgs& c, const Lanes<DP>& l, const uint8_t* from, uint32_t lds) {
-  if constexpr (D < DP / 32) {
-    if (WHOLE || l.k_in_head(c, D))
-      lds_dma16_at<64 * D, (1024 - 64) * D>(from, l.k, lds);  // the instruction's offset moves both addresses
-    dma_k_from<DP, WHOLE, D + 1>(c, l, from, lds);
+  if constexpr (X < DP / 32) {
+    if (WHOLE || l.k_in_head(c, X))
+      dma_k_one<X>(l.k, from, lds);
+    dma_k_from<DP, WHOLE, X + 1>(c, l, from, lds);
   }
 }
 
@@ -710,6 +718,21 @@ __device__ __forceinline__ void dma_v_from(const CacheArgs& c, const Lanes<DP>& 
     if (WHOLE || l.v_in_head(c, X))
       lds_dma16_at<0, 1024 * X>(from, l.v[X], lds);
     dma_v_from<DP, WHOLE, X + 1>(c, l, from, lds);
+  }
+}
+
+// The transfer x of an unrolled loop.
+template <int DP, int X = 0>
+__device__ __forceinline__ void dma_at(int x, bool k, bool v, const Lanes<DP>& l, const uint8_t* from_k, const uint8_t* from_v, uint32_t lds, uint32_t lds_v) {
+  if constexpr (X < DP / 32) {
+    if (x == X) {
+      if (k)
+        dma_k_one<X>(l.k, from_k, lds);
+      if (v)
+        lds_dma16_at<0, 1024 * X>(from_v, l.v[X], lds_v);
+      return;
+    }
+    dma_at<DP, X + 1>(x, k, v, l, from_k, from_v, lds, lds_v);
   }
 }
 
@@ -913,7 +936,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const uint8_t* const k_head = uniform_ptr(static_cast<const uint8_t*>(c.k) + (int64_t)p.head * c.head_stride * 2);
     const uint8_t* const v_head = uniform_ptr(static_cast<const uint8_t*>(c.v) + (int64_t)p.head * c.head_stride * 2);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(lds) + group * (DP / 32) * 1024);
-    const auto fetch = [&](int t, int buffer) {
+    constexpr bool kBoth = NW == NA;
+    const bool k_mine = kBoth || wave < NA, v_mine = kBoth || wave >= NA;
+    const uint8_t *k_next = nullptr, *v_next = nullptr;  // where the next tile's transfers come from and go to
+    uint32_t to_next = 0;
+    const auto find = [&](int t, int buffer) {
       const int key = u.lo + t * TK, mine = key + 16 * group;
       pages.reach(a, key >> c.page_log);
       const int page = pages.page(mine >> c.page_log);
@@ -926,23 +953,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           there |= pages.page((key + 16 * b) >> c.page_log) >= 0 ? 1u << b : 0u;
       }
       const int64_t at = Pages::bytes(c, page, mine);
-      const uint32_t here = to + buffer * 2 * kTile;
-      if (NW == NA || wave < NA)
-        dma_k<DP>(c, from, k_head + at, here);
-      if (NW == NA || wave >= NA)
-        dma_v<DP>(c, from, v_head + at, here + kTile);
+      k_next = k_head + at;
+      v_next = v_head + at;
+      to_next = to + buffer * 2 * kTile;
+    };
+    const auto fetch = [&]() {
+      if (k_mine)
+        dma_k<DP>(c, from, k_next, to_next);
+      if (v_mine)
+        dma_v<DP>(c, from, v_next, to_next + kTile);
     };
     if (!none) {
       __syncthreads();  // the buffers' last readers are done
       __builtin_amdgcn_sched_barrier(0);
-      fetch(t0, 0);
+      find(t0, 0);
+      fetch();
       for (int t = 0; t < n; ++t) {
         const uint32_t here = there;
         wait_loads<0>();
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
-        if (t + 1 < n)
-          fetch(t0 + t + 1, (t + 1) & 1);
+        bool asks = t + 1 < n;
+        if (asks)
+          find(t0 + t + 1, (t + 1) & 1);
         const int key = u.lo + (t0 + t) * TK;
         uint8_t* const k = lds + (t & 1) * 2 * kTile;
         const bool most = active && key < hi_most && key + TK > lo_least;
@@ -957,11 +990,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             __syncthreads();
           }
         }
+        // The next tile's transfers go between the first products: all at once they
+        // would wait for the way to the caches before the products begin (1130 to 2510
+        // clocks of a tile of 5700).
+        if (asks && (!most || c.dim != DP)) {
+          fetch();
+          asks = false;
+        }
         if (!most)
           continue;
         const bool whole = key + TK <= hi_least && key >= lo_most && here == (1u << NA) - 1;
         f4_t s[NA][NQ];
-        scores<T, DP, NQ, NA>(k, rows, s);
+        scores<T, DP, NQ, NA>(k, rows, s, [&](int d) {
+          if (asks)
+            dma_at<DP>(d, k_mine, v_mine, from, k_next, v_next, to_next, to_next + kTile);
+        });
         finish_scores<T, DP, NQ, NA>(a, rows, key, whole, here, FORM, s);
         sums.weigh(s, [&](int y) { return FORM ? 1.0f : rows.factor(y); });
 #pragma unroll
@@ -1095,7 +1138,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         const bool whole = key + TK <= hi_least && key >= lo_most && here == 3u, more = t + NW < n;
         wait_loads<kLoads>();  // K is here, V may be on its way
         f4_t s[2][NQ];
-        scores<T, DP, NQ, 2>(mine, rows, s);
+        scores<T, DP, NQ, 2>(mine, rows, s, [](int) {});
         wait_lds();
         if (more) {
           open(t0 + t + NW);
