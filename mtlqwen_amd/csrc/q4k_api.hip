@@ -2118,8 +2118,9 @@ int check_pool(const q4k_pool* p, const int32_t* tables, const int32_t* lengths,
       (uint64_t)p->blocks * p->page_size * p->token_bytes > (1ull << 34))
     return fail(Q4K_ESHAPE, "pages must be of 1 or more blocks of up to 2^30 bytes, 2^34 in all, token_bytes a multiple of 16 (got %u blocks of %u x %u)",
                 p->blocks, p->page_size, p->token_bytes);
-  if (slots > Q4K_MAX_SLOTS || (uint64_t)width * p->page_size > (1u << 30))
-    return fail(Q4K_ESHAPE, "up to %u slots of up to 2^30 tokens (got %u of %u pages of %u)", Q4K_MAX_SLOTS, slots, width, p->page_size);
+  if (slots > Q4K_MAX_SLOTS || (uint64_t)width * p->page_size > (1u << 30) || (uint64_t)slots * width > 0x7fffffffu)
+    return fail(Q4K_ESHAPE, "up to %u slots of up to 2^30 tokens, 2^31 - 1 entries in all (got %u of %u pages of %u)", Q4K_MAX_SLOTS, slots, width,
+                p->page_size);
   if (!p->data || (slots && (!lengths || (width && (!tables || !new_tables)))))
     return fail(Q4K_EINVAL, "data, tables, lengths and new_tables must be non-NULL");
   if ((uintptr_t)p->data % 16 != 0)

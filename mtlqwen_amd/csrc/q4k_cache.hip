@@ -50,11 +50,14 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs c, CacheRows
 // ----------------------------------------------------------------------------
 // Tables.  One workgroup of 1024 threads per call: which pages are held is a
 // bit per page in LDS (up to 2^18 pages, 32 KB), so nothing about the pool is
-// kept between calls, and the lowest free pages are found by counting bits.
+// kept between calls, and pages are found by counting bits: `rank` holds, per word,
+// the pages counted before it.  Bound by latency: what each step reads it reads with
+// all threads at once, over slots and entries alike.
 // ----------------------------------------------------------------------------
 constexpr int kTableThreads = 1024;
+constexpr int kWords = (int)kMaxPages / 32;
 
-// Sum over the threads before this one, and over all of them.  `sums` holds 17
+// Sum over the threads before this one, and over all of them.  `sums` holds 16
 // words; free for the next call behind the caller's next barrier.
 __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* sums, uint32_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -67,9 +70,11 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* sums, uint
     sums[wave] = s;
   __syncthreads();
   uint32_t before = 0, all = 0;
+#pragma unroll
   for (int w = 0; w < kTableThreads / 64; ++w) {
-    before += w < wave ? sums[w] : 0;
-    all += sums[w];
+    const uint32_t x = sums[w];
+    before += w < wave ? x : 0;
+    all += x;
   }
   __syncthreads();
   *total = all;
@@ -80,10 +85,32 @@ __device__ __forceinline__ bool bit_of(const uint32_t* bits, uint32_t p) {
   return (bits[p >> 5] >> (p & 31)) & 1;
 }
 
-// Bits of the words past the last page are set: no page there is free.
-__device__ __forceinline__ void clear_bits(uint32_t* bits, uint32_t pages) {
-  for (uint32_t w = threadIdx.x; w < kMaxPages / 32; w += kTableThreads)
-    bits[w] = 32 * w >= pages ? ~0u : pages - 32 * w < 32 ? ~0u << (pages - 32 * w) : 0u;
+__device__ __forceinline__ void set_bit(uint32_t* bits, uint32_t p) {
+  atomicOr(&bits[p >> 5], 1u << (p & 31));
+}
+
+__device__ __forceinline__ int words_of(const TableArgs& a) {
+  return (int)((a.pages + 31) >> 5);
+}
+
+// rank[w] = set bits in the words before w; their number.  Ends with a barrier.
+__device__ __forceinline__ uint32_t count_bits(const uint32_t* bits, uint32_t* rank, int words, uint32_t* sums) {
+  const int each = (words + kTableThreads - 1) / kTableThreads, from = threadIdx.x * each;
+  uint32_t n = 0, all;
+  for (int w = from; w < from + each && w < words; ++w)
+    n += __popc(bits[w]);
+  uint32_t before = scan_before(n, sums, &all);
+  for (int w = from; w < from + each && w < words; ++w) {
+    rank[w] = before;
+    before += __popc(bits[w]);
+  }
+  __syncthreads();
+  return all;
+}
+
+// Set bits before page p.
+__device__ __forceinline__ uint32_t rank_of(const uint32_t* bits, const uint32_t* rank, uint32_t p) {
+  return rank[p >> 5] + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1));
 }
 
 // A slot's tokens: not negative, no more than its table holds.
@@ -92,101 +119,112 @@ __device__ __forceinline__ int32_t tokens_of(int32_t length, const TableArgs& a)
   return length < 0 ? 0 : length > most ? (int32_t)most : length;
 }
 
+// Calls f(slot, entry) for all entries of all slots, the threads side by side.
+template <typename F>
+__device__ __forceinline__ void each_entry(const TableArgs& a, const F& f) {
+  const uint32_t all = (uint32_t)a.slots * (uint32_t)a.width;  // below 2^31: checked by the caller
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < all; i += kTableThreads) {
+    const uint32_t s = i / (uint32_t)a.width;
+    f((int)s, (int)(i - s * (uint32_t)a.width));
+  }
+}
+
 // Slot s takes the first lengths[p] tokens of its parent p.  Pages full of tokens are
 // shared.  A page that is not full will be written on, so it can stay with one
 // slot only: with the lowest of those that hold it, unless another holds it as a
 // full page; the others get a page of their own and a copy (page_fork_kernel).
 // Then, slot by slot, the lowest free pages for counts[s] more tokens.
 __global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a) {
-  __shared__ uint32_t bits[kMaxPages / 32], sums[17], before[kMaxSlots + 1];
-  __shared__ int32_t parent[kMaxSlots], last[kMaxSlots], full[kMaxSlots], first[kMaxSlots], kept[kMaxSlots];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  clear_bits(bits, a.pages);
-  int32_t length = 0;
+  __shared__ uint32_t bits[kWords], rank[kWords], sums[16], before[kMaxSlots + 1], beyond;
+  __shared__ __attribute__((aligned(16))) int32_t last[kMaxSlots];
+  __shared__ int32_t parent[kMaxSlots], full[kMaxSlots], first[kMaxSlots], kept[kMaxSlots];
+  const int tid = threadIdx.x, words = words_of(a);
+  for (int w = tid; w < words; w += kTableThreads)
+    bits[w] = 0;
+  int32_t length = 0, tail = -1;
+  bool part = false;
   if (tid < a.slots) {
     const int32_t p = a.parents ? a.parents[tid] : tid;
     const bool live = (uint32_t)p < (uint32_t)a.slots;
     length = live ? tokens_of(a.lengths[p], a) : 0;
+    part = length & ((1 << a.page_log) - 1);
     parent[tid] = live ? p : 0;
     full[tid] = length >> a.page_log;
+    a.new_lengths[tid] = length;
+    if (part)
+      tail = a.tables[(int64_t)p * a.width + full[tid]];
   }
+  last[tid] = (uint32_t)tail < a.pages ? tail : -1;
+  if (tid == 0)
+    beyond = 0;
   __syncthreads();
-  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
-    const int32_t* t = a.tables + (int64_t)parent[s] * a.width;
-    for (int e = lane; e < full[s]; e += 64) {
-      const uint32_t p = (uint32_t)t[e];
+  each_entry(a, [&](int s, int e) {
+    if (e < full[s]) {
+      const uint32_t p = (uint32_t)a.tables[(int64_t)parent[s] * a.width + e];
       if (p < a.pages)
-        atomicOr(&bits[p >> 5], 1u << (p & 31));
+        set_bit(bits, p);
     }
-  }
-  const bool part = length & ((1 << a.page_log) - 1);
-  if (tid < a.slots) {
-    const int32_t p = part ? a.tables[(int64_t)parent[tid] * a.width + full[tid]] : -1;
-    last[tid] = (uint32_t)p < a.pages ? p : -1;
-  }
-  __syncthreads();
-  bool keep = false;
-  if (tid < a.slots && last[tid] >= 0) {
-    keep = !bit_of(bits, (uint32_t)last[tid]);
-    for (int s = 0; s < tid && keep; ++s)
-      keep = last[s] != last[tid];
+  });
+  bool keep = last[tid] >= 0;
+  const int4* lasts = reinterpret_cast<const int4*>(last);
+#pragma unroll 4
+  for (int s = 0; s < (a.slots + 3) / 4; ++s) {  // the slots before this one
+    const int4 o = lasts[s];
+    keep = keep && !((4 * s < tid && o.x == last[tid]) | (4 * s + 1 < tid && o.y == last[tid]) | (4 * s + 2 < tid && o.z == last[tid]) |
+                     (4 * s + 3 < tid && o.w == last[tid]));
   }
   __syncthreads();
-  uint32_t wants = 0, beyond = 0;
+  keep = keep && !bit_of(bits, (uint32_t)last[tid]);
+  __syncthreads();
+  uint32_t wants = 0;
   if (tid < a.slots) {
     if (keep)
-      atomicOr(&bits[last[tid] >> 5], 1u << (last[tid] & 31));
+      set_bit(bits, (uint32_t)last[tid]);
     // A page that the parent's table lacks stays lacking.
     const int32_t from = full[tid] + (part && (keep || last[tid] < 0));
     const int32_t count = a.counts ? a.counts[tid] : 0;
     const int64_t need = ((int64_t)length + (count > 0 ? count : 0) + (1 << a.page_log) - 1) >> a.page_log;
     const int64_t most = need < a.width ? need : a.width;
     wants = most > from ? (uint32_t)(most - from) : 0;
-    beyond = (uint32_t)(need - most);
+    if (need > most)
+      atomicAdd(&beyond, (uint32_t)(need - most));
     first[tid] = from;
     kept[tid] = keep;
-    a.new_lengths[tid] = length;
   }
-  uint32_t asked, lacking, there;
+  uint32_t asked;
   const uint32_t mine = scan_before(wants, sums, &asked);
   if (tid < a.slots)
     before[tid] = mine;
   if (tid == 0)
     before[a.slots] = asked;
-  (void)scan_before(beyond, sums, &lacking);
-  constexpr int kWords = kMaxPages / 32 / kTableThreads;
-  uint32_t n = 0;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w)
-    n += 32 - __popc(bits[tid * kWords + w]);
-  uint32_t rank = scan_before(n, sums, &there);
+  const uint32_t there = a.pages - count_bits(bits, rank, words, sums);
   if (tid == 0 && a.missing)
-    *a.missing = (int32_t)(lacking + (asked > there ? asked - there : 0));
+    *a.missing = (int32_t)(beyond + (asked > there ? asked - there : 0));
   // Request r of slot s (before[s] <= r < before[s + 1]) takes the r-th free page.
-  for (int w = 0; w < kWords && rank < asked; ++w) {
-    uint32_t open = ~bits[tid * kWords + w];
-    for (; open && rank < asked; open &= open - 1, ++rank) {
-      int lo = 0, hi = a.slots;  // before[lo] <= rank < before[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        (before[mid] <= rank ? lo : hi) = mid;
-      }
-      a.new_tables[(int64_t)lo * a.width + first[lo] + (rank - before[lo])] = 32 * (tid * kWords + w) + __ffs(open) - 1;
-    }
-  }
   const uint32_t given = asked < there ? asked : there;
-  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
-    const int32_t* t = a.tables + (int64_t)parent[s] * a.width;
-    int32_t* y = a.new_tables + (int64_t)s * a.width;
-    const int64_t to = first[s] + (before[s] >= given ? 0 : (int64_t)(before[s + 1] < given ? before[s + 1] : given) - before[s]);
-    for (int e = lane; e < a.width; e += 64) {
-      if (e >= first[s] && e < to)
-        continue;  // given above
-      const bool old = e < full[s] || (e == full[s] && kept[s]);
-      const int32_t p = old ? t[e] : -1;
-      y[e] = (uint32_t)p < a.pages ? p : -1;
+  for (uint32_t p0 = 0; p0 < a.pages && p0 - rank[p0 >> 5] < given; p0 += kTableThreads) {
+    const uint32_t p = p0 + tid;
+    if (p >= a.pages || bit_of(bits, p))
+      continue;
+    const uint32_t r = p - rank_of(bits, rank, p);
+    if (r >= given)
+      continue;
+    int lo = 0, hi = a.slots;  // before[lo] <= r < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (before[mid] <= r ? lo : hi) = mid;
     }
+    a.new_tables[(int64_t)lo * a.width + first[lo] + (r - before[lo])] = (int32_t)p;
   }
+  each_entry(a, [&](int s, int e) {
+    const bool asks = e >= first[s] && e - first[s] < (int)(before[s + 1] - before[s]);
+    if (asks && before[s] + (uint32_t)(e - first[s]) < given)
+      return;  // given above
+    const bool old = e < full[s] || (e == full[s] && kept[s]);
+    const int32_t p = old ? a.tables[(int64_t)parent[s] * a.width + e] : -1;
+    a.new_tables[(int64_t)s * a.width + e] = (uint32_t)p < a.pages ? p : -1;
+  });
 }
 
 // The pages that cache_assign_kernel gave in place of ones that are shared: what
@@ -234,70 +272,44 @@ __global__ __launch_bounds__(256) void page_fork_kernel(TableArgs a, PoolArgs p)
 // free one before it: no page is read that another is written over.  moves[0]
 // = their number, then the pairs.
 __global__ __launch_bounds__(kTableThreads) void cache_compact_kernel(TableArgs a, int32_t* moves) {
-  __shared__ uint32_t bits[kMaxPages / 32], sums[17], chunk[kTableThreads];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int w = tid; w < (int)(kMaxPages / 32); w += kTableThreads)
+  __shared__ uint32_t bits[kWords], rank[kWords], sums[16];
+  __shared__ int32_t held[kMaxSlots];
+  const int tid = threadIdx.x, words = words_of(a);
+  for (int w = tid; w < words; w += kTableThreads)
     bits[w] = 0;
+  if (tid < a.slots)
+    held[tid] = (int32_t)(((int64_t)tokens_of(a.lengths[tid], a) + (1 << a.page_log) - 1) >> a.page_log);
   __syncthreads();
-  const int round = (1 << a.page_log) - 1;
-  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
-    const int held = (int)(((int64_t)tokens_of(a.lengths[s], a) + round) >> a.page_log);
-    for (int e = lane; e < held; e += 64) {
+  each_entry(a, [&](int s, int e) {
+    if (e < held[s]) {
       const uint32_t p = (uint32_t)a.tables[(int64_t)s * a.width + e];
       if (p < a.pages)
-        atomicOr(&bits[p >> 5], 1u << (p & 31));
+        set_bit(bits, p);
     }
-  }
+  });
   __syncthreads();
-  constexpr int kWords = kMaxPages / 32 / kTableThreads;
-  uint32_t n = 0, used;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w)
-    n += __popc(bits[tid * kWords + w]);
-  const uint32_t mine = scan_before(n, sums, &used);
-  chunk[tid] = mine;
-  __syncthreads();
-  const auto held_before = [&](uint32_t p) {
-    uint32_t r = chunk[p / (32 * kWords)];
-    for (uint32_t w = p / (32 * kWords) * kWords; w < (p >> 5); ++w)
-      r += __popc(bits[w]);
-    return r + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1));
-  };
-  const uint32_t low = used < kMaxPages ? held_before(used) : used;  // pages that stay
+  const uint32_t used = count_bits(bits, rank, words, sums);
+  const uint32_t low = used < a.pages ? rank_of(bits, rank, used) : used;  // pages that stay
   if (tid == 0) {
     moves[0] = (int32_t)(used - low);
     if (a.missing)
       *a.missing = (int32_t)used;
   }
-  uint32_t rank = mine;  // held pages before the present one
-  for (int w = 0; w < kWords; ++w) {
-    const uint32_t word = bits[tid * kWords + w], p0 = 32 * (tid * kWords + w);
-    if (p0 < used)  // holes before page `used`
-      for (uint32_t open = ~word; open; open &= open - 1) {
-        const uint32_t b = (uint32_t)__ffs(open) - 1, p = p0 + b;
-        if (p < used)
-          moves[2 + 2 * (p - rank - __popc(word & ((1u << b) - 1)))] = (int32_t)p;
-      }
-    if (p0 + 31 >= used)  // pages to move
-      for (uint32_t held = word; held; held &= held - 1) {
-        const uint32_t b = (uint32_t)__ffs(held) - 1, p = p0 + b;
-        if (p >= used)
-          moves[1 + 2 * (rank + __popc(word & ((1u << b) - 1)) - low)] = (int32_t)p;
-      }
-    rank += __popc(word);
+  for (uint32_t p = tid; p < a.pages; p += kTableThreads) {
+    const uint32_t r = rank_of(bits, rank, p);
+    const bool is = bit_of(bits, p);
+    if (p < used ? !is : is)
+      moves[p < used ? 2 + 2 * (p - r) : 1 + 2 * (r - low)] = (int32_t)p;
   }
   __threadfence_block();
   __syncthreads();
-  for (int s = wave; s < a.slots; s += kTableThreads / 64) {
-    const int held = (int)(((int64_t)tokens_of(a.lengths[s], a) + round) >> a.page_log);
-    for (int e = lane; e < a.width; e += 64) {
-      const uint32_t p = e < held ? (uint32_t)a.tables[(int64_t)s * a.width + e] : ~0u;
-      int32_t to = p < a.pages ? (int32_t)p : -1;
-      if (p < a.pages && p >= used)
-        to = moves[2 + 2 * (held_before(p) - low)];
-      a.new_tables[(int64_t)s * a.width + e] = to;
-    }
-  }
+  each_entry(a, [&](int s, int e) {
+    const uint32_t p = e < held[s] ? (uint32_t)a.tables[(int64_t)s * a.width + e] : ~0u;
+    int32_t to = p < a.pages ? (int32_t)p : -1;
+    if (p < a.pages && p >= used)
+      to = moves[2 + 2 * (rank_of(bits, rank, p) - low)];
+    a.new_tables[(int64_t)s * a.width + e] = to;
+  });
 }
 
 __global__ __launch_bounds__(256) void page_move_kernel(const int32_t* moves, PoolArgs p) {
