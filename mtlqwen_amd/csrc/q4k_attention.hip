@@ -162,21 +162,23 @@ __device__ __forceinline__ int scan_lanes(int v) {
   return v;
 }
 
-// 64 units from u0 on, one per lane, and the tiles up to each.
+// A unit takes EXTRA places of the line before its tiles: what its beginning and
+// end cost a workgroup, in tiles.
+// 64 units from u0 on, one per lane, and the places up to each.
 struct Units {
   Unit unit;
   int upto;
 };
 
-template <int QB, int TK>
+template <int QB, int TK, int EXTRA>
 __device__ __forceinline__ Units units_from(const AttentionArgs& a, const Sequences& q, int u0) {
   Units x;
   x.unit = unit_of<QB, TK>(a, q, u0 + (threadIdx.x & 63));
-  x.upto = scan_lanes(x.unit.tiles);
+  x.upto = scan_lanes(x.unit.tiles ? x.unit.tiles + EXTRA : 0);
   return x;
 }
 
-// The line: tiles of one cache head and in all, and the tiles of a stretch: a
+// The line: places of one cache head and in all, and those of a stretch: a
 // multiple of LEAST, so that the line makes no more stretches than workgroups.
 // Wave-uniform.
 struct Line {
@@ -196,25 +198,26 @@ struct Line {
 };
 
 // `near`: the first 64 units.
-template <int QB, int TK, int LEAST>
+template <int QB, int TK, int EXTRA, int LEAST>
 __device__ __forceinline__ Line make_line(const AttentionArgs& a, const Sequences& q, const Units& near) {
   Line x;
   x.per_head = lane_value(near.upto, 63);
   for (int u0 = 64; u0 < a.units; u0 += 64)
-    x.per_head += lane_value(units_from<QB, TK>(a, q, u0).upto, 63);
+    x.per_head += lane_value(units_from<QB, TK, EXTRA>(a, q, u0).upto, 63);
   x.total = x.per_head * (int)a.cache.heads;
   const int each = (int)divided((uint32_t)(x.total + a.stretches - 1), (uint32_t)a.stretches, a.stretches_inverse);
   x.step = (each + LEAST - 1) & -LEAST;
   return x;
 }
 
-// The unit that holds place x of the line, and the place of its first tile (wave-uniform).
+// The unit that holds place x of the line, and the place of its first tile, behind
+// the extra ones (wave-uniform).
 struct Place {
   Unit unit;
   int head, at, index;
 };
 
-template <int QB, int TK>
+template <int QB, int TK, int EXTRA>
 __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences& q, const Line& line, const Units& near, int x) {
   Place p;
   p.head = Line::quotient(x, line.per_head);
@@ -224,7 +227,7 @@ __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences&
   while (y >= before + lane_value(here.upto, 63)) {  // ends: y < per_head
     before += lane_value(here.upto, 63);
     start += 64;
-    here = units_from<QB, TK>(a, q, start);
+    here = units_from<QB, TK, EXTRA>(a, q, start);
   }
   const int lane = __ffsll((unsigned long long)__ballot(here.upto > y - before)) - 1;
   p.unit.seq = lane_value(here.unit.seq, lane);
@@ -239,9 +242,9 @@ __device__ __forceinline__ Place locate(const AttentionArgs& a, const Sequences&
 }
 
 // The unit behind p's on the line.
-template <int QB, int TK>
+template <int QB, int TK, int EXTRA>
 __device__ __forceinline__ Place behind(const AttentionArgs& a, const Sequences& q, Place p) {
-  p.at += p.unit.tiles;
+  p.at += p.unit.tiles + EXTRA;
   const bool last = p.index + 1 == a.units;
   p.index = last ? 0 : p.index + 1;
   p.head += last ? 1 : 0;
@@ -804,7 +807,7 @@ __device__ __forceinline__ float2 load_part(const float* p) {
 // Called by all threads once their sums are stored: the last workgroup of the unit
 // joins them.  A lane holds 4 values of a row; what bounds it is the way to memory,
 // so the loads of RU rows and PU stretches are on their way at once.
-template <typename T, int DP, int QB, int NW, int RU, int PU>
+template <typename T, int DP, int QB, int EXTRA, int NW, int RU, int PU>
 __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& line, const Place& p, int start, int wave) {
   constexpr int kLanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kRows = NW * (64 / kLanes);  // lanes of a row, rows at once
   __shared__ int arrived;
@@ -821,7 +824,7 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
   if (threadIdx.x == 0)
     reset_counter(a.counters + r0);
   // Stretch r0 began before the unit, or with it; the others within it.
-  const int late = line.start(r0) < p.at ? 1 : 0;
+  const int late = line.start(r0) < p.at - EXTRA ? 1 : 0;
 #pragma unroll 1
   for (int first = row; first - row < rows; first += RU * kRows) {
     float m[RU], l[RU];
@@ -877,14 +880,14 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW, int TK, bool FORM>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void attention_chunk_kernel(AttentionArgs a) {
-  constexpr int QB = 16 * NW * NQ, NA = TK / 16, kTile = TK * DP * 2;
+  constexpr int QB = 16 * NW * NQ, NA = TK / 16, kTile = TK * DP * 2, kExtra = AttentionShape::chunk_extra;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // K, V of two tiles
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   __shared__ int kept[kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Units near = units_from<QB, TK>(a, loaded, 0);
-  const Line line = make_line<QB, TK, AttentionShape::chunk_least>(a, loaded, near);
+  const Units near = units_from<QB, TK, kExtra>(a, loaded, 0);
+  const Line line = make_line<QB, TK, kExtra, AttentionShape::chunk_least>(a, loaded, near);
   const int stretches = line.stretches();
   if ((int)blockIdx.x >= stretches)
     return;
@@ -895,8 +898,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // on XCD L % 8).
   const int xcd = (int)blockIdx.x & 7, more = stretches & 7;
   const int wg = xcd * (stretches >> 3) + (xcd < more ? xcd : more) + ((int)blockIdx.x >> 3);
-  int x = line.start(wg);
-  const int end = line.end(wg);
+  const int begin = line.start(wg), end = line.end(wg);
   if (c.dim != DP) {
     for (int i = tid; i < 4 * kTile / 16; i += 64 * NW)
       reinterpret_cast<u4_t*>(lds)[i] = u4_t{0, 0, 0, 0};
@@ -904,18 +906,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   }
   Lanes<DP> from;
   from.set(c);
-  Place p = locate<QB, TK>(a, loaded, line, near, x);
+  Place p = locate<QB, TK, kExtra>(a, loaded, line, near, begin);
+  int t0 = begin > p.at ? begin - p.at : 0;  // the unit's first tile in the stretch
   bool leading = true;  // the stretch's first unit
   while (true) {
     const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
-    const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
-    Rows<T, DP, NQ> rows;
+    const int left = u.tiles - t0, room = end - p.at - t0, n = room < left ? room : left;
+    if (n <= 0)
+      return;  // the stretch ends before the unit's tiles
     const int row = u.row + wave * 16 * NQ;
-    rows.load(a, seqs, u, p.head, row);
-    Sums<DP, NQ> sums;
-    sums.clear();
     // What the wave's rows see, at most and at least.
     const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
     const int last = (row + 16 * NQ < u.row_end ? row + 16 * NQ : u.row_end) - 1;
@@ -964,10 +965,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         dma_v<DP>(c, from, v_next, to_next + kTile);
     };
     if (!none) {
+      find(t0, 0);
       __syncthreads();  // the buffers' last readers are done
       __builtin_amdgcn_sched_barrier(0);
-      find(t0, 0);
       fetch();
+    }
+    Rows<T, DP, NQ> rows;  // on their way with the first tile
+    rows.load(a, seqs, u, p.head, row);
+    Sums<DP, NQ> sums;
+    sums.clear();
+    if (!none) {
       for (int t = 0; t < n; ++t) {
         const uint32_t here = there;
         wait_loads<0>();
@@ -1043,12 +1050,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       }
     }
     if (!done)
-      join_unit<T, DP, QB, NW, 8, 2>(a, line, p, start, wave);
-    x += n;
-    if (x >= end)
+      join_unit<T, DP, QB, kExtra, NW, 8, 2>(a, line, p, start, wave);
+    if (p.at + t0 + n >= end)
       return;
     leading = false;
-    p = behind<QB, TK>(a, kept_sequences(kept), p);
+    t0 = 0;
+    p = behind<QB, TK, kExtra>(a, kept_sequences(kept), p);
   }
 }
 
@@ -1060,7 +1067,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW>
 __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a) {
-  constexpr int QB = 16 * NQ, TK = 32, kTile = TK * DP * 2, kLoads = DP / 16;
+  constexpr int QB = 16 * NQ, TK = 32, kTile = TK * DP * 2, kExtra = AttentionShape::rows_extra, kLoads = DP / 16;
   static_assert(NW * 16 * DP * 4 <= NW * 2 * kTile, "the waves' sums fit into the buffers");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * 2 * kTile];
   __shared__ float sm[NW][QB], sl[NW][QB];
@@ -1068,28 +1075,30 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   __shared__ int kept[kSequenceInts];
   const Sequences loaded = load_sequences(a);
-  const Units near = units_from<QB, TK>(a, loaded, 0);
-  const Line line = make_line<QB, TK, NW>(a, loaded, near);
+  const Units near = units_from<QB, TK, kExtra>(a, loaded, 0);
+  const Line line = make_line<QB, TK, kExtra, NW>(a, loaded, near);
   const int wg = (int)blockIdx.x;
   if (wg >= line.stretches())
     return;
   if (wave == 0)
     keep_sequences(loaded, kept);
   __syncthreads();
-  int x = line.start(wg);
-  const int end = line.end(wg);
+  const int begin = line.start(wg), end = line.end(wg);
   Lanes<DP> from;
   from.set(c);
   uint8_t* const mine = lds + wave * 2 * kTile;
   const uint32_t at = __builtin_amdgcn_readfirstlane(lds_addr(mine));
   const bool formed = a.softcap > 0.0f || a.slopes;
-  Place p = locate<QB, TK>(a, loaded, line, near, x);
+  Place p = locate<QB, TK, kExtra>(a, loaded, line, near, begin);
+  int t0 = begin > p.at ? begin - p.at : 0;  // the unit's first tile in the stretch
   bool leading = true;
   while (true) {
     const Sequences seqs = kept_sequences(kept);  // anew for each unit: no registers under its products
     const Unit& u = p.unit;
     const int start = lane_value(seqs.start, u.seq);
-    const int t0 = x - p.at, left = u.tiles - t0, n = end - x < left ? end - x : left;
+    const int left = u.tiles - t0, room = end - p.at - t0, n = room < left ? room : left;
+    if (n <= 0)
+      return;  // the stretch ends before the unit's tiles
     const int first = lane_value(seqs.first, u.seq), cap = lane_value(seqs.cap, u.seq);
     const int ta = first + token_of(a, u.row) + 1, tb = first + token_of(a, u.row_end - 1) + 1;
     const int hi_least = ta < cap ? ta : cap, lo_most = a.window && tb > a.window ? tb - a.window : 0;
@@ -1210,12 +1219,12 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
       }
     }
     if (!done)
-      join_unit<T, DP, QB, NW, 1, 8>(a, line, p, start, wave);
-    x += n;
-    if (x >= end)
+      join_unit<T, DP, QB, kExtra, NW, 1, 8>(a, line, p, start, wave);
+    if (p.at + t0 + n >= end)
       return;
     leading = false;
-    p = behind<QB, TK>(a, kept_sequences(kept), p);
+    t0 = 0;
+    p = behind<QB, TK, kExtra>(a, kept_sequences(kept), p);
     __syncthreads();  // before the buffers and statistics are used again
   }
 }
@@ -1278,7 +1287,8 @@ int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats) {
     a.units += (int)(((int64_t)c.count[s] * a.group + qb - 1) / qb);
   }
   // No more workgroups than tiles: as many as a table holds, for every unit.
-  const int64_t tiles = (int64_t)a.units * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1);
+  const int extra = a.row_tiles ? AttentionShape::rows_extra : AttentionShape::chunk_extra;
+  const int64_t tiles = (int64_t)a.units * ((((int64_t)c.width << c.page_log) + tk - 1) / tk + 1 + extra);
   const int wgs = a.row_tiles ? cus : 8 / AttentionShape::chunk_waves(dp, f32) * cus;
   a.stretches = tiles * c.heads < wgs ? (int)(tiles * c.heads) : wgs;
   const auto inverse = [](int y) { return y == 1 ? ~0u : (uint32_t)((1ull << 32) / (uint32_t)y); };

@@ -635,6 +635,8 @@ struct AttentionShape {
   static constexpr int chunk_waves(int dp, bool f32) { return dp > (f32 ? 128 : 192) ? 8 : 4; }
   static constexpr int chunk_keys(int dp, bool f32) { return dp > (f32 ? 64 : 128) && chunk_waves(dp, f32) == 4 ? 32 : 64; }
   static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
+  // What a unit's beginning and end cost, in tiles of chunk_keys and of 32 keys.
+  static constexpr int chunk_extra = 4, rows_extra = 16;
 };
 // Sets the plan and the floats of `part`; the cache heads that a launch may take.
 int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats);

@@ -245,38 +245,40 @@ def _sequences(query_counts, rows):
     return (_COUNTS[n] if n < len(_COUNTS) else struct.Struct(f"={n}I").pack)(*query_counts), n, covered
 
 
-def _cache(k_cache, v_cache, tables, slots, positions, sequences, device):
-    """A q4k_cache, and the address of the positions."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError(f"k_cache and v_cache must be [pages, heads, page_size, head_dim] alike, got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
+def _cache(k_cache, v_cache, shape, tables, slots, positions, sequences, device):
+    """A q4k_cache of caches of ``shape``, and the address of the positions."""
+    pages, heads, size, dim = shape
+    strides = k_cache.stride()
     if k_cache.dtype is not torch.float16 or v_cache.dtype is not torch.float16:
         raise TypeError(f"k_cache and v_cache must be float16, got {k_cache.dtype} and {v_cache.dtype}")
     if k_cache.get_device() != device or v_cache.get_device() != device:
         raise ValueError(f"k_cache and v_cache must be on cuda:{device}")
-    pages, heads, size, dim = k_cache.shape
-    strides = k_cache.stride()
     if strides != v_cache.stride() or (strides[3] != 1 and dim > 1):
         raise ValueError("k_cache and v_cache must have the same strides and contiguous tokens")
-    if tables.dim() != 2:
+    table = tables.shape
+    if len(table) != 2:
         raise ValueError("tables must be [table rows, width]")
-    rows, width = tables.shape
+    rows, width = table
     if (pages | heads | size | dim | rows | width) >> 32:
         raise _cut(pages, heads, size, dim, rows, width)
-    i32 = torch.int32
-    return (_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], _address(tables, i32, 0, device, "tables"),
-                   _address(slots, i32, sequences, device, "slots"), pages, size, heads, dim, rows, width),
-            _address(positions, i32, sequences, device, "positions"))
+    return (_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], _address(tables, torch.int32, 0, device, "tables"),
+                   _address(slots, torch.int32, sequences, device, "slots"), pages, size, heads, dim, rows, width),
+            _address(positions, torch.int32, sequences, device, "positions"))
 
 
-def _rows_of(t, like, what):
-    """A q4k_heads of ``t``, read only, of the dtype, GPU, rows and head_dim of ``like``."""
-    if t.dim() != 3 or t.dtype is not like.dtype or t.get_device() != like.get_device() or t.shape[0] != like.shape[0]:
-        raise ValueError(f"{what} must be [rows, heads, head_dim], of k's dtype, GPU and rows")
+def _cache_shape(k_cache, v_cache):
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"k_cache and v_cache must be [pages, heads, page_size, head_dim] alike, got {tuple(shape)} and {tuple(v_cache.shape)}")
+    return shape
+
+
+def _rows_of(t, heads, what):
+    """A q4k_heads of ``t``, read only."""
     row, head, element = t.stride()
     if element != 1 and t.shape[2] > 1:
         raise ValueError(f"the elements of a head of {what} must be contiguous")
-    return _HEADS(t.data_ptr(), 0, 0, row, head, 0, 0, t.shape[1])
+    return _HEADS(t.data_ptr(), 0, 0, row, head, 0, 0, heads)
 
 
 def cache_write(k, v, k_cache, v_cache, tables, positions, query_counts=None, slots=None, stream=None):
@@ -291,15 +293,19 @@ def cache_write(k, v, k_cache, v_cache, tables, positions, query_counts=None, sl
     pages that are not there.  Rows behind the last sequence, and rows whose place
     is not there, are not written."""
     code, device = _activations(k, "k")
-    if k.dim() != 3 or k_cache.dim() != 4 or k.shape[1] != k_cache.shape[1] or k.shape[2] != k_cache.shape[3] or v.shape != k.shape:
-        raise ValueError(f"k and v must be [rows, heads, head_dim] of the cache's heads, got {tuple(k.shape)} and {tuple(v.shape)} for a cache of "
-                         f"{tuple(k_cache.shape)}")
-    counts, sequences, rows = _sequences(query_counts, k.shape[0])
+    shape, of = k.shape, _cache_shape(k_cache, v_cache)
+    if len(shape) != 3 or v.shape != shape or shape[1] != of[1] or shape[2] != of[3]:
+        raise ValueError(f"k and v must be [rows, heads, head_dim] of the cache's heads, got {tuple(shape)} and {tuple(v.shape)} for a cache of "
+                         f"{tuple(of)}")
+    if v.dtype is not k.dtype or v.get_device() != device:
+        raise ValueError("k and v must share dtype and GPU")
+    counts, sequences, rows = _sequences(query_counts, shape[0])
     if rows >> 32:
         raise _cut(rows)
-    cache, at = _cache(k_cache, v_cache, tables, slots, positions, sequences, device)
-    rc = _cache_write(_raw_stream(device) if stream is None else _stream_of(stream), device, cache, _rows_of(k, k, "k"), _rows_of(v, k, "v"), at,
-                      counts, sequences, rows, code)
+    cache, at = _cache(k_cache, v_cache, of, tables, slots, positions, sequences, device)
+    heads = of[1]
+    rc = _cache_write(_raw_stream(device) if stream is None else _stream_of(stream), device, cache, _rows_of(k, heads, "k"), _rows_of(v, heads, "v"),
+                      at, counts, sequences, rows, code)
     if rc:
         check(rc)
     return k_cache, v_cache
@@ -319,14 +325,14 @@ def attention(q, k_cache, v_cache, tables, positions, out, query_counts=None, sl
     becomes zero; rows behind the last sequence are left as they were."""
     code, device = _activations(q, "q")
     heads = _heads(q, out, 0, "q")
-    if k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3]:
-        raise ValueError(f"q must have the cache's head_dim, got {tuple(q.shape)} for a cache of {tuple(k_cache.shape)}")
-    counts, sequences, rows = _sequences(query_counts, q.shape[0])
+    shape, of = q.shape, _cache_shape(k_cache, v_cache)
+    if shape[2] != of[3]:
+        raise ValueError(f"q must have the cache's head_dim, got {tuple(shape)} for a cache of {tuple(of)}")
+    counts, sequences, rows = _sequences(query_counts, shape[0])
     if rows >> 32 or window >> 32:
         raise _cut(rows, window)
-    cache, at = _cache(k_cache, v_cache, tables, slots, positions, sequences, device)
-    params = _ATTENTION(q.shape[2] ** -0.5 if scale is None else scale, softcap, _address(slopes, torch.float32, q.shape[1], device, "slopes"),
-                        window)
+    cache, at = _cache(k_cache, v_cache, of, tables, slots, positions, sequences, device)
+    params = _ATTENTION(shape[2] ** -0.5 if scale is None else scale, softcap, _address(slopes, torch.float32, shape[1], device, "slopes"), window)
     rc = _attention(_raw_stream(device) if stream is None else _stream_of(stream), device, heads, cache, params, at, counts, sequences, rows, code)
     if rc:
         check(rc)

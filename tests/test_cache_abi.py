@@ -1,5 +1,7 @@
 """attention, cache_write, cache_assign and cache_compact without a GPU: every
 refusal comes before any HIP call."""
+import struct
+
 import pytest
 import torch
 
@@ -156,14 +158,22 @@ def test_python_checks(q4k):
         ops._sequences([3, 2], 4)
     assert ops._sequences([3], 4) == (counts(3), 1, 3) and ops._sequences(None, 4)[2] == 4
     with pytest.raises(ValueError):
-        ops._cache(c, c[:, :1], i, None, i[0], 1, -1)
+        ops._cache_shape(c, c[:, :1])
+    with pytest.raises(ValueError):
+        ops._cache_shape(c[0], c[0])
+    of = ops._cache_shape(c, c)
     with pytest.raises(TypeError):
-        ops._cache(c.float(), c.float(), i, None, i[0], 1, -1)
+        ops._cache(c.float(), c.float(), of, i, None, i[0], 1, -1)
     with pytest.raises(ValueError):
-        ops._cache(c, c.transpose(2, 3).contiguous().transpose(2, 3), i, None, i[0], 1, -1)
+        t = c.transpose(2, 3).contiguous().transpose(2, 3)
+        ops._cache(c, t, of, i, None, i[0], 1, -1)
     with pytest.raises(TypeError):
-        ops._cache(c, c, i.long(), None, i[0], 1, -1)
+        ops._cache(c, c, of, i.long(), None, i[0], 1, -1)
     with pytest.raises(ValueError):
-        ops._cache(c, c, i, i[0, :0], i[0], 1, -1)
+        ops._cache(c, c, of, i, None, i[0, :0], 1, -1)
     with pytest.raises(ValueError):
-        ops._cache(c, c, i[0], None, i[0], 1, -1)
+        ops._cache(c, c, of, i[0], None, i[0], 1, -1)
+    with pytest.raises(ValueError):
+        ops._rows_of(x.transpose(1, 2), 64, "k")
+    with pytest.raises(struct.error):
+        ops._sequences([3, -1], 4)
