@@ -136,7 +136,8 @@ __device__ __forceinline__ void each_entry(const TableArgs& a, const F& f) {
 // full page; the others get a page of their own and a copy (page_fork_kernel).
 // Then, slot by slot, the lowest free pages for counts[s] more tokens.
 __global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a) {
-  __shared__ uint32_t bits[kWords], rank[kWords], sums[16], before[kMaxSlots + 1], beyond;
+  __shared__ uint32_t bits[kWords], rank[kWords], sums[16], before[kMaxSlots + 1];
+  __shared__ unsigned long long beyond;  // pages that tables have no entries for
   __shared__ __attribute__((aligned(16))) int32_t last[kMaxSlots];
   __shared__ int32_t parent[kMaxSlots], full[kMaxSlots], first[kMaxSlots], kept[kMaxSlots];
   const int tid = threadIdx.x, words = words_of(a);
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a
     const int64_t most = need < a.width ? need : a.width;
     wants = most > from ? (uint32_t)(most - from) : 0;
     if (need > most)
-      atomicAdd(&beyond, (uint32_t)(need - most));
+      atomicAdd(&beyond, (unsigned long long)(need - most));
     first[tid] = from;
     kept[tid] = keep;
   }
@@ -199,8 +200,10 @@ __global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a
   if (tid == 0)
     before[a.slots] = asked;
   const uint32_t there = a.pages - count_bits(bits, rank, words, sums);
-  if (tid == 0 && a.missing)
-    *a.missing = (int32_t)(beyond + (asked > there ? asked - there : 0));
+  if (tid == 0 && a.missing) {
+    const unsigned long long n = beyond + (asked > there ? asked - there : 0);
+    *a.missing = n < 0x7fffffff ? (int32_t)n : 0x7fffffff;
+  }
   // Request r of slot s (before[s] <= r < before[s + 1]) takes the r-th free page.
   const uint32_t given = asked < there ? asked : there;
   for (uint32_t p0 = 0; p0 < a.pages && p0 - rank[p0 >> 5] < given; p0 += kTableThreads) {
@@ -259,13 +262,12 @@ __global__ __launch_bounds__(256) void page_fork_kernel(TableArgs a, PoolArgs p)
   const int32_t src = a.tables[(int64_t)from * a.width + full], dst = a.new_tables[(int64_t)s * a.width + full];
   if ((uint32_t)src >= a.pages || (uint32_t)dst >= a.pages || src == dst)
     return;
-  const uint64_t bytes = (uint64_t)tokens * p.token_bytes;
-  const uint32_t block = blockIdx.x / p.parts;
-  const uint64_t at = (uint64_t)(blockIdx.x - block * p.parts) * kCopyBytes;
-  if (at >= bytes)
-    return;
-  const uint64_t off = (uint64_t)block * p.block_bytes + at, page = (uint64_t)p.blocks * p.block_bytes;
-  copy_bytes(p.data + (uint64_t)src * page + off, p.data + (uint64_t)dst * page + off, (uint32_t)(bytes - at < kCopyBytes ? bytes - at : kCopyBytes));
+  const uint64_t bytes = (uint64_t)tokens * p.token_bytes, page = (uint64_t)p.blocks * p.block_bytes, all = (uint64_t)p.blocks * p.parts;
+  for (uint64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const uint64_t block = i / p.parts, at = (i - block * p.parts) * kCopyBytes, off = block * p.block_bytes + at;
+    if (at < bytes)
+      copy_bytes(p.data + (uint64_t)src * page + off, p.data + (uint64_t)dst * page + off, (uint32_t)(bytes - at < kCopyBytes ? bytes - at : kCopyBytes));
+  }
 }
 
 // Of the n pages held by any slot, the i-th at or behind page n moves to the i-th
@@ -335,7 +337,8 @@ hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a) {
 
 hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p) {
   p.parts = (p.block_bytes + kCopyBytes - 1) / kCopyBytes;
-  return dispatch(page_fork_kernel, dim3(p.blocks * p.parts, a.slots), dim3(256), s, a, p);
+  const uint64_t all = (uint64_t)p.blocks * p.parts;
+  return dispatch(page_fork_kernel, dim3(all < 4096 ? (uint32_t)all : 4096, a.slots), dim3(256), s, a, p);
 }
 
 hipError_t launch_cache_compact(hipStream_t s, const TableArgs& a, int32_t* moves) {

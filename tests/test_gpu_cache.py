@@ -183,3 +183,24 @@ def test_nothing_to_do(q4k, gpu):
     length = _i32(gpu, [7, 7])
     q4k.cache_assign(pool, flat, _i32(gpu, [3, 4]), _i32(gpu, [1, 0]), flat.clone(), length, counts=_i32(gpu, [1, 17]), missing=n)
     assert length.tolist() == [0, 0] and n.tolist() == [3]
+
+
+def test_assign_missing_at_most(q4k, gpu):
+    """More pages asked for than 32 bits count: 40 slots of 2^27 each."""
+    pool = torch.zeros((3, 1, 16, 16), device=gpu, dtype=torch.uint8)
+    for n, want in ((40, 2 ** 31 - 1), (15, 15 * 2 ** 27 - 3)):
+        tables, lengths = _i32(gpu, [[-1]] * n), _i32(gpu, [0] * n)
+        new, length, missing = torch.empty_like(tables), torch.empty_like(lengths), _i32(gpu, [55])
+        q4k.cache_assign(pool, tables, lengths, None, new, length, counts=_i32(gpu, [2 ** 31 - 1] * n), missing=missing)
+        assert missing.item() == want and new.flatten().tolist() == [0, 1, 2] + [-1] * (n - 3)
+
+
+def test_assign_many_blocks(q4k, gpu):
+    """A page of 2^24 blocks: more than a launch has workgroups for, one each."""
+    blocks = 1 << 24
+    pool = torch.zeros((2, blocks, 2, 16), device=gpu, dtype=torch.uint8)
+    pool[0] = torch.arange(blocks, device=gpu).view(blocks, 1, 1).remainder(251).to(torch.uint8)
+    new, length = _i32(gpu, [[9], [9]]), _i32(gpu, [9, 9])
+    q4k.cache_assign(pool, _i32(gpu, [[0], [-1]]), _i32(gpu, [1, 0]), _i32(gpu, [0, 0]), new, length)
+    assert new.tolist() == [[0], [1]] and length.tolist() == [1, 1]
+    assert torch.equal(pool[0, :, 0], pool[1, :, 0]) and (pool[1, :, 1] == 0).all()
