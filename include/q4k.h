@@ -20,8 +20,8 @@
  *  - The workspace lives until the process ends.  The first projection on a
  *    device, of any shape, reserves 94 MB (hipMalloc); a call that
  *    needs more (mostly by staging more activations: m * k above 4.3 million,
- *    m rounded up to 128, or m above 1024) grows it.  Which kernel a call takes depends on its
- *    shape alone, so a captured call gives the bits of the eager one.  A call
+ *    m rounded up to 128, or m above 1024; attention of chunks) grows it.
+ *    Which kernel a call takes depends on its shape alone, so a captured call gives the bits of the eager one.  A call
  *    made while its stream captures a HIP graph must not need growth: the
  *    launch that would need it fails with Q4K_ECAPTURE before allocating
  *    (q4k_mlp and the two-call form of q4k_mlp_gate_up may have enqueued
@@ -348,9 +348,9 @@ int q4k_linear_lora(void* stream, q4k_weight* w, const q4k_adapters* adapters, c
  * here for any number of heads and of pages, and what a server does with the
  * pages.  A cache is fp16 pages in device memory: element d of token t of head
  * h of page p is at p * page_stride + h * head_stride + t * token_stride + d of
- * k and of v alike (strides in elements, multiples of 8; k and v 16-byte
- * aligned).  Tokens 0, 1, ... of a sequence lie in the pages that its row of
- * `tables` lists; a number outside [0, pages) means that the page is not there.
+ * k and of v alike (strides in elements, multiples of 8, token_stride up to 2^26;
+ * k and v 16-byte aligned).  Tokens 0, 1, ... of a sequence lie in the pages
+ * that its row of `tables` lists; a number outside [0, pages) means that the page is not there.
  * Tables, slots, positions and all that follows them are device memory, read
  * when the call runs, so a captured call follows them from replay to replay;
  * the counts of new rows are host values, as for q4k_linear. */
@@ -372,13 +372,13 @@ typedef struct q4k_cache {
  * position positions[q] + t.  `in` and the input strides of k and v are used,
  * their heads are the cache's.  Values are rounded to fp16.  A row whose
  * position is negative, behind the table or in a page that is not there is not
- * written; of rows with one place, one's values stay there. */
+ * written; where rows have one place, every 8 values there are some one row's. */
 int q4k_cache_write(void* stream, int device, const q4k_cache* cache, const q4k_heads* k, const q4k_heads* v, const int32_t* positions,
                     const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype);
 
 typedef struct q4k_attention_params {
   float scale;         /* of q.k */
-  float softcap;       /* above 0: x becomes softcap * tanh(x / softcap) */
+  float softcap;       /* 0, or 2^-64..2^64: x becomes softcap * tanh(x / softcap) */
   const float* slopes; /* [heads] or NULL: slopes[h] * (key's position - row's) is added */
   uint32_t window;     /* above 0: a row sees its own position and the window - 1 before it */
 } q4k_attention_params;
@@ -390,9 +390,15 @@ typedef struct q4k_attention_params {
  * A row that sees no key (a position below 0, pages that are not there) becomes
  * zero; what a row does not see does not reach it, infinities and NaN included.
  * Scores, statistics and sums are fp32.  fp16 q are multiplied as they are and
- * weights enter the products with v as fp16; fp32 q, and their weights, with 22 bits.  q and out as in q4k_rope, but they must not overlap.  Positions lie
- * in [-2^30, 2^30].  Work is split by the lengths that the device holds; sums
- * of the parts live in the device's workspace, as the projections' do. */
+ * weights enter the products with v as fp16; fp32 q, and their weights, with 22
+ * bits.  q and out as in q4k_rope, but they must not overlap.  Positions lie
+ * in [-2^30, 2^30] (others are taken as the nearer end), rows * q->heads is at
+ * most 2^30.  Work is split by the lengths that the device holds: one cache
+ * head's key tiles, with full tables, must not pass 2^31 (Q4K_ESHAPE).  Sums of
+ * the parts live in the device's workspace, as the projections' do: its first
+ * reservation holds those of calls with up to 48 rows times heads of a group per
+ * sequence (32 for head_dim above 128), others take up to 102 MB.  Outputs do not
+ * depend on the order in which workgroups run. */
 int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache* cache, const q4k_attention_params* params,
                   const int32_t* positions, const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype);
 
@@ -413,7 +419,8 @@ typedef struct q4k_pool {
  * slot that holds it (if no other holds it as a full one), the others get a
  * page with a copy of its tokens.  New pages are the lowest that no slot's new
  * tokens lie in, in the order of the slots.  Entries without a page are -1;
- * *missing (may be NULL) is the number of pages asked for and not given.  A page
+ * *missing (may be NULL) is the number of pages asked for and not given (at most
+ * 2^31 - 1).  A page
  * counts as held where it lies below a slot's length (clamped to its table), so
  * the caller adds the tokens it has written to the lengths.  tables and lengths are
  * read, new_tables and new_lengths written; none may overlap.  Forks, beams in

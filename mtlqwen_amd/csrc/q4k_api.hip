@@ -2416,12 +2416,13 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
     rc = check_cache(cache, positions, nq);
   if (rc)
     return rc;
-  if ((uint64_t)rows * q->heads > 0x7fffffffu)
-    return fail(Q4K_ESHAPE, "at most 2^31 - 1 rows of heads (got %u of %u)", rows, q->heads);
+  if ((uint64_t)rows * q->heads > (1u << 30))
+    return fail(Q4K_ESHAPE, "at most 2^30 rows of heads (got %u of %u)", rows, q->heads);
   if (q->heads % cache->heads != 0)
     return fail(Q4K_ESHAPE, "the heads of q must be a multiple of the cache's (got %u and %u)", q->heads, cache->heads);
-  if (!std::isfinite(params->scale) || !std::isfinite(params->softcap) || params->softcap < 0.0f || params->window > 0x7fffffffu)
-    return fail(Q4K_EINVAL, "scale must be finite, softcap finite and not negative, window below 2^31");
+  if (!std::isfinite(params->scale) || !(params->softcap == 0.0f || (params->softcap >= 0x1p-64f && params->softcap <= 0x1p64f)) ||
+      params->window > 0x7fffffffu)
+    return fail(Q4K_EINVAL, "scale must be finite, softcap 0 or in [2^-64, 2^64], window below 2^31");
   const size_t es = dtype == Q4K_DTYPE_F32 ? 4 : 2;
   HeadSpan in, out;
   rc = check_heads("q", q, rows, cache->head_dim, es, &in, &out);
@@ -2445,9 +2446,7 @@ int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache*
   a.sign = params->scale > 0.0f ? 1.0f : params->scale < 0.0f ? -1.0f : 0.0f;
   a.scale = params->scale == 0.0f ? 1.0f : std::fabs(params->scale);
   a.softcap = params->softcap;
-  a.heads = (int)q->heads;
   a.group = (int)(q->heads / cache->heads);
-  a.rows = (int)rows;
   a.window = (int)params->window;
   DeviceScope scope(device);
   if (scope.rc)

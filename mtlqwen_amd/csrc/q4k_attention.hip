@@ -70,8 +70,8 @@ __device__ __forceinline__ int lane_value(int v, int lane) {
 
 // ---- the line of work --------------------------------------------------------
 // Whole numbers of 32 bits throughout (attention_plan bounds the line): what is
-// computed once per launch or unit is computed by code that was never fetched
-// before, at about 140 clocks for every 64 bytes of it.
+// computed once per launch or unit is a chain of dependent instructions with little
+// beside it, and a call of one row is hardly more than that.
 
 // x / y for any x, m = 2^32 / y rounded down (2^32 - 1 for y = 1): the product is
 // one too small at most.
@@ -334,6 +334,8 @@ struct Rows {
         }
       }
       __builtin_amdgcn_sched_barrier(0);
+      // Neither 0 nor infinite, which would make NaN of what is not seen or of zeros.
+      c[kParts ? n : 0] = __builtin_amdgcn_fmed3f(c[kParts ? n : 0], 0x1p-126f, 0x1p127f);
       slope[n] = live && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
       pos[n] = live ? first + t : -1;
     }

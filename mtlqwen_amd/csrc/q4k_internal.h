@@ -617,7 +617,7 @@ struct AttentionArgs {
   const float* slopes = nullptr;  // [heads] or nullptr
   float scale = 1.0f, sign = 1.0f;  // of q.k; scale is positive, q is taken times sign (1, -1 or 0)
   float softcap = 0.0f;
-  int heads = 0, group = 1, rows = 0;
+  int group = 1;   // heads of q to a head of the cache
   int window = 0;  // keys that a row sees, its own the last; 0: all before it
   // Set by attention_plan: the 16-row tiles of a unit (0: a chunk's), the units and
   // those before each sequence, the workgroups.

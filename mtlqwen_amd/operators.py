@@ -317,9 +317,9 @@ def attention(q, k_cache, v_cache, tables, positions, out, query_counts=None, sl
     the new tokens' own keys and values among them): row t of sequence q of ``q``
     [rows, heads, head_dim] stands at positions[q] + t and sees the keys up to
     there, head h those of cache head h // (heads / cache heads).  Scores are
-    ``scale`` (default 1 / sqrt(head_dim)) times the products; above 0,
-    ``softcap`` bounds them (softcap * tanh(score / softcap)) and ``window`` is the
-    number of keys that a row sees, its own the last; ``slopes`` (float32 [heads])
+    ``scale`` (default 1 / sqrt(head_dim)) times the products; ``softcap`` (2^-64
+    to 2^64; 0: none) bounds them (softcap * tanh(score / softcap)); ``window``,
+    above 0, is the number of keys that a row sees, its own the last; ``slopes`` (float32 [heads])
     times the (negative) distance to the key is added.  ``out`` is like ``q``, of
     any row and head strides, and must not overlap it.  A row that sees no key
     becomes zero; rows behind the last sequence are left as they were."""

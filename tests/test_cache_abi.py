@@ -76,6 +76,7 @@ def test_caches(q4k, c, code):
     ({"h": heads(o=S), "c": cache(s=S)}, EALIAS), ({"h": heads(o=S), "pr": params(slopes=S + 28)}, EALIAS),
     ({"pr": params(scale=float("inf"))}, EINVAL), ({"pr": params(scale=float("nan"))}, EINVAL), ({"pr": params(cap=-1.0)}, EINVAL),
     ({"pr": params(cap=float("nan"))}, EINVAL), ({"pr": params(window=1 << 31)}, EINVAL),
+    ({"pr": params(cap=2.0 ** -65)}, EINVAL), ({"pr": params(cap=2.0 ** 65)}, EINVAL), ({"rows": (1 << 24) - 1, "h": heads(n=66)}, ESHAPE),
     ({"c": cache(rows=2), "counts": counts(1, 2, 5), "nq": 3}, ESHAPE),
 ])
 def test_attention_refusals(q4k, kw, code):

@@ -244,3 +244,30 @@ def test_no_rows(q4k, gpu):
     out.fill_(1.0)
     q4k.attention(q, cache[:, 0], cache[:, 1], torch.empty((1, 0), device=gpu, dtype=torch.int32), _i32(gpu, [0]), out)
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("counts", [[1, 3], [40, 17]])
+def test_smallest_scores(q4k, gpu, counts, dtype):
+    """Scores that underflow: a plain mean of the values that a row sees."""
+    _check(q4k, gpu, counts, [77, 130], 4, 2, 128, 16, dtype, scale=1e-38)
+    _check(q4k, gpu, counts, [77, 130], 4, 2, 128, 16, dtype, scale=1e-30, size=1e-7 if dtype == F16 else 1e-35)
+    _check(q4k, gpu, counts, [77, 130], 4, 2, 128, 16, dtype, softcap=2.0 ** -64, window=30)
+
+
+@pytest.mark.parametrize("counts", [[1, 3], [40, 17]])
+def test_largest_cap(q4k, gpu, counts):
+    """A cap of 2^64 leaves scores as they are: their cubes over 3 * 2^128 are
+    nothing.  The cap's function is good to 2^-21 of its value, so scores up to x
+    are off by 2^-21 x more, and outputs by twice that of the largest value."""
+    rng = np.random.default_rng(5)
+    tables, pages = _tables(rng, [77, 130], 16)
+    cache = _cache(rng, gpu, pages, 2, 16, 64)
+    q = torch.from_numpy(rng.standard_normal((sum(counts), 4, 64)).astype(np.float32))
+    first = [77 - counts[0], 130 - counts[1]]
+    out = q4k.attention(q.to(gpu), cache[:, 0], cache[:, 1], _i32(gpu, tables), _i32(gpu, first), torch.empty_like(q, device=gpu), query_counts=counts,
+                        softcap=2.0 ** 64)
+    c = cache.cpu().numpy()
+    want, bound = ref.attention(q.numpy(), c[:, 0], c[:, 1], tables, first, counts)
+    x = 0.125 * np.sqrt((q.numpy() ** 2).sum(-1).max() * (c[:, 0].astype(np.float64) ** 2).sum(-1).max())  # no score is above
+    _close(out, want, bound + 2 * 2.0 ** -21 * x * np.abs(c[:, 1]).max(), "cap of 2^64")
