@@ -397,7 +397,7 @@ typedef struct q4k_attention_params {
  * head's key tiles, with full tables, must not pass 2^31 (Q4K_ESHAPE).  Sums of
  * the parts live in the device's workspace, as the projections' do: its first
  * reservation holds those of calls with up to 48 rows times heads of a group per
- * sequence (32 for head_dim above 128), others take up to 102 MB.  Outputs do not
+ * sequence (16 for head_dim above 128), others take up to 102 MB.  Outputs do not
  * depend on the order in which workgroups run. */
 int q4k_attention(void* stream, int device, const q4k_heads* q, const q4k_cache* cache, const q4k_attention_params* params,
                   const int32_t* positions, const uint32_t* query_counts, uint32_t nqueries, uint32_t rows, uint32_t dtype);

@@ -290,40 +290,31 @@ struct Rows {
       const T* x = static_cast<const T*>(a.q) + (int64_t)(start + t) * a.q_row + (int64_t)h * a.q_head + 8 * g;
       c[kParts ? n : 0] = a.scale * kLog2e;
       if constexpr (kParts) {
-        // Read twice, for the row's largest value and for its parts: 8 values at a
-        // time in registers.
-        const auto part = [&](int d, float (&f)[8]) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            f[e] = 0.0f;
-          if (live && 32 * d + 8 * g < a.cache.dim)
-            load8(x + 32 * d, f);
-          asm volatile("" ::: "memory");
-        };
-        float mx = 0.0f, up, down;
+        float f[DP / 32][8], mx = 0.0f, up, down;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          float f[8];
-          part(d, f);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            mx = fmaxf(mx, fabsf(f[e]));
+            f[d][e] = 0.0f;
+          if (live && 32 * d + 8 * g < a.cache.dim)
+            load8(x + 32 * d, f[d]);
         }
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            mx = fmaxf(mx, fabsf(f[d][e]));
         pow2_scale(row_max(mx), up, down);
         c[n] *= down;
         up *= a.sign;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          float f[8];
-          part(d, f);
+        for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float v = f[e] * up;
+            const float v = f[d][e] * up;
             q[n][d][e] = (_Float16)v;
             ql[n][d][e] = (_Float16)(v - (float)q[n][d][e]);
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
       } else {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
@@ -878,7 +869,13 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
 // ----------------------------------------------------------------------------
 // Chunks of tokens: NW waves of 16 NQ query rows each over the same key tiles,
 // two buffers of K and V in LDS, the next tile's transfers under the present
-// tile's products.
+// tile's products.  8192 fp16 rows of 32 / 8 heads of 128 take 603 us (912 TFLOP/s):
+// of a tile's 4000 clocks, a wave spends 660 to 950 on K Q^T, 1100 to 1220 on the weights
+// and 970 to 1020 on V P^T, and the other wave of its SIMD does not always have
+// what would fill them.  2048 rows of 16 / 4 heads of 256 take 263 us (690 TFLOP/s),
+// bound by LDS: a fragment feeds the products of 16 rows there, not 32.  Ragged
+// prompts (821 fp32 rows, window 1024) take 81 us: 17 tiles a workgroup, 35 us of it at
+// 8192 rows' pace, and the beginnings and ends of units, nearly all of them shared.
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW, int TK, bool FORM>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void attention_chunk_kernel(AttentionArgs a) {
@@ -1065,7 +1062,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 // Few query rows: every wave takes every NW-th tile of 32 keys of its workgroup's
 // stretch, with a buffer for K and one for V of its own, refilled as soon as each
 // has been read; the waves' sums join in LDS at the end of a unit.  Bound by the
-// reading of K and V.
+// reading of K and V: 8 rows of 16 / 4 heads of 256 over 1.2 GB of them take 210 us
+// (5.75 TB/s), 40 capped fp32 rows of 32 / 8 heads of 128 over 304 MB 70 us.  One
+// row over 777 keys takes 14 us, the latency of its steps: units of the line, rows
+// and keys, the waves' sums, the stretches' sums.  Four waves: with eight, heads of 128
+// of 8 sequences take 20.1 us in place of 17.0 (fp32 rows, 1024 keys; fp16 16.6 and
+// 15.3) and, over 16384 keys, 54.4 in place of 56.4 (fp16; fp32 57.7 and 57.1).
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW>
 __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a) {
@@ -1234,16 +1236,13 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
 template <typename T, int DP>
 hipError_t launch_t(hipStream_t s, const AttentionArgs& a) {
   if (a.row_tiles) {
-    hipError_t e;
-    if (a.row_tiles == 1)
-      e = dispatch(attention_rows_kernel<T, DP, 1, DP <= 128 ? 8 : 4>, dim3(a.stretches), dim3(DP <= 128 ? 512 : 256), s, a);
-    else if (a.row_tiles == 2)
-      e = dispatch(attention_rows_kernel<T, DP, 2, 4>, dim3(a.stretches), dim3(256), s, a);
-    else if constexpr (DP <= 128)
-      e = dispatch(attention_rows_kernel<T, DP, 3, 4>, dim3(a.stretches), dim3(256), s, a);
-    else
-      e = hipErrorInvalidValue;
-    return e;
+    if constexpr (AttentionShape::most_row_tiles(DP) > 1) {
+      if (a.row_tiles == 2)
+        return dispatch(attention_rows_kernel<T, DP, 2, 4>, dim3(a.stretches), dim3(256), s, a);
+      if (a.row_tiles == 3)
+        return dispatch(attention_rows_kernel<T, DP, 3, 4>, dim3(a.stretches), dim3(256), s, a);
+    }
+    return dispatch(attention_rows_kernel<T, DP, 1, 4>, dim3(a.stretches), dim3(256), s, a);
   }
   constexpr bool kF = sizeof(T) == 4;
   constexpr int NQ = AttentionShape::chunk_tiles(DP, kF), NW = AttentionShape::chunk_waves(DP, kF), TK = AttentionShape::chunk_keys(DP, kF);
@@ -1279,7 +1278,7 @@ int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats) {
     most = c.count[s] > most ? c.count[s] : most;
   const int rows = most * a.group;
   const int dp = AttentionShape::padded(c.dim);
-  a.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && dp <= 128 ? 3 : 0;
+  a.row_tiles = rows <= 16 * AttentionShape::most_row_tiles(dp) ? (rows + 15) / 16 : 0;
   const bool f32 = dtype == kF32;
   const int qb = a.row_tiles ? 16 * a.row_tiles : 16 * AttentionShape::chunk_waves(dp, f32) * AttentionShape::chunk_tiles(dp, f32);
   const int tk = a.row_tiles ? 32 : AttentionShape::chunk_keys(dp, f32);

@@ -628,13 +628,22 @@ struct AttentionArgs {
   int* counters = nullptr;   // [stretches], zero between launches
 };
 // Head sizes, as the kernels are built for them, and their chunks: 16-row tiles of
-// a wave, keys of a tile.
+// a wave, keys of a tile.  Two 16-row tiles a wave where two waves a SIMD still find
+// registers for them (2048 fp16 rows of heads of 256: 385 us with two tiles and one
+// wave, 291 with one and two waves), and 64 keys where these fit (8192 fp32 rows
+// of 128: 1703 us with 64 and one wave a SIMD, 1076 with 32 and two).
 struct AttentionShape {
   static constexpr int padded(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
   static constexpr int chunk_tiles(int dp, bool f32) { return dp > (f32 ? 128 : 192) ? 1 : 2; }
   static constexpr int chunk_waves(int dp, bool f32) { return dp > (f32 ? 128 : 192) ? 8 : 4; }
   static constexpr int chunk_keys(int dp, bool f32) { return dp > (f32 ? 64 : 128) && chunk_waves(dp, f32) == 4 ? 32 : 64; }
   static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
+  // Up to 16 times as many query rows of a cache head go to the kernel of few rows.
+  // 8 sequences, 1024 | 16384 keys, us with it and with chunks: 16 rows of 256 (fp16)
+  // 25.7, 26.8 | 119, 129; 32 rows 35.6, 28.0 | 130, 135; 16 rows of 128 15.3, 23.6 |
+  // 56, 73; 32 rows 21.6, 24.8 | 62, 75; 48 rows 27.1, 26.0 | 70, 76 (fp32 33.8,
+  // 29.9 | 80, 101).
+  static constexpr int most_row_tiles(int dp) { return dp <= 128 ? 3 : 1; }
   // What a unit's beginning and end cost, in tiles of chunk_keys and of 32 keys.
   static constexpr int chunk_extra = 4, rows_extra = 16;
 };
