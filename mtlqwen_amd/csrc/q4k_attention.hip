@@ -779,9 +779,9 @@ __device__ __forceinline__ T* out_row(const AttentionArgs& a, int start, int hea
 
 // ---- units that stretches share ------------------------------------------------------
 // The sums of stretch r's first unit are in slot 2 r of the workspace, those of its
-// last one in slot 2 r + 1: QB rows of DP values, and behind all slots each row's
-// maximum and sum of weights.  They are written and read past the caches, which
-// workgroups on different XCDs do not share.
+// last one in slot 2 r + 1: QB rows of DP values (chunks: as their waves hold them),
+// and behind all slots each row's maximum and sum of weights.  They are written and
+// read past the caches, which workgroups on different XCDs do not share.
 
 template <int DP, int QB>
 __device__ __forceinline__ float* part_row(const AttentionArgs& a, int64_t slot, int row) {
@@ -797,25 +797,33 @@ __device__ __forceinline__ float2 load_part(const float* p) {
   return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM));
 }
 
-// Called by all threads once their sums are stored: the last workgroup of the unit
-// joins them.  A lane holds 4 values of a row; what bounds it is the way to memory,
-// so the loads of RU rows and PU stretches are on their way at once.
-template <typename T, int DP, int QB, int EXTRA, int NW, int RU, int PU>
-__device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& line, const Place& p, int start, int wave) {
-  constexpr int kLanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kRows = NW * (64 / kLanes);  // lanes of a row, rows at once
+// Called by all threads once their sums are stored: whether this workgroup is the
+// last of the unit's `parts` stretches from r0 on.
+__device__ __forceinline__ bool last_of_unit(const AttentionArgs& a, int r0, int parts) {
   __shared__ int arrived;
-  const int lane = threadIdx.x & 63, d = 4 * (lane & (kLanes - 1)), row = wave * (64 / kLanes) + lane / kLanes;
-  const Unit& u = p.unit;
-  const int r0 = line.of(p.at), parts = line.of(p.at + u.tiles - 1) - r0 + 1, rows = u.row_end - u.row;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
     arrived = count_arrival(a.counters + r0);
   __syncthreads();
   if (arrived != parts - 1)
-    return;
+    return false;
   if (threadIdx.x == 0)
     reset_counter(a.counters + r0);
+  return true;
+}
+
+// Few rows: the last workgroup joins the sums.  A lane holds 4 values of a row; what
+// bounds it is the way to memory, so the loads of RU rows and PU stretches are on
+// their way at once.
+template <typename T, int DP, int QB, int EXTRA, int NW, int RU, int PU>
+__device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& line, const Place& p, int start, int wave) {
+  constexpr int kLanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kRows = NW * (64 / kLanes);  // lanes of a row, rows at once
+  const int lane = threadIdx.x & 63, d = 4 * (lane & (kLanes - 1)), row = wave * (64 / kLanes) + lane / kLanes;
+  const Unit& u = p.unit;
+  const int r0 = line.of(p.at), parts = line.of(p.at + u.tiles - 1) - r0 + 1, rows = u.row_end - u.row;
+  if (!last_of_unit(a, r0, parts))
+    return;
   // Stretch r0 began before the unit, or with it; the others within it.
   const int late = line.start(r0) < p.at - EXTRA ? 1 : 0;
 #pragma unroll 1
@@ -863,6 +871,88 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
     for (int y = 0; y < RU; ++y)
       if (first + y * kRows < rows && d < a.cache.dim)
         store4(out_row<T>(a, start, p.head, u.row + first + y * kRows) + d, l[y] == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[y] * (1.0f / l[y]));
+  }
+}
+
+// Chunks: every wave stores the sums of its 16 NQ rows as its lanes hold them, 1 KB
+// at a time, and the waves of the last workgroup add those of the other stretches to
+// their own (at their place in the order), all of a stretch on their way at once.
+// 821 fp32 rows take 66 us so, 76 with the values laid out by rows and the loads of 8
+// rows and 2 stretches at once; 8192 rows 572 and 586.
+template <int DP, int NQ, int NW>
+__device__ __forceinline__ void store_sums(const AttentionArgs& a, int slot, int wave, const Sums<DP, NQ>& sums, const float (&l)[NQ]) {
+  constexpr int QB = 16 * NW * NQ;
+  const int lane = threadIdx.x & 63;
+  float* o = part_row<DP, QB>(a, slot, wave * 16 * NQ) + lane * 4;
+#pragma unroll
+  for (int y = 0; y < NQ; ++y) {
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      store_coherent4(o + (y * (DP / 16) + d) * 256, sums.o[y][d]);
+    if (lane < 16) {
+      float* ml = part_weights<DP, QB>(a, slot, wave * 16 * NQ + 16 * y + lane);
+      store_coherent(ml, sums.m[y]);
+      store_coherent(ml + 1, l[y]);
+    }
+  }
+}
+
+// `own`: this workgroup's stretch, whose sums become the unit's.
+template <int DP, int NQ, int NW>
+__device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, int parts, int late, int own, int wave, Sums<DP, NQ>& sums, float (&l)[NQ]) {
+  constexpr int QB = 16 * NW * NQ, ND = DP / 16;
+  constexpr int kAtOnce = NQ * DP <= 256 ? NQ : 1;  // 16-row tiles beside the wave's own in registers
+  constexpr int kPastCaches = 17;                   // sc0 sc1
+  const int lane = threadIdx.x & 63;
+  const uint32_t floats = 2 * (uint32_t)a.stretches * QB * DP;
+  const auto from = __builtin_amdgcn_make_buffer_rsrc(a.part, 0, (int)((floats + 2 * (uint32_t)a.stretches * QB * 2) * 4), 0x00020000);
+#pragma unroll
+  for (int y0 = 0; y0 < NQ; y0 += kAtOnce) {
+    f4_t o[kAtOnce][ND];
+    float m[kAtOnce], w[kAtOnce];
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      m[y] = -INFINITY;
+      w[y] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        o[y][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll 1
+    for (int s = 0; s < parts; ++s) {
+      const uint32_t row = (uint32_t)(2 * (r0 + s) + (s == 0 ? late : 0)) * QB + wave * 16 * NQ;  // wave-uniform
+#pragma unroll
+      for (int y = 0; y < kAtOnce; ++y) {
+        f4_t f[ND];
+        float in = sums.m[y0 + y], weights = l[y0 + y];
+        if (r0 + s == own) {
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+            f[d] = sums.o[y0 + y][d];
+        } else {
+          const auto ml = __builtin_amdgcn_raw_buffer_load_b64(from, (lane & 15) * 8, (int)((floats + (row + 16 * (y0 + y)) * 2) * 4), kPastCaches);
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+            f[d] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(from, lane * 16, (int)((row * DP + ((y0 + y) * ND + d) * 256) * 4), kPastCaches));
+          in = __builtin_bit_cast(float, (uint32_t)ml[0]);
+          weights = __builtin_bit_cast(float, (uint32_t)ml[1]);
+        }
+        const float top = fmaxf(m[y], in);
+        const float old = m[y] == top ? 1.0f : __builtin_amdgcn_exp2f(m[y] - top), now = in == top ? 1.0f : __builtin_amdgcn_exp2f(in - top);
+        m[y] = top;
+        w[y] = w[y] * old + now * weights;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          o[y][d] = o[y][d] * old + now * f[d];
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      l[y0 + y] = w[y];
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        sums.o[y0 + y][d] = o[y][d];
+    }
   }
 }
 
@@ -1020,36 +1110,36 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       }
     }
     sums.settle();
-    // Whole units are done; of others the sums go to the workspace.
-    const bool done = n == u.tiles;
-    const int64_t slot = 2 * (int64_t)wg + (leading ? 0 : 1);
+    float l[NQ];
 #pragma unroll
-    for (int y = 0; y < NQ; ++y) {
-      const float l = row_sum(sums.l[y]);
-      const int r = row + 16 * y + (lane & 15);
-      if (r >= u.row_end)
-        continue;
-      if (done) {
+    for (int y = 0; y < NQ; ++y)
+      l[y] = row_sum(sums.l[y]);
+    // Whole units are done; the sums of others go to the workspace, and the last of
+    // their workgroups goes on with all of them.
+    bool done = n == u.tiles;
+    if (!done) {
+      if (active)
+        store_sums<DP, NQ, NW>(a, 2 * wg + (leading ? 0 : 1), wave, sums, l);
+      const int r0 = line.of(p.at), parts = line.of(p.at + u.tiles - 1) - r0 + 1;
+      done = last_of_unit(a, r0, parts);
+      // Stretch r0 began before the unit, or with it; the others within it.
+      if (done && active)
+        add_stretches<DP, NQ, NW>(a, r0, parts, line.start(r0) < p.at - kExtra ? 1 : 0, wg, wave, sums, l);
+    }
+    if (done) {
+#pragma unroll
+      for (int y = 0; y < NQ; ++y) {
+        const int r = row + 16 * y + (lane & 15);
+        if (r >= u.row_end)
+          continue;
         T* o = out_row<T>(a, start, p.head, r);
-        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        const float f = l[y] == 0.0f ? 0.0f : 1.0f / l[y];
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
           if (16 * d + 4 * g < c.dim)
-            store4(o + 16 * d + 4 * g, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : sums.o[y][d] * f);
-      } else {
-        float* o = part_row<DP, QB>(a, slot, r - u.row);
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-          store_coherent4(o + 16 * d + 4 * g, sums.o[y][d]);
-        if (g == 0) {
-          float* ml = part_weights<DP, QB>(a, slot, r - u.row);
-          store_coherent(ml, sums.m[y]);
-          store_coherent(ml + 1, l);
-        }
+            store4(o + 16 * d + 4 * g, l[y] == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : sums.o[y][d] * f);
       }
     }
-    if (!done)
-      join_unit<T, DP, QB, kExtra, NW, 8, 2>(a, line, p, start, wave);
     if (p.at + t0 + n >= end)
       return;
     leading = false;

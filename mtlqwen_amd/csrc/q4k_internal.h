@@ -644,8 +644,10 @@ struct AttentionShape {
   // 56, 73; 32 rows 21.6, 24.8 | 62, 75; 48 rows 27.1, 26.0 | 70, 76 (fp32 33.8,
   // 29.9 | 80, 101).
   static constexpr int most_row_tiles(int dp) { return dp <= 128 ? 3 : 1; }
-  // What a unit's beginning and end cost, in tiles of chunk_keys and of 32 keys.
-  static constexpr int chunk_extra = 4, rows_extra = 16;
+  // What a unit's beginning and end cost, in tiles of chunk_keys and of 32 keys (us
+  // with 4, 6 and 8 for chunks: 821 fp32 rows 66.1, 63.5, 67.1, 2048 rows of heads of
+  // 256 239, 237, 239, 8192 of 128 573, 576, 580).
+  static constexpr int chunk_extra = 6, rows_extra = 16;
 };
 // Sets the plan and the floats of `part`; the cache heads that a launch may take.
 int attention_plan(AttentionArgs& a, int dtype, int cus, size_t* floats);
