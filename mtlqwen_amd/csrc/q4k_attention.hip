@@ -959,12 +959,12 @@ __device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, in
 // ----------------------------------------------------------------------------
 // Chunks of tokens: NW waves of 16 NQ query rows each over the same key tiles,
 // two buffers of K and V in LDS, the next tile's transfers under the present
-// tile's products.  8192 fp16 rows of 32 / 8 heads of 128 take 603 us (912 TFLOP/s):
+// tile's products.  8192 fp16 rows of 32 / 8 heads of 128 take 568 us (968 TFLOP/s):
 // of a tile's 4000 clocks, a wave spends 660 to 950 on K Q^T, 1100 to 1220 on the weights
 // and 970 to 1020 on V P^T, and the other wave of its SIMD does not always have
-// what would fill them.  2048 rows of 16 / 4 heads of 256 take 263 us (690 TFLOP/s),
+// what would fill them.  2048 rows of 16 / 4 heads of 256 take 239 us (761 TFLOP/s),
 // bound by LDS: a fragment feeds the products of 16 rows there, not 32.  Ragged
-// prompts (821 fp32 rows, window 1024) take 81 us: 17 tiles a workgroup, 35 us of it at
+// prompts (821 fp32 rows, window 1024) take 63 us: 17 tiles a workgroup, 35 us of it at
 // 8192 rows' pace, and the beginnings and ends of units, nearly all of them shared.
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW, int TK, bool FORM>
@@ -1153,7 +1153,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 // stretch, with a buffer for K and one for V of its own, refilled as soon as each
 // has been read; the waves' sums join in LDS at the end of a unit.  Bound by the
 // reading of K and V: 8 rows of 16 / 4 heads of 256 over 1.2 GB of them take 210 us
-// (5.75 TB/s), 40 capped fp32 rows of 32 / 8 heads of 128 over 304 MB 70 us.  One
+// (5.75 TB/s), 40 capped fp32 rows of 32 / 8 heads of 128 over 304 MB 64 us.  One
 // row over 777 keys takes 14 us, the latency of its steps: units of the line, rows
 // and keys, the waves' sums, the stretches' sums.  Four waves: with eight, heads of 128
 // of 8 sequences take 20.1 us in place of 17.0 (fp32 rows, 1024 keys; fp16 16.6 and
