@@ -755,6 +755,26 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// Of a tile's transfers of K by dma_k, one after another, only those that have a lane in the
+// head are made: where a head's last 32 elements are all padding, one less of each
+// 16 tokens.  (Those of V have lanes in the head all.)
+constexpr bool one_transfer_at_most() {
+  for (int dim = 8; dim <= 256; dim += 8)
+    if ((dim + 31) / 32 < AttentionShape::padded(dim) / 32 - 1)
+      return false;
+  return true;
+}
+static_assert(one_transfer_at_most(), "one transfer of 16 tokens may be left out, not two");
+
+// All transfers are done but those of K of the 32 tokens asked for last.
+template <int DP>
+__device__ __forceinline__ void wait_loads_before_k(const CacheArgs& c) {
+  if (c.dim + 32 <= DP)
+    wait_loads<DP / 16 - 2>();
+  else
+    wait_loads<DP / 16>();
+}
+
 // Every read of LDS so far is done (a transfer may overwrite what it read).
 __device__ __forceinline__ void wait_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1239,7 +1259,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         const int key = u.lo + (t0 + t) * TK;
         const uint32_t here = there;
         const bool whole = key + TK <= hi_least && key >= lo_most && here == 3u, more = t + NW < n;
-        wait_loads<kLoads>();  // K is here, V may be on its way
+        wait_loads<kLoads>();  // K is here, V (kLoads transfers, whatever the head) may be on its way
         f4_t s[2][NQ];
         scores<T, DP, NQ, 2>(mine, rows, s, [](int) {});
         wait_lds();
@@ -1250,7 +1270,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         finish_scores<T, DP, NQ, 2>(a, rows, key, whole, here, formed, s);
         sums.weigh(s, [&](int y) { return formed ? 1.0f : rows.factor(y); });
         if (more)
-          wait_loads<kLoads>();
+          wait_loads_before_k<DP>(c);
         else
           wait_loads<0>();
         if (!whole && __any(odd_values<64, kTile>(mine + kTile, lane))) {
