@@ -389,6 +389,8 @@ typedef struct q4k_attention_params {
  *   out = sum_j exp(x_j) v_j / sum_j exp(x_j),   x_j = scale (q . k_j), capped, then biased.
  * A row that sees no key (a position below 0, pages that are not there) becomes
  * zero; what a row does not see does not reach it, infinities and NaN included.
+ * A row whose scores are all -inf becomes NaN (0 / 0); an infinity in a key that a
+ * row of fp32 q, which is two parts, sees makes it NaN.
  * Scores, statistics and sums are fp32.  fp16 q are multiplied as they are and
  * weights enter the products with v as fp16; fp32 q, and their weights, with 22
  * bits.  q and out as in q4k_rope, but they must not overlap.  Positions lie

@@ -21,6 +21,8 @@
 // number of workgroups and each takes an equal stretch of that line (locate());
 // a unit that several share leaves its sums, one per stretch, in the workspace,
 // and the workgroup that comes last adds them, in the order of the stretches.
+#include <cfloat>
+
 #include "q4k_device.h"
 
 namespace q4k {
@@ -384,10 +386,10 @@ __device__ __forceinline__ void scores(const uint8_t* k, const Rows<T, DP, NQ>& 
 // Products become t: capped, biased and, in a tile that not every row sees whole,
 // -inf for the keys that a row does not see.  `there`: a bit per 16 keys whose page
 // is there.  With neither cap nor bias products stay as they are (c turns them into
-// t where the weights are formed).
+// t where the weights are formed).  `some`: a bit per row that sees a key.
 template <typename T, int DP, int NQ, int NA>
 __device__ __forceinline__ void finish_scores(const AttentionArgs& a, const Rows<T, DP, NQ>& r, int key, bool whole, uint32_t there, bool formed,
-                                              f4_t (&s)[NA][NQ]) {
+                                              f4_t (&s)[NA][NQ], uint32_t (&some)[NQ]) {
   const int g = (threadIdx.x & 63) >> 4;
   if (formed) {
     const float in = a.softcap > 0.0f ? 1.0f / (a.softcap * kLog2e) : 0.0f, out = a.softcap * kLog2e;
@@ -409,27 +411,52 @@ __device__ __forceinline__ void finish_scores(const AttentionArgs& a, const Rows
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       int low, high;
+      bool any = false;
       r.seen(a, n, key + 4 * g, low, high);
 #pragma unroll
       for (int b = 0; b < NA; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!((there >> b) & 1) || 16 * b + e <= low || 16 * b + e > high)
+        for (int e = 0; e < 4; ++e) {
+          const bool sees = ((there >> b) & 1) && 16 * b + e > low && 16 * b + e <= high;
+          any = any || sees;
+          if (!sees)
             s[b][n][e] = -INFINITY;
+        }
+      const uint64_t lanes = __ballot(any), half = lanes | lanes >> 32;
+      some[n] |= (uint32_t)(half | half >> 16);
     }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+      some[n] = ~0u;
   }
 }
 
-// The running sums of NQ column tiles: O^T, the maximum that its weights refer to
-// and this lane's part of their sum.
+// What a row becomes.  One that sees nothing (its maximum is -inf) is zero; scores that are
+// all -inf have a maximum (Sums::settle) and no weights: 0 / 0.
+__device__ __forceinline__ f4_t row_values(f4_t o, float l, float m) {
+  const float f = l == 0.0f ? __builtin_nanf("") : 1.0f / l;
+  return m == -INFINITY ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * f;
+}
+
+// The running sums of NQ column tiles: O^T, the maximum that its weights refer to,
+// this lane's part of their sum, and a bit per row that sees a key.
 template <int DP, int NQ>
 struct Sums {
   f4_t o[NQ][DP / 16];
   float m[NQ], l[NQ];
+  uint32_t some[NQ];
   uint32_t up[NQ][(DP + 127) / 128], down[NQ][(DP + 127) / 128];  // sums that infinities and NaN reach: bit 4 d + e
 
-  // They reach them: infinity, -infinity, or both, a NaN.
+  // They reach them: infinity, -infinity, or both, a NaN.  And a row that sees keys whose scores
+  // are all -inf gets the lowest maximum: other stretches' weights leave nothing of
+  // its sums, and alone it is no row that sees nothing.
   __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const bool sees = (some[n] >> (threadIdx.x & 15)) & 1;
+      m[n] = m[n] == -INFINITY && sees ? -FLT_MAX : m[n];
+    }
     uint32_t any = 0;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -455,6 +482,7 @@ struct Sums {
         o[n][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
       m[n] = -INFINITY;
       l[n] = 0.0f;
+      some[n] = 0;
 #pragma unroll
       for (int i = 0; i < (DP + 127) / 128; ++i)
         up[n][i] = down[n][i] = 0;
@@ -890,7 +918,7 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
 #pragma unroll
     for (int y = 0; y < RU; ++y)
       if (first + y * kRows < rows && d < a.cache.dim)
-        store4(out_row<T>(a, start, p.head, u.row + first + y * kRows) + d, l[y] == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o[y] * (1.0f / l[y]));
+        store4(out_row<T>(a, start, p.head, u.row + first + y * kRows) + d, row_values(o[y], l[y], m[y]));
   }
 }
 
@@ -968,6 +996,7 @@ __device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, in
     }
 #pragma unroll
     for (int y = 0; y < kAtOnce; ++y) {
+      sums.m[y0 + y] = m[y];
       l[y0 + y] = w[y];
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -1121,7 +1150,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           if (asks)
             dma_at<DP>(d, k_mine, v_mine, from, k_next, v_next, to_next, to_next + kTile);
         });
-        finish_scores<T, DP, NQ, NA>(a, rows, key, whole, here, FORM, s);
+        finish_scores<T, DP, NQ, NA>(a, rows, key, whole, here, FORM, s, sums.some);
         sums.weigh(s, [&](int y) { return FORM ? 1.0f : rows.factor(y); });
 #pragma unroll
         for (int h = 0; h < NA / 2; ++h) {
@@ -1153,11 +1182,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         if (r >= u.row_end)
           continue;
         T* o = out_row<T>(a, start, p.head, r);
-        const float f = l[y] == 0.0f ? 0.0f : 1.0f / l[y];
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
           if (16 * d + 4 * g < c.dim)
-            store4(o + 16 * d + 4 * g, l[y] == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : sums.o[y][d] * f);
+            store4(o + 16 * d + 4 * g, row_values(sums.o[y][d], l[y], sums.m[y]));
       }
     }
     if (p.at + t0 + n >= end)
@@ -1267,7 +1295,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
           open(t0 + t + NW);
           fetch_k();
         }
-        finish_scores<T, DP, NQ, 2>(a, rows, key, whole, here, formed, s);
+        finish_scores<T, DP, NQ, 2>(a, rows, key, whole, here, formed, s, sums.some);
         sums.weigh(s, [&](int y) { return formed ? 1.0f : rows.factor(y); });
         if (more)
           wait_loads_before_k<DP>(c);
@@ -1321,7 +1349,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
           o += f * *reinterpret_cast<const f4_t*>(buffer + (w * 16 + rr) * DP + d);
         }
         if (done) {
-          store4(out_row<T>(a, start, p.head, r) + d, l == 0.0f ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / l));
+          store4(out_row<T>(a, start, p.head, r) + d, row_values(o, l, top));
         } else {
           store_coherent4(part_row<DP, QB>(a, slot, 16 * y + rr) + d, o);
           if (d == 0) {

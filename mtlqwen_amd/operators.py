@@ -322,7 +322,8 @@ def attention(q, k_cache, v_cache, tables, positions, out, query_counts=None, sl
     above 0, is the number of keys that a row sees, its own the last; ``slopes`` (float32 [heads])
     times the (negative) distance to the key is added.  ``out`` is like ``q``, of
     any row and head strides, and must not overlap it.  A row that sees no key
-    becomes zero; rows behind the last sequence are left as they were."""
+    becomes zero (one whose scores are all -inf NaN); rows behind the last sequence
+    are left as they were."""
     code, device = _activations(q, "q")
     heads = _heads(q, out, 0, "q")
     shape, of = q.shape, _cache_shape(k_cache, v_cache)

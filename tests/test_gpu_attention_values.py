@@ -1,0 +1,71 @@
+"""Attention over scores and values that are not finite and that a row does see:
+what the formula gives, in tiles that all rows of a unit see and in others, in one
+stretch of the keys or several."""
+import numpy as np
+import pytest
+import torch
+
+import cache_ref as ref
+from test_gpu_attention import _cache, _close, _i32, _tables
+
+pytestmark = pytest.mark.gpu
+F32, F16 = torch.float32, torch.float16
+
+
+def _case(gpu, counts, contexts, heads, kv, dim, page, dtype):
+    rng = np.random.default_rng(sum(contexts) + dim)
+    tables, pages = _tables(rng, contexts, page)
+    cache = _cache(rng, gpu, pages, kv, page, dim)
+    q = torch.from_numpy(rng.standard_normal((sum(counts), heads, dim)).astype(np.float32)).to(dtype)
+    return tables, cache, q, [c - n for c, n in zip(contexts, counts)]
+
+
+def _attend(q4k, gpu, q, cache, tables, first, counts, window=0):
+    out = torch.full(q.shape, 9.0, device=gpu, dtype=q.dtype)
+    q4k.attention(q.to(gpu), cache[:, 0], cache[:, 1], _i32(gpu, tables), _i32(gpu, first), out, query_counts=counts, window=window)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim", [64, 80, 128, 200, 256])
+@pytest.mark.parametrize("counts,contexts,window", [([1], [40], 0), ([1, 2], [1, 3000], 0), ([5], [90], 7), ([70], [200], 0), ([3, 90], [50, 4000], 333)])
+def test_scores_of_minus_infinity_alone(q4k, gpu, counts, contexts, window, dim, dtype):
+    """An infinite element of a query whose products are all -inf: 0 / 0, not a row that sees nothing."""
+    tables, cache, q, first = _case(gpu, counts, contexts, 4, 2, dim, 16, dtype)
+    cache[:, 0, :, :, 5] = -cache[:, 0, :, :, 5].abs() - 0.5
+    r, h = sum(counts) - 1, 2
+    q[r, h, 5] = float("inf")
+    out = _attend(q4k, gpu, q, cache, tables, first, counts, window)
+    c = cache.cpu().numpy()
+    want, bound = ref.attention(q.float().numpy(), c[:, 0], c[:, 1], tables, first, counts, window=window, f16=dtype == F16)
+    assert np.isnan(want[r, h]).all()
+    _close(out, want, bound, "one row of -inf")
+
+
+@pytest.mark.parametrize("dim", [64, 80, 128, 200, 256])
+@pytest.mark.parametrize("counts,contexts", [([1, 2], [40, 6000]), ([4, 5], [30, 8000]), ([70], [200]), ([100, 90], [6000, 500])])
+def test_scores_of_minus_infinity_among_others(q4k, gpu, counts, contexts, dim):
+    """Keys with an infinite element leave nothing in rows that see others, in whichever part of the keys they are,
+    and make those that see no other NaN.  fp16 rows: fp32 ones, of two parts, become NaN.  For the bounds those keys have a score of
+    -4000 / sqrt(dim), whose weight is below 2^-300."""
+    page, window = 16, 0
+    for window in (0, 3):
+        tables, cache, q, first = _case(gpu, counts, contexts, 4, 2, dim, page, F16)
+        q[:, :, 5] = 4.0
+        cache[:, 0, :, :, 5] = 0.0
+        plain = cache.clone()
+        # The first half of the last sequence's tokens before its rows, and its rows' own but the last three.
+        n, t = contexts[-1], tables[-1]
+        bad = [at for at in range(n - 3) if at >= first[-1] or at < first[-1] // 2]
+        for at in bad:
+            cache[t[at // page], 0, :, at % page, 5] = float("-inf")
+            plain[t[at // page], 0, :, at % page, 5] = -1000.0
+        out = _attend(q4k, gpu, q, cache, tables, first, counts, window)
+        c = plain.cpu().numpy()
+        want, bound = ref.attention(q.float().numpy(), c[:, 0], c[:, 1], tables, first, counts, window=window, f16=True)
+        for i in range(counts[-1]):
+            p, r = first[-1] + i, sum(counts[:-1]) + i
+            if all(at in set(bad) for at in range(max(0, p + 1 - window) if window else 0, p + 1)):
+                want[r] = np.nan
+        _close(out, want, bound, f"window {window}")
