@@ -570,8 +570,8 @@ template <int THREADS, int BYTES>
 __device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
   uint32_t bits = 0;
 #pragma unroll 4
-  for (int i = 0; i < BYTES / 16 / THREADS; ++i) {
-    const u4_t f = *reinterpret_cast<const u4_t*>(v + (i * THREADS + thread) * 16);
+  for (int at = thread * 16; at < BYTES; at += THREADS * 16) {
+    const u4_t f = *reinterpret_cast<const u4_t*>(v + at);
     // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
     bits |= ((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
             ((f.w & 0x7fff7fffu) + 0x04000400u);
@@ -582,12 +582,12 @@ __device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
 template <int THREADS, int BYTES>
 __device__ __forceinline__ void clear_values(uint8_t* v, int thread) {
 #pragma unroll 1
-  for (int i = 0; i < BYTES / 16 / THREADS; ++i) {
-    h8_t f = *reinterpret_cast<const h8_t*>(v + (i * THREADS + thread) * 16);
+  for (int at = thread * 16; at < BYTES; at += THREADS * 16) {
+    h8_t f = *reinterpret_cast<const h8_t*>(v + at);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       f[e] = __builtin_fabsf16(f[e]) <= (_Float16)65504.0f ? f[e] : (_Float16)0.0f;
-    *reinterpret_cast<h8_t*>(v + (i * THREADS + thread) * 16) = f;
+    *reinterpret_cast<h8_t*>(v + at) = f;
   }
 }
 

@@ -69,3 +69,32 @@ def test_scores_of_minus_infinity_among_others(q4k, gpu, counts, contexts, dim):
             if all(at in set(bad) for at in range(max(0, p + 1 - window) if window else 0, p + 1)):
                 want[r] = np.nan
         _close(out, want, bound, f"window {window}")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim", [8, 64, 72, 80, 96, 112, 128, 160, 192, 200, 256])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("counts,contexts,window", [([1, 3], [77, 500], 60), ([5], [900], 65), ([70], [130], 0), ([150], [900], 500)])
+def test_values_that_no_row_sees(q4k, gpu, counts, contexts, window, bad, dim, dtype):
+    """Keys and values before every row's window and behind the last token, then
+    values of one token that some rows see, at every place of a tile."""
+    tables, cache, q, first = _case(gpu, counts, contexts, 2, 1, dim, 32, dtype)
+    for t, n, p in zip(tables, contexts, first):
+        for at in list(range(0, max(0, p + 1 - window) if window else 0)) + list(range(n, -(-n // 32) * 32)):
+            cache[t[at // 32], :, :, at % 32] = bad
+    out = _attend(q4k, gpu, q, cache, tables, first, counts, window)
+    c = cache.cpu().numpy()
+    want, bound = ref.attention(q.float().numpy(), c[:, 0], c[:, 1], tables, first, counts, window=window, f16=dtype == F16)
+    assert np.isfinite(want).all()
+    _close(out, want, bound, f"{bad} that no row sees")
+    # A token that the first row of the last sequence does not see yet, or does not see any more.
+    at = contexts[-1] - 1 if counts[-1] > 1 and not window else max(0, first[-1] + 1 - window)
+    cache[tables[-1][at // 32], 1, :, at % 32] = bad
+    out = _attend(q4k, gpu, q, cache, tables, first, counts, window)
+    c = cache.cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want, bound = ref.attention(q.float().numpy(), c[:, 0], c[:, 1], tables, first, counts, window=window, f16=dtype == F16)
+    fine = np.isfinite(want)
+    got = out.cpu().double().numpy()
+    assert np.isfinite(got[fine]).all() and not np.isfinite(got[~fine]).any() and fine.any() and not fine.all()
+    _close(torch.from_numpy(np.where(fine, got, 0.0)), np.where(fine, want, 0.0), np.where(fine, bound, 1.0), f"{bad} that some rows see")
