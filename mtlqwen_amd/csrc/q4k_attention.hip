@@ -439,6 +439,12 @@ __device__ __forceinline__ f4_t row_values(f4_t o, float l, float m) {
   return m == -INFINITY ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * f;
 }
 
+// What sums under the maximum m count for under `top`.  Never 0: an infinite sum
+// stays infinite, and 2^-126 of a finite one is nothing beside weights of 2^kTop.
+__device__ __forceinline__ float share(float m, float top) {
+  return m == top ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f);
+}
+
 // The running sums of NQ column tiles: O^T, the maximum that its weights refer to,
 // this lane's part of their sum, and a bit per row that sees a key.
 template <int DP, int NQ>
@@ -469,9 +475,24 @@ struct Sums {
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[n][d][e] += ((up[n][d / 8] >> (4 * (d % 8) + e)) & 1 ? INFINITY : 0.0f) - ((down[n][d / 8] >> (4 * (d % 8) + e)) & 1 ? INFINITY : 0.0f);
+          for (int e = 0; e < 4; ++e) {
+            const bool u = (up[n][d / 8] >> (4 * (d % 8) + e)) & 1, v = (down[n][d / 8] >> (4 * (d % 8) + e)) & 1;
+            o[n][d][e] = u || v ? (u ? INFINITY : 0.0f) - (v ? INFINITY : 0.0f) : o[n][d][e];
+          }
     }
+  }
+
+  // Whether a sum of this lane is infinite or NaN: only those leave 0 * o other than 0.
+  __device__ __forceinline__ bool odd() const {
+    float z = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          z = fmaf(o[n][d][e], 0.0f, z);
+    return !(z == 0.0f);
   }
 
   __device__ __forceinline__ void clear() {
@@ -565,7 +586,11 @@ __device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
 // tile that some row does not see whole is looked over first (odd_values, by
 // THREADS threads together).  If it holds one, a product of the places of infinities and
 // NaN with who sees them says which sums they reach (mark_values: a bit per sum,
-// for settle()), and they become zero in LDS (clear_values).
+// for settle()), and they become zero in LDS (clear_values).  Tiles that all rows see
+// are not looked over (it would be an eighth of their reads of LDS, and a barrier more).
+// An infinity there makes a sum infinite, or NaN where its weight, or the second part of one, is
+// zero or negative in fp16; so where a sum comes out as either (Sums::odd), V of
+// the stretch is fetched once more and marked.
 template <int THREADS, int BYTES>
 __device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
   uint32_t bits = 0;
@@ -906,8 +931,7 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
 #pragma unroll
         for (int y = 0; y < RU; ++y) {
           const float in = s0 + s < parts ? w[y][s].x : -INFINITY, top = fmaxf(m[y], in);
-          const float old = m[y] == top ? 1.0f : __builtin_amdgcn_exp2f(m[y] - top);
-          const float f = s0 + s < parts ? (in == top ? 1.0f : __builtin_amdgcn_exp2f(in - top)) : 0.0f;
+          const float old = share(m[y], top), f = share(in, top);
           m[y] = top;
           if (s0 + s < parts) {
             l[y] = l[y] * old + f * w[y][s].y;
@@ -986,7 +1010,7 @@ __device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, in
           weights = __builtin_bit_cast(float, (uint32_t)ml[1]);
         }
         const float top = fmaxf(m[y], in);
-        const float old = m[y] == top ? 1.0f : __builtin_amdgcn_exp2f(m[y] - top), now = in == top ? 1.0f : __builtin_amdgcn_exp2f(in - top);
+        const float old = share(m[y], top), now = share(in, top);
         m[y] = top;
         w[y] = w[y] * old + now * weights;
 #pragma unroll
@@ -1157,6 +1181,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           add_values<T, DP, NQ>(k + kTile + h * 32 * DP * 2, s[2 * h], s[2 * h + 1], sums);
         }
       }
+      if (__syncthreads_or(sums.odd())) {
+#pragma unroll 1
+        for (int t = t0; t < t0 + n; ++t) {
+          const int key = u.lo + t * TK;
+          find(t, 0);
+          __syncthreads();  // the buffer's last readers are done
+          if (v_mine)
+            dma_v<DP>(c, from, v_next, to_next + kTile);
+          wait_loads<0>();
+          __syncthreads();
+          __builtin_amdgcn_sched_barrier(0);
+          if (active && key < hi_most && key + TK > lo_least)
+#pragma unroll 1
+            for (int h = 0; h < NA / 2; ++h)
+              mark_values<T, DP, NQ>(a, lds + kTile + h * 32 * DP * 2, rows, key + 32 * h, there >> (2 * h), sums);
+        }
+      }
     }
     sums.settle();
     float l[NQ];
@@ -1312,6 +1353,16 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         if (more)
           fetch_v();
       }
+      if (__any(sums.odd())) {
+#pragma unroll 1
+        for (int t = wave; t < n; t += NW) {
+          open(t0 + t);
+          fetch_v();
+          wait_loads<0>();
+          mark_values<T, DP, NQ>(a, mine + kTile, rows, u.lo + (t0 + t) * TK, there, sums);
+          wait_lds();
+        }
+      }
     }
     sums.settle();
     // The waves' sums of each 16 rows, joined by all threads.
@@ -1344,7 +1395,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          const float m = sm[w][16 * y + rr], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+          const float f = share(sm[w][16 * y + rr], top);
           l = fmaf(f, sl[w][16 * y + rr], l);
           o += f * *reinterpret_cast<const f4_t*>(buffer + (w * 16 + rr) * DP + d);
         }

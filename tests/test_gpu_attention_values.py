@@ -98,3 +98,36 @@ def test_values_that_no_row_sees(q4k, gpu, counts, contexts, window, bad, dim, d
     got = out.cpu().double().numpy()
     assert np.isfinite(got[fine]).all() and not np.isfinite(got[~fine]).any() and fine.any() and not fine.all()
     _close(torch.from_numpy(np.where(fine, got, 0.0)), np.where(fine, want, 0.0), np.where(fine, bound, 1.0), f"{bad} that some rows see")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim", [64, 80, 128, 200, 256])
+@pytest.mark.parametrize("size", [1.0, 20.0])
+@pytest.mark.parametrize("counts,contexts,window", [([1, 1], [150, 5000], 0), ([5], [700], 0), ([70], [500], 0), ([90, 3], [4000, 3000], 0),
+                                                    ([150], [900], 500), ([2, 4], [900, 4000], 1500)])
+def test_values_of_infinity(q4k, gpu, counts, contexts, window, size, dim, dtype):
+    """Values of infinity, -infinity, both and NaN that rows see, among keys of weights of any size (those of 2^-200 too, whose
+    share no fp32 holds), in tiles that all rows see: weights are positive, so the sum is what it is in the reals."""
+    tables, cache, q, first = _case(gpu, counts, contexts, 4, 2, dim, 32, dtype)
+    q *= size
+    for t, n in zip(tables, contexts):
+        for at in range(n):
+            if at % 41 == 7:
+                cache[t[at // 32], 1, :, at % 32, 3] = float("inf")
+            if at % 611 == 40:
+                cache[t[at // 32], 1, :, at % 32, 8] = float("-inf")
+            if at % 300 == 50:
+                cache[t[at // 32], 1, :, at % 32, 15] = float("-inf") if at % 600 == 50 else float("inf")
+            if at == 111:
+                cache[t[at // 32], 1, :, at % 32, dim - 1] = float("nan")
+    out = _attend(q4k, gpu, q, cache, tables, first, counts, window)
+    c = cache.cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want, bound = ref.attention(q.float().numpy(), c[:, 0], c[:, 1], tables, first, counts, window=window, f16=dtype == F16)
+    got = out.cpu().double().numpy()
+    assert np.isinf(want).any() and np.isnan(want).any()
+    for what in (np.isposinf, np.isneginf, np.isnan):
+        off = np.argwhere(what(got) != what(want))
+        assert not len(off), f"{what.__name__}: {len(off)} places, row, head and element {off[0]}"
+    fine = np.isfinite(want)
+    _close(torch.from_numpy(np.where(fine, got, 0.0)), np.where(fine, want, 0.0), np.where(fine, bound, 1.0), "finite ones")
