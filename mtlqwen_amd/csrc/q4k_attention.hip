@@ -262,6 +262,12 @@ __device__ __forceinline__ Place behind(const AttentionArgs& a, const Sequences&
 
 // ---- query rows ----------------------------------------------------------------
 
+// The row at `pos` (-1: none) sees key j + x for low < x <= high.
+__device__ __forceinline__ void seen_keys(const AttentionArgs& a, int pos, int cap, int j, int& low, int& high) {
+  high = (pos < cap ? pos : cap - 1) - j;
+  low = a.window && pos >= a.window ? pos - a.window - j : -j - 1;
+}
+
 // NQ column tiles of 16 query rows: their fragments (fp32 rows as two fp16 parts
 // under a power of two, 22 bits), what turns a product into t, and where the rows
 // stand (-1: no row; it sees nothing).
@@ -274,11 +280,7 @@ struct Rows {
 
   __device__ __forceinline__ float factor(int n) const { return c[kParts ? n : 0]; }
 
-  // The row of tile n sees key j + x for low < x <= high.
-  __device__ __forceinline__ void seen(const AttentionArgs& a, int n, int j, int& low, int& high) const {
-    high = (pos[n] < cap ? pos[n] : cap - 1) - j;
-    low = a.window && pos[n] >= a.window ? pos[n] - a.window - j : -j - 1;
-  }
+  __device__ __forceinline__ void seen(const AttentionArgs& a, int n, int j, int& low, int& high) const { seen_keys(a, pos[n], cap, j, low, high); }
 
   __device__ __forceinline__ void load(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -439,8 +441,8 @@ __device__ __forceinline__ f4_t row_values(f4_t o, float l, float m) {
   return m == -INFINITY ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : o * f;
 }
 
-// What sums under the maximum m count for under `top`.  Never 0: an infinite sum
-// stays infinite, and 2^-126 of a finite one is nothing beside weights of 2^kTop.
+// What a wave's or stretch's sums under the maximum m count for under `top`.  Never 0: an
+// infinite sum stays infinite, and 2^-126 of a finite one is nothing beside weights of 2^kTop.
 __device__ __forceinline__ float share(float m, float top) {
   return m == top ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f);
 }
@@ -482,17 +484,21 @@ struct Sums {
     }
   }
 
-  // Whether a sum of this lane is infinite or NaN: only those leave 0 * o other than 0.
-  __device__ __forceinline__ bool odd() const {
-    float z = 0.0f;
+  // Whether a sum of this lane is infinite or NaN (only those leave 0 * o other than 0)
+  // in a row whose sum of weights is not.
+  __device__ __forceinline__ bool odd(const float (&weights)[NQ]) const {
+    bool any = false;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n) {
+      f4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          z = fmaf(o[n][d][e], 0.0f, z);
-    return !(z == 0.0f);
+          z[e] = fmaf(o[n][d][e], 0.0f, z[e]);
+      any = any || (!(z[0] + z[1] + z[2] + z[3] == 0.0f) && weights[n] == weights[n]);
+    }
+    return any;
   }
 
   __device__ __forceinline__ void clear() {
@@ -589,19 +595,21 @@ __device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
 // for settle()), and they become zero in LDS (clear_values).  Tiles that all rows see
 // are not looked over (it would be an eighth of their reads of LDS, and a barrier more).
 // An infinity there makes a sum infinite, or NaN where its weight, or the second part of one, is
-// zero or negative in fp16; so where a sum comes out as either (Sums::odd), V of
-// the stretch is fetched once more and marked.
+// zero or negative in fp16; so a wave some of whose sums come out as either
+// (Sums::odd) reads V once more and marks it (mark_again).
+// A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
+__device__ __forceinline__ uint32_t odd_bits(u4_t f) {
+  return (((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
+          ((f.w & 0x7fff7fffu) + 0x04000400u)) & 0x80008000u;
+}
+
 template <int THREADS, int BYTES>
 __device__ __forceinline__ bool odd_values(const uint8_t* v, int thread) {
   uint32_t bits = 0;
 #pragma unroll 4
-  for (int at = thread * 16; at < BYTES; at += THREADS * 16) {
-    const u4_t f = *reinterpret_cast<const u4_t*>(v + at);
-    // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
-    bits |= ((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
-            ((f.w & 0x7fff7fffu) + 0x04000400u);
-  }
-  return (bits & 0x80008000u) != 0;
+  for (int at = thread * 16; at < BYTES; at += THREADS * 16)
+    bits |= odd_bits(*reinterpret_cast<const u4_t*>(v + at));
+  return bits != 0;
 }
 
 template <int THREADS, int BYTES>
@@ -745,6 +753,65 @@ struct Lanes {
     return 8 * ((n - row * (DP / 8)) ^ v_swizzle<DP>(row)) < c.dim;
   }
 };
+
+// Marks the infinities and NaN of V of keys `key` .. `end` - 1, whole groups of 16, out
+// of memory, for the wave's rows from `row` on.  The lanes look over 16 tokens together; those of a group
+// that holds some are gone through one by one.  Neither LDS nor barriers, all found
+// anew, and expected of no wave: laid out among the tiles' code, or with registers of its own
+// under the products, it took 8192 fp16 rows of heads of 64 from 391 to 420 us.
+template <int DP, int NQ>
+__device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row, int key, int end,
+                                           Sums<DP, NQ>& sums) {
+  typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+  const CacheArgs& c = a.cache;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane), "+s"(head), "+s"(row));
+  const int g = lane >> 4, first = lane_value(s.first, u.seq), cap = lane_value(s.cap, u.seq);
+  const uint8_t* const v = static_cast<const uint8_t*>(c.v) + (int64_t)head * c.head_stride * 2;
+  Pages pages;
+  pages.open(a, s, u.seq);
+#pragma unroll 1
+  for (; key < end; key += 16) {
+    pages.reach(a, key >> c.page_log);
+    const int page = pages.page(key >> c.page_log);
+    if (page < 0)
+      continue;
+    const uint8_t* const tokens = v + Pages::bytes(c, page, key);
+    uint32_t bits = 0;
+#pragma unroll 1
+    for (int d = 8 * g; d < c.dim; d += 32)
+      bits |= odd_bits(*reinterpret_cast<const u4_t*>(tokens + ((lane & 15) * c.token_stride + d) * 2));
+    if (!__any(bits != 0))
+      continue;
+#pragma unroll 1
+    for (int i = 0; i < DP; ++i) {  // token i % 16, d of 16 (i / 16)
+      const int t = i & 15, d = i >> 4;
+      if (16 * d + 4 * g >= c.dim)
+        continue;
+      const h4_t f = *reinterpret_cast<const h4_t*>(tokens + (t * c.token_stride + 16 * d + 4 * g) * 2);
+      uint32_t up = 0, down = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        up |= f[e] <= (_Float16)65504.0f ? 0u : 1u << e;
+        down |= f[e] >= (_Float16)-65504.0f ? 0u : 1u << e;
+      }
+      up <<= 4 * (d & 7);
+      down <<= 4 * (d & 7);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        int low, high;
+        const int mine = row + 16 * n + (lane & 15);
+        seen_keys(a, mine < u.row_end ? first + token_of(a, mine) : -1, cap, key, low, high);
+        const bool sees = t > low && t <= high;
+#pragma unroll
+        for (int x = 0; x < (DP + 127) / 128; ++x) {
+          sums.up[n][x] |= sees && d >> 3 == x ? up : 0u;
+          sums.down[n][x] |= sees && d >> 3 == x ? down : 0u;
+        }
+      }
+    }
+  }
+}
 
 // Transfer X of K or V of 16 tokens.
 template <int X>
@@ -1010,7 +1077,7 @@ __device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, in
           weights = __builtin_bit_cast(float, (uint32_t)ml[1]);
         }
         const float top = fmaxf(m[y], in);
-        const float old = share(m[y], top), now = share(in, top);
+        const float old = m[y] == top ? 1.0f : __builtin_amdgcn_exp2f(m[y] - top), now = in == top ? 1.0f : __builtin_amdgcn_exp2f(in - top);
         m[y] = top;
         w[y] = w[y] * old + now * weights;
 #pragma unroll
@@ -1181,29 +1248,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           add_values<T, DP, NQ>(k + kTile + h * 32 * DP * 2, s[2 * h], s[2 * h + 1], sums);
         }
       }
-      if (__syncthreads_or(sums.odd())) {
-#pragma unroll 1
-        for (int t = t0; t < t0 + n; ++t) {
-          const int key = u.lo + t * TK;
-          find(t, 0);
-          __syncthreads();  // the buffer's last readers are done
-          if (v_mine)
-            dma_v<DP>(c, from, v_next, to_next + kTile);
-          wait_loads<0>();
-          __syncthreads();
-          __builtin_amdgcn_sched_barrier(0);
-          if (active && key < hi_most && key + TK > lo_least)
-#pragma unroll 1
-            for (int h = 0; h < NA / 2; ++h)
-              mark_values<T, DP, NQ>(a, lds + kTile + h * 32 * DP * 2, rows, key + 32 * h, there >> (2 * h), sums);
-        }
-      }
     }
-    sums.settle();
     float l[NQ];
 #pragma unroll
     for (int y = 0; y < NQ; ++y)
       l[y] = row_sum(sums.l[y]);
+    sums.settle();
     // Whole units are done; the sums of others go to the workspace, and the last of
     // their workgroups goes on with all of them.
     bool done = n == u.tiles;
@@ -1217,6 +1267,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         add_stretches<DP, NQ, NW>(a, r0, parts, line.start(r0) < p.at - kExtra ? 1 : 0, wg, wave, sums, l);
     }
     if (done) {
+      if (__builtin_expect(__any(sums.odd(l)), 0)) {
+        mark_again<DP, NQ>(a, kept_sequences(kept), u, p.head, row, u.lo, u.lo + u.tiles * TK, sums);
+        sums.settle();
+      }
 #pragma unroll
       for (int y = 0; y < NQ; ++y) {
         const int r = row + 16 * y + (lane & 15);
@@ -1353,25 +1407,20 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
         if (more)
           fetch_v();
       }
-      if (__any(sums.odd())) {
-#pragma unroll 1
-        for (int t = wave; t < n; t += NW) {
-          open(t0 + t);
-          fetch_v();
-          wait_loads<0>();
-          mark_values<T, DP, NQ>(a, mine + kTile, rows, u.lo + (t0 + t) * TK, there, sums);
-          wait_lds();
-        }
-      }
     }
+    float l[NQ];
+#pragma unroll
+    for (int y = 0; y < NQ; ++y)
+      l[y] = row_sum(sums.l[y]);
+    if (__builtin_expect(__any(sums.odd(l)), 0))
+      mark_again<DP, NQ>(a, kept_sequences(kept), u, p.head, u.row, u.lo + t0 * TK, u.lo + (t0 + n) * TK, sums);
     sums.settle();
     // The waves' sums of each 16 rows, joined by all threads.
 #pragma unroll
     for (int y = 0; y < NQ; ++y) {
-      const float l = row_sum(sums.l[y]);
       if (g == 0) {
         sm[wave][16 * y + (lane & 15)] = sums.m[y];
-        sl[wave][16 * y + (lane & 15)] = l;
+        sl[wave][16 * y + (lane & 15)] = l[y];
       }
     }
     const bool done = n == u.tiles;
