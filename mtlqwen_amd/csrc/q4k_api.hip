@@ -2509,7 +2509,7 @@ int q4k_cache_assign(void* stream, int device, const q4k_pool* pool, const int32
     LaunchTimer timer(s, Q4K_KERNEL_AUX);
     Q4K_TRY_HIP(launch_cache_assign(s, a), "cache assign launch");
   }
-  if (slots < 2 || width == 0 || pool->page_size == 1)  // no page can have two holders, or none is filled in part
+  if (slots == 0 || width == 0 || pool->page_size == 1)  // no page is filled in part
     return Q4K_OK;
   LaunchTimer timer(s, Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_page_fork(s, a, pool_args(pool)), "page fork launch");
