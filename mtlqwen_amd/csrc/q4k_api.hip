@@ -2507,9 +2507,9 @@ int q4k_cache_assign(void* stream, int device, const q4k_pool* pool, const int32
   hipStream_t s = static_cast<hipStream_t>(stream);
   {
     LaunchTimer timer(s, Q4K_KERNEL_AUX);
-    Q4K_TRY_HIP(launch_cache_assign(s, a), "cache assign launch");
+    Q4K_TRY_HIP(launch_cache_assign(s, a, pool_args(pool)), "cache assign launch");
   }
-  if (slots == 0 || width == 0 || pool->page_size == 1)  // no page is filled in part
+  if (slots < 2 || width == 0 || pool->page_size == 1)  // copied already, or no page is filled in part
     return Q4K_OK;
   LaunchTimer timer(s, Q4K_KERNEL_AUX);
   Q4K_TRY_HIP(launch_page_fork(s, a, pool_args(pool)), "page fork launch");

@@ -130,12 +130,31 @@ __device__ __forceinline__ void each_entry(const TableArgs& a, const F& f) {
   }
 }
 
+// What a workgroup copies of a block at a time.
+constexpr uint32_t kCopyBytes = 16384;
+
+template <int THREADS = 256>
+__device__ __forceinline__ void copy_bytes(const uint8_t* from, uint8_t* to, uint32_t bytes) {
+  constexpr int kDeep = 4;
+  u4_t v[kDeep];
+  for (uint32_t at = threadIdx.x * 16; at < bytes; at += THREADS * 16 * kDeep) {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (at + i * THREADS * 16 < bytes)
+        v[i] = *reinterpret_cast<const u4_t*>(from + at + i * THREADS * 16);
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (at + i * THREADS * 16 < bytes)
+        *reinterpret_cast<u4_t*>(to + at + i * THREADS * 16) = v[i];
+  }
+}
+
 // Slot s takes the first lengths[p] tokens of its parent p.  Pages full of tokens are
 // shared.  A page that is not full will be written on, so it can stay with one
 // slot only: with the lowest of those that hold it, unless another holds it as a
 // full page; the others get a page of their own and a copy (page_fork_kernel).
 // Then, slot by slot, the lowest free pages for counts[s] more tokens.
-__global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a) {
+__global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a, PoolArgs pool) {
   __shared__ uint32_t bits[kWords], rank[kWords], sums[16], before[kMaxSlots + 1];
   __shared__ unsigned long long beyond;  // pages that tables have no entries for
   __shared__ __attribute__((aligned(16))) int32_t last[kMaxSlots];
@@ -228,28 +247,25 @@ __global__ __launch_bounds__(kTableThreads) void cache_assign_kernel(TableArgs a
     const int32_t p = old ? a.tables[(int64_t)parent[s] * a.width + e] : -1;
     a.new_tables[(int64_t)s * a.width + e] = (uint32_t)p < a.pages ? p : -1;
   });
+  // One slot alone: only a last page that its table lists as a full one too is copied,
+  // by this workgroup.  Hardly a call has one, and a launch for it takes 2 us.
+  if (a.slots != 1 || last[0] < 0 || kept[0])
+    return;
+  __threadfence_block();
+  __syncthreads();
+  const int32_t target = a.new_tables[full[0]];
+  if (target < 0)
+    return;
+  const uint64_t page = (uint64_t)pool.blocks * pool.block_bytes;
+  const uint32_t bytes = (uint32_t)(a.new_lengths[0] & ((1 << a.page_log) - 1)) * pool.token_bytes;
+  for (uint32_t b = 0; b < pool.blocks; ++b)
+    copy_bytes<kTableThreads>(pool.data + (uint64_t)last[0] * page + (uint64_t)b * pool.block_bytes,
+                              pool.data + (uint64_t)target * page + (uint64_t)b * pool.block_bytes, bytes);
 }
 
 // The pages that cache_assign_kernel gave in place of ones that are shared: what
 // their slots hold of them, `part` tokens of every block.  A workgroup copies up
 // to kCopyBytes of a block.
-constexpr uint32_t kCopyBytes = 16384;
-
-__device__ __forceinline__ void copy_bytes(const uint8_t* from, uint8_t* to, uint32_t bytes) {
-  constexpr int kDeep = 4;
-  u4_t v[kDeep];
-  for (uint32_t at = threadIdx.x * 16; at < bytes; at += 256 * 16 * kDeep) {
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (at + i * 4096 < bytes)
-        v[i] = *reinterpret_cast<const u4_t*>(from + at + i * 4096);
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (at + i * 4096 < bytes)
-        *reinterpret_cast<u4_t*>(to + at + i * 4096) = v[i];
-  }
-}
-
 __global__ __launch_bounds__(256) void page_fork_kernel(TableArgs a, PoolArgs p) {
   const uint32_t s = blockIdx.y;
   const int32_t from = a.parents ? a.parents[s] : (int32_t)s;
@@ -331,8 +347,8 @@ hipError_t launch_cache_write(hipStream_t s, const CacheArgs& c, const CacheRows
                        : dispatch(cache_write_kernel<_Float16>, grid, block, s, c, in, per_row, rows);
 }
 
-hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a) {
-  return dispatch(cache_assign_kernel, dim3(1), dim3(kTableThreads), s, a);
+hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a, const PoolArgs& p) {
+  return dispatch(cache_assign_kernel, dim3(1), dim3(kTableThreads), s, a, p);
 }
 
 hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p) {
