@@ -2512,7 +2512,7 @@ int q4k_cache_assign(void* stream, int device, const q4k_pool* pool, const int32
   if (slots < 2 || width == 0 || pool->page_size == 1)  // copied already, or no page is filled in part
     return Q4K_OK;
   LaunchTimer timer(s, Q4K_KERNEL_AUX);
-  Q4K_TRY_HIP(launch_page_fork(s, a, pool_args(pool)), "page fork launch");
+  Q4K_TRY_HIP(launch_page_fork(s, a, pool_args(pool), device_cus(device)), "page fork launch");
   return Q4K_OK;
 }
 

@@ -674,7 +674,7 @@ struct PoolArgs {
   uint32_t parts = 0;  // set by the launch: workgroups of a block
 };
 hipError_t launch_cache_assign(hipStream_t s, const TableArgs& a, const PoolArgs& p);  // and the copy of one slot alone
-hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p);
+hipError_t launch_page_fork(hipStream_t s, const TableArgs& a, PoolArgs p, int cus);
 // moves: 1 + pages + pages % 2 values.
 hipError_t launch_cache_compact(hipStream_t s, const TableArgs& a, int32_t* moves);
 hipError_t launch_page_move(hipStream_t s, const int32_t* moves, const PoolArgs& p, uint32_t pages, int cus);
