@@ -662,22 +662,26 @@ __device__ __forceinline__ void mark_values(const AttentionArgs& a, const uint8_
   }
 }
 
-// O^T += V^T P^T of 32 keys.
-template <typename T, int DP, int NQ>
+// O^T += V^T P^T of 32 keys.  PARTS: weights as two fp16 parts, 22 bits, and not one, 11
+// bits.  One is the output's own precision in fp16 and adds as much again to its
+// error (2.9e-4 of the values in all, 2.1e-4 with two parts).  Few rows take two, which they hardly
+// notice beside the reading of keys (8 rows 209.1 us with one, 210.8 with two; 5 of 8
+// sequences 59.0, 60.0; one row 14.2, 14.5); chunks of fp16 rows take one: 8192 rows 586 us with
+// one, 807 with two, 2048 of heads of 256 235 and 298.
+template <typename T, int DP, int NQ, bool PARTS>
 __device__ __forceinline__ void add_values(const uint8_t* v, const f4_t (&p0)[NQ], const f4_t (&p1)[NQ], Sums<DP, NQ>& sums) {
-  constexpr bool kParts = Rows<T, DP, NQ>::kParts;
-  constexpr int kAhead = kParts && DP == 256 ? 1 : 4;
+  constexpr int kAhead = PARTS && DP == 256 ? 1 : 4;
   uint32_t base = v_base<DP>(v);
   asm volatile("" : "+v"(base));  // one register, not one per fragment
   h8_t f[kAhead + 1];
 #pragma unroll
   for (int d = 0; d < kAhead; ++d)
     f[d] = v_fragment<DP>(base, d);
-  h8_t w[NQ], wl[kParts ? NQ : 1];
+  h8_t w[NQ], wl[PARTS ? NQ : 1];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     w[n] = pack_weights(p0[n], p1[n]);
-    if constexpr (kParts)
+    if constexpr (PARTS)
       wl[n] = pack_rest(p0[n], p1[n], w[n]);
   }
 #pragma unroll
@@ -688,7 +692,7 @@ __device__ __forceinline__ void add_values(const uint8_t* v, const f4_t (&p0)[NQ
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d % (kAhead + 1)], w[n], sums.o[n][d], 0, 0, 0);
-      if constexpr (kParts)
+      if constexpr (PARTS)
         sums.o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[d % (kAhead + 1)], wl[n], sums.o[n][d], 0, 0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -1245,7 +1249,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         sums.weigh(s, [&](int y) { return FORM ? 1.0f : rows.factor(y); });
 #pragma unroll
         for (int h = 0; h < NA / 2; ++h) {
-          add_values<T, DP, NQ>(k + kTile + h * 32 * DP * 2, s[2 * h], s[2 * h + 1], sums);
+          add_values<T, DP, NQ, Rows<T, DP, NQ>::kParts>(k + kTile + h * 32 * DP * 2, s[2 * h], s[2 * h + 1], sums);
         }
       }
     }
@@ -1402,7 +1406,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
           clear_values<64, kTile>(mine + kTile, lane);
           wait_lds();
         }
-        add_values<T, DP, NQ>(mine + kTile, s[0], s[1], sums);
+        add_values<T, DP, NQ, true>(mine + kTile, s[0], s[1], sums);
         wait_lds();
         if (more)
           fetch_v();
