@@ -958,11 +958,12 @@ __device__ __forceinline__ bool last_of_unit(const AttentionArgs& a, int r0, int
 }
 
 // Few rows: the last workgroup joins the sums.  A lane holds 4 values of a row; what
-// bounds it is the way to memory, so the loads of RU rows and PU stretches are on
-// their way at once.
-template <typename T, int DP, int QB, int EXTRA, int NW, int RU, int PU>
+// bounds it is the way to memory, so the loads of eight stretches are on their way at
+// once.
+template <typename T, int DP, int QB, int EXTRA, int NW>
 __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& line, const Place& p, int start, int wave) {
   constexpr int kLanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kRows = NW * (64 / kLanes);  // lanes of a row, rows at once
+  constexpr int kAtOnce = 8;
   const int lane = threadIdx.x & 63, d = 4 * (lane & (kLanes - 1)), row = wave * (64 / kLanes) + lane / kLanes;
   const Unit& u = p.unit;
   const int r0 = line.of(p.at), parts = line.of(p.at + u.tiles - 1) - r0 + 1, rows = u.row_end - u.row;
@@ -971,49 +972,33 @@ __device__ __forceinline__ void join_unit(const AttentionArgs& a, const Line& li
   // Stretch r0 began before the unit, or with it; the others within it.
   const int late = line.start(r0) < p.at - EXTRA ? 1 : 0;
 #pragma unroll 1
-  for (int first = row; first - row < rows; first += RU * kRows) {
-    float m[RU], l[RU];
-    f4_t o[RU];
-#pragma unroll
-    for (int y = 0; y < RU; ++y) {
-      m[y] = -INFINITY;
-      l[y] = 0.0f;
-      o[y] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+  for (int r = row; r < rows; r += kRows) {
+    float m = -INFINITY, l = 0.0f;
+    f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int s0 = 0; s0 < parts; s0 += PU) {
-      float2 w[RU][PU], lo[RU][PU], hi[RU][PU];
+    for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
+      float2 w[kAtOnce], lo[kAtOnce], hi[kAtOnce];
 #pragma unroll
-      for (int s = 0; s < PU; ++s) {
-        // Past the last stretch, row or value: the last one again, left out below.
+      for (int s = 0; s < kAtOnce; ++s) {
+        // Past the last stretch or value: the last one again, left out below.
         const int at = s0 + s < parts ? s0 + s : parts - 1;
         const int64_t slot = 2 * (int64_t)(r0 + at) + (at == 0 ? late : 0);
-#pragma unroll
-        for (int y = 0; y < RU; ++y) {
-          const int r = first + y * kRows < rows ? first + y * kRows : rows - 1;
-          const float* v = part_row<DP, QB>(a, slot, r) + (d < DP ? d : 0);
-          w[y][s] = load_part(part_weights<DP, QB>(a, slot, r));
-          lo[y][s] = load_part(v);
-          hi[y][s] = load_part(v + 2);
-        }
+        const float* v = part_row<DP, QB>(a, slot, r) + (d < DP ? d : 0);
+        w[s] = load_part(part_weights<DP, QB>(a, slot, r));
+        lo[s] = load_part(v);
+        hi[s] = load_part(v + 2);
       }
 #pragma unroll
-      for (int s = 0; s < PU; ++s)
-#pragma unroll
-        for (int y = 0; y < RU; ++y) {
-          const float in = s0 + s < parts ? w[y][s].x : -INFINITY, top = fmaxf(m[y], in);
-          const float old = share(m[y], top), f = share(in, top);
-          m[y] = top;
-          if (s0 + s < parts) {
-            l[y] = l[y] * old + f * w[y][s].y;
-            o[y] = o[y] * old + f * f4_t{lo[y][s].x, lo[y][s].y, hi[y][s].x, hi[y][s].y};
-          }
+      for (int s = 0; s < kAtOnce; ++s)
+        if (s0 + s < parts) {
+          const float in = w[s].x, top = fmaxf(m, in), old = share(m, top), f = share(in, top);
+          m = top;
+          l = l * old + f * w[s].y;
+          o = o * old + f * f4_t{lo[s].x, lo[s].y, hi[s].x, hi[s].y};
         }
     }
-#pragma unroll
-    for (int y = 0; y < RU; ++y)
-      if (first + y * kRows < rows && d < a.cache.dim)
-        store4(out_row<T>(a, start, p.head, u.row + first + y * kRows) + d, row_values(o[y], l[y], m[y]));
+    if (d < a.cache.dim)
+      store4(out_row<T>(a, start, p.head, u.row + r) + d, row_values(o, l, m));
   }
 }
 
@@ -1465,7 +1450,7 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
       }
     }
     if (!done)
-      join_unit<T, DP, QB, kExtra, NW, 1, 8>(a, line, p, start, wave);
+      join_unit<T, DP, QB, kExtra, NW>(a, line, p, start, wave);
     if (p.at + t0 + n >= end)
       return;
     leading = false;

@@ -640,9 +640,10 @@ struct AttentionShape {
   static constexpr int chunk_least = 2;  // tiles of a workgroup, at least
   // Up to 16 times as many query rows of a cache head go to the kernel of few rows.
   // 8 sequences, 1024 | 16384 keys, us with it and with chunks: 16 rows of 256 (fp16)
-  // 25.7, 26.8 | 119, 129; 32 rows 35.6, 28.0 | 130, 135; 16 rows of 128 15.3, 23.6 |
-  // 56, 73; 32 rows 21.6, 24.8 | 62, 75; 48 rows 27.1, 26.0 | 70, 76 (fp32 33.8,
-  // 29.9 | 80, 101).
+  // 26.1, 21.4 | 119, 122; 32 rows 35.6, 21.9 | 130, 128; 16 rows of 128 15.3, 19.9 |
+  // 56, 67; 32 rows 21.4, 20.5 | 62, 68 (fp32 23.5, 23.8 | 64, 82); 48 rows 27.2, 22.3 |
+  // 72, 73 (fp32 31.6, 26.9 | 77, 94): the lengths are on the device, and long
+  // contexts, where a step takes longest, gain more than short ones lose.
   static constexpr int most_row_tiles(int dp) { return dp <= 128 ? 3 : 1; }
   // What a unit's beginning and end cost, in tiles of chunk_keys and of 32 keys (us
   // with 4, 6 and 8 for chunks: 821 fp32 rows 66.1, 63.5, 67.1, 2048 rows of heads of
