@@ -36,6 +36,10 @@ typedef __attribute__((address_space(3))) s4_t lds_s4_t;
 // (2^(kTop + kSlack) is still finite), which is rare after the first tiles.
 constexpr float kTop = 8.0f, kSlack = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
+// Maxima from here on leave t - m + kTop to a sum of its own (sum_again).  The products'
+// multiply-add keeps what the maximum's own rounding took off, half a step, and kTop takes part in that rounding:
+// from 2^27 on 8 and more, weights past fp16, or of nothing.
+constexpr float kFar = 0x1p26f;
 
 // tanh within 2^-21 of the value: the odd series below 1/4 (its next term is
 // 2^-26 of the value there), 1 - 2 / (e^2x + 1) above, whose error is 2^-23.
@@ -453,6 +457,7 @@ template <int DP, int NQ>
 struct Sums {
   f4_t o[NQ][DP / 16];
   float m[NQ], l[NQ];
+  bool far;  // a maximum of the wave's rows has passed kFar or -kFar
   uint32_t some[NQ];
   uint32_t up[NQ][(DP + 127) / 128], down[NQ][(DP + 127) / 128];  // sums that infinities and NaN reach: bit 4 d + e
 
@@ -502,6 +507,7 @@ struct Sums {
   }
 
   __device__ __forceinline__ void clear() {
+    far = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -532,12 +538,13 @@ struct Sums {
       top[n] = row_max(v) * c(n);
       rise = rise || top[n] > m[n] + kSlack;
     }
-    if (__any(rise)) {
+    if (__builtin_expect(__any(rise), 0)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         const float now = fmaxf(m[n], top[n]);
         const float f = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
         m[n] = now;
+        far = far || __any(fabsf(now) >= kFar && now > -INFINITY);
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
@@ -814,6 +821,82 @@ __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequenc
         }
       }
     }
+  }
+}
+
+// The sums of the wave's rows from `row` on over the keys of tiles of TK from `key` on,
+// every `step` keys, before `end`, for scores too large for the tiles' way with weights
+// (Sums::far): a key at a time, out of memory, t rounded once and its distance from the
+// maximum exact.  The four lanes of a row share its products and hold its values as after the tiles.
+// Expected of no wave, as mark_again: slow, and found anew.
+template <typename T, int DP, int NQ, int TK>
+__device__ __forceinline__ void sum_again(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row, int key, int end, int step,
+                                          Sums<DP, NQ>& sums) {
+#pragma clang fp contract(off)
+  typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+  typedef T t4_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  const CacheArgs& c = a.cache;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane), "+s"(head), "+s"(row));
+  const int g = lane >> 4, first = lane_value(s.first, u.seq), start = lane_value(s.start, u.seq), cap = lane_value(s.cap, u.seq);
+  const float scale = __builtin_amdgcn_fmed3f(a.scale * kLog2e, 0x1p-126f, 0x1p127f);
+  Pages pages;
+  pages.open(a, s, u.seq);
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = row + 16 * n + (lane & 15), token = token_of(a, r), h = head * a.group + (r - token * a.group);
+    const bool live = r < u.row_end;
+    const T* const q = static_cast<const T*>(a.q) + (int64_t)(start + token) * a.q_row + (int64_t)h * a.q_head + 4 * g;
+    const int pos = live ? first + token : -1;
+    const float slope = live && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+    sums.m[n] = -INFINITY;
+    sums.l[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      sums.o[n][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int tile = key; tile < end; tile += step)
+#pragma unroll 1
+      for (int j = tile; j < tile + TK; ++j) {
+        int low, high;
+        seen_keys(a, pos, cap, j, low, high);
+        const bool sees = 0 > low && 0 <= high;
+        pages.reach(a, j >> c.page_log);
+        const int page = pages.page(j >> c.page_log);
+        if (page < 0 || !__any(sees))
+          continue;
+        const int64_t at = (int64_t)head * c.head_stride * 2 + Pages::bytes(c, page, j) + 8 * g;
+        const uint8_t* const k = static_cast<const uint8_t*>(c.k) + at;
+        const uint8_t* const v = static_cast<const uint8_t*>(c.v) + at;
+        float x = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < c.dim; d += 16)
+          if (live && d + 4 * g < c.dim) {
+            const t4_t left = *reinterpret_cast<const t4_t*>(q + d);
+            const h4_t right = *reinterpret_cast<const h4_t*>(k + 2 * d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x = fmaf((float)left[e], (float)right[e], x);
+          }
+        float t = row_sum(x) * a.sign * scale;
+        if (a.softcap > 0.0f)
+          t = a.softcap * kLog2e * tanh_score(t / (a.softcap * kLog2e));
+        t = sees ? fmaf(slope, (float)(j - pos), t) : -INFINITY;
+        const float now = fmaxf(sums.m[n], t), f = now == sums.m[n] ? 1.0f : __builtin_amdgcn_exp2f(sums.m[n] - now);
+        const float w = t == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((t - now) + kTop);
+        sums.m[n] = now;
+        sums.l[n] = sums.l[n] * f + (g == 0 ? w : 0.0f);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          h4_t y = {};
+          if (sees && 16 * d + 4 * g < c.dim)
+            y = *reinterpret_cast<const h4_t*>(v + 32 * d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sums.o[n][d][e] = fmaf(w, (float)y[e], sums.o[n][d][e] * f);
+          asm volatile("" ::: "memory");  // one after another: no registers for more
+        }
+      }
   }
 }
 
@@ -1204,7 +1287,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const int key = u.lo + (t0 + t) * TK;
         uint8_t* const k = lds + (t & 1) * 2 * kTile;
         const bool most = active && key < hi_most && key + TK > lo_least;
-        if (key + TK > unit_hi || key < unit_lo || here != (1u << NA) - 1) {
+        if (__builtin_expect(key + TK > unit_hi || key < unit_lo || here != (1u << NA) - 1, 0)) {
           if (__syncthreads_or(odd_values<64 * NW, kTile>(k + kTile, tid))) {
             if (most)
 #pragma unroll
@@ -1218,11 +1301,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         // The next tile's transfers go between the first products: all at once they
         // would wait for the way to the caches before the products begin (1130 to 2510
         // clocks of a tile of 5700).
-        if (asks && (!most || c.dim != DP)) {
+        if (__builtin_expect(asks && (!most || c.dim != DP), 0)) {
           fetch();
           asks = false;
         }
-        if (!most)
+        if (__builtin_expect(!most, 0))
           continue;
         const bool whole = key + TK <= hi_least && key >= lo_most && here == (1u << NA) - 1;
         f4_t s[NA][NQ];
@@ -1238,6 +1321,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
       }
     }
+    if (__builtin_expect(sums.far, 0))
+      sum_again<T, DP, NQ, TK>(a, kept_sequences(kept), u, p.head, row, u.lo + t0 * TK, u.lo + (t0 + n) * TK, TK, sums);
     float l[NQ];
 #pragma unroll
     for (int y = 0; y < NQ; ++y)
@@ -1397,6 +1482,8 @@ __global__ __launch_bounds__(64 * NW) void attention_rows_kernel(AttentionArgs a
           fetch_v();
       }
     }
+    if (__builtin_expect(sums.far, 0))
+      sum_again<T, DP, NQ, TK>(a, kept_sequences(kept), u, p.head, u.row, u.lo + (t0 + wave) * TK, u.lo + (t0 + n) * TK, NW * TK, sums);
     float l[NQ];
 #pragma unroll
     for (int y = 0; y < NQ; ++y)

@@ -131,3 +131,41 @@ def test_values_of_infinity(q4k, gpu, counts, contexts, window, size, dim, dtype
         assert not len(off), f"{what.__name__}: {len(off)} places, row, head and element {off[0]}"
     fine = np.isfinite(want)
     _close(torch.from_numpy(np.where(fine, got, 0.0)), np.where(fine, want, 0.0), np.where(fine, bound, 1.0), "finite ones")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 24, 2.0 ** 26, 1.3 * 2.0 ** 27, 1.7 * 2.0 ** 27, 2.0 ** 29, 2.0 ** 33])
+@pytest.mark.parametrize("counts,contexts", [([1, 2], [70, 3000]), ([5], [900]), ([70], [300]), ([90, 40], [3000, 500])])
+@pytest.mark.parametrize("dim,softcap,slopes", [(64, 0.0, False), (128, 0.0, True), (256, 0.0, False), (80, 2.0 ** 40, False)])
+def test_scores_of_any_size(q4k, gpu, counts, contexts, size, dim, softcap, slopes, dtype):
+    """One key whose score is above all others', by a hundredth of `size` and more, where scores of that size have steps of
+    2^-23 of it: its values, but for the roundings of one weight and the output (2^-11 each in fp16).  Once with all scores above zero, once
+    below, once with that key's at zero and the others' far below."""
+    rng = np.random.default_rng(dim)
+    for sign in (1.0, -1.0, 0.0):
+        tables, cache, q, first = _case(gpu, counts, contexts, 4, 2, dim, 32, dtype)
+        cache[:, 0] = 0.0
+        # Scores are size * k[0] (fp16 k): q[0] k[0] / sqrt(dim).
+        a = float(np.sqrt(size * np.sqrt(dim)))
+        small = min(a, 30000.0)
+        q.zero_()
+        q[:, :, 0] = a * a / small if dtype is F32 else min(a * a / small, 60000.0)
+        q[:, :, 1] = 0.5
+        best = [min(f, n - 3) for f, n in zip(first, contexts)]
+        for t, n, b in zip(tables, contexts, best):
+            for at in range(n):
+                x = 1.0 if at == b else float(rng.uniform(0.25, 0.99))
+                x = small * (x if sign > 0 else x - 1.25 if sign < 0 else 0.0 if at == b else -x)
+                cache[t[at // 32], 0, :, at % 32, 0] = x
+        sl = torch.full((4,), 0.25, device=gpu) if slopes else None
+        out = torch.full(q.shape, 9.0, device=gpu, dtype=dtype)
+        q4k.attention(q.to(gpu), cache[:, 0], cache[:, 1], _i32(gpu, tables), _i32(gpu, first), out, query_counts=counts, softcap=softcap, slopes=sl)
+        torch.cuda.synchronize()
+        v, got, r = cache[:, 1].double().cpu().numpy(), out.double().cpu().numpy(), 0
+        for s, (t, n, b) in enumerate(zip(tables, counts, best)):
+            want = v[t[b // 32], :, b % 32]  # [kv, dim]
+            want = np.repeat(want, 2, axis=0)[None]
+            off = np.abs(got[r:r + n] - want)
+            bad = ~(off <= 2.0 ** -10 * np.abs(want) + 2.0 ** -24)
+            assert not bad.any(), f"{sign} sequence {s}: {bad.sum()} of {bad.size}, {np.isnan(off).sum()} NaN"
+            r += n
