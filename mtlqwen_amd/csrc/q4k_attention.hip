@@ -544,7 +544,7 @@ struct Sums {
         const float now = fmaxf(m[n], top[n]);
         const float f = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
         m[n] = now;
-        far = far || __any(fabsf(now) >= kFar && now > -INFINITY);
+        far = far || __any(fabsf(now) >= kFar && fabsf(now) < INFINITY);
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
@@ -766,10 +766,11 @@ struct Lanes {
 };
 
 // Marks the infinities and NaN of V of keys `key` .. `end` - 1, whole groups of 16, out
-// of memory, for the wave's rows from `row` on.  The lanes look over 16 tokens together; those of a group
-// that holds some are gone through one by one.  Neither LDS nor barriers, all found
-// anew, and expected of no wave: laid out among the tiles' code, or with registers of its own
-// under the products, it took 8192 fp16 rows of heads of 64 from 391 to 420 us.
+// of memory, for the wave's rows from `row` on.  The lanes look over 16 tokens together; those
+// that hold some are gone through one by one.  Neither LDS nor barriers, all found
+// anew, and expected of no wave: laid out among the tiles' code it took 8192 fp16 rows of heads of 64
+// from 391 to 420 us.  8192 rows of 128 take 2.1 ms in place of 0.58 where every
+// page holds an infinity, 35 ms where every token does.
 template <int DP, int NQ>
 __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row, int key, int end,
                                            Sums<DP, NQ>& sums) {
@@ -792,32 +793,34 @@ __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequenc
 #pragma unroll 1
     for (int d = 8 * g; d < c.dim; d += 32)
       bits |= odd_bits(*reinterpret_cast<const u4_t*>(tokens + ((lane & 15) * c.token_stride + d) * 2));
-    if (!__any(bits != 0))
-      continue;
+    const uint64_t lanes = __ballot(bits != 0), half = lanes | lanes >> 32;
 #pragma unroll 1
-    for (int i = 0; i < DP; ++i) {  // token i % 16, d of 16 (i / 16)
-      const int t = i & 15, d = i >> 4;
-      if (16 * d + 4 * g >= c.dim)
-        continue;
-      const h4_t f = *reinterpret_cast<const h4_t*>(tokens + (t * c.token_stride + 16 * d + 4 * g) * 2);
-      uint32_t up = 0, down = 0;
+    for (uint32_t odd = (uint32_t)(half | half >> 16) & 0xffff; odd; odd &= odd - 1) {
+      const int t = __builtin_ctz(odd);
+#pragma unroll 1
+      for (int d = 0; d < DP / 16; ++d) {
+        if (16 * d + 4 * g >= c.dim)
+          continue;
+        const h4_t f = *reinterpret_cast<const h4_t*>(tokens + (t * c.token_stride + 16 * d + 4 * g) * 2);
+        uint32_t up = 0, down = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        up |= f[e] <= (_Float16)65504.0f ? 0u : 1u << e;
-        down |= f[e] >= (_Float16)-65504.0f ? 0u : 1u << e;
-      }
-      up <<= 4 * (d & 7);
-      down <<= 4 * (d & 7);
+        for (int e = 0; e < 4; ++e) {
+          up |= f[e] <= (_Float16)65504.0f ? 0u : 1u << e;
+          down |= f[e] >= (_Float16)-65504.0f ? 0u : 1u << e;
+        }
+        up <<= 4 * (d & 7);
+        down <<= 4 * (d & 7);
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        int low, high;
-        const int mine = row + 16 * n + (lane & 15);
-        seen_keys(a, mine < u.row_end ? first + token_of(a, mine) : -1, cap, key, low, high);
-        const bool sees = t > low && t <= high;
+        for (int n = 0; n < NQ; ++n) {
+          int low, high;
+          const int mine = row + 16 * n + (lane & 15);
+          seen_keys(a, mine < u.row_end ? first + token_of(a, mine) : -1, cap, key, low, high);
+          const bool sees = t > low && t <= high;
 #pragma unroll
-        for (int x = 0; x < (DP + 127) / 128; ++x) {
-          sums.up[n][x] |= sees && d >> 3 == x ? up : 0u;
-          sums.down[n][x] |= sees && d >> 3 == x ? down : 0u;
+          for (int x = 0; x < (DP + 127) / 128; ++x) {
+            sums.up[n][x] |= sees && d >> 3 == x ? up : 0u;
+            sums.down[n][x] |= sees && d >> 3 == x ? down : 0u;
+          }
         }
       }
     }
@@ -828,7 +831,8 @@ __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequenc
 // every `step` keys, before `end`, for scores too large for the tiles' way with weights
 // (Sums::far): a key at a time, out of memory, t rounded once and its distance from the
 // maximum exact.  The four lanes of a row share its products and hold its values as after the tiles.
-// Expected of no wave, as mark_again: slow, and found anew.
+// Expected of no wave, as mark_again: slow (8192 rows of 128 93 ms, 8 rows of up to 65536
+// keys 6 ms), and found anew.
 template <typename T, int DP, int NQ, int TK>
 __device__ __forceinline__ void sum_again(const AttentionArgs& a, const Sequences& s, const Unit& u, int head, int row, int key, int end, int step,
                                           Sums<DP, NQ>& sums) {
