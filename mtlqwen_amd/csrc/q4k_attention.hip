@@ -459,34 +459,29 @@ struct Sums {
   float m[NQ], l[NQ];
   bool far;  // a maximum of the wave's rows has passed kFar or -kFar
   uint32_t some[NQ];
-  uint32_t up[NQ][(DP + 127) / 128], down[NQ][(DP + 127) / 128];  // sums that infinities and NaN reach: bit 4 d + e
 
-  // They reach them: infinity, -infinity, or both, a NaN.  And a row that sees keys whose scores
-  // are all -inf gets the lowest maximum: other stretches' weights leave nothing of
-  // its sums, and alone it is no row that sees nothing.
+  // A row that sees keys whose scores are all -inf gets the lowest maximum: other
+  // stretches' weights leave nothing of its sums, and alone it is no row that sees nothing.
   __device__ __forceinline__ void settle() {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const bool sees = (some[n] >> (threadIdx.x & 15)) & 1;
       m[n] = m[n] == -INFINITY && sees ? -FLT_MAX : m[n];
     }
-    uint32_t any = 0;
+  }
+
+  // Sums that infinities, -infinities or both (NaN) reach: bit 4 d + e of `up` and `down`.
+  static constexpr int kWords = (DP + 127) / 128;
+  __device__ __forceinline__ void put(const uint32_t (&up)[NQ][kWords], const uint32_t (&down)[NQ][kWords]) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < (DP + 127) / 128; ++i)
-        any |= up[n][i] | down[n][i];
-    if (__any(any != 0)) {
+      for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool u = (up[n][d / 8] >> (4 * (d % 8) + e)) & 1, v = (down[n][d / 8] >> (4 * (d % 8) + e)) & 1;
-            o[n][d][e] = u || v ? (u ? INFINITY : 0.0f) - (v ? INFINITY : 0.0f) : o[n][d][e];
-          }
-    }
+        for (int e = 0; e < 4; ++e) {
+          const bool u = (up[n][d / 8] >> (4 * (d % 8) + e)) & 1, v = (down[n][d / 8] >> (4 * (d % 8) + e)) & 1;
+          o[n][d][e] = u || v ? (u ? INFINITY : 0.0f) - (v ? INFINITY : 0.0f) : o[n][d][e];
+        }
   }
 
   // Whether a sum of this lane is infinite or NaN (only those leave 0 * o other than 0)
@@ -516,9 +511,6 @@ struct Sums {
       m[n] = -INFINITY;
       l[n] = 0.0f;
       some[n] = 0;
-#pragma unroll
-      for (int i = 0; i < (DP + 127) / 128; ++i)
-        up[n][i] = down[n][i] = 0;
     }
   }
 
@@ -598,12 +590,12 @@ __device__ __forceinline__ h8_t v_fragment(uint32_t base, int dt) {
 // A weight of zero does not keep an infinity or NaN of V out of a product, so a
 // tile that some row does not see whole is looked over first (odd_values, by
 // THREADS threads together).  If it holds one, a product of the places of infinities and
-// NaN with who sees them says which sums they reach (mark_values: a bit per sum,
-// for settle()), and they become zero in LDS (clear_values).  Tiles that all rows see
-// are not looked over (it would be an eighth of their reads of LDS, and a barrier more).
-// An infinity there makes a sum infinite, or NaN where its weight, or the second part of one, is
-// zero or negative in fp16; so a wave some of whose sums come out as either
-// (Sums::odd) reads V once more and marks it (mark_again).
+// NaN with who sees them says which sums they reach, which become NaN (mark_values), and
+// they become zero in LDS (clear_values).  Tiles that all rows see are not looked over (it
+// would be an eighth of their reads of LDS, and a barrier more).  An infinity there
+// makes a sum infinite, or NaN where its weight, or the second part of one, is zero or
+// negative in fp16.  So a wave some of whose sums come out as either (Sums::odd) reads V
+// once more for what they are to be (mark_again).
 // A half's exponent plus one step reaches its sign bit for infinities and NaN alone.
 __device__ __forceinline__ uint32_t odd_bits(u4_t f) {
   return (((f.x & 0x7fff7fffu) + 0x04000400u) | ((f.y & 0x7fff7fffu) + 0x04000400u) | ((f.z & 0x7fff7fffu) + 0x04000400u) |
@@ -634,8 +626,10 @@ __device__ __forceinline__ void clear_values(uint8_t* v, int thread) {
 template <typename T, int DP, int NQ>
 __device__ __forceinline__ void mark_values(const AttentionArgs& a, const uint8_t* v, const Rows<T, DP, NQ>& r, int key, uint32_t there,
                                             Sums<DP, NQ>& sums) {
+  constexpr int kWords = Sums<DP, NQ>::kWords;
   const int g = (threadIdx.x & 63) >> 4;
   const uint32_t base = v_base<DP>(v);
+  uint32_t reached[NQ][kWords], any = 0;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     int low, high;
@@ -646,27 +640,29 @@ __device__ __forceinline__ void mark_values(const AttentionArgs& a, const uint8_
       const int k = 16 * (e >> 2) + (e & 3);
       one[e] = ((there >> (e >> 2)) & 1) && k > low && k <= high ? (_Float16)1.0f : (_Float16)0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      reached[n][i] = 0;
 #pragma unroll 1
-    for (int step = 0; step < DP / 8; ++step) {  // d and sign: a fragment at a time in registers
-      const int d = step >> 1;
-      const bool below = step & 1;
+    for (int d = 0; d < DP / 16; ++d) {  // a fragment at a time in registers
       h8_t f = v_fragment<DP>(base, d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // infinity and NaN, -infinity and NaN
-        f[e] = (below ? -f[e] : f[e]) <= (_Float16)65504.0f ? (_Float16)0.0f : (_Float16)1.0f;
+      for (int e = 0; e < 8; ++e)
+        f[e] = __builtin_fabsf16(f[e]) <= (_Float16)65504.0f ? (_Float16)0.0f : (_Float16)1.0f;
       const f4_t many = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
       uint32_t bits = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         bits |= many[e] > 0.0f ? 1u << e : 0u;
+      any |= bits;
       bits <<= 4 * (d & 7);
 #pragma unroll
-      for (int i = 0; i < (DP + 127) / 128; ++i) {
-        sums.up[n][i] |= !below && d >> 3 == i ? bits : 0u;
-        sums.down[n][i] |= below && d >> 3 == i ? bits : 0u;
-      }
+      for (int i = 0; i < kWords; ++i)
+        reached[n][i] |= d >> 3 == i ? bits : 0u;
     }
   }
+  if (__any(any != 0))
+    sums.put(reached, reached);
 }
 
 // O^T += V^T P^T of 32 keys.  PARTS: weights as two fp16 parts, 22 bits, and not one, 11
@@ -782,6 +778,7 @@ __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequenc
   const uint8_t* const v = static_cast<const uint8_t*>(c.v) + (int64_t)head * c.head_stride * 2;
   Pages pages;
   pages.open(a, s, u.seq);
+  uint32_t all_up[NQ][Sums<DP, NQ>::kWords] = {}, all_down[NQ][Sums<DP, NQ>::kWords] = {};
 #pragma unroll 1
   for (; key < end; key += 16) {
     pages.reach(a, key >> c.page_log);
@@ -817,14 +814,15 @@ __device__ __forceinline__ void mark_again(const AttentionArgs& a, const Sequenc
           seen_keys(a, mine < u.row_end ? first + token_of(a, mine) : -1, cap, key, low, high);
           const bool sees = t > low && t <= high;
 #pragma unroll
-          for (int x = 0; x < (DP + 127) / 128; ++x) {
-            sums.up[n][x] |= sees && d >> 3 == x ? up : 0u;
-            sums.down[n][x] |= sees && d >> 3 == x ? down : 0u;
+          for (int x = 0; x < Sums<DP, NQ>::kWords; ++x) {
+            all_up[n][x] |= sees && d >> 3 == x ? up : 0u;
+            all_down[n][x] |= sees && d >> 3 == x ? down : 0u;
           }
         }
       }
     }
   }
+  sums.put(all_up, all_down);
 }
 
 // The sums of the wave's rows from `row` on over the keys of tiles of TK from `key` on,
@@ -1294,7 +1292,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         if (__builtin_expect(key + TK > unit_hi || key < unit_lo || here != (1u << NA) - 1, 0)) {
           if (__syncthreads_or(odd_values<64 * NW, kTile>(k + kTile, tid))) {
             if (most)
-#pragma unroll
+#pragma unroll 1
               for (int h = 0; h < NA / 2; ++h)
                 mark_values<T, DP, NQ>(a, k + kTile + h * 32 * DP * 2, rows, key + 32 * h, here >> (2 * h), sums);
             __syncthreads();
@@ -1345,10 +1343,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         add_stretches<DP, NQ, NW>(a, r0, parts, line.start(r0) < p.at - kExtra ? 1 : 0, wg, wave, sums, l);
     }
     if (done) {
-      if (__builtin_expect(__any(sums.odd(l)), 0)) {
+      if (__builtin_expect(__any(sums.odd(l)), 0))
         mark_again<DP, NQ>(a, kept_sequences(kept), u, p.head, row, u.lo, u.lo + u.tiles * TK, sums);
-        sums.settle();
-      }
 #pragma unroll
       for (int y = 0; y < NQ; ++y) {
         const int r = row + 16 * y + (lane & 15);
