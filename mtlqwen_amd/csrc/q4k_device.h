@@ -246,20 +246,24 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
   return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
+// Such a load wants a wait state behind the write of m0, and five behind a vector
+// instruction's write of sbase (a spill's reload, say); the compiler, which sees to both
+// in its own code, does not look into an asm block.  With one more here the orders that it
+// makes of these kernels leave five.
 template <int OFFSET>
 __device__ __forceinline__ void lds_dma16(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET) : "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET) : "m0");
 }
 
 template <int OFFSET>
 __device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET) : "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 1\n\tglobal_load_lds_dword %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET) : "m0");
 }
 
 // The same with a constant added to the LDS address.
 template <int OFFSET, int LDS>
 __device__ __forceinline__ void lds_dma16_at(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_add_u32 m0, %2, %4\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET), "n"(LDS) : "m0", "scc");
+  asm volatile("s_add_u32 m0, %2, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(sbase), "s"(lds), "n"(OFFSET), "n"(LDS) : "m0", "scc");
 }
 
 // Stores and loads that bypass every cache level (sc0 sc1: system
