@@ -36,9 +36,9 @@ typedef __attribute__((address_space(3))) s4_t lds_s4_t;
 // (2^(kTop + kSlack) is still finite), which is rare after the first tiles.
 constexpr float kTop = 8.0f, kSlack = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
-// Maxima from here on leave t - m + kTop to a sum of its own (sum_again).  The products'
-// multiply-add keeps what the maximum's own rounding took off, half a step, and kTop takes part in that rounding:
-// from 2^27 on 8 and more, weights past fp16, or of nothing.
+// Rows whose maximum passes this are summed apart (sum_again): the multiply-add that
+// makes t - m + kTop keeps what the maximum's own rounding took off, half a step, and
+// rounds kTop with it, from 2^27 on by 8 and more, which makes weights that pass fp16 or are nothing.
 constexpr float kFar = 0x1p26f;
 
 // tanh within 2^-21 of the value: the odd series below 1/4 (its next term is
@@ -1173,12 +1173,12 @@ __device__ __forceinline__ void add_stretches(const AttentionArgs& a, int r0, in
 // ----------------------------------------------------------------------------
 // Chunks of tokens: NW waves of 16 NQ query rows each over the same key tiles,
 // two buffers of K and V in LDS, the next tile's transfers under the present
-// tile's products.  8192 fp16 rows of 32 / 8 heads of 128 take 568 us (968 TFLOP/s):
+// tile's products.  8192 fp16 rows of 32 / 8 heads of 128 take 579 us (950 TFLOP/s):
 // of a tile's 4000 clocks, a wave spends 660 to 950 on K Q^T, 1100 to 1220 on the weights
 // and 970 to 1020 on V P^T, and the other wave of its SIMD does not always have
-// what would fill them.  2048 rows of 16 / 4 heads of 256 take 239 us (761 TFLOP/s),
+// what would fill them.  2048 rows of 16 / 4 heads of 256 take 231 us (788 TFLOP/s),
 // bound by LDS: a fragment feeds the products of 16 rows there, not 32.  Ragged
-// prompts (821 fp32 rows, window 1024) take 63 us: 17 tiles a workgroup, 35 us of it at
+// prompts (821 fp32 rows, window 1024) take 65 us: 17 tiles a workgroup, 35 us of it at
 // 8192 rows' pace, and the beginnings and ends of units, nearly all of them shared.
 // ----------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int NW, int TK, bool FORM>
@@ -1370,8 +1370,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 // stretch, with a buffer for K and one for V of its own, refilled as soon as each
 // has been read; the waves' sums join in LDS at the end of a unit.  Bound by the
 // reading of K and V: 8 rows of 16 / 4 heads of 256 over 1.2 GB of them take 210 us
-// (5.75 TB/s), 40 capped fp32 rows of 32 / 8 heads of 128 over 304 MB 64 us.  One
-// row over 777 keys takes 14 us, the latency of its steps: units of the line, rows
+// (5.75 TB/s), 40 capped fp32 rows of 32 / 8 heads of 128 over 304 MB 70 us.  One
+// row over 777 keys takes 15 us, the latency of its steps: units of the line, rows
 // and keys, the waves' sums, the stretches' sums.  Four waves: with eight, heads of 128
 // of 8 sequences take 20.1 us in place of 17.0 (fp32 rows, 1024 keys; fp16 16.6 and
 // 15.3) and, over 16384 keys, 54.4 in place of 56.4 (fp16; fp32 57.7 and 57.1).
