@@ -392,9 +392,9 @@ typedef struct q4k_attention_params {
  * A row whose scores are all -inf becomes NaN (0 / 0); an infinity in a key that a
  * row of fp32 q, which is two parts, sees makes it NaN.
  * Scores, statistics and sums are fp32.  fp16 q are multiplied as they are, fp32 q
- * with 22 bits; weights enter the products with v with 22 bits, of fp16 q with more
- * than 48 rows times heads of a group per sequence (16 for head_dim above 128) as
- * fp16.  q and out as in q4k_rope, but they must not overlap.  Positions lie
+ * with 22 bits; weights enter the products with v with 22 bits, but as fp16 where q
+ * is fp16 and some sequence of the call has more than 48 rows times heads of a group
+ * (16 for head_dim above 128).  q and out as in q4k_rope, but they must not overlap.  Positions lie
  * in [-2^30, 2^30] (others are taken as the nearer end), rows * q->heads is at
  * most 2^30.  Work is split by the lengths that the device holds: one cache
  * head's key tiles, with full tables, must not pass 2^31 (Q4K_ESHAPE).  Sums of

@@ -169,3 +169,56 @@ def test_scores_of_any_size(q4k, gpu, counts, contexts, size, dim, softcap, slop
             bad = ~(off <= 2.0 ** -10 * np.abs(want) + 2.0 ** -24)
             assert not bad.any(), f"{sign} sequence {s}: {bad.sum()} of {bad.size}, {np.isnan(off).sum()} NaN"
             r += n
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim", [64, 80, 160, 256])
+@pytest.mark.parametrize("n,window", [(1, 0), (3, 3000), (40, 0), (60, 2500)])
+def test_rare_sums_of_long_contexts(q4k, gpu, n, window, dim, dtype):
+    """Infinite values, then scores too large for the tiles' way with weights, in eight sequences whose waves have several tiles each,
+    some of whose pages are not there: two heads of two sequences against 64 bits, every output for NaN."""
+    rng = np.random.default_rng(dim + n)
+    kv, heads, page = 4, 8, 16
+    contexts = [4000 + 311 * i for i in range(8)]
+    counts, first = [n] * 8, [c - n for c in contexts]
+    tables, pages = _tables(rng, contexts, page)
+    for t, c in zip(tables, contexts):
+        for e in range(5, c // page - 20, 17):
+            t[e] = -1
+    cache = _cache(rng, gpu, pages, kv, page, dim)
+    q = torch.from_numpy(rng.standard_normal((8 * n, heads, dim)).astype(np.float32)).to(dtype)
+    probes = ((1, 0), (6, 7))
+
+    def compare(out, far):
+        for s, h in probes:
+            mine = [p for p in tables[s] if p >= 0]
+            c = cache[torch.tensor(mine, device=gpu), :, h // 2].cpu().numpy()[:, :, None]
+            table = [mine.index(p) if p >= 0 else -1 for p in tables[s]]
+            rows = slice(s * n, (s + 1) * n)
+            with np.errstate(invalid="ignore"):
+                want, bound = ref.attention(q[rows, h:h + 1].float().numpy(), c[:, 0], c[:, 1], [table], [first[s]], [n], window=window, f16=dtype == F16)
+            got = out[rows, h:h + 1].cpu().double().numpy()
+            if far:  # one key alone has a weight, one of 22 or 11 bits
+                bound = 2.0 ** -10 * np.abs(want) + 2.0 ** -24
+            for what in (np.isposinf, np.isneginf, np.isnan):
+                assert np.array_equal(what(got), what(want)), (what.__name__, s, h)
+            fine = np.isfinite(want)
+            _close(torch.from_numpy(np.where(fine, got, 0.0)), np.where(fine, want, 0.0), np.where(fine, bound, 1.0), f"sequence {s} head {h}")
+
+    for t, c in zip(tables, contexts):
+        for at in range(c % 50, c, 97):
+            if t[at // page] >= 0:
+                cache[t[at // page], 1, :, at % page, 3] = float("inf")
+                cache[t[at // page], 1, :, at % page, dim - 1] = float("inf") if at % 2 else float("-inf")
+    compare(_attend(q4k, gpu, q, cache, tables, first, counts, window), False)
+    # One key's score 2^30 / sqrt(dim), which passes 2^26 / log2(e), all others' at most 0.9 of it.
+    cache = _cache(rng, gpu, pages, kv, page, dim)
+    cache[:, 0] = 0.0
+    cache[:, 0, :, :, 0] = torch.from_numpy(rng.uniform(-0.9, 0.9, (pages, 1, page))).to(gpu).to(F16) * 2.0 ** 15
+    q.zero_()
+    q[:, :, 0] = 2.0 ** 15
+    for t, f in zip(tables, first):
+        at = f - n if t[(f - n) // page] >= 0 else f - n - page
+        assert t[at // page] >= 0
+        cache[t[at // page], 0, :, at % page, 0] = 2.0 ** 15
+    compare(_attend(q4k, gpu, q, cache, tables, first, counts, window), True)
