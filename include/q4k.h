@@ -421,7 +421,8 @@ typedef struct q4k_pool {
  * Full pages are shared.  A last page that is not full stays with the lowest
  * slot that holds it (if no other holds it as a full one), the others get a
  * page with a copy of its tokens.  New pages are the lowest that no slot's new
- * tokens lie in, in the order of the slots.  Entries without a page are -1;
+ * tokens lie in, in the order of the slots.  Entries without a page are -1, and a
+ * page below its length that the parent lacks stays lacking;
  * *missing (may be NULL) is the number of pages asked for and not given (at most
  * 2^31 - 1).  A page
  * counts as held where it lies below a slot's length (clamped to its table), so
